@@ -17,7 +17,9 @@ LIB_PATH = os.path.join(HERE, "lib", os.environ.get("BWGEMM_LIB") or "libbwgemm.
 HEADER = os.path.join(os.path.dirname(HERE), "include", "bwgemm.h")
 
 BW_OK, BW_ERR_SHAPE, BW_ERR_LAUNCH, BW_ERR_TIMEOUT, BW_ERR_ARG, BW_ERR_DEVICE = 0, 1, 2, 3, 4, 5
+BW_ERR_SCRATCH = 6
 BW_KERNEL_TILE, BW_KERNEL_SWAP, BW_KERNEL_PAIR = 0, 1, 2
+BW_TYPE_F16, BW_TYPE_BF16, BW_TYPE_F32 = 0, 1, 2
 
 
 class Plan(ctypes.Structure):
@@ -108,6 +110,17 @@ def lib():
         L.bw_gemm_f16_rs.restype = i
         L.bw_rs_destroy.argtypes = [vp]
         L.bw_rs_destroy.restype = i
+        ll, sz = ctypes.c_longlong, ctypes.c_size_t
+        L.bw_quant_rows_i8.argtypes = [vp, i, ll, vp, vp, i, i, vp]
+        L.bw_quant_rows_i8.restype = i
+        L.bw_gemm_i8_work_bytes.argtypes = [i, i, i, i, i, i, ctypes.POINTER(sz)]
+        L.bw_gemm_i8_work_bytes.restype = i
+        L.bw_gemm_i8.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
+        L.bw_gemm_i8.restype = i
+        L.bw_gemm_i8_swiglu.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, sz, vp]
+        L.bw_gemm_i8_swiglu.restype = i
+        L.bw_linear_i8.argtypes = [vp, i, ll, vp, vp, vp, i, i, i, i, vp, sz, vp]
+        L.bw_linear_i8.restype = i
         L.bw_status_string.argtypes = [i]
         L.bw_status_string.restype = ctypes.c_char_p
         L.bw_last_error_string.argtypes = []
@@ -237,6 +250,163 @@ def gemm_swiglu(A, B, C=None, stream=None):
     s = stream if stream is not None else torch.cuda.current_stream(A.device)
     with torch.cuda.device(A.device):
         check(lib().bw_gemm_f16_swiglu(A.data_ptr(), B.data_ptr(), C.data_ptr(), M, N, K, s.cuda_stream))
+    return C
+
+
+# ---------------------------------------------------------------------------------- 8-bit integer products
+def _types():
+    import torch
+
+    return {torch.float16: BW_TYPE_F16, torch.bfloat16: BW_TYPE_BF16, torch.float32: BW_TYPE_F32}
+
+
+class _On:
+    """The tensors' device made current and `stream` (None: that device's current stream) the current one there, so
+    that memory made inside belongs to the stream the call runs on; does nothing where both already are."""
+
+    def __init__(self, device, stream):
+        import torch
+
+        self.ctx = []
+        if stream is not None and stream != torch.cuda.current_stream(device):
+            self.ctx.append(torch.cuda.stream(stream))
+        elif torch.cuda.current_device() != device.index:
+            self.ctx.append(torch.cuda.device(device))
+        self.device = device
+
+    def __enter__(self):
+        import torch
+
+        for c in self.ctx:
+            c.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        for c in reversed(self.ctx):
+            c.__exit__(*exc)
+
+
+def _rows16(X, what):
+    """X as rows of 16-bit values a kernel reads as they are: (rows, cols, elements from row to row)."""
+    import torch
+
+    if X.dtype not in (torch.float16, torch.bfloat16) or not X.is_cuda or X.dim() != 2:
+        raise ValueError(f"{what} must be a 2-D fp16 or bf16 CUDA tensor")
+    rows, cols = X.shape
+    if cols > 1 and X.stride(1) != 1:
+        raise ValueError(f"{what}'s rows must be contiguous")
+    ld = X.stride(0) if rows > 1 else cols
+    if ld < cols or ld % 8 or X.data_ptr() % 16:
+        raise ValueError(f"{what}'s rows must start on 16-byte boundaries and not overlap")
+    return rows, cols, ld
+
+
+def _i8_weight(B, b_scale, device):
+    import torch
+
+    if B.dtype != torch.int8 or B.dim() != 2 or B.device != device or not B.is_contiguous():
+        raise ValueError("B must be a contiguous int8 N x K tensor on A's device")
+    if b_scale.dtype != torch.float32 or b_scale.shape != (B.shape[0],) or b_scale.device != device or \
+            not b_scale.is_contiguous():
+        raise ValueError("b_scale must be a contiguous fp32 tensor of B's N scales on A's device")
+
+
+def _i8_out(C, shape, dtype, device):
+    import torch
+
+    if C is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(C.shape) != tuple(shape) or C.dtype != dtype or C.device != device or not C.is_contiguous():
+        raise ValueError(f"C must be a contiguous {dtype} tensor of {shape[0]} x {shape[1]} on A's device")
+    return C
+
+
+_i8_work_bytes = {}  # (device, M, N, K, type, swiglu, linear) -> bytes: the plan's, a constant of the device
+
+
+def _i8_work(device, M, N, K, out_type, swiglu, linear):
+    """The call's own workspace from torch's allocator (so of the stream, or the CUDA graph, that the call is part of)."""
+    import torch
+
+    key = (device.index, M, N, K, out_type, swiglu, linear)
+    n = _i8_work_bytes.get(key)
+    if n is None:
+        size = ctypes.c_size_t()
+        check(lib().bw_gemm_i8_work_bytes(M, N, K, out_type, swiglu, linear, ctypes.byref(size)))
+        if len(_i8_work_bytes) >= 4096:
+            _i8_work_bytes.clear()
+        n = _i8_work_bytes[key] = size.value
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+
+
+def quantize_rows(X, Q=None, scale=None, stream=None):
+    """(Q, scale): the rows of a 2-D fp16 or bf16 CUDA tensor (rows may be strided) as int8 and their fp32 scales,
+    scale = max|row| / 127, Q = round-half-even(127 X / max|row|); made if not given.  X's columns: a multiple of 16."""
+    import torch
+
+    rows, cols, ld = _rows16(X, "X")
+    with _On(X.device, stream) as s:
+        Q = _i8_out(Q, (rows, cols), torch.int8, X.device)
+        if scale is None:
+            scale = torch.empty((rows,), dtype=torch.float32, device=X.device)
+        elif scale.shape != (rows,) or scale.dtype != torch.float32 or scale.device != X.device or \
+                not scale.is_contiguous():
+            raise ValueError("scale must be a contiguous fp32 tensor of X's rows")
+        check(lib().bw_quant_rows_i8(X.data_ptr(), _types()[X.dtype], ld, Q.data_ptr(), scale.data_ptr(), rows, cols, s))
+    return Q, scale
+
+
+def _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, swiglu):
+    import torch
+
+    dtype = torch.float16 if dtype is None else dtype
+    types = _types()
+    if dtype not in types or (swiglu and dtype == torch.float32):
+        raise ValueError(f"C cannot be {dtype}")
+    if A.dtype != torch.int8 or A.dim() != 2 or not A.is_cuda or not A.is_contiguous():
+        raise ValueError("A must be a contiguous int8 M x K CUDA tensor")
+    M, K = A.shape
+    if a_scale.dtype != torch.float32 or a_scale.shape != (M,) or a_scale.device != A.device or \
+            not a_scale.is_contiguous():
+        raise ValueError("a_scale must be a contiguous fp32 tensor of A's M scales on A's device")
+    _i8_weight(B, b_scale, A.device)
+    N, K2 = B.shape
+    if K2 != K:
+        raise ValueError(f"A is {M} x {K} but B is {N} x {K2}")
+    with _On(A.device, stream) as s:
+        C = _i8_out(C, (M, N // 2 if swiglu else N), dtype, A.device)
+        work, n = _i8_work(A.device, M, N, K, types[dtype], swiglu, 0)
+        f = lib().bw_gemm_i8_swiglu if swiglu else lib().bw_gemm_i8
+        check(f(A.data_ptr(), a_scale.data_ptr(), B.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, types[dtype],
+                work.data_ptr() if n else None, n, s))
+    return C
+
+
+def gemm_i8(A, a_scale, B, b_scale, C=None, dtype=None, stream=None):
+    """C (M x N) = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k] for int8 CUDA tensors A (M x K) and B (N x K), exact integer
+    sums, in `dtype` (fp16 by default, bf16 or fp32)."""
+    return _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, 0)
+
+
+def gemm_i8_swiglu(A, a_scale, B, b_scale, C=None, dtype=None, stream=None):
+    """C (M x N/2, fp16 or bf16) = silu(gate) * up of the scaled products, B's rows in groups of 128 gate then 128 up."""
+    return _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, 1)
+
+
+def linear_i8(X, B, b_scale, C=None, swiglu=False, stream=None):
+    """C = X B^T in X's type (fp16 or bf16): X (M x K, rows may be strided) quantised to int8 by row (quantize_rows), B
+    (N x K) int8 with a scale per row; swiglu: silu(gate) * up, M x N/2, B's rows in groups of 128 gate then 128 up."""
+    M, K, ld = _rows16(X, "X")
+    _i8_weight(B, b_scale, X.device)
+    N, K2 = B.shape
+    if K2 != K:
+        raise ValueError(f"X is {M} x {K} but B is {N} x {K2}")
+    t, swiglu = _types()[X.dtype], int(bool(swiglu))
+    with _On(X.device, stream) as s:
+        C = _i8_out(C, (M, N // 2 if swiglu else N), X.dtype, X.device)
+        work, n = _i8_work(X.device, M, N, K, t, swiglu, 1)
+        check(lib().bw_linear_i8(X.data_ptr(), t, ld, B.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, swiglu,
+                                 work.data_ptr() if n else None, n, s))
     return C
 
 

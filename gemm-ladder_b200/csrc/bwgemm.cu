@@ -11,6 +11,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <atomic>
 
 #include "bwgemm.h"
 #include "gemm_kernel.cuh"
@@ -255,7 +256,7 @@ const int* held_of(const DeviceState& d) { return BW_KSPLIT ? d.held : nullptr; 
 
 template <int BN, bool SWAP, bool PAIR, int EPI = kEpiF16, int WM = 1>
 int launch_kernel(DeviceState& d, unsigned long long bit, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my,
-                  const CUtensorMap& mc, const Params& p, cudaStream_t st)
+                  const CUtensorMap& mc, const Params& p, cudaStream_t st, bool pdl = false)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     // K split: what a block receives from the others of its cluster lands in its idle stage ring
@@ -270,7 +271,7 @@ int launch_kernel(DeviceState& d, unsigned long long bit, const bw_plan& q, cons
     cudaLaunchAttribute attr[2];
     // the reduce-scatter kernel keeps the plain stream order: its peers' calls pair with this one by epoch
     const cudaLaunchConfig_t cfg = launch_config<BN, SWAP, PAIR, WM, EPI>(q.grid, st, attr, q.ksplit,
-                                                                          g_pdl && EPI != kEpiRS);
+                                                                          (g_pdl && EPI != kEpiRS) || pdl);
     cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_kernel<BN, SWAP, PAIR, EPI, WM>, mx, my, mc, p);
     if (e != cudaSuccess) return cuda_fail(e, "kernel launch");
     return BW_OK;
@@ -667,6 +668,9 @@ BW_API int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw
                                     bw::held_of(*d));
     return bw::make_plan(M, N, K, d->sms, d->pairs, variant, out, 0u, bw::held_of(*d));
 }
+
+// ------------------------------------------------------------------ the 8-bit integer entries
+#include "gemm_i8.cuh"
 
 #ifdef BW_TRACE
 // The timeline of the last launch (a -DBW_TRACE build only; not part of the C ABI of bwgemm.h).

@@ -6,6 +6,56 @@
 
 namespace bw {
 
+// ------------------------------------------------------------------ 8-bit integer sums (kEpiI8*)
+// A 32-bit integer sum travels through the epilogue as the bits of a float (tensor memory, partials, shared memory
+// and the in-warp transposes only move it); it is added to other partials as an integer, so a split tile's sum is
+// exact, and turned into a value once, where C is stored: (float(s) * row scale) * column scale, three roundings of
+// 2^-24 each, then the one to C's type.
+template <int EPI>
+__device__ __forceinline__ float part_add(float a, float b)
+{
+    if constexpr (epi_i8(EPI)) return __int_as_float((int)((unsigned)__float_as_int(a) + (unsigned)__float_as_int(b)));
+    return a + b;
+}
+__device__ __forceinline__ float i8_value(float bits, float row_scale, float col_scale)
+{
+    return (float)__float_as_int(bits) * row_scale * col_scale;
+}
+// NC columns n .. n + NC - 1 (inside C) of row m: the scaled values; a row past M (never stored) gets scale 0.
+template <int NC>
+__device__ __forceinline__ void i8_row_values(const Params& p, int m, int n, const float (&s)[NC], float (&v)[NC])
+{
+    const float rs = m < p.s.M ? __ldg(p.row_scale + m) : 0.f;
+#pragma unroll
+    for (int j = 0; j < NC; j += 4) {
+        const float4 cs = *reinterpret_cast<const float4*>(p.col_scale + n + j);  // one address per warp: a broadcast
+        v[j] = i8_value(s[j], rs, cs.x);
+        v[j + 1] = i8_value(s[j + 1], rs, cs.y);
+        v[j + 2] = i8_value(s[j + 2], rs, cs.z);
+        v[j + 3] = i8_value(s[j + 3], rs, cs.w);
+    }
+}
+// Two values of C in its 16-bit type, the first in the low half.
+template <int EPI>
+__device__ __forceinline__ uint32_t pack2(const Params& p, float a, float b)
+{
+    if (epi_i8(EPI) && p.out_bf16) {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&y);
+    }
+    const __half2 x = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+template <int EPI>
+__device__ __forceinline__ __half half_bits(const Params& p, float a)  // one value, as the 16 bits of a __half
+{
+    if (epi_i8(EPI) && p.out_bf16) {
+        const __nv_bfloat16 y = __float2bfloat16_rn(a);
+        return *reinterpret_cast<const __half*>(&y);
+    }
+    return __float2half_rn(a);
+}
+
 // ------------------------------------------------------------------ the epilogue's stores
 // 16 accumulator columns of TMEM lane `lane` (v) -> C, by all 128 epilogue threads together.
 // Not swapped: C[m0 + lane][n0 + c0 .. +15], two 16-byte stores per thread.
@@ -18,6 +68,25 @@ __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int
                                             __half* cst)
 {
     const Sched& s = p.s;
+    if constexpr (epi_i8(EPI) && !SWAP) {  // the scaled values, then as the fp16 and fp32 outputs below
+        const int m = m0 + lane, n = n0 + c0;
+        if (m >= s.M || n >= s.N) return;
+        float w[16];
+        i8_row_values(p, m, n, v, w);
+        if (EPI == kEpiI8F32) {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.C) + (size_t)m * s.N + n);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) dst[q] = make_float4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        } else {
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = pack2<EPI>(p, w[2 * j], w[2 * j + 1]);
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.C) + (size_t)m * s.N + n);
+            dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        return;
+    }
     if (EPI == kEpiF32) {  // fp32 C (not swapped): four 16-byte stores
         const int m = m0 + lane, n = n0 + c0;
         if (m >= s.M || n >= s.N) return;
@@ -40,8 +109,18 @@ __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int
         dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
     } else {
         __half* buf = cst + ((c0 >> 4) & 1) * (16 * 128);
+        if constexpr (epi_i8(EPI)) {  // the lane's column scale, the chunk's 16 row scales
+            const int wb = BT ? c0 / BT : 0, tok = c0 - wb * BT, n = n0 + wb * 128 + lane;
+            const float cs = n < s.N ? __ldg(p.col_scale + n) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = __float2half_rn(v[j]);
+            for (int j = 0; j < 16; ++j) {
+                const float rs = tok + j < s.M ? __ldg(p.row_scale + tok + j) : 0.f;
+                buf[j * 128 + lane] = half_bits<EPI>(p, i8_value(v[j], rs, cs));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = __float2half_rn(v[j]);
+        }
         named_bar_sync(1, 128);
         const int t = threadIdx.x - kEpiThread0;
         // accumulator column c0: token c0 % BT of weight block c0 / BT (BT tokens per block; 0: one block)
@@ -88,21 +167,20 @@ __device__ __forceinline__ void transpose_pieces(uint32_t (&x)[P][4], int lane)
 }
 
 template <int EPI>
-__device__ __forceinline__ void store_rows64(const Params& p, int r0, int n, int lane, const float (&v)[64])
+__device__ __forceinline__ void store_lines64(const Params& p, int r0, int n, int lane, const float (&v)[64])
 {
-    static_assert(EPI == kEpiF16 || EPI == kEpiF32, "fp16 or fp32 C");
-    constexpr int P = EPI == kEpiF32 ? 16 : 8;
+    constexpr bool kF32 = EPI == kEpiF32 || EPI == kEpiI8F32;
+    constexpr int P = kF32 ? 16 : 8;
     const Sched& s = p.s;
     uint32_t x[P][4];
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            if (EPI == kEpiF32) {
+            if (kF32) {
                 x[i][w] = __float_as_uint(v[4 * i + w]);
             } else {
-                const __half2 h = __floats2half2_rn(v[8 * i + 2 * w], v[8 * i + 2 * w + 1]);
-                x[i][w] = *reinterpret_cast<const uint32_t*>(&h);
+                x[i][w] = pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w + 1]);
             }
         }
     transpose_pieces<P>(x, lane);
@@ -112,12 +190,29 @@ __device__ __forceinline__ void store_rows64(const Params& p, int r0, int n, int
     for (int e = 0; e < P; ++e) {
         const int m = r0 + g * P + e;
         if (m < s.M) {
-            uint4* dst = EPI == kEpiF32
+            uint4* dst = kF32
                              ? reinterpret_cast<uint4*>(static_cast<float*>(p.C) + (size_t)m * s.N + n) + q
                              : reinterpret_cast<uint4*>(static_cast<__half*>(p.C) + (size_t)m * s.N + n) + q;
             *dst = make_uint4(x[e][0], x[e][1], x[e][2], x[e][3]);
         }
     }
+}
+
+template <int EPI>
+__device__ __forceinline__ void store_rows64(const Params& p, int r0, int n, int lane, const float (&v)[64])
+{
+    static_assert(EPI == kEpiF16 || EPI == kEpiF32, "fp16 or fp32 C");
+    store_lines64<EPI>(p, r0, n, lane, v);
+}
+
+// The 64 columns' integer sums (kEpiI8, kEpiI8F32), scaled, the same way.
+template <int EPI>
+__device__ __forceinline__ void store_rows64_i8(const Params& p, int r0, int n, int lane, const float (&sum)[64])
+{
+    if (n >= p.s.N) return;  // N % 64 == 0: the 64 columns are all in C or all outside
+    float v[64];
+    i8_row_values(p, r0 + lane, n, sum, v);
+    store_lines64<EPI>(p, r0, n, lane, v);
 }
 
 // The same 64 columns of C from one warp's 32 rows by a TMA store (TILE and PAIR, fp16, BW_EPI_TMA): the warp writes
@@ -148,6 +243,69 @@ __device__ __forceinline__ void store_rows64_tma(const CUtensorMap* tmc, uint8_t
     if (lane == 0) {
         tma_store_2d(tmc, quarter, n, r0);
         bulk_commit();
+    }
+}
+
+// A whole tile of kEpiI8SwiGLU: silu(gate) * up from the scaled sums, in C's 16-bit type.  Columns of C come in groups
+// of 256 weight rows of B, 128 gate then 128 up.
+//   PAIR: accumulator columns [0, BN / 2) are gate, [BN / 2, BN) up, of row m0 + row: columns n0 / 2 + c of the M x N/2 C.
+//   SWAP (two weight blocks): lane `row` holds output column n0 / 2 + row; accumulator columns [0, BN) are its gate sums
+//   by token, [BN, 2 BN) its up sums.
+// The logistic takes the fast exponential: its relative error is within (2 + 1.16 |g|) 2^-23 by CUDA's bound, 1.3e-5
+// at the |g| = 88 where exp leaves fp32, against the 2^-8 (bf16) or 2^-11 (fp16) of the one rounding that follows.
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+
+template <int BN, bool SWAP>
+__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row)
+{
+    const Sched& s = p.s;
+    if constexpr (!SWAP) {
+        const int m = m0 + row;
+        const float rs = m < s.M ? __ldg(p.row_scale + m) : 0.f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < BN / 2; c0 += 16) {
+            uint32_t gr[16], ur[16];
+            tmem_ld16(tbase + (uint32_t)c0, gr);
+            tmem_ld16(tbase + (uint32_t)(BN / 2 + c0), ur);
+            tmem_wait_ld();
+            if (m >= s.M || n0 >= s.N) continue;
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float a[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = c0 + 2 * j + e;
+                    a[e] = silu_mul(i8_value(__uint_as_float(gr[2 * j + e]), rs, __ldg(p.col_scale + n0 + c)),
+                                    i8_value(__uint_as_float(ur[2 * j + e]), rs, __ldg(p.col_scale + n0 + BN / 2 + c)));
+                }
+                h[j] = pack2<kEpiI8SwiGLU>(p, a[0], a[1]);
+            }
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.C) + (size_t)m * (s.N / 2) + n0 / 2 + c0);
+            dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+    } else {
+        const bool in = n0 < s.N;  // N % 256 == 0: a tile is in C or outside
+        const float gs = in ? __ldg(p.col_scale + n0 + row) : 0.f, us = in ? __ldg(p.col_scale + n0 + 128 + row) : 0.f;
+        __half* C = static_cast<__half*>(p.C);
+#pragma unroll 1
+        for (int c0 = 0; c0 < BN; c0 += 16) {
+            uint32_t gr[16], ur[16];
+            tmem_ld16(tbase + (uint32_t)c0, gr);
+            tmem_ld16(tbase + (uint32_t)(BN + c0), ur);
+            tmem_wait_ld();
+            // a warp's 32 lanes write 64 contiguous bytes of one token's row
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int m = c0 + j;
+                if (m < s.M && in) {
+                    const float rs = __ldg(p.row_scale + m);
+                    C[(size_t)m * (s.N / 2) + n0 / 2 + row] = half_bits<kEpiI8SwiGLU>(
+                        p, silu_mul(i8_value(__uint_as_float(gr[j]), rs, gs), i8_value(__uint_as_float(ur[j]), rs, us)));
+                }
+            }
+        }
     }
 }
 
@@ -214,7 +372,7 @@ __device__ __noinline__ void reduce_tile(const Params& p, int P, int tile, int r
                         for (int e = 0; e < 16; ++e) v[e] = own[e];
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] += own[e];
+                        for (int e = 0; e < 16; ++e) v[e] = part_add<EPI>(v[e], own[e]);
                     }
                     own_added = true;
                 }
@@ -232,12 +390,12 @@ __device__ __noinline__ void reduce_tile(const Params& p, int P, int tile, int r
                     for (int e = 0; e < 16; ++e) v[e] = x[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] += x[e];
+                    for (int e = 0; e < 16; ++e) v[e] = part_add<EPI>(v[e], x[e]);
                 }
                 if (j == L - 1) {  // the chunk is complete
                     if (own_mine && !own_added) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] += own[e];
+                        for (int e = 0; e < 16; ++e) v[e] = part_add<EPI>(v[e], own[e]);
                     }
                     store_chunk<SWAP, EPI, BT>(p, m0, n0, row, chunk * 16, v, cst);
                 }
@@ -309,16 +467,16 @@ __device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, 
                 } else {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        acc[q].x += w[q].x;
-                        acc[q].y += w[q].y;
-                        acc[q].z += w[q].z;
-                        acc[q].w += w[q].w;
+                        acc[q].x = part_add<EPI>(acc[q].x, w[q].x);
+                        acc[q].y = part_add<EPI>(acc[q].y, w[q].y);
+                        acc[q].z = part_add<EPI>(acc[q].z, w[q].z);
+                        acc[q].w = part_add<EPI>(acc[q].w, w[q].w);
                     }
                 }
             }
         }
     };
-    if constexpr (!SWAP && BN % 64 == 0 && BW_EPI_LINES && (EPI == kEpiF16 || EPI == kEpiF32)) {
+    if constexpr (!SWAP && BN % 64 == 0 && BW_EPI_LINES && (EPI == kEpiF16 || EPI == kEpiF32 || epi_i8(EPI))) {
         // 64 columns at a time, stored as whole lines of C (store_rows64)
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 64) {
@@ -335,7 +493,10 @@ __device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, 
                     v[16 * h + 4 * q + 3] = acc[q].w;
                 }
             }
-            store_rows64<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v);
+            if constexpr (epi_i8(EPI))
+                store_rows64_i8<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v);
+            else
+                store_rows64<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v);
         }
     } else {
 #pragma unroll 1

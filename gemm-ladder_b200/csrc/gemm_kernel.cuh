@@ -32,6 +32,10 @@
 // accumulator's 16-column chunks.
 // Outputs (EPI): fp16 C; fp32 C; the SwiGLU activation of a gate / up tile; or the fused reduce-scatter of a
 // row-parallel layer (kEpiRS: partial tiles of other ranks' rows pushed into their memory, this rank's rows summed).
+// 8-bit integers (kEpiI8*): A (M x K) and B (N x K) as int8 rows of K bytes.  A 128-byte swizzle row holds 128 of them
+// where it holds 64 fp16, and an MMA's 32-byte slice 32 where it holds 16, so to everything but the MMA and the
+// epilogue an int8 row of K is an fp16 row of K / 2: the maps, stages, descriptors, schedules and partials are the fp16
+// ones (the maps' zero fill past K adds zeros), the MMA is kind::i8 and the sums are 32-bit integers (epilogue.cuh).
 // Every wait on a barrier is bounded (ptx.cuh, wait_bounded): a stalled pipeline ends the kernel with an error status
 // instead of hanging the GPU.
 #pragma once
@@ -47,7 +51,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     constexpr int AN = G::kAccN;  // accumulator columns (TMEM)
-    static_assert(!SWAP || EPI == kEpiF16, "fp32 and SwiGLU outputs are written by the TILE and PAIR forms");
+    static_assert(!SWAP || EPI == kEpiF16 || EPI == kEpiI8 || EPI == kEpiI8SwiGLU,
+                  "fp32 and fp16 SwiGLU outputs are written by the TILE and PAIR forms");
+    static_assert(!SWAP || EPI != kEpiI8SwiGLU || WM == 2, "swap-AB SwiGLU: the tile's two weight blocks are gate and up");
     static_assert(EPI != kEpiSwiGLU || BN % 32 == 0, "SwiGLU pairs the two halves of a tile");
     static_assert(EPI != kEpiRS || (PAIR && BN == 256 && WM == 1), "the fused reduce-scatter runs on pair tiles");
     constexpr int S = G::kStages;
@@ -254,7 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && leader) {
             // B (the MMA's A operand in swap-AB) is MN-major when K x N, K-major when N x K (p.tn)
             constexpr uint32_t idesc_nn = idesc_f16_f32(PAIR ? 256 : 128, G::kMmaN, SWAP, !SWAP);
-            constexpr uint32_t idesc_tn = idesc_f16_f32(PAIR ? 256 : 128, G::kMmaN, false, false);
+            constexpr uint32_t idesc_tn = epi_i8(EPI) ? idesc_i8_s32(PAIR ? 256 : 128, G::kMmaN)
+                                                      : idesc_f16_f32(PAIR ? 256 : 128, G::kMmaN, false, false);
             const uint32_t idesc = p.tn ? idesc_tn : idesc_nn;
             const bool bk = p.tn != 0;
             SegIter it(s, c, P);
@@ -310,7 +317,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint64_t ad = (SWAP && !bk) ? desc_mnmajor(xw, k) : desc_kmajor(xw, k);
                             const uint64_t bd = (SWAP || bk) ? desc_kmajor(yw, k) : desc_mnmajor(yw, k);
                             const uint32_t dw = d + (uint32_t)(w * (SWAP ? BN : G::kMmaN));
-                            if (PAIR)
+                            if constexpr (epi_i8(EPI) && PAIR)
+                                mma_i8_pair(dw, ad, bd, idesc, accumulate);
+                            else if constexpr (epi_i8(EPI))
+                                mma_i8(dw, ad, bd, idesc, accumulate);
+                            else if (PAIR)
                                 mma_f16_pair(dw, ad, bd, idesc, accumulate);
                             else
                                 mma_f16(dw, ad, bd, idesc, accumulate);
@@ -492,6 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 rs_tile(p, rs_epoch, tm, tn, rank, tbase, row, lane, q, abort_flag, recv_flag, reduce_flag, rs_acked,
                         smem + G::kWindowOffset, rbar, krecv, win_ph, win_next, seg);
                 release_all(acc);
+            } else if constexpr (EPI == kEpiI8SwiGLU) {
+                i8_swiglu_tile<BN, SWAP>(p, tbase, m0, n0, row);
+                release_all(acc);
             } else if (EPI == kEpiSwiGLU) {
                 // a whole tile (the plan splits none): gate columns [0, BN/2), up columns [BN/2, BN) of the tile,
                 // silu(gate) * up to columns [n0 / 2, n0 / 2 + BN / 2) of the M x N/2 output
@@ -606,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 }
                             }
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = sb == 0 ? x[e] : v[e] + x[e];
+                            for (int e = 0; e < 16; ++e) v[e] = sb == 0 ? x[e] : part_add<EPI>(v[e], x[e]);
                         }
                         store_chunk<SWAP, EPI, BN>(p, m0, n0, row, ch * 16, v, cst);
                     }
@@ -640,10 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const float4 w = peer[(c0 / 4 + j) * 128];
-                                v[4 * j] = __uint_as_float(r[4 * j]) + w.x;
-                                v[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + w.y;
-                                v[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + w.z;
-                                v[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + w.w;
+                                v[4 * j] = part_add<EPI>(__uint_as_float(r[4 * j]), w.x);
+                                v[4 * j + 1] = part_add<EPI>(__uint_as_float(r[4 * j + 1]), w.y);
+                                v[4 * j + 2] = part_add<EPI>(__uint_as_float(r[4 * j + 2]), w.z);
+                                v[4 * j + 3] = part_add<EPI>(__uint_as_float(r[4 * j + 3]), w.w);
                             }
                             store_chunk<SWAP, EPI, BN>(p, m0, n0, row, c0, v, cst);
                         }
@@ -693,7 +707,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float v[64];
 #pragma unroll
                         for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j / 16][j % 16]);
-                        store_rows64<EPI == kEpiF32 ? kEpiF32 : kEpiF16>(p, m0 + q * 32, n0 + c0, lane, v);
+                        if constexpr (epi_i8(EPI))
+                            store_rows64_i8<EPI>(p, m0 + q * 32, n0 + c0, lane, v);
+                        else
+                            store_rows64<EPI == kEpiF32 ? kEpiF32 : kEpiF16>(p, m0 + q * 32, n0 + c0, lane, v);
                     } else {
 #pragma unroll
                         for (int h = 0; h < kLdw / 16; ++h) {

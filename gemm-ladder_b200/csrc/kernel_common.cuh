@@ -3,6 +3,7 @@
 // the shared-memory matrix descriptors of the stage tiles.  gemm_kernel.cuh describes the kernel as a whole.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "plan.h"
 #include "ptx.cuh"
@@ -22,7 +23,12 @@ enum : int {
                      // M x N/2 (a gated MLP's activation, from the accumulators: the gateup result never exists)
     kEpiRS = 3,      // the fused reduce-scatter: C (fp16, this rank's M / world rows) = the sum over the ranks of
                      // their A_r B_r, the partials exchanged tile by tile through the ranks' memory (RsTable)
+    // A (M x K) and B (N x K) in 8-bit signed integers, 32-bit integer sums s, a scale per row of A and per row of B:
+    kEpiI8 = 4,        // C = row_scale[m] col_scale[n] s in fp16 or bf16 (Params.out_bf16)
+    kEpiI8F32 = 5,     // the same in fp32
+    kEpiI8SwiGLU = 6,  // the activation of kEpiSwiGLU from the scaled sums, fp16 or bf16
 };
+__host__ __device__ constexpr bool epi_i8(int epi) { return epi == kEpiI8 || epi == kEpiI8F32 || epi == kEpiI8SwiGLU; }
 
 constexpr int kRsMaxWorld = 8;
 
@@ -59,6 +65,9 @@ struct Params {
                                       // than wait_ns: the ranks' processes reach their first call out of step
     int tn;                      // 1: B is N x K row-major (K-major for the tensor core, like A); 0: K x N
     const RsTable* rs;           // kEpiRS only: the ranks' regions
+    const float* row_scale;      // kEpiI8*: M scales of A's rows
+    const float* col_scale;      // kEpiI8*: N scales of B's rows (C's columns)
+    int out_bf16;                // kEpiI8, kEpiI8SwiGLU: C in bf16 (0: fp16)
 };
 
 __host__ __device__ constexpr int pow2_at_least(int v, int p) { return p >= v ? p : pow2_at_least(v, 2 * p); }

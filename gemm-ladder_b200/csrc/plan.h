@@ -311,6 +311,8 @@ enum : unsigned {
     kPlanNoSwap = 1u,   // A is the MMA's A operand (fp32 and fused outputs are written by TILE and PAIR only)
     kPlanNoSplit = 2u,  // whole tiles only (a fused epilogue needs the complete sums)
     kPlanNarrow = 4u,   // swap-AB tiles of 128 weight columns, pair tiles of 256 (half the partials' scratch)
+    kPlanGateUp = 16u,  // swap-AB tiles of 256 weight columns, 128 gate and 128 up, at every M (a fused activation)
+    kPlanNoStage = 32u, // no staging for TMA stores of C (BW_EPI_TMA): the 8-bit entries store from registers
     kPlanRsWindow = 8u, // shared memory for the fused reduce-scatter's window (kPlanRsWindowBytes), fewer stages
 };
 
@@ -412,6 +414,11 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
         q.tiles_n = tiles256;
         q.tiles = q.tiles_n;
     }
+    if (swap && (flags & kPlanGateUp)) {
+        q.wm = 2;
+        q.tiles_n = tiles256;
+        q.tiles = q.tiles_n;
+    }
     // BW_SWAP_PAIR: the stream-K swap-AB tiles on SM pairs instead, from 33 tokens, the MMA's N rounded up to 64 or
     // 128 (half per block; the pair MMA's N kept to those two); tiles of 2 x 128 weight columns, or 2 x 256 while those
     // still outnumber the pairs
@@ -475,7 +482,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     }
     q.grid = P * ranks;
     // shared memory after the ring: the fused reduce-scatter's window, or the fp16 TILE / PAIR epilogue's staging
-    const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow));
+    const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow | kPlanNoStage));
     const int reserve = (flags & kPlanRsWindow) ? kPlanRsWindowBytes : epi_tma ? kPlanEpiStageBytes : 0;
     q.stages = plan_stages(q.bn, ranks, swap, q.wm, reserve);
     q.smem_bytes = plan_smem_bytes(q.bn, ranks, swap, q.wm, reserve);

@@ -583,6 +583,62 @@ inline void mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool
     }
 }
 
+// The same in 8-bit signed integers (kind::i8): K32 slices, both operands K-major, 32-bit integer accumulators.
+inline void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate, bool pair)
+{
+    for (uint64_t desc : {adesc, bdesc})
+        if ((desc >> 61) != 2u || ((desc >> 46) & 3u) != 1u) finding("a descriptor that is not sm_100 128-byte swizzle");
+    const int N = (int)((idesc >> 17) & 0x3Fu) << 3, M = (int)((idesc >> 24) & 0x1Fu) << 4;
+    if (((idesc >> 4) & 3u) != 2u || ((idesc >> 7) & 7u) != 1u || ((idesc >> 10) & 7u) != 1u || ((idesc >> 15) & 3u))
+        finding("an integer MMA that is not signed 8-bit, K-major, with 32-bit accumulators");
+    const int ranks = pair ? 2 : 1;
+    if (M != 128 * ranks || N < 16 * ranks || N > 256 || N % (16 * ranks)) {
+        finding("an integer MMA of M %d N %d (cta_group::%d)", M, N, ranks);
+        return;
+    }
+    Cta* cta[2] = {t_cta, t_cta};
+    if (pair) {
+        if (!t_cta->cluster || t_cta->cluster->size != 2) {
+            finding("a cta_group::2 MMA outside a cluster of two");
+            return;
+        }
+        cta[0] = t_cta->cluster->cta[0];
+        cta[1] = t_cta->cluster->cta[1];
+    }
+    const uint32_t lane0 = d >> 16, col0 = d & 0xFFFFu;
+    if (lane0 != 0 || col0 + (uint32_t)N > (uint32_t)kTmemCols) {
+        finding("an MMA accumulator at lane %u column %u (N %d) outside tensor memory", lane0, col0, N);
+        return;
+    }
+    auto load = [](const Cta* c, uint64_t desc, int row, int k) -> int {
+        const uint32_t start = (uint32_t)(desc & 0x3FFFu) << 4, sbo = (uint32_t)((desc >> 32) & 0x3FFFu) << 4;
+        const uint32_t p = swizzle128(start + (uint32_t)(row >> 3) * sbo + (uint32_t)(row & 7) * 128u + (uint32_t)k);
+        if (p >= (uint32_t)kSmemBytes) {
+            finding("an MMA operand read past the end of shared memory");
+            return 0;
+        }
+        return static_cast<int8_t>(c->smem[p]);
+    };
+    std::vector<int> b((size_t)N * 32), a(128 * 32);
+    for (int n = 0; n < N; ++n) {
+        const int r = n / (N / ranks), local = n % (N / ranks);
+        for (int k = 0; k < 32; ++k) b[(size_t)n * 32 + k] = load(cta[r], bdesc, local, k);
+    }
+    for (int r = 0; r < ranks; ++r) {
+        for (int m = 0; m < 128; ++m)
+            for (int k = 0; k < 32; ++k) a[(size_t)m * 32 + k] = load(cta[r], adesc, m, k);
+        if (cta[r]->tmem_cols < (int)(col0 + N)) finding("an MMA into tensor memory not allocated");
+        for (int m = 0; m < 128; ++m) {
+            uint32_t* row = cta[r]->tmem.data() + (size_t)m * kTmemCols + col0;
+            for (int n = 0; n < N; ++n) {
+                int s = 0;
+                for (int k = 0; k < 32; ++k) s += a[(size_t)m * 32 + k] * b[(size_t)n * 32 + k];
+                row[n] = accumulate ? row[n] + (uint32_t)s : (uint32_t)s;
+            }
+        }
+    }
+}
+
 // tcgen05.ld 32x32b.x16: lane = the address's lane + the thread's lane in its warp, 16 columns
 inline void tmem_ld(uint32_t taddr, uint32_t (&r)[16])
 {
@@ -630,6 +686,19 @@ inline float __uint_as_float(uint32_t u)
     std::memcpy(&f, &u, 4);
     return f;
 }
+inline int __float_as_int(float f)
+{
+    int u;
+    std::memcpy(&u, &f, 4);
+    return u;
+}
+inline float __int_as_float(int u)
+{
+    float f;
+    std::memcpy(&f, &u, 4);
+    return f;
+}
+inline float __ldg(const float* p) { return *p; }
 inline uint32_t __float_as_uint(float f)
 {
     uint32_t u;

@@ -199,7 +199,7 @@ MUTATIONS = [
      "mbar_arrive_cluster(mapa_shared(smem_u32(kgo), 0));", 0, "halves"),
     ("khalf_recv_wait_gone", GK, "const bool ok = wait_bounded(krecv, 0, abort_flag, p.wait_ns, site(2, 5, 0), seg);\n                        if (!ok) wait_drain(krecv, 0, p.wait_ns);  // st.async",
      "const bool ok = true;\n                        if (!ok) wait_drain(krecv, 0, p.wait_ns);  // st.async", 0, "halves"),
-    ("khalf_other_half_dropped", GK, "v[4 * j] = __uint_as_float(r[4 * j]) + w.x;", "v[4 * j] = __uint_as_float(r[4 * j]);",
+    ("khalf_other_half_dropped", GK, "v[4 * j] = part_add<EPI>(__uint_as_float(r[4 * j]), w.x);", "v[4 * j] = __uint_as_float(r[4 * j]);",
      0, "halves"),
     ("khalf_send_stride", GK, "st_async_v4(dst + (uint32_t)((c0 / 4 + j) * 128 * 16), r[4 * j], r[4 * j + 1],",
      "st_async_v4(dst + (uint32_t)((c0 / 4 + j) * 128 * 8), r[4 * j], r[4 * j + 1],", 0, "halves"),
@@ -228,8 +228,8 @@ MUTATIONS = [
     ("geom_b_part", KC, "static constexpr int kBPart = BN / kRanks / kWN;", "static constexpr int kBPart = BN / kWN;", 0,
      "library"),
     # ---------------------------------------------------------------- stores of C, reductions (epilogue.cuh)
-    ("store_f32_row_bound", EP, "if (m >= s.M || n >= s.N) return;", "if (m > s.M || n >= s.N) return;", 0, "library"),
-    ("store_f16_row_bound", EP, "if (m >= s.M || n >= s.N) return;", "if (m > s.M || n >= s.N) return;", 1, "library"),
+    ("store_f32_row_bound", EP, "if (m >= s.M || n >= s.N) return;", "if (m > s.M || n >= s.N) return;", 1, "library"),
+    ("store_f16_row_bound", EP, "if (m >= s.M || n >= s.N) return;", "if (m > s.M || n >= s.N) return;", 2, "library"),
     ("store_f16_pair_order", EP, "const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);",
      "const __half2 x = __floats2half2_rn(v[2 * j + 1], v[2 * j]);", 0, "library"),
     ("store_swap_lane", EP, "buf[j * 128 + lane] = __float2half_rn(v[j]);", "buf[j * 128 + (lane ^ 1)] = __float2half_rn(v[j]);",
@@ -239,25 +239,25 @@ MUTATIONS = [
     ("store_swap_row_bound", EP, "if (m < s.M && n < s.N)\n", "if (m <= s.M && n < s.N)\n", 0, "library"),
     ("store_swap_tokens_wm", EP, "const int wb = BT ? c0 / BT : 0, tok = c0 - wb * BT;", "const int wb = BT ? c0 / BT : 0, tok = c0;",
      0, "library"),
-    ("store_swap_no_barrier", EP, "buf[j * 128 + lane] = __float2half_rn(v[j]);\n        named_bar_sync(1, 128);",
-     "buf[j * 128 + lane] = __float2half_rn(v[j]);", 0, "library"),
+    ("store_swap_no_barrier", EP, "buf[j * 128 + lane] = __float2half_rn(v[j]);\n        }\n        named_bar_sync(1, 128);",
+     "buf[j * 128 + lane] = __float2half_rn(v[j]);\n        }", 0, "library"),
     ("transpose_direction", EP, "const bool hi = (q & m) != 0;", "const bool hi = (q & m) == 0;", 0, "library"),
     ("transpose_partner", EP, "const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, m);",
      "const uint32_t recv = __shfl_xor_sync(0xffffffffu, send, m == 1 ? 2 : m);", 0, "library"),
     ("lines_group_rows", EP, "const int q = lane & (P - 1), g = lane / P;", "const int q = lane & (P - 1), g = (lane / P) ^ 1;",
      0, "library"),
     ("lines_row_bound", EP, "if (m < s.M) {", "if (m <= s.M) {", 0, "library"),
-    ("lines_f16_pair_order", EP, "__floats2half2_rn(v[8 * i + 2 * w], v[8 * i + 2 * w + 1])",
-     "__floats2half2_rn(v[8 * i + 2 * w], v[8 * i + 2 * w])", 0, "library"),
+    ("lines_f16_pair_order", EP, "pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w + 1])",
+     "pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w])", 0, "library"),
     ("reduce_column_group", EP, "w[q] = __ldcg(slot_vec<BN>(p, slot, row, chunk * 4 + q));",
      "w[q] = __ldcg(slot_vec<BN>(p, slot, row, chunk * 4 + (q ^ 1)));", 0, "library"),
     ("reduce_reads_own_slot", EP, "const int L = f.nseg - (own_mine ? 1 : 0);  // partials read from memory",
      "const int L = f.nseg;", 0, "library"),
     ("reduce_skips_own_index", EP, "auto index_of = [&](int j) { return (own_mine && j >= f.mine) ? j + 1 : j; };",
      "auto index_of = [&](int j) { return j; };", 0, "library"),
-    ("reduce_overwrites", EP, "for (int e = 0; e < 16; ++e) v[e] += x[e];", "for (int e = 0; e < 16; ++e) v[e] = x[e];", 0,
+    ("reduce_overwrites", EP, "for (int e = 0; e < 16; ++e) v[e] = part_add<EPI>(v[e], x[e]);", "for (int e = 0; e < 16; ++e) v[e] = x[e];", 0,
      "library"),
-    ("reduce_own_dropped", EP, "for (int e = 0; e < 16; ++e) v[e] += own[e];", "for (int e = 0; e < 16; ++e) v[e] += 0.f;", 1,
+    ("reduce_own_dropped", EP, "for (int e = 0; e < 16; ++e) v[e] = part_add<EPI>(v[e], own[e]);", "for (int e = 0; e < 16; ++e) v[e] += 0.f;", 1,
      "library"),
     ("bulk_expect_short", EP, "mbar_arrive_expect_tx(rbar, (uint32_t)(L * kSlotBytes));",
      "mbar_arrive_expect_tx(rbar, (uint32_t)(L * kSlotBytes / 2));", 0, "library"),
@@ -265,7 +265,7 @@ MUTATIONS = [
      "const int n = kSlotBytes - off < 32768 ? kSlotBytes - off : 16384;", 0, "library"),
     ("bulk_ring_place", EP, "const int j = (own_mine && i > f.mine) ? i - 1 : i;  // its place in the ring",
      "const int j = i;", 0, "library"),
-    ("bulk_sum_sign", EP, "acc[q].x += w[q].x;", "acc[q].x -= w[q].x;", 0, "library"),
+    ("bulk_sum_sign", EP, "acc[q].x = part_add<EPI>(acc[q].x, w[q].x);", "acc[q].x -= w[q].x;", 0, "library"),
     ("bulk_wait_gone", EP, "if (!wait_bounded(rbar, 0, abort_flag, p.wait_ns, site(2, 4, 0), seg)) return false;",
      "(void)seg;", 0, "library"),
     ("bulk_wait_parity", EP, "if (!wait_bounded(rbar, 0, abort_flag, p.wait_ns, site(2, 4, 0), seg)) return false;",

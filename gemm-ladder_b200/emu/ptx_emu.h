@@ -230,6 +230,24 @@ inline void mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32
         --tc.mmas;
     });
 }
+inline void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    emu::Engine& tc = emu::t_cta->tc;
+    ++tc.mmas;
+    tc.post([=, &tc] {
+        emu::mma_i8(d_tmem, adesc, bdesc, idesc, accumulate != 0, false);
+        --tc.mmas;
+    });
+}
+inline void mma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    emu::Engine& tc = emu::t_cta->tc;
+    ++tc.mmas;
+    tc.post([=, &tc] {
+        emu::mma_i8(d_tmem, adesc, bdesc, idesc, accumulate != 0, true);
+        --tc.mmas;
+    });
+}
 inline void mma_commit_pair(uint32_t bar)
 {
     emu::t_cta->tc.post([=] { emu::mb_arrive(emu::cta_of(bar), emu::off_of(bar), 0); });
@@ -253,6 +271,11 @@ constexpr uint32_t idesc_f16_f32(int m, int n, bool a_mn_major, bool b_mn_major)
 {
     return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
+}
+
+constexpr uint32_t idesc_i8_s32(int m, int n)
+{
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // ------------------------------------------------------------------ global memory ordering, named barriers

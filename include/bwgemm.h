@@ -77,6 +77,47 @@ int bw_gemm_f16_f32out(const void* A, const void* B, void* C, int M, int N, int 
  */
 int bw_gemm_f16_swiglu(const void* A, const void* B, void* C, int M, int N, int K, void* stream);
 
+/*
+ * 8-bit integer products with a scale per token and per channel.  A (M x K) and B (N x K, a linear layer's weight
+ * layout) are row-major int8; a_scale[m] and b_scale[n] (fp32) are the scales of their rows; the sums are exact 32-bit
+ * integers:
+ *   C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k]      rounded once to C's type (out_type, BW_TYPE_*).
+ * N % 64 == 0, K % 16 == 0, 16 <= K <= 131056 (where the sum of K products of magnitude 2^14 stays below 2^31), any M;
+ * A, B, C and b_scale 16-byte aligned, a_scale 4-byte aligned.  The same rule and plans as the fp16 entries, an int8 row
+ * of K taking the place of an fp16 row of K / 2 (out_type BW_TYPE_F32: SM-pair tiles at every M).
+ *
+ * bw_gemm_i8_swiglu is the gated MLP's activation in one product, as bw_gemm_f16_swiglu is for fp16: B's rows in groups
+ * of 256, 128 gate then the 128 matching up rows (N % 256 == 0), C (M x N/2) = silu(gate) * up from the scaled sums,
+ * fp16 or bf16.
+ *
+ * bw_quant_rows_i8 makes such rows of fp16 or bf16 (x_type) ones, ld elements from row to row (ld >= cols, ld % 8 == 0,
+ * cols % 16 == 0, X and Q 16-byte aligned; Q is rows x cols, contiguous):
+ *   scale[m] = max_k |X[m][k]| / 127,  Q[m][k] = round-half-even(127 X[m][k] / max_k |X[m][k]|)
+ * exactly as written, whatever the values.  A row of zeros gets scale 0; one that holds an infinity or a NaN gets scale
+ * NaN (so every product with it is NaN).
+ *
+ * bw_linear_i8 is both in one call: C = X B^T with X (fp16 or bf16, M x K, ld as above) quantised by row on the way
+ * (swiglu 1: the activation as above), C in X's type.
+ *
+ * These entries keep nothing between calls: `work` is the caller's (256-byte aligned, at least the bytes that
+ * bw_gemm_i8_work_bytes gives for the call; it may be null where that is 0), is written by the call, and must not be
+ * shared by calls that may overlap on the GPU.  With a buffer each, calls may overlap on several streams and be made
+ * from several host threads.  Asynchronous, capturable in a CUDA graph (the graph then uses that buffer).
+ * bw_gemm_i8_work_bytes: linear 1 for bw_linear_i8, 0 for the others; swiglu and out_type as in the call.
+ * M == 0 is a call that does nothing.  No reference counterpart: the reference multiplies fp16 only.
+ */
+#define BW_TYPE_F16 0
+#define BW_TYPE_BF16 1
+#define BW_TYPE_F32 2
+int bw_quant_rows_i8(const void* X, int x_type, long long ld, void* Q, void* scale, int rows, int cols, void* stream);
+int bw_gemm_i8_work_bytes(int M, int N, int K, int out_type, int swiglu, int linear, size_t* bytes);
+int bw_gemm_i8(const void* A, const void* a_scale, const void* B, const void* b_scale, void* C, int M, int N, int K,
+               int out_type, void* work, size_t work_bytes, void* stream);
+int bw_gemm_i8_swiglu(const void* A, const void* a_scale, const void* B, const void* b_scale, void* C, int M, int N,
+                      int K, int out_type, void* work, size_t work_bytes, void* stream);
+int bw_linear_i8(const void* X, int x_type, long long ld, const void* B, const void* b_scale, void* C, int M, int N,
+                 int K, int swiglu, void* work, size_t work_bytes, void* stream);
+
 /* The number of variants.  Replaces: the weak `int g_nvar` (probe/probe.cu:40, hopper/verif.cu:38,
  * hopper/step7.cu:16). */
 int bw_gemm_variant_count(void);
