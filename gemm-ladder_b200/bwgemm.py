@@ -121,6 +121,10 @@ def lib():
         L.bw_gemm_i8_swiglu.restype = i
         L.bw_linear_i8.argtypes = [vp, i, ll, vp, vp, vp, i, i, i, i, vp, sz, vp]
         L.bw_linear_i8.restype = i
+        L.bw_moe_work_bytes.argtypes = [i, i, i, i, i, ctypes.POINTER(sz)]
+        L.bw_moe_work_bytes.restype = i
+        L.bw_moe_mlp.argtypes = [vp, ll, vp, vp, vp, vp, i, i, i, i, i, i, i, vp, vp, vp, sz, vp]
+        L.bw_moe_mlp.restype = i
         L.bw_status_string.argtypes = [i]
         L.bw_status_string.restype = ctypes.c_char_p
         L.bw_last_error_string.argtypes = []
@@ -311,13 +315,13 @@ def _i8_weight(B, b_scale, device):
         raise ValueError("b_scale must be a contiguous fp32 tensor of B's N scales on A's device")
 
 
-def _i8_out(C, shape, dtype, device):
+def _i8_out(C, shape, dtype, device, what="C"):
     import torch
 
     if C is None:
         return torch.empty(shape, dtype=dtype, device=device)
     if tuple(C.shape) != tuple(shape) or C.dtype != dtype or C.device != device or not C.is_contiguous():
-        raise ValueError(f"C must be a contiguous {dtype} tensor of {shape[0]} x {shape[1]} on A's device")
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {shape[0]} x {shape[1]} on the inputs' device")
     return C
 
 
@@ -408,6 +412,47 @@ def linear_i8(X, B, b_scale, C=None, swiglu=False, stream=None):
         check(lib().bw_linear_i8(X.data_ptr(), t, ld, B.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, swiglu,
                                  work.data_ptr() if n else None, n, s))
     return C
+
+
+# ---------------------------------------------------------------------------------- mixture of experts
+MOE_MAX_TOKENS = 128
+_moe_work_bytes = {}  # (device, T, E, top_k, D, F) -> bytes
+
+
+def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=None, stream=None):
+    """Y (T x D): the mixture-of-experts MLP of up to 128 tokens, fp16 or bf16 throughout.  X (T x D, rows may be
+    strided), R (E x D) the router, W1 (E x 2F x D) the experts' gate rows then up rows, W2 (E x D x F); each token takes
+    its top_k experts by logit (equal ones: the lower index) with softmax weights over them (renormalize) or over all
+    experts.  ids (T x top_k int32) and weights (T x top_k fp32), where given, receive the routing."""
+    import torch
+
+    T, D, ld = _rows16(X, "X")
+    for t, what, dim in ((R, "R", 2), (W1, "W1", 3), (W2, "W2", 3)):
+        if t.dtype != X.dtype or t.device != X.device or t.dim() != dim or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {dim}-D tensor of X's type on X's device")
+    E, F = R.shape[0], W2.shape[2]
+    if R.shape[1] != D or tuple(W1.shape) != (E, 2 * F, D) or tuple(W2.shape) != (E, D, F):
+        raise ValueError(f"X {tuple(X.shape)}, R {tuple(R.shape)}, W1 {tuple(W1.shape)} and W2 {tuple(W2.shape)} do not "
+                         "make a layer (T x D, E x D, E x 2F x D, E x D x F)")
+    for t, what, dtype in ((ids, "ids", torch.int32), (weights, "weights", torch.float32)):
+        if t is not None and (tuple(t.shape) != (T, top_k) or t.dtype != dtype or t.device != X.device or
+                              not t.is_contiguous()):
+            raise ValueError(f"{what} must be a contiguous {dtype} T x top_k tensor on X's device")
+    with _On(X.device, stream) as s:
+        Y = _i8_out(Y, (T, D), X.dtype, X.device, "Y")
+        key = (X.device.index, T, E, top_k, D, F)
+        n = _moe_work_bytes.get(key)
+        if n is None:
+            size = ctypes.c_size_t()
+            check(lib().bw_moe_work_bytes(T, E, top_k, D, F, ctypes.byref(size)))
+            if len(_moe_work_bytes) >= 4096:
+                _moe_work_bytes.clear()
+            n = _moe_work_bytes[key] = size.value
+        work = torch.empty(n, dtype=torch.uint8, device=X.device)
+        check(lib().bw_moe_mlp(X.data_ptr(), ld, R.data_ptr(), W1.data_ptr(), W2.data_ptr(), Y.data_ptr(), T, E, top_k, D, F,
+                               _types()[X.dtype], int(bool(renormalize)), ids.data_ptr() if ids is not None else None,
+                               weights.data_ptr() if weights is not None else None, work.data_ptr() if n else None, n, s))
+    return Y
 
 
 def status():

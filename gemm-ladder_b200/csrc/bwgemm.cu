@@ -576,7 +576,7 @@ BW_API const char* bw_status_string(int status)
 {
     switch (status) {
     case BW_OK: return "ok";
-    case BW_ERR_SHAPE: return "shape not supported (M, N, K positive; N % 64 and K % 64 must be 0)";
+    case BW_ERR_SHAPE: return "shape not supported (GEMM: M, N, K positive, N % 64 and K % 64 must be 0; other entries: see bwgemm.h)";
     case BW_ERR_LAUNCH: return "CUDA error (see bw_last_error_string)";
     case BW_ERR_TIMEOUT: return "a bounded wait on a barrier gave up (see bw_gemm_status)";
     case BW_ERR_ARG: return "bad argument (null or misaligned pointer, unknown variant)";
@@ -671,6 +671,9 @@ BW_API int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw
 
 // ------------------------------------------------------------------ the 8-bit integer entries
 #include "gemm_i8.cuh"
+
+// ------------------------------------------------------------------ the mixture-of-experts layer
+#include "moe_mlp.cuh"
 
 #ifdef BW_TRACE
 // The timeline of the last launch (a -DBW_TRACE build only; not part of the C ABI of bwgemm.h).

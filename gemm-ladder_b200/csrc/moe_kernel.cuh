@@ -1,0 +1,515 @@
+// moe_kernel.cuh -- a mixture-of-experts MLP layer for few tokens (T <= 128), in two kernels:
+//
+//   router    logits l_te = x_t . r_e;  S_t = the top_k experts of token t (equal logits: the lower index);
+//             p_te = exp(l_te - max) / sum over S_t (or over all experts)
+//   experts   g = x_t W1[e][:F]^T, u = x_t W1[e][F:]^T;  h_te = p_te silu(g) u (0 where e is not in S_t);
+//             y_t = sum_e h_te W2[e]^T
+//
+// With few tokens the layer is a stream of the active experts' weights: 6 D F bytes each, read once, against 2 T
+// multiplications per weight at most.  So the experts kernel is one persistent block per SM whose TMA producer streams
+// weights without a pause from the first to the last byte:
+//   - as in the swap-AB GEMM the weights fill the MMA's 128 rows (two MMAs per stage: gate and up rows, or 256 rows of
+//     W2) and the tokens its N.  All T tokens are multiplied with every active expert (the tensor core idles anyway);
+//     a token that did not choose the expert gets p = 0, so no rows are gathered or sorted.
+//   - the router's weights are folded into h, so that the down product of all experts is one product whose K is the
+//     active experts' F one after the other: the sum over the experts happens in the accumulator.
+//   - both products are cut evenly over the blocks by K-blocks (moe_sched.h); split tiles are summed in block order
+//     (the same bits on every run).
+//   - between the products a block waits for the activations it needs, by active expert, but only its token-side loads
+//     do: the weights of W2 are already on their way into the ring (up to 200 KB per SM, 30 MB in all), so the wait
+//     costs no memory time.
+// One thread per role: warp 0 the weights' producer, warp 6 the tokens' (both arrive on a stage's full barrier), warp 1
+// the MMA issuer, warps 2-5 the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
+// resident); every wait is bounded (ptx.cuh).
+//
+// Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32), y once at the end; sums in fp32.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernel_common.cuh"
+#include "moe_sched.h"
+
+namespace bw {
+
+constexpr int kMoeThreads = 224;  // 7 warps
+constexpr int kMoeXBytes = 32768; // a stage's weights: 256 rows x 64 values
+constexpr int kMoeMaxStages = 6;
+constexpr int kMoeEpiThread0 = 64;
+
+struct MoeParams {
+    int T, Tp;          // tokens; rounded up to 16 (the MMA's N, the rows of a token box)
+    int E, top_k, D, F;
+    int bf16;           // the tokens', weights' and results' type: 1 bf16, 0 fp16
+    int stages, stage_bytes;
+    const int* ids;     // T x top_k
+    const float* weights;
+    uint16_t* H;        // [active expert][T][F]
+    uint16_t* Y;        // T x D
+    float* partials;
+    long long slot_floats;
+    int* ready;         // finished gate/up tiles per active expert
+    int* counters;      // the split tiles' (moe_counter)
+    unsigned long long wait_ns;
+};
+
+// Shared memory after the ring (offsets from its end).
+struct MoeSmem {
+    static constexpr int kBars = 0;  // weights in, tokens in, empty (6 each), tfull, tempty (2 each), drain
+    static constexpr int kMisc = kBars + (3 * kMoeMaxStages + 5) * 8 + 8;  // tmem slot, flags
+    static constexpr int kMask = kMisc + 64;                       // a bit per expert
+    static constexpr int kExpert = kMask + kMoeMaxExperts / 8;     // the active experts, 16 bits each
+    static constexpr int kGate = kExpert + 2 * kMoeMaxExperts;     // p of every token for the epilogue's expert
+    static constexpr int kBytes = kGate + 4 * kMoeMaxTokens;
+};
+__host__ __device__ constexpr int moe_stage_bytes(int tp) { return kMoeXBytes + tp * 128; }
+__host__ __device__ constexpr int moe_stages(int tp)
+{
+    const int fit = (BW_SMEM_LIMIT - 1024 - MoeSmem::kBytes) / moe_stage_bytes(tp);
+    return fit < kMoeMaxStages ? fit : kMoeMaxStages;
+}
+__host__ __device__ constexpr int moe_smem_bytes(int tp)
+{
+    return 1024 + moe_stages(tp) * moe_stage_bytes(tp) + MoeSmem::kBytes;
+}
+
+// Spins until the counter at p reaches `want`, the abort flag rises or the limit passes.  One thread calls it.
+__device__ __noinline__ bool moe_wait_count(const int* p, int want, volatile int* abort_flag, uint64_t limit_ns,
+                                            uint32_t where, int seg)
+{
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (ld_acquire_gpu(p) >= want) return true;
+        if ((i & 15u) == 0) {
+            if (*abort_flag) return false;
+            if (globaltimer_ns() - t0 > limit_ns) {
+                record_timeout(abort_flag, where, seg);
+                return false;
+            }
+        }
+    }
+}
+
+// A producer's loads in flight land before its block may leave (on the normal path they all have): the last S stages
+// it filled.
+__device__ __forceinline__ void moe_drain(uint64_t* full, int issued, int S, uint64_t limit_ns)
+{
+    const int n = issued < S ? issued : S;
+    for (int i = 1; i <= n; ++i) wait_drain(&full[(issued - i) % S], (uint32_t)(((issued - i) / S) & 1), limit_ns);
+}
+
+__device__ __forceinline__ uint16_t moe_bits16(float v, int bf16)
+{
+    if (bf16) {
+        const __nv_bfloat16 b = __float2bfloat16_rn(v);
+        return *reinterpret_cast<const uint16_t*>(&b);
+    }
+    const __half h = __float2half_rn(v);
+    return *reinterpret_cast<const uint16_t*>(&h);
+}
+
+// kind::f16 with fp16 (format 0) or bf16 (format 1) operands, both K-major, fp32 accumulators.
+__device__ __forceinline__ uint32_t moe_idesc(int n, int bf16)
+{
+    return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// tmw1: W1 as {D, F, 2 E} (gate and up halves of an expert are two planes), boxes of 64 x 128; tmw2: W2 as {F, D, E},
+// boxes of 64 x 256; tmx: X as {D, T}, tmh: H as {F, T, slots}, boxes of 64 x Tp.  Zeros outside all of them.
+__global__ void __launch_bounds__(kMoeThreads, 1)
+    moe_experts_kernel(const __grid_constant__ CUtensorMap tmw1, const __grid_constant__ CUtensorMap tmw2,
+                       const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmh,
+                       const MoeParams p)
+{
+#ifdef BW_EMULATE
+    uint8_t* smem_raw = emu::cta_smem();
+#else
+    extern __shared__ uint8_t smem_raw[];
+#endif
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* misc = smem + (size_t)p.stages * p.stage_bytes;
+    uint64_t* wfull = reinterpret_cast<uint64_t*>(misc + MoeSmem::kBars);  // a barrier per stage and producer, so that
+    uint64_t* xfull = wfull + kMoeMaxStages;                               // each can drain its own loads
+    uint64_t* empty = xfull + kMoeMaxStages;
+    uint64_t* tfull = empty + kMoeMaxStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* epi_go = abort_flag + 1;    // two slots, alternating by segment
+    volatile int* epi_last = abort_flag + 3;  // the outcome of a split tile's count or wait
+    uint32_t* mask = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMask);
+    uint16_t* expert = reinterpret_cast<uint16_t*>(misc + MoeSmem::kExpert);
+    float* gate = reinterpret_cast<float*>(misc + MoeSmem::kGate);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+    const int S = p.stages, Tp = p.Tp;
+    int tmem_cols = 32;
+    while (tmem_cols < 4 * Tp) tmem_cols *= 2;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&wfull[i], 1);  // the producer's arrive.expect_tx
+            mbar_init(&xfull[i], 1);
+            mbar_init(&empty[i], 1);  // one tcgen05.commit
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 4);  // one arrival per epilogue warp
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (threadIdx.x < kMoeMaxExperts / 32) mask[threadIdx.x] = 0u;
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tmw1);
+        prefetch_tmap(&tmw2);
+        prefetch_tmap(&tmx);
+        prefetch_tmap(&tmh);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, (uint32_t)tmem_cols);
+        tmem_relinquish();
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    // nothing above touches global memory: from here on the router has finished
+    griddep_wait();
+
+    // the experts that some token chose, in index order
+    for (int i = threadIdx.x; i < p.T * p.top_k; i += kMoeThreads) {
+        const int e = p.ids[i];
+        atomicOr(&mask[e >> 5], 1u << (e & 31));
+    }
+    __syncthreads();
+    int active = 0;
+    for (int w = 0; w < (p.E + 31) / 32; ++w) active += __popc(mask[w]);
+    for (int e = threadIdx.x; e < p.E; e += kMoeThreads) {
+        if (!(mask[e >> 5] >> (e & 31) & 1u)) continue;
+        int pos = __popc(mask[e >> 5] & ((1u << (e & 31)) - 1u));
+        for (int w = 0; w < e >> 5; ++w) pos += __popc(mask[w]);
+        expert[pos] = (uint16_t)e;
+    }
+    __syncthreads();
+    const MoeSched s = moe_sched(p.T, p.D, p.F, active, gridDim.x);
+
+    if (warp == 0) {
+        // ---------------------------------------------------------- the weights' producer
+        if (lane == 0) {
+            const uint64_t pol = policy_evict_first();  // read once
+            MoeIter it(s, c);
+            MoeSeg sg;
+            int stage = 0, seg = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            while (ok && it.next(s, sg)) {
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = smem + (size_t)stage * p.stage_bytes;
+                    mbar_arrive_expect_tx(&wfull[stage], kMoeXBytes);
+                    if (sg.phase == 0) {
+                        const int e = expert[sg.tile / s.f_tiles], f0 = sg.tile % s.f_tiles * 128;
+                        tma_load_3d_hint(dst, &tmw1, kb * 64, f0, 2 * e, &wfull[stage], pol);
+                        tma_load_3d_hint(dst + kMoeXBytes / 2, &tmw1, kb * 64, f0, 2 * e + 1, &wfull[stage], pol);
+                    } else {
+                        const int sl = kb / s.kbf;
+                        tma_load_3d_hint(dst, &tmw2, (kb - sl * s.kbf) * 64, sg.tile * 256, expert[sl], &wfull[stage],
+                                         pol);
+                    }
+                    ++issued;
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                ++seg;
+            }
+            moe_drain(wfull, issued, S, p.wait_ns);
+        }
+    } else if (warp == 6) {
+        // ---------------------------------------------------------- the tokens' producer
+        if (lane == 0) {
+            MoeIter it(s, c);
+            MoeSeg sg;
+            int stage = 0, seg = 0, seen = -1, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            while (ok && it.next(s, sg)) {
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(3, 1, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    const int sl = sg.phase ? kb / s.kbf : 0;
+                    if (sg.phase && sl != seen) {  // the expert's activations are complete and visible to the TMA engine
+                        if (!moe_wait_count(p.ready + sl, s.f_tiles, abort_flag, p.wait_ns, site(3, 10, sl & 255), seg)) {
+                            ok = false;
+                            break;
+                        }
+                        fence_proxy_async_global();
+                        seen = sl;
+                    }
+                    uint8_t* dst = smem + (size_t)stage * p.stage_bytes + kMoeXBytes;
+                    mbar_arrive_expect_tx(&xfull[stage], (uint32_t)Tp * 128u);
+                    if (sg.phase == 0)
+                        tma_load_2d(dst, &tmx, kb * 64, 0, &xfull[stage]);
+                    else
+                        tma_load_3d(dst, &tmh, (kb - sl * s.kbf) * 64, 0, sl, &xfull[stage]);
+                    ++issued;
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                ++seg;
+            }
+            moe_drain(xfull, issued, S, p.wait_ns);
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------- the MMA issuer
+        if (lane == 0) {
+            const uint32_t idesc = moe_idesc(Tp, p.bf16);
+            MoeIter it(s, c);
+            MoeSeg sg;
+            int stage = 0, acc = 0, seg = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            while (ok && it.next(s, sg)) {
+                if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + (uint32_t)(acc * 2 * Tp);
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (!wait_bounded(&wfull[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg) ||
+                        !wait_bounded(&xfull[stage], ph, abort_flag, p.wait_ns, site(1, 12, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sx = smem_u32(smem + (size_t)stage * p.stage_bytes), sy = sx + kMoeXBytes;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t accumulate = (kb > sg.k0 || k > 0) ? 1u : 0u;
+                        mma_f16(d, desc_kmajor(sx, k), desc_kmajor(sy, k), idesc, accumulate);
+                        mma_f16(d + (uint32_t)Tp, desc_kmajor(sx + kMoeXBytes / 2, k), desc_kmajor(sy, k), idesc, accumulate);
+                    }
+                    mma_commit(&empty[stage]);
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                mma_commit(&tfull[acc]);
+                if (++acc == 2) {
+                    acc = 0;
+                    aph ^= 1u;
+                }
+                ++seg;
+            }
+            mma_commit(drain);  // the MMAs in flight finish before the tensor memory is freed
+            wait_drain(drain, 0, p.wait_ns);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------- the epilogue
+        const int q = warp & 3, row = q * 32 + lane;  // the TMEM lane: a row of each of the stage's two weight blocks
+        const int tq = (p.T + 3) / 4;                 // groups of four tokens
+        const int tid = threadIdx.x - kMoeEpiThread0;
+        MoeIter it(s, c);
+        MoeSeg sg, pend[2];
+        int acc = 0, seg = 0, n_pend = 0, gate_slot = -1;
+        uint32_t aph = 0;
+        bool ok = true;
+        // a partial: [block w of 2][group of 4 tokens][row][4]
+        auto slot_of = [&](int blk, const MoeSeg& g) {
+            return reinterpret_cast<float4*>(p.partials + (size_t)moe_slot(g, blk) * p.slot_floats);
+        };
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
+        };
+        while (it.next(s, sg)) {
+            if (threadIdx.x == kMoeEpiThread0)
+                epi_go[seg & 1] = wait_bounded(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, acc), seg) ? 1 : 0;
+            named_bar_sync(1, 128);
+            if (epi_go[seg & 1] != 1) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 2 * Tp);
+            bool sum_here = sg.nseg == 1;  // this block has (or gathers) the whole sums of the tile
+            if (sg.nseg > 1) {
+                float4* dst = slot_of(c, sg) + row;
+#pragma unroll 1
+                for (int w = 0; w < 2; ++w)
+#pragma unroll 1
+                    for (int c0 = 0; c0 < p.T; c0 += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(tbase + (uint32_t)(w * Tp + c0), r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (c0 + 4 * j < p.T)
+                                __stcg(dst + (size_t)(w * tq + c0 / 4 + j) * 128,
+                                       make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                   __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
+                    }
+                __threadfence();
+                named_bar_sync(1, 128);
+                if (threadIdx.x == kMoeEpiThread0) {
+                    const int old = atomicAdd(p.counters + moe_counter(sg), 1);
+                    __threadfence();
+                    *epi_last = old == sg.nseg - 1 ? 1 : 0;
+                }
+                if (sg.phase == 0) {  // the last block of a split gate/up tile sums it
+                    named_bar_sync(1, 128);
+                    sum_here = *epi_last != 0;
+                } else {
+                    pend[n_pend++] = sg;  // a split down tile is summed below, by all its blocks
+                }
+            }
+            if (sum_here) {
+                const int sl = sg.tile / s.f_tiles, f = sg.tile % s.f_tiles * 128 + row;
+                if (sg.phase == 0 && sl != gate_slot) {  // p of every token for this expert
+                    named_bar_sync(1, 128);              // the previous expert's have been read
+                    if (tid < p.T) {
+                        const int e = expert[sl];
+                        float v = 0.f;
+                        for (int j = 0; j < p.top_k; ++j)
+                            if (p.ids[tid * p.top_k + j] == e) v = p.weights[tid * p.top_k + j];
+                        gate[tid] = v;
+                    }
+                    gate_slot = sl;
+                    named_bar_sync(1, 128);
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < p.T; c0 += 16) {
+                    float a[2][16];
+                    if (sg.nseg == 1) {
+                        uint32_t r[2][16];
+                        tmem_ld16(tbase + (uint32_t)c0, r[0]);
+                        tmem_ld16(tbase + (uint32_t)(Tp + c0), r[1]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int w = 0; w < 2; ++w)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) a[w][j] = __uint_as_float(r[w][j]);
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 2; ++w)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) a[w][j] = 0.f;
+#pragma unroll 1
+                        for (int b = sg.first; b < sg.first + sg.nseg; ++b) {  // in block order
+                            const float4* src = slot_of(b, sg) + row;
+#pragma unroll
+                            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    if (c0 + 4 * j >= p.T) continue;
+                                    const float4 v = __ldcg(src + (size_t)(w * tq + c0 / 4 + j) * 128);
+                                    a[w][4 * j] += v.x;
+                                    a[w][4 * j + 1] += v.y;
+                                    a[w][4 * j + 2] += v.z;
+                                    a[w][4 * j + 3] += v.w;
+                                }
+                        }
+                    }
+                    if (sg.phase == 0) {
+                        if (f < p.F) {
+                            uint16_t* dst = p.H + ((size_t)sl * p.T + c0) * p.F + f;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                if (c0 + j >= p.T) break;
+                                const float pr = gate[c0 + j];
+                                // a token that did not choose the expert contributes nothing, whatever its products
+                                const float h = pr == 0.f ? 0.f : pr * (a[0][j] / (1.0f + __expf(-a[0][j])) * a[1][j]);
+                                dst[(size_t)j * p.F] = moe_bits16(h, p.bf16);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const int d = sg.tile * 256 + w * 128 + row;
+                            if (d >= p.D) continue;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (c0 + j < p.T) p.Y[(size_t)(c0 + j) * p.D + d] = moe_bits16(a[w][j], p.bf16);
+                        }
+                    }
+                }
+                if (sg.phase == 0) {
+                    __threadfence();  // h before the count
+                    named_bar_sync(1, 128);
+                    if (threadIdx.x == kMoeEpiThread0) {
+                        __threadfence();
+                        atomicAdd(p.ready + sl, 1);
+                    }
+                }
+            }
+            release();
+            if (++acc == 2) {
+                acc = 0;
+                aph ^= 1u;
+            }
+            ++seg;
+        }
+        // the split down tiles (at most two per block): every block of a tile sums a part of it once all have written
+        // theirs.  A block writes its own partials before it waits for any, so no wait can close a circle.
+        for (int i = 0; ok && i < n_pend; ++i) {
+            const MoeSeg& g = pend[i];
+            if (threadIdx.x == kMoeEpiThread0)
+                *epi_last = moe_wait_count(p.counters + moe_counter(g), g.nseg, abort_flag, p.wait_ns,
+                                           site(2, 11, g.first & 255), seg)
+                                ? 1
+                                : 0;
+            named_bar_sync(1, 128);
+            ok = *epi_last != 0;
+            named_bar_sync(1, 128);
+            if (!ok) break;
+            __threadfence();
+            const int items = 2 * tq * 128, mine = c - g.first;
+            const int i1 = (int)((long long)items * (mine + 1) / g.nseg);
+            for (int x = (int)((long long)items * mine / g.nseg) + tid; x < i1; x += 128) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int b = g.first; b < g.first + g.nseg; ++b) {
+                    const float4 u = __ldcg(slot_of(b, g) + x);
+                    v.x += u.x;
+                    v.y += u.y;
+                    v.z += u.z;
+                    v.w += u.w;
+                }
+                const int w = x / (tq * 128), t0 = (x - w * tq * 128) / 128 * 4;
+                const int d = g.tile * 256 + w * 128 + (x & 127);
+                if (d >= p.D) continue;
+                uint16_t* dst = p.Y + (size_t)t0 * p.D + d;
+                dst[0] = moe_bits16(v.x, p.bf16);
+                if (t0 + 1 < p.T) dst[(size_t)p.D] = moe_bits16(v.y, p.bf16);
+                if (t0 + 2 < p.T) dst[2 * (size_t)p.D] = moe_bits16(v.z, p.bf16);
+                if (t0 + 3 < p.T) dst[3 * (size_t)p.D] = moe_bits16(v.w, p.bf16);
+            }
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem_base, (uint32_t)tmem_cols);
+    }
+}
+
+}  // namespace bw

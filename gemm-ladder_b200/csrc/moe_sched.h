@@ -1,0 +1,128 @@
+// moe_sched.h -- the work of one block of the mixture-of-experts kernel (moe_kernel.cuh): which tiles of the two
+// products, and which K-blocks of them.  Host and device: the kernel runs it, the CPU tests check it.
+//
+// Both products are streams of K-blocks (256 weight rows x 64 values, 32 KB) read once, cut evenly over the blocks
+// whatever the number of active experts:
+//   gate/up  tile (s, j): active expert s's gate rows [128 j, 128 j + 128) and the up rows of the same, K = D
+//   down     tile i: output columns [256 i, 256 i + 256), K = the active experts' F one after the other, so the sum
+//            over the experts is the accumulator's own
+// A share of P >= 1 blocks out of U K-blocks: block c takes [U c / P, U (c + 1) / P), P <= U, so no share is empty.
+#pragma once
+#if defined(__CUDACC__)
+#define BW_MOE_HD __host__ __device__
+#else
+#define BW_MOE_HD
+#endif
+
+namespace bw {
+
+constexpr int kMoeMaxTokens = 128;
+constexpr int kMoeMaxExperts = 512;
+constexpr int kMoeMaxTopK = 32;
+constexpr int kMoeMinBlocks = 4;  // K-blocks of a share at least, where there are as many: a share's fixed cost is
+                                  // that of a few K-blocks
+
+struct MoeSched {
+    int T, D, F;
+    int active;           // experts that some token chose
+    int f_tiles;          // gate/up tiles per expert
+    int kb1, kbf;         // K-blocks of a gate/up tile; of one expert in a down tile
+    int d_tiles;
+    long long u1, u2;     // K-blocks of each product
+    int p1, p2;           // blocks that share them
+};
+
+BW_MOE_HD inline int moe_share_blocks(long long u, int grid)
+{
+    const long long want = u / kMoeMinBlocks;
+    return want < 1 ? 1 : want < grid ? (int)want : grid;
+}
+
+BW_MOE_HD inline MoeSched moe_sched(int T, int D, int F, int active, int grid)
+{
+    MoeSched s;
+    s.T = T;
+    s.D = D;
+    s.F = F;
+    s.active = active;
+    s.f_tiles = (F + 127) / 128;
+    s.kb1 = D / 64;
+    s.kbf = F / 64;
+    s.d_tiles = (D + 255) / 256;
+    s.u1 = (long long)active * s.f_tiles * s.kb1;
+    s.u2 = (long long)s.d_tiles * active * s.kbf;
+    s.p1 = moe_share_blocks(s.u1, grid);
+    s.p2 = moe_share_blocks(s.u2, grid);
+    return s;
+}
+
+BW_MOE_HD inline long long moe_begin(long long u, int p, int c) { return u * c / p; }
+// The block whose share holds K-block g: the largest c with moe_begin(c) <= g.
+BW_MOE_HD inline int moe_owner(long long u, int p, long long g) { return (int)(((g + 1) * p - 1) / u); }
+
+struct MoeSeg {
+    int phase;        // 0: gate/up, 1: down
+    int tile, k0, k1; // K-blocks [k0, k1) of the tile
+    int first, nseg;  // the first block that works on the tile, and how many do
+};
+
+// A block's segments in order: its share of the first product, then of the second.
+struct MoeIter {
+    long long g, end;
+    int phase, c;
+    BW_MOE_HD MoeIter(const MoeSched& s, int c_) : g(0), end(0), phase(-1), c(c_) { (void)s; }
+    BW_MOE_HD bool next(const MoeSched& s, MoeSeg& seg)
+    {
+        while (g >= end) {
+            if (++phase > 1) return false;
+            const long long u = phase ? s.u2 : s.u1;
+            const int p = phase ? s.p2 : s.p1;
+            if (c >= p) continue;
+            g = moe_begin(u, p, c);
+            end = moe_begin(u, p, c + 1);
+        }
+        const long long u = phase ? s.u2 : s.u1;
+        const int p = phase ? s.p2 : s.p1, kb = phase ? s.active * s.kbf : s.kb1;
+        const long long t = g / kb;
+        seg.phase = phase;
+        seg.tile = (int)t;
+        seg.k0 = (int)(g - t * kb);
+        seg.k1 = end - g < (long long)(kb - seg.k0) ? seg.k0 + (int)(end - g) : kb;
+        seg.first = moe_owner(u, p, t * kb);
+        seg.nseg = moe_owner(u, p, (t + 1) * kb - 1) - seg.first + 1;
+        g += seg.k1 - seg.k0;
+        return true;
+    }
+};
+
+// Block c's slot for its partial of a split tile: one for the tile its share of a product starts in, one for the tile
+// it ends in (whole tiles in between need none), in each product.
+BW_MOE_HD inline int moe_slot(const MoeSeg& seg, int c) { return 4 * c + 2 * seg.phase + (c == seg.first ? 1 : 0); }
+// The counter of a split tile: a block is the first of at most one split tile in each product.
+BW_MOE_HD inline int moe_counter(const MoeSeg& seg) { return 2 * seg.first + seg.phase; }
+
+// The workspace of a call on `grid` blocks (offsets in bytes): the chosen experts and their weights, the activations of
+// the active experts, the partials, then the words that start at zero (a count of finished gate/up tiles per active
+// expert, the split tiles' counters).
+struct MoeWork {
+    long long ids, weights, h, partials, zero, bytes;
+    int slots, zero_words;
+    long long slot_floats;
+};
+BW_MOE_HD inline long long moe_up(long long v) { return (v + 255) / 256 * 256; }
+BW_MOE_HD inline MoeWork moe_work(int T, int E, int k, int F, int grid)
+{
+    MoeWork w;
+    w.slots = T * k < E ? T * k : E;
+    w.slot_floats = 256LL * ((T + 3) / 4 * 4);
+    w.ids = 0;
+    w.weights = moe_up(w.ids + 4LL * T * k);
+    w.h = moe_up(w.weights + 4LL * T * k);
+    w.partials = moe_up(w.h + 2LL * w.slots * T * F);
+    w.zero = moe_up(w.partials + 4LL * 4 * grid * w.slot_floats);
+    w.zero_words = w.slots + 2 * grid;
+    w.bytes = moe_up(w.zero + 4LL * w.zero_words);
+    return w;
+}
+
+}  // namespace bw

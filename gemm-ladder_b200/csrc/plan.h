@@ -160,6 +160,9 @@
 #define BW_DYN_MAX_BYTES (32u << 20)  // the units' partials of a call at most this many bytes (longer units if need be;
                                       // so that the no-allocation entry's array holds them too)
 #endif
+#ifndef BW_MOE_PDL
+#define BW_MOE_PDL 1           // the mixture-of-experts kernel's set-up overlaps its router (programmatic serialisation)
+#endif
 #ifndef BW_SK_ONE_WAVE
 #define BW_SK_ONE_WAVE 1       // stream-K over every tile when they make one full wave and part of another (the
                                // split-K tail's units then double a block's work: measured qkv_m512 -12 %)

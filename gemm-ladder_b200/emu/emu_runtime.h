@@ -39,7 +39,10 @@ inline thread_local dim3 threadIdx, blockIdx, gridDim, blockDim;
 namespace bw {
 namespace emu {
 
-constexpr int kCtaThreads = 192;
+#ifndef BW_EMU_THREADS
+#define BW_EMU_THREADS 192  // the GEMM kernel's block
+#endif
+constexpr int kCtaThreads = BW_EMU_THREADS;
 constexpr int kSmemBytes = 232448 + 1024;  // the kernel's dynamic shared memory limit and alignment slack
 constexpr int kTmemLanes = 128, kTmemCols = 512;
 
@@ -511,7 +514,7 @@ inline void tmem_dealloc(uint32_t taddr, uint32_t ncols)
 }
 
 // operand element (row, k) of a K16 slice through a 128-byte-swizzled shared-memory descriptor
-inline float operand(const Cta* c, uint64_t desc, bool mn_major, int row, int k)
+inline float operand(const Cta* c, uint64_t desc, bool mn_major, int row, int k, bool bf16 = false)
 {
     const uint32_t start = (uint32_t)(desc & 0x3FFFu) << 4;
     const uint32_t lbo = (uint32_t)((desc >> 16) & 0x3FFFu) << 4;
@@ -523,6 +526,14 @@ inline float operand(const Cta* c, uint64_t desc, bool mn_major, int row, int k)
     if (p + 2 > (uint32_t)kSmemBytes) {
         finding("an MMA operand read past the end of shared memory");
         return 0.f;
+    }
+    if (bf16) {
+        uint16_t u;
+        std::memcpy(&u, c->smem + p, 2);
+        const uint32_t w = (uint32_t)u << 16;
+        float f;
+        std::memcpy(&f, &w, 4);
+        return f;
     }
     __half h;
     std::memcpy(&h, c->smem + p, 2);
@@ -538,6 +549,8 @@ inline void mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool
     const bool a_mn = (idesc >> 15) & 1u, b_mn = (idesc >> 16) & 1u;
     const int N = (int)((idesc >> 17) & 0x3Fu) << 3, M = (int)((idesc >> 24) & 0x1Fu) << 4;
     if (((idesc >> 4) & 3u) != 1u) finding("an MMA whose accumulator is not fp32");
+    const unsigned fmt = (idesc >> 7) & 7u;  // 0 fp16, 1 bf16
+    if (fmt > 1u || ((idesc >> 10) & 7u) != fmt) finding("an MMA whose operands are not both fp16 or both bf16");
     const int ranks = pair ? 2 : 1;
     // cta_group::1 with M = 128: N in 16 .. 256 by 16; cta_group::2 (M = 256): N in 32 .. 256 by 32, half per block
     if (M != 128 * ranks || N < 16 * ranks || N > 256 || N % (16 * ranks)) {
@@ -562,12 +575,12 @@ inline void mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool
     std::vector<float> b((size_t)N * 16);
     for (int n = 0; n < N; ++n) {
         const int r = n / (N / ranks), local = n % (N / ranks);
-        for (int k = 0; k < 16; ++k) b[(size_t)n * 16 + k] = operand(cta[r], bdesc, b_mn, local, k);
+        for (int k = 0; k < 16; ++k) b[(size_t)n * 16 + k] = operand(cta[r], bdesc, b_mn, local, k, fmt == 1u);
     }
     std::vector<float> a(128 * 16);
     for (int r = 0; r < ranks; ++r) {
         for (int m = 0; m < 128; ++m)
-            for (int k = 0; k < 16; ++k) a[(size_t)m * 16 + k] = operand(cta[r], adesc, a_mn, m, k);
+            for (int k = 0; k < 16; ++k) a[(size_t)m * 16 + k] = operand(cta[r], adesc, a_mn, m, k, fmt == 1u);
         if (cta[r]->tmem_cols < (int)(col0 + N)) finding("an MMA into tensor memory not allocated");
         for (int m = 0; m < 128; ++m) {
             uint32_t* row = cta[r]->tmem.data() + (size_t)m * kTmemCols + col0;
@@ -707,6 +720,8 @@ inline uint32_t __float_as_uint(float f)
 }
 inline int atomicAdd(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
 inline unsigned atomicAdd(unsigned* p, unsigned v) { return __atomic_fetch_add(p, v, __ATOMIC_SEQ_CST); }
+inline uint32_t atomicOr(uint32_t* p, uint32_t v) { return __atomic_fetch_or(p, v, __ATOMIC_SEQ_CST); }
+inline int __popc(uint32_t v) { return __builtin_popcount(v); }
 inline int atomicExch(int* p, int v) { return __atomic_exchange_n(p, v, __ATOMIC_SEQ_CST); }
 inline unsigned atomicCAS(unsigned* p, unsigned cmp, unsigned val)
 {

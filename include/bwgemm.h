@@ -118,6 +118,29 @@ int bw_gemm_i8_swiglu(const void* A, const void* a_scale, const void* B, const v
 int bw_linear_i8(const void* X, int x_type, long long ld, const void* B, const void* b_scale, void* C, int M, int N,
                  int K, int swiglu, void* work, size_t work_bytes, void* stream);
 
+/*
+ * A mixture-of-experts MLP layer for a few tokens (a decode step; T <= 128), in two kernels: the router, then all
+ * active experts' gate, up and down products, which stream each active expert's weights once.  type BW_TYPE_F16 or
+ * BW_TYPE_BF16 for X, R, W1, W2 and Y:
+ *   X   T x D (ldx elements from row to row)     R   E x D, the router
+ *   W1  E x 2F x D: an expert's F gate rows, then its F up rows     W2  E x D x F     Y  T x D
+ *   logits l = X R^T (fp32); S_t = the top_k experts of token t by logit (equal logits: the lower index);
+ *   p_te = softmax over S_t (renormalize 1) or over all experts (0);
+ *   Y_t = sum over S_t of p_te (silu(X_t G_e^T) * (X_t U_e^T)) W2_e^T
+ * in fp32 sums; p_te silu * up is rounded to the type before the down product, Y once.  D % 64 == 0, F % 64 == 0,
+ * E <= 512, top_k <= min(E, 32), ldx >= D, ldx % 8 == 0; X, R, W1 and W2 16-byte aligned.
+ * The down products of all active experts are one product for all tokens (with p = 0 where a token did not choose an
+ * expert), so a W2 that holds an infinity or a NaN reaches every token of a call in which any token chose its expert;
+ * an infinity or a NaN anywhere else stays with the tokens that meet it.
+ * ids (T x top_k int32, by falling logit) and weights (T x top_k fp32) receive the routing where not null.
+ * `work`: as for the 8-bit entries, at least bw_moe_work_bytes (T, E, top_k, D, F) bytes, 256-byte aligned.  The experts
+ * kernel is a cooperative launch of one block per SM.  T == 0 is a call that does nothing.  No reference counterpart.
+ */
+int bw_moe_work_bytes(int T, int E, int top_k, int D, int F, size_t* bytes);
+int bw_moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const void* W2, void* Y, int T, int E,
+               int top_k, int D, int F, int type, int renormalize, void* ids, void* weights, void* work,
+               size_t work_bytes, void* stream);
+
 /* The number of variants.  Replaces: the weak `int g_nvar` (probe/probe.cu:40, hopper/verif.cu:38,
  * hopper/step7.cu:16). */
 int bw_gemm_variant_count(void);
@@ -234,7 +257,8 @@ int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw_plan* 
  * gave up, *block its block, *segment the segment that block was on.  Kinds: 0 a full stage, 1 an empty stage, 2 a
  * finished accumulator, 3 a free accumulator, 4 partials copied in, 5 and 6 a K-split cluster's pieces and go signal,
  * 7 another rank's partial of the fused reduce-scatter (index: the sender), 8 a rank's ack of the previous call, 9 an
- * entry of the block's queue of units (a plan with dyn 1).
+ * entry of the block's queue of units (a plan with dyn 1); of the mixture-of-experts kernel (role 3: its tokens'
+ * producer) 10 an expert's activations, 11 a split output tile's other partials, 12 a stage's tokens.
  * Returns a CUDA error as BW_ERR_LAUNCH.
  * No reference counterpart as a function: the reference traps in its guarded wait (hopper/step2.cuh:128-145); this
  * rung's waits return instead and leave the context usable.

@@ -1,0 +1,216 @@
+"""The mixture-of-experts layer on a B200, through the public entry point, against the definition in 64 bits
+(tests/moe_ref.py derives how far a result may be from it): one token to 128, one expert to 512, ragged widths, ties,
+all tokens on one expert; strided rows, streams, overlapping calls and graphs, a stall's status."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import bwgemm  # noqa: E402
+import moe_ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.set_device(0)
+    bwgemm.clear_status()
+    yield
+    torch.cuda.synchronize()
+    assert bwgemm.status()[0] == 0
+
+
+def inputs(T, E, D, F, dtype, seed=0, pad=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    X = randn(T, D + pad).to(dtype)[:, :D]
+    R = (randn(E, D) * (1.5 / D ** 0.5)).to(dtype)
+    W1 = (randn(E, 2 * F, D) / D ** 0.5).to(dtype)
+    W2 = (randn(E, D, F) * (2 / F ** 0.5)).to(dtype)
+    return X, R, W1, W2
+
+
+def check(Y, X, R, W1, W2, k, renormalize=True):
+    ids, weights, err = moe_ref.route(X, R, k, renormalize)
+    y, tol = moe_ref.layer(X, ids, weights, err, W1, W2)
+    bad = ((Y.double() - y).abs() > tol) | ~torch.isfinite(Y.double())
+    assert not bad.any(), f"{int(bad.sum())} elements outside, first {bad.nonzero()[:3].tolist()}"
+    return ids, weights, err
+
+
+CASES = [  # T, E, k, D, F
+    (1, 1, 1, 64, 64), (1, 8, 2, 256, 128), (1, 64, 8, 2048, 1024), (2, 60, 4, 512, 192), (3, 4, 4, 128, 64),
+    (5, 16, 3, 4096, 128), (8, 128, 8, 1024, 448), (16, 8, 1, 320, 1344), (17, 8, 2, 2112, 320), (33, 8, 2, 1024, 1792),
+    (64, 128, 8, 512, 256), (77, 512, 6, 192, 64), (100, 32, 32, 256, 128), (128, 32, 4, 1472, 704), (128, 2, 2, 64, 4096)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(map(str, c)))
+def test_layer(case, dtype):
+    T, E, k, D, F = case
+    X, R, W1, W2 = inputs(T, E, D, F, dtype, seed=T + E + D, pad=8 if T % 2 else 0)
+    ids = torch.full((T, k), -1, dtype=torch.int32, device="cuda")
+    weights = torch.full((T, k), float("nan"), device="cuda")
+    buf = torch.full((T + 4, D), float("nan"), dtype=dtype, device="cuda")
+    Y = bwgemm.moe_mlp(X, R, W1, W2, k, Y=buf[:T], ids=ids, weights=weights)
+    torch.cuda.synchronize()
+    assert bwgemm.status()[0] == 0, bwgemm.status()
+    want, p, err = check(Y, X, R, W1, W2, k)
+    assert torch.equal(ids.long(), want)
+    assert ((weights.double() - p).abs() <= p * err).all()
+    assert torch.isnan(buf[T:]).all()
+    assert torch.equal(Y, bwgemm.moe_mlp(X, R, W1, W2, k)), "calls differ"
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_weights_over_the_chosen_or_over_all(renormalize):
+    X, R, W1, W2 = inputs(6, 40, 256, 128, torch.bfloat16, 3)
+    weights = torch.empty((6, 4), device="cuda")
+    Y = bwgemm.moe_mlp(X, R, W1, W2, 4, renormalize=renormalize, weights=weights)
+    check(Y, X, R, W1, W2, 4, renormalize)
+    assert (weights.sum(1) - 1).abs().max() < 1e-5 if renormalize else (weights.sum(1) < 1).all()
+
+
+def test_equal_logits_go_to_the_lower_index():
+    X, R, W1, W2 = inputs(9, 100, 256, 64, torch.float16, 4)
+    R[:] = R[torch.arange(100, device="cuda") % 7]  # every logit about 14 times
+    X[4] = 0  # every logit equal
+    ids = torch.empty((9, 5), dtype=torch.int32, device="cuda")
+    Y = bwgemm.moe_mlp(X, R, W1, W2, 5, ids=ids)
+    want, _, _ = check(Y, X, R, W1, W2, 5)
+    assert torch.equal(ids.long(), want)
+    assert ids[4].tolist() == [0, 1, 2, 3, 4] and (Y[4] == 0).all()
+
+
+def test_every_token_on_one_expert():
+    X, R, W1, W2 = inputs(50, 16, 512, 320, torch.bfloat16, 5)
+    X = X.abs() + 0.1
+    R[:] = 0
+    R[11] = 1
+    ids = torch.empty((50, 1), dtype=torch.int32, device="cuda")
+    Y = bwgemm.moe_mlp(X, R, W1, W2, 1, ids=ids)
+    check(Y, X, R, W1, W2, 1)
+    assert (ids == 11).all()
+
+
+def test_a_token_with_nan_or_infinity_reaches_no_other_token():
+    X, R, W1, W2 = inputs(20, 16, 256, 128, torch.float16, 6)
+    want = bwgemm.moe_mlp(X, R, W1, W2, 3)
+    X[7, 3] = float("nan")
+    X[13, 100] = float("inf")
+    ids = torch.empty((20, 3), dtype=torch.int32, device="cuda")
+    got = bwgemm.moe_mlp(X, R, W1, W2, 3, ids=ids)
+    others = [t for t in range(20) if t not in (7, 13)]
+    assert torch.isnan(got[7]).all()
+    assert torch.equal(got[others], want[others])
+    assert ((ids >= 0) & (ids < 16)).all()
+
+
+def test_inactive_experts_weights_are_not_met():
+    X, R, W1, W2 = inputs(4, 32, 256, 128, torch.bfloat16, 7)
+    ids, _, _ = moe_ref.route(X, R, 2)
+    want = bwgemm.moe_mlp(X, R, W1, W2, 2)
+    idle = [e for e in range(32) if e not in set(ids.flatten().tolist())]
+    W1[idle] = float("nan")
+    W2[idle] = float("nan")
+    assert torch.equal(bwgemm.moe_mlp(X, R, W1, W2, 2), want)
+
+
+def test_inputs_are_left_alone():
+    a = inputs(12, 16, 512, 192, torch.float16, 8)
+    before = [t.clone() for t in a]
+    bwgemm.moe_mlp(*a, 4)
+    assert all(torch.equal(x, y) for x, y in zip(a, before))
+
+
+def test_no_tokens():
+    X, R, W1, W2 = inputs(1, 4, 64, 64, torch.float16)
+    assert bwgemm.moe_mlp(X[:0], R, W1, W2, 2).shape == (0, 64)
+
+
+def test_streams_and_overlapping_calls():
+    sets = [inputs(t, 32, 1024, 512, torch.bfloat16, 20 + t) for t in (3, 24)]
+    want = [bwgemm.moe_mlp(*a, 4) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):  # cooperative launches on both streams
+        for i in range(2):
+            got[i].append(bwgemm.moe_mlp(*sets[i], 4, stream=streams[i]))
+    torch.cuda.synchronize()
+    assert bwgemm.status()[0] == 0, bwgemm.status()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_beside_a_long_gemm():
+    """The blocks of a GEMM on another stream hold the SMs: the layer's blocks start once all of them fit."""
+    A = torch.randn((8192, 8192), device="cuda").half()
+    a = inputs(8, 32, 1024, 512, torch.float16, 31)
+    want = bwgemm.moe_mlp(*a, 4)
+    C = bwgemm.gemm(A, A)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    out = []
+    for _ in range(8):
+        C2 = bwgemm.gemm(A, A)
+        out.append(bwgemm.moe_mlp(*a, 4, stream=side))
+    torch.cuda.synchronize()
+    assert bwgemm.status()[0] == 0
+    assert all(torch.equal(y, want) for y in out) and torch.equal(C, C2)
+
+
+def test_graphs_with_new_contents_replayed_at_once():
+    sets = [inputs(t, 32, 512, 256, torch.bfloat16, 40 + t) for t in (1, 16)]
+    for a in sets:
+        bwgemm.moe_mlp(*a, 4)
+    torch.cuda.synchronize()
+    graphs, out = [], []
+    for a in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(bwgemm.moe_mlp(*a, 4))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(10):
+        for a in sets:
+            a[0].copy_(torch.randn_like(a[0]))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert bwgemm.status()[0] == 0, bwgemm.status()
+        for i in range(2):
+            assert torch.equal(out[i], bwgemm.moe_mlp(*sets[i], 4))
+
+
+def test_refused_tensors():
+    X, R, W1, W2 = inputs(4, 8, 128, 64, torch.float16, 9)
+    for call in (lambda: bwgemm.moe_mlp(X.float(), R, W1, W2, 2), lambda: bwgemm.moe_mlp(X, R.bfloat16(), W1, W2, 2),
+                 lambda: bwgemm.moe_mlp(X, R, W1[:, :64], W2, 2), lambda: bwgemm.moe_mlp(X, R, W1, W2.transpose(1, 2), 2),
+                 lambda: bwgemm.moe_mlp(X, R[:4], W1, W2, 2), lambda: bwgemm.moe_mlp(X[:, :64], R, W1, W2, 2),
+                 lambda: bwgemm.moe_mlp(X, R, W1, W2, 2, ids=torch.empty((4, 3), dtype=torch.int32, device="cuda")),
+                 lambda: bwgemm.moe_mlp(X, R, W1, W2, 2, weights=torch.empty((4, 2), dtype=torch.float64, device="cuda")),
+                 lambda: bwgemm.moe_mlp(X, R, W1, W2, 2, Y=torch.empty((4, 64), dtype=torch.float16, device="cuda"))):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: bwgemm.moe_mlp(X, R, W1, W2, 0), lambda: bwgemm.moe_mlp(X, R, W1, W2, 9),
+                 lambda: bwgemm.moe_mlp(X.repeat(33, 1), R, W1, W2, 2)):
+        with pytest.raises(bwgemm.BwError):
+            call()
+    n = ctypes.c_size_t()
+    L = bwgemm.lib()
+    assert L.bw_moe_work_bytes(4, 8, 2, 128, 64, ctypes.byref(n)) == 0
+    w = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    rc = L.bw_moe_mlp(X.data_ptr(), 128, R.data_ptr(), W1.data_ptr(), W2.data_ptr(), X.data_ptr(), 4, 8, 2, 128, 64, 0, 1,
+                      None, None, w.data_ptr(), n.value - 1, None)
+    assert rc == bwgemm.BW_ERR_SCRATCH
