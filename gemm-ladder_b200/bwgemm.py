@@ -258,51 +258,49 @@ def gemm_swiglu(A, B, C=None, stream=None):
 
 
 # ---------------------------------------------------------------------------------- 8-bit integer products
+# These calls are made once per layer of a decode step, so their host side is kept short: plain comparisons, the raw
+# stream handle, torch's allocator only for what the call needs.
+_type_codes = {}
+
+
 def _types():
+    if not _type_codes:
+        import torch
+
+        _type_codes.update({torch.float16: BW_TYPE_F16, torch.bfloat16: BW_TYPE_BF16, torch.float32: BW_TYPE_F32})
+    return _type_codes
+
+
+def _on(device, stream, call):
+    """call(stream handle) with `device` current and `stream` (None: the device's current stream) the current stream there,
+    so that memory made inside belongs to the stream the call runs on."""
     import torch
 
-    return {torch.float16: BW_TYPE_F16, torch.bfloat16: BW_TYPE_BF16, torch.float32: BW_TYPE_F32}
-
-
-class _On:
-    """The tensors' device made current and `stream` (None: that device's current stream) the current one there, so
-    that memory made inside belongs to the stream the call runs on; does nothing where both already are."""
-
-    def __init__(self, device, stream):
-        import torch
-
-        self.ctx = []
-        if stream is not None and stream != torch.cuda.current_stream(device):
-            self.ctx.append(torch.cuda.stream(stream))
-        elif torch.cuda.current_device() != device.index:
-            self.ctx.append(torch.cuda.device(device))
-        self.device = device
-
-    def __enter__(self):
-        import torch
-
-        for c in self.ctx:
-            c.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        for c in reversed(self.ctx):
-            c.__exit__(*exc)
+    if stream is None:
+        if torch.cuda.current_device() == device.index:
+            return call(torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(device):
+            return call(torch._C._cuda_getCurrentRawStream(device.index))
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    with torch.cuda.stream(stream):
+        return call(stream.cuda_stream)
 
 
 def _rows16(X, what):
-    """X as rows of 16-bit values a kernel reads as they are: (rows, cols, elements from row to row)."""
-    import torch
-
-    if X.dtype not in (torch.float16, torch.bfloat16) or not X.is_cuda or X.dim() != 2:
+    """X as rows of 16-bit values a kernel reads as they are: (rows, cols, elements from row to row, type code)."""
+    code = _types().get(X.dtype)
+    if code is None or code == BW_TYPE_F32 or not X.is_cuda or X.dim() != 2:
         raise ValueError(f"{what} must be a 2-D fp16 or bf16 CUDA tensor")
     rows, cols = X.shape
-    if cols > 1 and X.stride(1) != 1:
+    ld, step = X.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{what}'s rows must be contiguous")
-    ld = X.stride(0) if rows > 1 else cols
+    if rows <= 1:
+        ld = cols
     if ld < cols or ld % 8 or X.data_ptr() % 16:
         raise ValueError(f"{what}'s rows must start on 16-byte boundaries and not overlap")
-    return rows, cols, ld
+    return rows, cols, ld, code
 
 
 def _i8_weight(B, b_scale, device):
@@ -310,37 +308,41 @@ def _i8_weight(B, b_scale, device):
 
     if B.dtype != torch.int8 or B.dim() != 2 or B.device != device or not B.is_contiguous():
         raise ValueError("B must be a contiguous int8 N x K tensor on A's device")
-    if b_scale.dtype != torch.float32 or b_scale.shape != (B.shape[0],) or b_scale.device != device or \
-            not b_scale.is_contiguous():
+    if b_scale.dtype != torch.float32 or b_scale.dim() != 1 or b_scale.shape[0] != B.shape[0] or \
+            b_scale.device != device or not b_scale.is_contiguous():
         raise ValueError("b_scale must be a contiguous fp32 tensor of B's N scales on A's device")
 
 
-def _i8_out(C, shape, dtype, device, what="C"):
-    import torch
-
+def _out(C, like, rows, cols, dtype, what="C"):
+    """C, checked, or a new one on `like`'s device (and the current stream)."""
     if C is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(C.shape) != tuple(shape) or C.dtype != dtype or C.device != device or not C.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {shape[0]} x {shape[1]} on the inputs' device")
+        return like.new_empty((rows, cols), dtype=dtype)
+    if C.dim() != 2 or C.shape[0] != rows or C.shape[1] != cols or C.dtype != dtype or C.device != like.device or \
+            not C.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of {rows} x {cols} on the inputs' device")
     return C
 
 
-_i8_work_bytes = {}  # (device, M, N, K, type, swiglu, linear) -> bytes: the plan's, a constant of the device
+_work_sizes = {}  # (entry, device, sizes ...) -> bytes of workspace: the plan's, a constant of the device
 
 
-def _i8_work(device, M, N, K, out_type, swiglu, linear):
-    """The call's own workspace from torch's allocator (so of the stream, or the CUDA graph, that the call is part of)."""
+def _work(query, like, *sizes):
+    """The call's own workspace from torch's allocator (so of the stream, or the CUDA graph, that the call is part of):
+    (tensor or None, address, bytes)."""
     import torch
 
-    key = (device.index, M, N, K, out_type, swiglu, linear)
-    n = _i8_work_bytes.get(key)
+    key = (query, like.device.index, *sizes)
+    n = _work_sizes.get(key)
     if n is None:
         size = ctypes.c_size_t()
-        check(lib().bw_gemm_i8_work_bytes(M, N, K, out_type, swiglu, linear, ctypes.byref(size)))
-        if len(_i8_work_bytes) >= 4096:
-            _i8_work_bytes.clear()
-        n = _i8_work_bytes[key] = size.value
-    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+        check(getattr(lib(), query)(*sizes, ctypes.byref(size)))
+        if len(_work_sizes) >= 4096:
+            _work_sizes.clear()
+        n = _work_sizes[key] = size.value
+    if not n:
+        return None, None, 0
+    t = like.new_empty((n,), dtype=torch.uint8)
+    return t, t.data_ptr(), n
 
 
 def quantize_rows(X, Q=None, scale=None, stream=None):
@@ -348,42 +350,47 @@ def quantize_rows(X, Q=None, scale=None, stream=None):
     scale = max|row| / 127, Q = round-half-even(127 X / max|row|); made if not given.  X's columns: a multiple of 16."""
     import torch
 
-    rows, cols, ld = _rows16(X, "X")
-    with _On(X.device, stream) as s:
-        Q = _i8_out(Q, (rows, cols), torch.int8, X.device)
-        if scale is None:
-            scale = torch.empty((rows,), dtype=torch.float32, device=X.device)
-        elif scale.shape != (rows,) or scale.dtype != torch.float32 or scale.device != X.device or \
-                not scale.is_contiguous():
-            raise ValueError("scale must be a contiguous fp32 tensor of X's rows")
-        check(lib().bw_quant_rows_i8(X.data_ptr(), _types()[X.dtype], ld, Q.data_ptr(), scale.data_ptr(), rows, cols, s))
-    return Q, scale
+    rows, cols, ld, code = _rows16(X, "X")
+    if scale is not None and (scale.dim() != 1 or scale.shape[0] != rows or scale.dtype != torch.float32 or
+                              scale.device != X.device or not scale.is_contiguous()):
+        raise ValueError("scale must be a contiguous fp32 tensor of X's rows")
+
+    def call(s):
+        q = _out(Q, X, rows, cols, torch.int8, "Q")
+        sc = X.new_empty((rows,), dtype=torch.float32) if scale is None else scale
+        check(lib().bw_quant_rows_i8(X.data_ptr(), code, ld, q.data_ptr(), sc.data_ptr(), rows, cols, s))
+        return q, sc
+
+    return _on(X.device, stream, call)
 
 
 def _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, swiglu):
     import torch
 
     dtype = torch.float16 if dtype is None else dtype
-    types = _types()
-    if dtype not in types or (swiglu and dtype == torch.float32):
+    code = _types().get(dtype)
+    if code is None or (swiglu and code == BW_TYPE_F32):
         raise ValueError(f"C cannot be {dtype}")
     if A.dtype != torch.int8 or A.dim() != 2 or not A.is_cuda or not A.is_contiguous():
         raise ValueError("A must be a contiguous int8 M x K CUDA tensor")
     M, K = A.shape
-    if a_scale.dtype != torch.float32 or a_scale.shape != (M,) or a_scale.device != A.device or \
+    if a_scale.dtype != torch.float32 or a_scale.dim() != 1 or a_scale.shape[0] != M or a_scale.device != A.device or \
             not a_scale.is_contiguous():
         raise ValueError("a_scale must be a contiguous fp32 tensor of A's M scales on A's device")
     _i8_weight(B, b_scale, A.device)
     N, K2 = B.shape
     if K2 != K:
         raise ValueError(f"A is {M} x {K} but B is {N} x {K2}")
-    with _On(A.device, stream) as s:
-        C = _i8_out(C, (M, N // 2 if swiglu else N), dtype, A.device)
-        work, n = _i8_work(A.device, M, N, K, types[dtype], swiglu, 0)
+
+    def call(s):
+        out = _out(C, A, M, N // 2 if swiglu else N, dtype)
+        _t, work, n = _work("bw_gemm_i8_work_bytes", A, M, N, K, code, swiglu, 0)
         f = lib().bw_gemm_i8_swiglu if swiglu else lib().bw_gemm_i8
-        check(f(A.data_ptr(), a_scale.data_ptr(), B.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, types[dtype],
-                work.data_ptr() if n else None, n, s))
-    return C
+        check(f(A.data_ptr(), a_scale.data_ptr(), B.data_ptr(), b_scale.data_ptr(), out.data_ptr(), M, N, K, code, work, n,
+                s))
+        return out
+
+    return _on(A.device, stream, call)
 
 
 def gemm_i8(A, a_scale, B, b_scale, C=None, dtype=None, stream=None):
@@ -400,23 +407,25 @@ def gemm_i8_swiglu(A, a_scale, B, b_scale, C=None, dtype=None, stream=None):
 def linear_i8(X, B, b_scale, C=None, swiglu=False, stream=None):
     """C = X B^T in X's type (fp16 or bf16): X (M x K, rows may be strided) quantised to int8 by row (quantize_rows), B
     (N x K) int8 with a scale per row; swiglu: silu(gate) * up, M x N/2, B's rows in groups of 128 gate then 128 up."""
-    M, K, ld = _rows16(X, "X")
+    M, K, ld, code = _rows16(X, "X")
     _i8_weight(B, b_scale, X.device)
     N, K2 = B.shape
     if K2 != K:
         raise ValueError(f"X is {M} x {K} but B is {N} x {K2}")
-    t, swiglu = _types()[X.dtype], int(bool(swiglu))
-    with _On(X.device, stream) as s:
-        C = _i8_out(C, (M, N // 2 if swiglu else N), X.dtype, X.device)
-        work, n = _i8_work(X.device, M, N, K, t, swiglu, 1)
-        check(lib().bw_linear_i8(X.data_ptr(), t, ld, B.data_ptr(), b_scale.data_ptr(), C.data_ptr(), M, N, K, swiglu,
-                                 work.data_ptr() if n else None, n, s))
-    return C
+    swiglu = 1 if swiglu else 0
+
+    def call(s):
+        out = _out(C, X, M, N // 2 if swiglu else N, X.dtype)
+        _t, work, n = _work("bw_gemm_i8_work_bytes", X, M, N, K, code, swiglu, 1)
+        check(lib().bw_linear_i8(X.data_ptr(), code, ld, B.data_ptr(), b_scale.data_ptr(), out.data_ptr(), M, N, K, swiglu,
+                                 work, n, s))
+        return out
+
+    return _on(X.device, stream, call)
 
 
 # ---------------------------------------------------------------------------------- mixture of experts
 MOE_MAX_TOKENS = 128
-_moe_work_bytes = {}  # (device, T, E, top_k, D, F) -> bytes
 
 
 def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=None, stream=None):
@@ -426,7 +435,7 @@ def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=Non
     experts.  ids (T x top_k int32) and weights (T x top_k fp32), where given, receive the routing."""
     import torch
 
-    T, D, ld = _rows16(X, "X")
+    T, D, ld, code = _rows16(X, "X")
     for t, what, dim in ((R, "R", 2), (W1, "W1", 3), (W2, "W2", 3)):
         if t.dtype != X.dtype or t.device != X.device or t.dim() != dim or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous {dim}-D tensor of X's type on X's device")
@@ -438,21 +447,16 @@ def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=Non
         if t is not None and (tuple(t.shape) != (T, top_k) or t.dtype != dtype or t.device != X.device or
                               not t.is_contiguous()):
             raise ValueError(f"{what} must be a contiguous {dtype} T x top_k tensor on X's device")
-    with _On(X.device, stream) as s:
-        Y = _i8_out(Y, (T, D), X.dtype, X.device, "Y")
-        key = (X.device.index, T, E, top_k, D, F)
-        n = _moe_work_bytes.get(key)
-        if n is None:
-            size = ctypes.c_size_t()
-            check(lib().bw_moe_work_bytes(T, E, top_k, D, F, ctypes.byref(size)))
-            if len(_moe_work_bytes) >= 4096:
-                _moe_work_bytes.clear()
-            n = _moe_work_bytes[key] = size.value
-        work = torch.empty(n, dtype=torch.uint8, device=X.device)
-        check(lib().bw_moe_mlp(X.data_ptr(), ld, R.data_ptr(), W1.data_ptr(), W2.data_ptr(), Y.data_ptr(), T, E, top_k, D, F,
-                               _types()[X.dtype], int(bool(renormalize)), ids.data_ptr() if ids is not None else None,
-                               weights.data_ptr() if weights is not None else None, work.data_ptr() if n else None, n, s))
-    return Y
+
+    def call(s):
+        out = _out(Y, X, T, D, X.dtype, "Y")
+        _t, work, n = _work("bw_moe_work_bytes", X, T, E, top_k, D, F)
+        check(lib().bw_moe_mlp(X.data_ptr(), ld, R.data_ptr(), W1.data_ptr(), W2.data_ptr(), out.data_ptr(), T, E, top_k, D,
+                               F, code, 1 if renormalize else 0, ids.data_ptr() if ids is not None else None,
+                               weights.data_ptr() if weights is not None else None, work, n, s))
+        return out
+
+    return _on(X.device, stream, call)
 
 
 def status():

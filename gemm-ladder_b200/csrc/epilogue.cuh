@@ -248,14 +248,29 @@ __device__ __forceinline__ void store_rows64_tma(const CUtensorMap* tmc, uint8_t
 
 // A whole tile of kEpiI8SwiGLU: silu(gate) * up from the scaled sums, in C's 16-bit type.  Columns of C come in groups
 // of 256 weight rows of B, 128 gate then 128 up.
-//   PAIR: accumulator columns [0, BN / 2) are gate, [BN / 2, BN) up, of row m0 + row: columns n0 / 2 + c of the M x N/2 C.
+//   PAIR: accumulator columns [0, 128) are gate, [128, 256) up, of row m0 + row: columns n0 / 2 + c of the M x N/2 C.
 //   SWAP (two weight blocks): lane `row` holds output column n0 / 2 + row; accumulator columns [0, BN) are its gate sums
 //   by token, [BN, 2 BN) its up sums.
 // The logistic takes the fast exponential: its relative error is within (2 + 1.16 |g|) 2^-23 by CUDA's bound, 1.3e-5
 // at the |g| = 88 where exp leaves fp32, against the 2^-8 (bf16) or 2^-11 (fp16) of the one rounding that follows.
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
-template <int BN, bool SWAP>
+// 16 tokens' activations of output column n0 / 2 + row (swap-AB), from the gate and up sums: a warp's 32 lanes write 64
+// contiguous bytes of each token's row.
+__device__ __forceinline__ void i8_swiglu_store16(const Params& p, const float (&g)[16], const float (&u)[16], int c0,
+                                                  int n0, int row, float gs, float us)
+{
+    __half* C = static_cast<__half*>(p.C) + (size_t)c0 * (p.s.N / 2) + n0 / 2 + row;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        if (c0 + j >= p.s.M) break;
+        const float rs = __ldg(p.row_scale + c0 + j);
+        C[(size_t)j * (p.s.N / 2)] =
+            half_bits<kEpiI8SwiGLU>(p, silu_mul(i8_value(g[j], rs, gs), i8_value(u[j], rs, us)));
+    }
+}
+
+template <bool SWAP, int BN>
 __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row)
 {
     const Sched& s = p.s;
@@ -263,10 +278,10 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
         const int m = m0 + row;
         const float rs = m < s.M ? __ldg(p.row_scale + m) : 0.f;
 #pragma unroll 1
-        for (int c0 = 0; c0 < BN / 2; c0 += 16) {
+        for (int c0 = 0; c0 < 128; c0 += 16) {
             uint32_t gr[16], ur[16];
             tmem_ld16(tbase + (uint32_t)c0, gr);
-            tmem_ld16(tbase + (uint32_t)(BN / 2 + c0), ur);
+            tmem_ld16(tbase + (uint32_t)(128 + c0), ur);
             tmem_wait_ld();
             if (m >= s.M || n0 >= s.N) continue;
             uint32_t h[8];
@@ -277,7 +292,7 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
                 for (int e = 0; e < 2; ++e) {
                     const int c = c0 + 2 * j + e;
                     a[e] = silu_mul(i8_value(__uint_as_float(gr[2 * j + e]), rs, __ldg(p.col_scale + n0 + c)),
-                                    i8_value(__uint_as_float(ur[2 * j + e]), rs, __ldg(p.col_scale + n0 + BN / 2 + c)));
+                                    i8_value(__uint_as_float(ur[2 * j + e]), rs, __ldg(p.col_scale + n0 + 128 + c)));
                 }
                 h[j] = pack2<kEpiI8SwiGLU>(p, a[0], a[1]);
             }
@@ -288,23 +303,19 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
     } else {
         const bool in = n0 < s.N;  // N % 256 == 0: a tile is in C or outside
         const float gs = in ? __ldg(p.col_scale + n0 + row) : 0.f, us = in ? __ldg(p.col_scale + n0 + 128 + row) : 0.f;
-        __half* C = static_cast<__half*>(p.C);
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 16) {
             uint32_t gr[16], ur[16];
             tmem_ld16(tbase + (uint32_t)c0, gr);
             tmem_ld16(tbase + (uint32_t)(BN + c0), ur);
             tmem_wait_ld();
-            // a warp's 32 lanes write 64 contiguous bytes of one token's row
+            float g[16], u[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const int m = c0 + j;
-                if (m < s.M && in) {
-                    const float rs = __ldg(p.row_scale + m);
-                    C[(size_t)m * (s.N / 2) + n0 / 2 + row] = half_bits<kEpiI8SwiGLU>(
-                        p, silu_mul(i8_value(__uint_as_float(gr[j]), rs, gs), i8_value(__uint_as_float(ur[j]), rs, us)));
-                }
+                g[j] = __uint_as_float(gr[j]);
+                u[j] = __uint_as_float(ur[j]);
             }
+            if (in) i8_swiglu_store16(p, g, u, c0, n0, row, gs, us);
         }
     }
 }
@@ -516,6 +527,57 @@ __device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, 
     }
     if (threadIdx.x == kEpiThread0) BW_TRACE_AT(11);
     return true;
+}
+
+// A split swap-AB tile of kEpiI8SwiGLU, by its last block: the gate and up sums of 16 tokens over the tile's partials (this
+// block's own from tensor memory when own_mine), exact in any order, then the activation.
+template <int BN>
+__device__ __noinline__ void i8_swiglu_reduce(const Params& p, int P, int tile, Fixup f, bool own_mine, uint32_t tbase,
+                                              int n0, int row)
+{
+    const Sched& s = p.s;
+    if (n0 >= s.N) return;
+    const float gs = __ldg(p.col_scale + n0 + row), us = __ldg(p.col_scale + n0 + 128 + row);
+#pragma unroll 1
+    for (int c0 = 0; c0 < BN; c0 += 16) {
+        if (c0 >= s.M) break;  // the last group's padding
+        float a[2][16];
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) a[w][j] = __int_as_float(0);
+        if (own_mine) {
+            uint32_t gr[16], ur[16];
+            tmem_ld16(tbase + (uint32_t)c0, gr);
+            tmem_ld16(tbase + (uint32_t)(BN + c0), ur);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                a[0][j] = __uint_as_float(gr[j]);
+                a[1][j] = __uint_as_float(ur[j]);
+            }
+        }
+#pragma unroll 2
+        for (int i = 0; i < f.nseg; ++i) {
+            if (own_mine && i == f.mine) continue;
+            const long long slot = fixup_slot(s, P, tile, f, i);
+            float4 v[2][4];
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[w][j] = __ldcg(slot_vec<2 * BN>(p, slot, row, (w * BN + c0) / 4 + j));
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[w][4 * j] = part_add<kEpiI8>(a[w][4 * j], v[w][j].x);
+                    a[w][4 * j + 1] = part_add<kEpiI8>(a[w][4 * j + 1], v[w][j].y);
+                    a[w][4 * j + 2] = part_add<kEpiI8>(a[w][4 * j + 2], v[w][j].z);
+                    a[w][4 * j + 3] = part_add<kEpiI8>(a[w][4 * j + 3], v[w][j].w);
+                }
+        }
+        i8_swiglu_store16(p, a[0], a[1], c0, n0, row, gs, us);
+    }
 }
 
 // ------------------------------------------------------------------ the fused reduce-scatter's epilogue

@@ -22,10 +22,24 @@ int i8_plan(DeviceState& d, int M, int N, int K, int epi, bw_plan* q)
     std::lock_guard<std::mutex> lock(g_mu);
     int rc = pair_occupancy(d);
     if (rc) return rc;
+    // the last plans, by shape (a plan depends on nothing else; making one takes a microsecond of the host's time)
+    struct Entry {
+        const DeviceState* d;
+        int M, N, K, epi;
+        bw_plan q;
+    };
+    static Entry cache[64];
+    Entry& at = cache[((unsigned)M * 31u + (unsigned)N / 64u * 7u + (unsigned)K / 16u + (unsigned)epi) % 64u];
+    if (at.d == &d && at.M == M && at.N == N && at.K == K && at.epi == epi) {
+        *q = at.q;
+        return BW_OK;
+    }
     const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap
-                           : epi == kEpiI8SwiGLU ? kPlanNoSplit | kPlanGateUp | (M > 128 ? kPlanNoSwap : 0u)
-                                                 : kPlanNoStage;
-    return make_plan(M, N, (K + 127) / 128 * 64, d.sms, d.pairs, 0, q, flags, held_of(d));
+                           : epi == kEpiI8SwiGLU ? kPlanGateUp | kPlanI8 | (M > 128 ? kPlanNoSplit : 0u)
+                                                 : kPlanI8;
+    if ((rc = make_plan(M, N, (K + 127) / 128 * 64, d.sms, d.pairs, 0, q, flags, held_of(d)))) return rc;
+    at = {&d, M, N, K, epi, *q};
+    return BW_OK;
 }
 
 // The workspace of a call: [linear: the quantised rows, their scales][partials of split tiles][their counters].
@@ -126,6 +140,7 @@ int i8_product(DeviceState& d, const bw_plan& q, const I8Work& w, const void* A,
     p.row_scale = a_scale;
     p.col_scale = b_scale;
     p.out_bf16 = bf16 ? 1 : 0;
+    p.early_weights = zeroed ? 1 : 0;
     return i8_dispatch(d, q, mx, my, p, st, epi, zeroed);
 }
 
@@ -169,25 +184,22 @@ int i8_gemm(const void* A, const void* a_scale, const void* B, const void* b_sca
                       epi, out_type == BW_TYPE_BF16, static_cast<uint8_t*>(work), false, st);
 }
 
-// The quantiser's instance: a warp per row up to 2048 elements, a block of 512 threads above, with as many 16-byte
-// vectors per thread in registers as the row needs (measured on rows of 8192 to 28672: one pass from memory).
+// The quantiser's instance: a warp per row up to 2048 elements, else a block whose threads hold 8 of the row's 16-byte
+// vectors each: 128 threads up to 8192 elements (more, smaller blocks per SM; many threads with few vectors each lose
+// to the blocks' fixed cost: 8192 x 8192 took 62 us with 512 threads where 128 took 50), 512 above.
 template <bool BF16>
 void quant_launch(const QuantParams& p, cudaStream_t st)
 {
     const int nv = p.cols / 8;
-    if (nv <= 256) {
-        const dim3 grid((p.rows + 7) / 8);
-        if (nv <= 64)
-            quant_rows_kernel<BF16, 32, 2><<<grid, 256, 0, st>>>(p);
-        else
-            quant_rows_kernel<BF16, 32, 8><<<grid, 256, 0, st>>>(p);
-    } else if (nv <= 512 * 2) {
-        quant_rows_kernel<BF16, 512, 2><<<p.rows, 512, 0, st>>>(p);
-    } else if (nv <= 512 * 4) {
-        quant_rows_kernel<BF16, 512, 4><<<p.rows, 512, 0, st>>>(p);
-    } else {
+    const dim3 warp_rows((p.rows + 7) / 8);
+    if (nv <= 64)
+        quant_rows_kernel<BF16, 32, 2><<<warp_rows, 256, 0, st>>>(p);
+    else if (nv <= 256)
+        quant_rows_kernel<BF16, 32, 8><<<warp_rows, 256, 0, st>>>(p);
+    else if (nv <= 1024)
+        quant_rows_kernel<BF16, 128, 8><<<p.rows, 128, 0, st>>>(p);
+    else
         quant_rows_kernel<BF16, 512, 8><<<p.rows, 512, 0, st>>>(p);
-    }
 }
 
 int quant_rows(const void* X, int x_type, long long ld, void* Q, void* scale, int rows, int cols, int* zero, int zero_n,

@@ -145,7 +145,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    // nothing above touches global memory: from here on the call ahead of this one (operands, counters, status word,
+    // kEpiI8*: the weights may be complete already (early_weights); their first stages are then on their way before the
+    // wait, while the kernel ahead quantises the tokens
+    int early = 0;
+    if constexpr (epi_i8(EPI) && SWAP) {
+        if (p.early_weights && threadIdx.x == 0) {
+            SegIter it(s, c, P);
+            Seg sg;
+            const uint64_t pol_sb = BW_SWAP_HINT_B ? l2_policy(BW_SWAP_HINT_B) : 0ull;
+            while (early < S && it.next(s, P, sg))
+                for (int kb = sg.k0; kb < sg.k1 && early < S; ++kb, ++early) {
+                    mbar_arrive_expect_tx(&full[early], G::kStageBytes);
+                    load_tile<PAIR, BW_SWAP_HINT_B>(smem + early * G::kStageBytes, &tmx, kb * kBK, sg.tile * 128 * WM,
+                                                    &full[early], 0u, pol_sb);
+                }
+        }
+    }
+    // nothing else above touches global memory: from here on the call ahead of this one (operands, counters, status word,
     // workspace) has finished and its writes are visible
     griddep_wait();
     if (threadIdx.x == 0) BW_TRACE_AT(1);
@@ -197,7 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint8_t* sy = sx + G::kXBytes;
                     // both blocks of a pair complete their halves on the leader's barrier, which expects them all
                     const uint32_t barc = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : 0u;
-                    if (!PAIR || leader) mbar_arrive_expect_tx(&full[stage], R * G::kStageBytes);
+                    const bool early_stage = epi_i8(EPI) && SWAP && issued < early;  // expected and its weights loaded
+                    if (!early_stage) {
+                        if (!PAIR || leader) mbar_arrive_expect_tx(&full[stage], R * G::kStageBytes);
+                    }
                     if (!SWAP) {
                         // A: 64 K x 128 rows (this block's rows of a pair tile)
                         load_tile<PAIR, BW_HINT_A>(sx, &tmx, kb * kBK, tm * G::kTileM + rank * 128, &full[stage], barc,
@@ -223,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // this block's weight columns (a pair: block r holds the tile's r-th run of 128 x WM), and
                         // its tokens (a pair: block r the r-th half of the BN, the MMA's N split over the pair)
                         const int wcol = (tn * R + rank) * 128 * WM;
-                        if (p.tn) {  // B (N x K): 128 (x WM) rows of B, 64 K each, one load
+                        if (early_stage) {
+                        } else if (p.tn) {  // B (N x K): 128 (x WM) rows of B, 64 K each, one load
                             load_tile<PAIR, BW_SWAP_HINT_B>(sx, &tmx, kb * kBK, wcol, &full[stage], barc, pol_sb);
                         } else if (BW_TMA3D) {  // B: 128 (x WM) columns, one load
                             load_blocks<PAIR, BW_SWAP_HINT_B>(sx, &tmx, wcol / 64, kb * kBK, &full[stage], barc, pol_sb);
@@ -248,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // this thread's abort, and after an abort elsewhere that left its last stages unconsumed (on the normal
             // path they have all landed: no wait)
             if (leader) {
+                if (issued < early) issued = early;
                 const int n = issued < S ? issued : S;
                 for (int i = 1; i <= n; ++i) {
                     const int q = issued - i;
@@ -503,9 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 rs_tile(p, rs_epoch, tm, tn, rank, tbase, row, lane, q, abort_flag, recv_flag, reduce_flag, rs_acked,
                         smem + G::kWindowOffset, rbar, krecv, win_ph, win_next, seg);
                 release_all(acc);
-            } else if constexpr (EPI == kEpiI8SwiGLU) {
-                i8_swiglu_tile<BN, SWAP>(p, tbase, m0, n0, row);
-                release_all(acc);
+            } else if (EPI == kEpiI8SwiGLU && sg.k0 == 0 && sg.k1 == s.kblocks) {
+                if constexpr (EPI == kEpiI8SwiGLU) {
+                    i8_swiglu_tile<SWAP, BN>(p, tbase, m0, n0, row);
+                    release_all(acc);
+                }
             } else if (EPI == kEpiSwiGLU) {
                 // a whole tile (the plan splits none): gate columns [0, BN/2), up columns [BN/2, BN) of the tile,
                 // silu(gate) * up to columns [n0 / 2, n0 / 2 + BN / 2) of the M x N/2 output
@@ -746,7 +769,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     BW_TRACE_VAL(8, (fast == 2 ? 2 : 3) | f.nseg << 8 | seg << 16);
                 }
                 if (fast == 2) {
-                    if (bulk)
+                    if constexpr (EPI == kEpiI8SwiGLU && SWAP)
+                        i8_swiglu_reduce<BN>(p, P, sg.tile, f, true, tbase, n0, row);
+                    else if (bulk)
                         reduce_tile_bulk<AN, SWAP, R, G::kMaxSum, EPI, BN>(p, P, sg.tile, rank, f, true, tbase, row, m0, n0,
                                                                   cst, smem, rbar, abort_flag, seg);
                     else
@@ -783,7 +808,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             BW_TRACE_AT(9);
                             BW_TRACE_VAL(8, 1 | f.nseg << 8 | seg << 16);
                         }
-                        if (bulk)
+                        if constexpr (EPI == kEpiI8SwiGLU && SWAP)
+                            i8_swiglu_reduce<BN>(p, P, sg.tile, f, last_seg, tbase, n0, row);
+                        else if (bulk)
                             reduce_tile_bulk<AN, SWAP, R, G::kMaxSum, EPI, BN>(p, P, sg.tile, rank, f, true, tbase, row, m0, n0,
                                                                       cst, smem, rbar, abort_flag, seg);
                         else

@@ -68,6 +68,8 @@ struct Params {
     const float* row_scale;      // kEpiI8*: M scales of A's rows
     const float* col_scale;      // kEpiI8*: N scales of B's rows (C's columns)
     int out_bf16;                // kEpiI8, kEpiI8SwiGLU: C in bf16 (0: fp16)
+    int early_weights;           // kEpiI8* swap-AB: the weights were complete before the kernel this one waits for
+                                 // (griddep_wait) began, so their first loads need not wait for it
 };
 
 __host__ __device__ constexpr int pow2_at_least(int v, int p) { return p >= v ? p : pow2_at_least(v, 2 * p); }

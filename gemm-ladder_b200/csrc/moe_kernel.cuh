@@ -18,8 +18,8 @@
 //   - between the products a block waits for the activations it needs, by active expert, but only its token-side loads
 //     do: the weights of W2 are already on their way into the ring (up to 200 KB per SM, 30 MB in all), so the wait
 //     costs no memory time.
-// One thread per role: warp 0 the weights' producer, warp 6 the tokens' (both arrive on a stage's full barrier), warp 1
-// the MMA issuer, warps 2-5 the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
+// Roles: one thread of warp 0 the weights' producer, one of warp 10 the tokens', one of warp 1 the MMA issuer, warps 2-9
+// the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
 // resident); every wait is bounded (ptx.cuh).
 //
 // Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32), y once at the end; sums in fp32.
@@ -33,7 +33,8 @@
 
 namespace bw {
 
-constexpr int kMoeThreads = 224;  // 7 warps
+constexpr int kMoeThreads = 352;  // 11 warps
+constexpr int kMoeEpiThreads = 256;
 constexpr int kMoeXBytes = 32768; // a stage's weights: 256 rows x 64 values
 constexpr int kMoeMaxStages = 6;
 constexpr int kMoeEpiThread0 = 64;
@@ -109,6 +110,101 @@ __device__ __forceinline__ uint16_t moe_bits16(float v, int bf16)
     return *reinterpret_cast<const uint16_t*>(&h);
 }
 
+// The other blocks' parts of a split tile added to this block's own (a: the two weight blocks' rows, 8 tokens from c0),
+// all in block order so that the bits do not depend on who is last; up to four parts' loads in flight.
+__device__ __forceinline__ void moe_sum_parts(const MoeParams& p, const MoeSeg& g, int c, int row, int c0, int tq,
+                                              float (&a)[2][8])
+{
+    float own[2][8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            own[w][j] = a[w][j];
+            a[w][j] = 0.f;
+        }
+#pragma unroll 1
+    for (int b0 = g.first; b0 < g.first + g.nseg; b0 += 4) {
+        float4 v[4][2][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = b0 + i;
+            if (b >= g.first + g.nseg || b == c) continue;
+            const float4* src = reinterpret_cast<const float4*>(p.partials + (size_t)moe_slot(g, b) * p.slot_floats) + row;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (c0 + 4 * j < p.T) v[i][w][j] = __ldcg(src + (size_t)(w * tq + c0 / 4 + j) * 128);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = b0 + i;
+            if (b >= g.first + g.nseg) break;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (b == c) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) a[w][4 * j + e] += own[w][4 * j + e];
+                    } else if (c0 + 4 * j < p.T) {
+                        a[w][4 * j] += v[i][w][j].x;
+                        a[w][4 * j + 1] += v[i][w][j].y;
+                        a[w][4 * j + 2] += v[i][w][j].z;
+                        a[w][4 * j + 3] += v[i][w][j].w;
+                    }
+                }
+        }
+    }
+}
+
+__device__ __forceinline__ float moe_shfl_xor(float v, int m)
+{
+    return __uint_as_float(__shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(v), m));
+}
+
+// This block's part of the sum of a split down tile: items (four tokens of one column) [n mine / nseg, n (mine + 1) /
+// nseg) of the tile's n.  With few tokens there are fewer items than threads: 2^ls lanes then share an item, each
+// adding every 2^ls-th part in block order, and their sums meet in a tree (ls depends on the sizes alone).
+__device__ __noinline__ void moe_sum_down(const MoeParams& p, const MoeSeg& g, int c, int tq, int tid, int lane)
+{
+    const int items = 2 * tq * 128, mine = c - g.first;
+    const int i0 = (int)((long long)items * mine / g.nseg), i1 = (int)((long long)items * (mine + 1) / g.nseg);
+    int ls = 0;
+    while (ls < 5 && (1 << ls) < g.nseg && ((i1 - i0) << (ls + 1)) <= kMoeEpiThreads) ++ls;
+    const int per = 32 >> ls, sub = lane / per;  // items per warp; this lane's share of its item
+    for (int base = i0 + (tid >> 5) * per; base < i1; base += (kMoeEpiThreads / 32) * per) {
+        const int x = base + lane % per;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (x < i1) {
+#pragma unroll 16
+            for (int b = g.first + sub; b < g.first + g.nseg; b += 1 << ls) {
+                const float4 u =
+                    __ldcg(reinterpret_cast<const float4*>(p.partials + (size_t)moe_slot(g, b) * p.slot_floats) + x);
+                v.x += u.x;
+                v.y += u.y;
+                v.z += u.z;
+                v.w += u.w;
+            }
+        }
+        for (int m = 16; m >= per; m >>= 1) {
+            v.x += moe_shfl_xor(v.x, m);
+            v.y += moe_shfl_xor(v.y, m);
+            v.z += moe_shfl_xor(v.z, m);
+            v.w += moe_shfl_xor(v.w, m);
+        }
+        const int w = x / (tq * 128), t0 = (x - w * tq * 128) / 128 * 4;
+        const int d = g.tile * 256 + w * 128 + (x & 127);
+        if (x >= i1 || sub || d >= p.D) continue;
+        uint16_t* dst = p.Y + (size_t)t0 * p.D + d;
+        dst[0] = moe_bits16(v.x, p.bf16);
+        if (t0 + 1 < p.T) dst[(size_t)p.D] = moe_bits16(v.y, p.bf16);
+        if (t0 + 2 < p.T) dst[2 * (size_t)p.D] = moe_bits16(v.z, p.bf16);
+        if (t0 + 3 < p.T) dst[3 * (size_t)p.D] = moe_bits16(v.w, p.bf16);
+    }
+}
+
 // kind::f16 with fp16 (format 0) or bf16 (format 1) operands, both K-major, fp32 accumulators.
 __device__ __forceinline__ uint32_t moe_idesc(int n, int bf16)
 {
@@ -138,7 +234,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMisc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* epi_go = abort_flag + 1;    // two slots, alternating by segment
-    volatile int* epi_last = abort_flag + 3;  // the outcome of a split tile's count or wait
+    volatile int* epi_sum = abort_flag + 3;   // two slots: this block sums the segment's tile
+    volatile int* epi_pend = abort_flag + 5;  // two slots: a split down tile's parts are all there
     uint32_t* mask = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMask);
     uint16_t* expert = reinterpret_cast<uint16_t*>(misc + MoeSmem::kExpert);
     float* gate = reinterpret_cast<float*>(misc + MoeSmem::kGate);
@@ -149,6 +246,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     while (tmem_cols < 4 * Tp) tmem_cols *= 2;
 
     if (threadIdx.x == 0) {
+        for (int i = 1; i < 12; ++i) BW_TRACE_VAL(i, 0);  // (12 to 15 are the router's)
+        BW_TRACE_AT(0);
         for (int i = 0; i < S; ++i) {
             mbar_init(&wfull[i], 1);  // the producer's arrive.expect_tx
             mbar_init(&xfull[i], 1);
@@ -156,7 +255,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], 4);  // one arrival per epilogue warp
+            mbar_init(&tempty[i], kMoeEpiThreads / 32);  // one arrival per epilogue warp
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -178,8 +277,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    // nothing above touches global memory: from here on the router has finished
-    griddep_wait();
+    if (threadIdx.x == 0) BW_TRACE_AT(1);
 
     // the experts that some token chose, in index order
     for (int i = threadIdx.x; i < p.T * p.top_k; i += kMoeThreads) {
@@ -197,6 +295,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     }
     __syncthreads();
     const MoeSched s = moe_sched(p.T, p.D, p.F, active, gridDim.x);
+    if (threadIdx.x == 0) BW_TRACE_AT(3);
 
     if (warp == 0) {
         // ---------------------------------------------------------- the weights' producer
@@ -234,7 +333,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             }
             moe_drain(wfull, issued, S, p.wait_ns);
         }
-    } else if (warp == 6) {
+    } else if (warp == 10) {
         // ---------------------------------------------------------- the tokens' producer
         if (lane == 0) {
             MoeIter it(s, c);
@@ -277,6 +376,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         // ---------------------------------------------------------- the MMA issuer
         if (lane == 0) {
             const uint32_t idesc = moe_idesc(Tp, p.bf16);
+#ifdef BW_TRACE
+            bool in_down = false;
+#endif
             MoeIter it(s, c);
             MoeSeg sg;
             int stage = 0, acc = 0, seg = 0;
@@ -292,6 +394,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         ok = false;
                         break;
                     }
+#ifdef BW_TRACE
+                    if (seg == 0 && kb == sg.k0) BW_TRACE_AT(4);     // the first weights are in
+                    if (sg.phase == 1 && !in_down) BW_TRACE_AT(6);   // the first activations are in
+                    in_down = sg.phase == 1;
+                    if (!in_down) BW_TRACE_AT(5);                    // the last gate/up stage
+                    else BW_TRACE_AT(7);                             // the last down stage
+#endif
                     tc_fence_after();
                     const uint32_t sx = smem_u32(smem + (size_t)stage * p.stage_bytes), sy = sx + kMoeXBytes;
 #pragma unroll
@@ -320,7 +429,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         __syncwarp();
     } else {
         // ---------------------------------------------------------- the epilogue
+        // warps 2-9: two per quarter of the TMEM lanes, taking turns at the groups of 8 tokens
         const int q = warp & 3, row = q * 32 + lane;  // the TMEM lane: a row of each of the stage's two weight blocks
+        const int half = (warp - 2) >> 2;
         const int tq = (p.T + 3) / 4;                 // groups of four tokens
         const int tid = threadIdx.x - kMoeEpiThread0;
         MoeIter it(s, c);
@@ -332,104 +443,86 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         auto slot_of = [&](int blk, const MoeSeg& g) {
             return reinterpret_cast<float4*>(p.partials + (size_t)moe_slot(g, blk) * p.slot_floats);
         };
-        auto release = [&] {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[acc]);
-        };
         while (it.next(s, sg)) {
-            if (threadIdx.x == kMoeEpiThread0)
+            int* counter = p.counters + moe_counter(sg);
+            const int sl = sg.tile / s.f_tiles, f = sg.tile % s.f_tiles * 128 + row;  // (gate/up)
+            if (sg.phase == 0 && sl != gate_slot) {  // p of every token for this expert, while the MMAs run
+                named_bar_sync(1, kMoeEpiThreads);   // the previous expert's have been read
+                if (tid < p.T) {
+                    const int e = expert[sl];
+                    float v = 0.f;
+                    for (int j = 0; j < p.top_k; ++j) {
+                        const float pr = p.weights[tid * p.top_k + j];
+                        if (p.ids[tid * p.top_k + j] == e) v = pr;
+                    }
+                    gate[tid] = v;  // (read after the barrier below)
+                }
+                gate_slot = sl;
+            }
+            if (threadIdx.x == kMoeEpiThread0) {
                 epi_go[seg & 1] = wait_bounded(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, acc), seg) ? 1 : 0;
-            named_bar_sync(1, 128);
+                // a split gate/up tile whose other parts are all there is summed here, without writing this one
+                epi_sum[seg & 1] = sg.nseg == 1 || (sg.phase == 0 && ld_acquire_gpu(counter) == sg.nseg - 1) ? 1 : 0;
+            }
+            named_bar_sync(1, kMoeEpiThreads);
             if (epi_go[seg & 1] != 1) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 2 * Tp);
-            bool sum_here = sg.nseg == 1;  // this block has (or gathers) the whole sums of the tile
-            if (sg.nseg > 1) {
+            bool sum_here = epi_sum[seg & 1] != 0;
+            if (!sum_here) {
                 float4* dst = slot_of(c, sg) + row;
 #pragma unroll 1
-                for (int w = 0; w < 2; ++w)
-#pragma unroll 1
-                    for (int c0 = 0; c0 < p.T; c0 += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(tbase + (uint32_t)(w * Tp + c0), r);
-                        tmem_wait_ld();
+                for (int c0 = 8 * half; c0 < p.T; c0 += 16) {
+                    uint32_t r[2][8];
+                    tmem_ld8(tbase + (uint32_t)c0, r[0]);
+                    tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
                             if (c0 + 4 * j < p.T)
                                 __stcg(dst + (size_t)(w * tq + c0 / 4 + j) * 128,
-                                       make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                                   __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
-                    }
-                __threadfence();
-                named_bar_sync(1, 128);
+                                       make_float4(__uint_as_float(r[w][4 * j]), __uint_as_float(r[w][4 * j + 1]),
+                                                   __uint_as_float(r[w][4 * j + 2]), __uint_as_float(r[w][4 * j + 3])));
+                }
+                named_bar_sync(1, kMoeEpiThreads);  // every thread's part is written (and epi_sum read)
                 if (threadIdx.x == kMoeEpiThread0) {
-                    const int old = atomicAdd(p.counters + moe_counter(sg), 1);
+                    __threadfence();  // cumulative: the other threads' stores, ordered before by the barrier, too
+                    const int old = atomicAdd(counter, 1);
                     __threadfence();
-                    *epi_last = old == sg.nseg - 1 ? 1 : 0;
+                    epi_sum[seg & 1] = sg.phase == 0 && old == sg.nseg - 1 ? 1 : 0;
                 }
                 if (sg.phase == 0) {  // the last block of a split gate/up tile sums it
-                    named_bar_sync(1, 128);
-                    sum_here = *epi_last != 0;
+                    named_bar_sync(1, kMoeEpiThreads);
+                    sum_here = epi_sum[seg & 1] != 0;
                 } else {
                     pend[n_pend++] = sg;  // a split down tile is summed below, by all its blocks
                 }
             }
             if (sum_here) {
-                const int sl = sg.tile / s.f_tiles, f = sg.tile % s.f_tiles * 128 + row;
-                if (sg.phase == 0 && sl != gate_slot) {  // p of every token for this expert
-                    named_bar_sync(1, 128);              // the previous expert's have been read
-                    if (tid < p.T) {
-                        const int e = expert[sl];
-                        float v = 0.f;
-                        for (int j = 0; j < p.top_k; ++j)
-                            if (p.ids[tid * p.top_k + j] == e) v = p.weights[tid * p.top_k + j];
-                        gate[tid] = v;
-                    }
-                    gate_slot = sl;
-                    named_bar_sync(1, 128);
-                }
 #pragma unroll 1
-                for (int c0 = 0; c0 < p.T; c0 += 16) {
-                    float a[2][16];
-                    if (sg.nseg == 1) {
-                        uint32_t r[2][16];
-                        tmem_ld16(tbase + (uint32_t)c0, r[0]);
-                        tmem_ld16(tbase + (uint32_t)(Tp + c0), r[1]);
+                for (int c0 = 8 * half; c0 < p.T; c0 += 16) {
+                    float a[2][8];
+                    {
+                        uint32_t r[2][8];
+                        tmem_ld8(tbase + (uint32_t)c0, r[0]);
+                        tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
                         tmem_wait_ld();
 #pragma unroll
                         for (int w = 0; w < 2; ++w)
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) a[w][j] = __uint_as_float(r[w][j]);
-                    } else {
-#pragma unroll
-                        for (int w = 0; w < 2; ++w)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) a[w][j] = 0.f;
-#pragma unroll 1
-                        for (int b = sg.first; b < sg.first + sg.nseg; ++b) {  // in block order
-                            const float4* src = slot_of(b, sg) + row;
-#pragma unroll
-                            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    if (c0 + 4 * j >= p.T) continue;
-                                    const float4 v = __ldcg(src + (size_t)(w * tq + c0 / 4 + j) * 128);
-                                    a[w][4 * j] += v.x;
-                                    a[w][4 * j + 1] += v.y;
-                                    a[w][4 * j + 2] += v.z;
-                                    a[w][4 * j + 3] += v.w;
-                                }
-                        }
+                            for (int j = 0; j < 8; ++j) a[w][j] = __uint_as_float(r[w][j]);
                     }
+                    if (sg.nseg > 1) moe_sum_parts(p, sg, c, row, c0, tq, a);
                     if (sg.phase == 0) {
                         if (f < p.F) {
                             uint16_t* dst = p.H + ((size_t)sl * p.T + c0) * p.F + f;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
+                            for (int j = 0; j < 8; ++j) {
                                 if (c0 + j >= p.T) break;
                                 const float pr = gate[c0 + j];
                                 // a token that did not choose the expert contributes nothing, whatever its products
@@ -443,62 +536,43 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                             const int d = sg.tile * 256 + w * 128 + row;
                             if (d >= p.D) continue;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
+                            for (int j = 0; j < 8; ++j)
                                 if (c0 + j < p.T) p.Y[(size_t)(c0 + j) * p.D + d] = moe_bits16(a[w][j], p.bf16);
                         }
                     }
                 }
                 if (sg.phase == 0) {
-                    __threadfence();  // h before the count
-                    named_bar_sync(1, 128);
+                    named_bar_sync(1, kMoeEpiThreads);
                     if (threadIdx.x == kMoeEpiThread0) {
-                        __threadfence();
+                        __threadfence();  // h before the count
                         atomicAdd(p.ready + sl, 1);
+                        BW_TRACE_AT(8);  // this block's last gate/up tile is done
                     }
                 }
             }
-            release();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);  // the accumulator is read
             if (++acc == 2) {
                 acc = 0;
                 aph ^= 1u;
             }
             ++seg;
         }
+        if (threadIdx.x == kMoeEpiThread0) BW_TRACE_AT(9);  // this block's partials are written
         // the split down tiles (at most two per block): every block of a tile sums a part of it once all have written
         // theirs.  A block writes its own partials before it waits for any, so no wait can close a circle.
         for (int i = 0; ok && i < n_pend; ++i) {
             const MoeSeg& g = pend[i];
             if (threadIdx.x == kMoeEpiThread0)
-                *epi_last = moe_wait_count(p.counters + moe_counter(g), g.nseg, abort_flag, p.wait_ns,
-                                           site(2, 11, g.first & 255), seg)
-                                ? 1
-                                : 0;
-            named_bar_sync(1, 128);
-            ok = *epi_last != 0;
-            named_bar_sync(1, 128);
-            if (!ok) break;
-            __threadfence();
-            const int items = 2 * tq * 128, mine = c - g.first;
-            const int i1 = (int)((long long)items * (mine + 1) / g.nseg);
-            for (int x = (int)((long long)items * mine / g.nseg) + tid; x < i1; x += 128) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                for (int b = g.first; b < g.first + g.nseg; ++b) {
-                    const float4 u = __ldcg(slot_of(b, g) + x);
-                    v.x += u.x;
-                    v.y += u.y;
-                    v.z += u.z;
-                    v.w += u.w;
-                }
-                const int w = x / (tq * 128), t0 = (x - w * tq * 128) / 128 * 4;
-                const int d = g.tile * 256 + w * 128 + (x & 127);
-                if (d >= p.D) continue;
-                uint16_t* dst = p.Y + (size_t)t0 * p.D + d;
-                dst[0] = moe_bits16(v.x, p.bf16);
-                if (t0 + 1 < p.T) dst[(size_t)p.D] = moe_bits16(v.y, p.bf16);
-                if (t0 + 2 < p.T) dst[2 * (size_t)p.D] = moe_bits16(v.z, p.bf16);
-                if (t0 + 3 < p.T) dst[3 * (size_t)p.D] = moe_bits16(v.w, p.bf16);
-            }
+                epi_pend[i] = moe_wait_count(p.counters + moe_counter(g), g.nseg, abort_flag, p.wait_ns,
+                                             site(2, 11, g.first & 255), seg)
+                                  ? 1
+                                  : 0;
+            named_bar_sync(1, kMoeEpiThreads);
+            ok = epi_pend[i] != 0;
+            if (threadIdx.x == kMoeEpiThread0) BW_TRACE_AT(10);  // the others' partials are in
+            if (ok) moe_sum_down(p, g, c, tq, tid, lane);
         }
     }
 
@@ -510,6 +584,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem_base, (uint32_t)tmem_cols);
     }
+    if (threadIdx.x == 0) BW_TRACE_AT(11);
 }
 
 }  // namespace bw

@@ -46,17 +46,23 @@ int moe_shape(int T, int E, int top_k, int D, int F)
 // The blocks of the experts kernel: one per SM (its shared memory allows one).
 int moe_grid(const DeviceState& d) { return d.sms; }
 
+template <bool BF16, int TG>
+void router_launch(const RouterParams& r, cudaStream_t st)
+{
+    const int grid = kRouterBlocks * ((r.T + TG - 1) / TG);
+    if (r.E <= 128)
+        moe_router_kernel<BF16, TG, 4><<<grid, kRouterThreads, 0, st>>>(r);
+    else
+        moe_router_kernel<BF16, TG, 16><<<grid, kRouterThreads, 0, st>>>(r);
+}
+// A token per cluster up to 16 tokens, where the clusters fit the GPU at once; 4 above, for the reuse of R.
 template <bool BF16>
 cudaError_t router_launch(const RouterParams& r, cudaStream_t st)
 {
-    // a token per cluster up to 4 tokens (R is small and read from L2 by the later clusters; the chain per warp is what
-    // counts), then 4 and 8 tokens per cluster: fewer reads of R per token once the clusters fill the GPU
-    if (r.T <= 4)
-        moe_router_kernel<BF16, 1><<<kRouterBlocks * r.T, kRouterThreads, 0, st>>>(r);
-    else if (r.T <= 32)
-        moe_router_kernel<BF16, 4><<<kRouterBlocks * ((r.T + 3) / 4), kRouterThreads, 0, st>>>(r);
+    if (r.T <= 16)
+        router_launch<BF16, 1>(r, st);
     else
-        moe_router_kernel<BF16, 8><<<kRouterBlocks * ((r.T + 7) / 8), kRouterThreads, 0, st>>>(r);
+        router_launch<BF16, 4>(r, st);
     return cudaGetLastError();
 }
 
@@ -118,8 +124,8 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
         done.store(true, std::memory_order_release);
     }
 
-    RouterParams r = {static_cast<const uint16_t*>(X), ldx, static_cast<const uint16_t*>(R), T, E, top_k, D, renormalize,
-                      ids, weights, p.ready, w.zero_words};
+    RouterParams r = {static_cast<const uint16_t*>(X), ldx, static_cast<const uint16_t*>(R), T, E, top_k, D,
+                      router_ranges(E), renormalize, ids, weights, p.ready, w.zero_words};
     e = p.bf16 ? router_launch<true>(r, st) : router_launch<false>(r, st);
     if (e != cudaSuccess) return cuda_fail(e, "kernel launch (router)");
 
@@ -128,13 +134,14 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     cfg.blockDim = dim3(kMoeThreads);
     cfg.dynamicSmemBytes = (size_t)moe_smem_bytes(p.Tp);
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeCooperative;  // the blocks wait for one another: all of them resident
+    // the blocks wait for one another, so all of them have to be resident.  (A cooperative launch does not overlap the
+    // router's end: measured, programmatic serialisation has no effect on it; without the cooperative attribute it saves
+    // 3.7 us a call, but then two overlapping calls could each hold SMs the other needs.)
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
     attr[0].val.cooperative = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // their set-up overlaps the router
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = BW_MOE_PDL ? 2 : 1;
+    cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, moe_experts_kernel, m1, m2, mx, mh, p);
     if (e != cudaSuccess) return cuda_fail(e, "kernel launch (experts)");
     return BW_OK;

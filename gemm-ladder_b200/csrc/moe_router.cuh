@@ -2,17 +2,20 @@
 // top_k experts of each token by logit (equal logits: the lower index), their softmax weights.
 //
 // A latency-bound kernel (E D values of R, 1 MB at 128 experts of 4096, and a choice per token), so its work is spread
-// for short chains rather than few bytes: a cluster of 8 blocks takes TG tokens, its 64 warps the experts (a warp two
-// at a time, lanes along D, 16-byte loads), the logits go to the block of the cluster that chooses for the token
-// through distributed shared memory, and one warp per token picks: no counters, no second kernel, R read once per TG
-// tokens (from L2 after the first).
-// The sums are 32 chains of D / 32 products, exact in fp32, added in fp32, then a tree: the choice between two experts
-// can differ from the exact one only where their logits agree to about 2^-21 of the products' magnitude.
+// for short chains: a cluster of 8 blocks takes TG tokens; each of its 128 warps takes four experts and one of `ds`
+// ranges of D (as many ranges as the experts leave warps for), so that a value of X or R is unpacked once for four
+// products and a warp's loads are all in flight at once.  The ranges are summed in shared memory, the logits go to the
+// block of the cluster that chooses for the token through distributed shared memory, and one warp per token picks: no
+// counters, no second kernel.
+// The sums are chains of fp32 additions of products that are exact in fp32 (22 bits), short ones (D / (32 ds)), then a
+// tree: the choice between two experts can differ from the exact one only where their logits agree to about 2^-21 of
+// the products' magnitude.
 // It also clears the words that the experts kernel counts on.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "kernel_common.cuh"
 #include "moe_sched.h"
 #include "quant_rows.cuh"
 
@@ -23,6 +26,7 @@ struct RouterParams {
     long long ldx;
     const uint16_t* R;  // E x D
     int T, E, top_k, D;
+    int ranges;         // router_ranges(E)
     int renormalize;    // 1: the weights' sum over the chosen experts is 1; 0: the softmax is over all experts
     int* ids;           // T x top_k, by falling logit
     float* weights;
@@ -30,8 +34,19 @@ struct RouterParams {
     int zero_words;
 };
 
-constexpr int kRouterBlocks = 8;  // of a cluster
-constexpr int kRouterThreads = 256;
+constexpr int kRouterBlocks = 8;     // of a cluster
+constexpr int kRouterThreads = 512;
+constexpr int kRouterWarps = kRouterThreads / 32;
+constexpr int kRouterTE = 4;         // experts of a warp
+
+// The ranges of D (a power of two up to a block's warps) that E experts leave warps for.
+__host__ __device__ inline int router_ranges(int E)
+{
+    const int groups = (E + kRouterTE - 1) / kRouterTE;
+    int ds = kRouterWarps;
+    while (ds > 1 && kRouterBlocks * (kRouterWarps / ds) < groups) ds >>= 1;
+    return ds;
+}
 
 // Larger logits get larger keys; 0 is below every key (NaN, of either sign, is above every number).
 __device__ __forceinline__ uint32_t router_key(float v)
@@ -41,73 +56,89 @@ __device__ __forceinline__ uint32_t router_key(float v)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-template <bool BF16, int TG>
-__global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterThreads)
+// TG tokens per cluster; up to 32 PER experts.
+template <bool BF16, int TG, int PER>
+__global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterThreads, 2)
     moe_router_kernel(const RouterParams p)
 {
-    __shared__ float logits[kMoeMaxExperts];  // of the token this block chooses for
-    griddep_launch();
-    griddep_wait();
+    __shared__ float logits[32 * PER];  // of the token this block chooses for
+    if (threadIdx.x == 0) BW_TRACE_AT(12);
     for (int i = blockIdx.x * kRouterThreads + threadIdx.x; i < p.zero_words; i += gridDim.x * kRouterThreads)
         p.zero[i] = 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     const int t0 = blockIdx.x / kRouterBlocks * TG;
-    const int warps = kRouterBlocks * (kRouterThreads / 32);
-    const int nv = p.D / 8;
-    for (int e = rank * (kRouterThreads / 32) + warp; e < p.E; e += 2 * warps) {
-        const bool two = e + warps < p.E;
-        const uint4* r0 = reinterpret_cast<const uint4*>(p.R + (size_t)e * p.D);
-        const uint4* r1 = reinterpret_cast<const uint4*>(p.R + (size_t)(two ? e + warps : e) * p.D);
-        float acc[2][TG];
+    constexpr int TE = kRouterTE, NV = TE * TG;
+    __shared__ float part[kRouterWarps][NV];  // the warps' sums
+    const int ds = p.ranges, gpb = kRouterWarps / ds;  // ranges of D; groups of experts per block
+    const int nv = p.D / 8, v0 = nv * (warp % ds) / ds, v1 = nv * (warp % ds + 1) / ds;
+    for (int g0 = 0; g0 * TE < p.E; g0 += kRouterBlocks * gpb) {
+        const int e0 = (g0 + rank * gpb + warp / ds) * TE;
+        float acc[TE][TG];
 #pragma unroll
-        for (int t = 0; t < TG; ++t) acc[0][t] = acc[1][t] = 0.f;
+        for (int i = 0; i < TE; ++i)
+#pragma unroll
+            for (int t = 0; t < TG; ++t) acc[i][t] = 0.f;
+        if (e0 < p.E) {
 #pragma unroll(TG == 1 ? 4 : 1)
-        for (int c = lane; c < nv; c += 32) {
-            const uint4 w0 = r0[c], w1 = r1[c];
-            uint4 x[TG];
+            for (int c = v0 + lane; c < v1; c += 32) {
+                uint4 w[TE], x[TG];
 #pragma unroll
-            for (int t = 0; t < TG; ++t) {
-                const int tok = t0 + t < p.T ? t0 + t : t0;  // rows past the last token repeat a row that exists
-                x[t] = reinterpret_cast<const uint4*>(p.X + (size_t)tok * p.ldx)[c];
-            }
-            const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
+                for (int i = 0; i < TE; ++i)  // (experts past the last repeat one that exists, tokens too)
+                    w[i] = reinterpret_cast<const uint4*>(p.R + (size_t)(e0 + i < p.E ? e0 + i : e0) * p.D)[c];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float u0, v0, u1, v1;
-                unpack2<BF16>(a0[j], u0, v0);
-                unpack2<BF16>(a1[j], u1, v1);
+                for (int t = 0; t < TG; ++t)
+                    x[t] = reinterpret_cast<const uint4*>(p.X + (size_t)(t0 + t < p.T ? t0 + t : t0) * p.ldx)[c];
 #pragma unroll
-                for (int t = 0; t < TG; ++t) {
-                    const uint32_t xw[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
-                    float xa, xb;
-                    unpack2<BF16>(xw[j], xa, xb);
-                    acc[0][t] = fmaf(v0, xb, fmaf(u0, xa, acc[0][t]));
-                    acc[1][t] = fmaf(v1, xb, fmaf(u1, xa, acc[1][t]));
+                for (int j = 0; j < 4; ++j) {
+                    float u[TE], v[TE];
+#pragma unroll
+                    for (int i = 0; i < TE; ++i) {
+                        const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        unpack2<BF16>(ww[j], u[i], v[i]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < TG; ++t) {
+                        const uint32_t xw[4] = {x[t].x, x[t].y, x[t].z, x[t].w};
+                        float xa, xb;
+                        unpack2<BF16>(xw[j], xa, xb);
+#pragma unroll
+                        for (int i = 0; i < TE; ++i) acc[i][t] = fmaf(v[i], xb, fmaf(u[i], xa, acc[i][t]));
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int t = 0; t < TG; ++t)
+        for (int i = 0; i < TE; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v = acc[h][t];
+            for (int t = 0; t < TG; ++t) {
+                float v = acc[i][t];
 #pragma unroll
                 for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
-                if (lane == t && (h == 0 || two)) {
-                    const uint32_t dst = mapa_shared(smem_u32(&logits[e + h * warps]), (uint32_t)t);
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
-                }
+                if (lane == (i * TG + t) % 32) part[warp][i * TG + t] = v;
             }
+        __syncthreads();
+        // a logit per thread: its ranges in order, to the block that chooses for its token
+        for (int n = threadIdx.x; n < gpb * NV; n += kRouterThreads) {
+            const int g = n / NV, i = n % NV / TG, t = n % TG, e = (g0 + rank * gpb + g) * TE + i;
+            float v = 0.f;
+            for (int r = 0; r < ds; ++r) v += part[g * ds + r][i * TG + t];
+            if (e < p.E) {
+                const uint32_t dst = mapa_shared(smem_u32(&logits[e]), (uint32_t)t);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+            }
+        }
+        if ((g0 + kRouterBlocks * gpb) * TE < p.E) __syncthreads();  // the sums are read before the next ones
     }
+    if (threadIdx.x == 0) BW_TRACE_AT(13);
     cluster_sync();  // the logits are in; nothing reaches another block's shared memory after this
     const int tok = t0 + rank;
     if (rank >= TG || tok >= p.T || warp != 0) return;
-    constexpr int kPer = kMoeMaxExperts / 32;
-    uint32_t key[kPer];
+    if (threadIdx.x == 0) BW_TRACE_AT(14);
+    uint32_t key[PER];
     uint32_t best = 0u;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const int e = lane + 32 * i;
         key[i] = e < p.E ? router_key(logits[e]) : 0u;
         best = max(best, key[i]);
@@ -117,13 +148,13 @@ __global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterT
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
         uint32_t at = 0xFFFFFFFFu;  // the lowest index among the largest keys
 #pragma unroll
-        for (int i = kPer - 1; i >= 0; --i)
+        for (int i = PER - 1; i >= 0; --i)
             if (key[i] == top && lane + 32 * i < p.E) at = (uint32_t)(lane + 32 * i);
         at = __reduce_min_sync(0xFFFFFFFFu, at);
         if (lane == j) mine = (int)at;
         best = 0u;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
+        for (int i = 0; i < PER; ++i) {
             if ((uint32_t)(lane + 32 * i) == at) key[i] = 0u;
             best = max(best, key[i]);
         }
@@ -142,6 +173,7 @@ __global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterT
         p.ids[(size_t)tok * p.top_k + lane] = mine;
         p.weights[(size_t)tok * p.top_k + lane] = ex / sum;
     }
+    if (threadIdx.x == 0) BW_TRACE_AT(15);
 }
 
 }  // namespace bw

@@ -66,32 +66,69 @@ struct MoeSeg {
     int first, nseg;  // the first block that works on the tile, and how many do
 };
 
-// A block's segments in order: its share of the first product, then of the second.
+// A block's segments in order: its share of the first product, then of the second.  In the first product its parts of
+// split tiles come first (the one its share ends in, then the one it starts in), so that their sums and the waits for
+// them hide behind the whole tiles; what the second product waits for at the end is one whole tile's epilogue.
 struct MoeIter {
-    long long g, end;
-    int phase, c;
-    BW_MOE_HD MoeIter(const MoeSched& s, int c_) : g(0), end(0), phase(-1), c(c_) { (void)s; }
+    long long begin, end;
+    int phase, c, step, tile, tiles;  // step: 0 the end's part, 1 the start's part, 2 whole tiles
+    BW_MOE_HD MoeIter(const MoeSched&, int c_) : begin(0), end(0), phase(-1), c(c_), step(3), tile(0), tiles(0) {}
     BW_MOE_HD bool next(const MoeSched& s, MoeSeg& seg)
     {
-        while (g >= end) {
-            if (++phase > 1) return false;
-            const long long u = phase ? s.u2 : s.u1;
-            const int p = phase ? s.p2 : s.p1;
-            if (c >= p) continue;
-            g = moe_begin(u, p, c);
-            end = moe_begin(u, p, c + 1);
+        for (;;) {
+            if (step == 3) {
+                if (++phase > 1) return false;
+                const int p = phase ? s.p2 : s.p1;
+                if (c >= p) continue;
+                const long long u = phase ? s.u2 : s.u1;
+                begin = moe_begin(u, p, c);
+                end = moe_begin(u, p, c + 1);
+                step = 0;
+            }
+            const int kb = phase ? s.active * s.kbf : s.kb1;
+            const int t0 = (int)(begin / kb), t1 = (int)((end - 1) / kb);
+            const int k0 = (int)(begin - (long long)t0 * kb), k1 = (int)(end - (long long)t1 * kb);
+            const int at = step;
+            if (step < 2) ++step;
+            if (at == 0) {
+                tile = k0 ? t0 + 1 : t0;                     // the whole tiles
+                tiles = k1 == kb ? t1 + 1 - tile : t1 - tile;
+                if (tiles < 0) tiles = 0;                    // (the share lies inside one tile)
+                if (phase || k1 == kb || t0 == t1) continue; // no part of a tile at the end (or it is the start's too)
+                set(s, seg, t1, 0, k1);
+                return true;
+            }
+            if (at == 1) {
+                if (t0 == t1 && (k0 || k1 < kb)) {
+                    set(s, seg, t0, k0, k1);
+                    return true;
+                }
+                if (!k0) continue;
+                set(s, seg, t0, k0, kb);
+                return true;
+            }
+            if (tiles > 0) {
+                --tiles;
+                set(s, seg, tile++, 0, kb);
+                return true;
+            }
+            step = 3;
+            if (phase && k1 < kb && t0 != t1) {
+                set(s, seg, t1, 0, k1);
+                return true;
+            }
         }
-        const long long u = phase ? s.u2 : s.u1;
-        const int p = phase ? s.p2 : s.p1, kb = phase ? s.active * s.kbf : s.kb1;
-        const long long t = g / kb;
+    }
+    BW_MOE_HD void set(const MoeSched& s, MoeSeg& seg, int t, int k0, int k1) const
+    {
+        const long long u = phase ? s.u2 : s.u1, kb = phase ? s.active * s.kbf : s.kb1;
+        const int p = phase ? s.p2 : s.p1;
         seg.phase = phase;
-        seg.tile = (int)t;
-        seg.k0 = (int)(g - t * kb);
-        seg.k1 = end - g < (long long)(kb - seg.k0) ? seg.k0 + (int)(end - g) : kb;
+        seg.tile = t;
+        seg.k0 = k0;
+        seg.k1 = k1;
         seg.first = moe_owner(u, p, t * kb);
         seg.nseg = moe_owner(u, p, (t + 1) * kb - 1) - seg.first + 1;
-        g += seg.k1 - seg.k0;
-        return true;
     }
 };
 

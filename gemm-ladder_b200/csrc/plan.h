@@ -122,6 +122,11 @@
 #ifndef BW_KS_BLOCK_US
 #define BW_KS_BLOCK_US 0.1     // per block of the grid (fitted: more blocks streaming the weights at once cost time)
 #endif
+#ifndef BW_KS_BLOCK_I8_US
+#define BW_KS_BLOCK_I8_US 0.03 // the same for the 8-bit entries (measured on 10240 x 8192 at 1 and 16 tokens: clusters of 3
+                               // over 120 blocks 22.4 us, which 0.1 us a block gives up for clusters of 2 over 80, 24.3 us;
+                               // 8192 x 8192 and 8192 x 28672 keep the fastest choice within 4 %)
+#endif
 #ifndef BW_KS_CLUSTER_US
 #define BW_KS_CLUSTER_US 0.5   // per block of a cluster beyond two (fitted: the larger clusters' longer hand-over)
 #endif
@@ -159,9 +164,6 @@
 #ifndef BW_DYN_MAX_BYTES
 #define BW_DYN_MAX_BYTES (32u << 20)  // the units' partials of a call at most this many bytes (longer units if need be;
                                       // so that the no-allocation entry's array holds them too)
-#endif
-#ifndef BW_MOE_PDL
-#define BW_MOE_PDL 1           // the mixture-of-experts kernel's set-up overlaps its router (programmatic serialisation)
 #endif
 #ifndef BW_SK_ONE_WAVE
 #define BW_SK_ONE_WAVE 1       // stream-K over every tile when they make one full wave and part of another (the
@@ -244,7 +246,7 @@ inline bool plan_ksplit_fits(int bn, int wm, int c)
 // the grid and per block of a cluster beyond two.  Every K-split plan streams the weights once, so the intake decides
 // between them where it exceeds the HBM time: at M = 128 the tokens cost as much intake per block as the weights of a
 // 128-column tile.
-inline double ksplit_cost(int M, int N, int K, int bn, int wm, int c)
+inline double ksplit_cost(int M, int N, int K, int bn, int wm, int c, double block_us = BW_KS_BLOCK_US)
 {
     const double kb = (double)((K / 64 + c - 1) / c);                      // the longest K range, in K-blocks
     const double intake = (128.0 * wm + bn) * 64 * 2 * kb;                  // bytes into the busiest block
@@ -253,7 +255,7 @@ inline double ksplit_cost(int M, int N, int K, int bn, int wm, int c)
     const double sent = (double)(chunks - chunks / c) * 8192;               // the busiest sender's pieces
     const int blocks = (N + 128 * wm - 1) / (128 * wm) * c;
     const double t_hbm = hbm / (BW_HBM_GBS * 1e3), t_in = intake / (BW_SM_INGEST_GBS * 1e3);
-    return (t_hbm > t_in ? t_hbm : t_in) + sent / (BW_DSMEM_GBS * 1e3) + BW_KS_BLOCK_US * blocks +
+    return (t_hbm > t_in ? t_hbm : t_in) + sent / (BW_DSMEM_GBS * 1e3) + block_us * blocks +
            BW_KS_CLUSTER_US * (c - 2);
 }
 
@@ -314,8 +316,11 @@ enum : unsigned {
     kPlanNoSwap = 1u,   // A is the MMA's A operand (fp32 and fused outputs are written by TILE and PAIR only)
     kPlanNoSplit = 2u,  // whole tiles only (a fused epilogue needs the complete sums)
     kPlanNarrow = 4u,   // swap-AB tiles of 128 weight columns, pair tiles of 256 (half the partials' scratch)
-    kPlanGateUp = 16u,  // swap-AB tiles of 256 weight columns, 128 gate and 128 up, at every M (a fused activation)
-    kPlanNoStage = 32u, // no staging for TMA stores of C (BW_EPI_TMA): the 8-bit entries store from registers
+    kPlanGateUp = 16u,  // tiles of whole 256-column gate/up groups (a fused activation): swap-AB tiles of 256 weight
+                        // columns, 128 gate and 128 up, stream-K over them; pair tiles of 256 columns (512:
+                        // measured 19 % slower at 1999 x 57344 x 8192, the activation then shows between tiles)
+    kPlanI8 = 32u,      // an 8-bit entry: no staging for TMA stores of C (BW_EPI_TMA; they store from registers),
+                        // BW_KS_BLOCK_I8_US
     kPlanRsWindow = 8u, // shared memory for the fused reduce-scatter's window (kPlanRsWindowBytes), fewer stages
 };
 
@@ -369,7 +374,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     const bool wide_ok = (variant == 0 || variant == 3) && !(flags & kPlanNarrow);
     const int tiles256 = (N + 255) / 256;
     int ks = 0, ks_wm = 0;
-    if (swap && variant != 1 && variant != 4 && q.kblocks >= 2) {
+    if (swap && variant != 1 && variant != 4 && q.kblocks >= 2 && !(flags & kPlanGateUp)) {
 #if BW_KSPLIT
         double best = 0.0;
         for (int c = 2; c <= BW_KSPLIT_MAX && c <= 8; ++c) {
@@ -380,7 +385,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
                 const int tiles = (N + 128 * wm - 1) / (128 * wm);
                 const int at_once = held ? held[c] : (c == 2 && pairs > 0) ? pairs : sms / c;
                 if (tiles > at_once || (c > 2 && q.kblocks < 4 * c) || !plan_ksplit_fits(q.bn, wm, c)) continue;
-                const double t = ksplit_cost(M, N, K, q.bn, wm, c);
+                const double t = ksplit_cost(M, N, K, q.bn, wm, c, flags & kPlanI8 ? BW_KS_BLOCK_I8_US : BW_KS_BLOCK_US);
                 if (!ks || t < best) {
                     best = t;
                     ks = c;
@@ -485,7 +490,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     }
     q.grid = P * ranks;
     // shared memory after the ring: the fused reduce-scatter's window, or the fp16 TILE / PAIR epilogue's staging
-    const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow | kPlanNoStage));
+    const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow | kPlanI8));
     const int reserve = (flags & kPlanRsWindow) ? kPlanRsWindowBytes : epi_tma ? kPlanEpiStageBytes : 0;
     q.stages = plan_stages(q.bn, ranks, swap, q.wm, reserve);
     q.smem_bytes = plan_smem_bytes(q.bn, ranks, swap, q.wm, reserve);

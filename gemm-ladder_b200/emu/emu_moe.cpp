@@ -1,5 +1,5 @@
 // emu_moe.cpp -- the host emulator over the mixture-of-experts kernel (test infrastructure; a build of its own with
-// -DBW_EMU_THREADS=224, the kernel's block).  The blocks wait for one another, so every block of the grid runs at once,
+// -DBW_EMU_THREADS=352, the kernel's block).  The blocks wait for one another, so every block of the grid runs at once,
 // as the library's cooperative launch has it; the router is given (ids, weights).
 //
 // C entry:

@@ -52,8 +52,8 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     std::memset(g_status, 0, sizeof g_status);
     const int epi = swiglu ? kEpiI8SwiGLU : out_type == BW_TYPE_F32 ? kEpiI8F32 : kEpiI8;
     const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap
-                           : epi == kEpiI8SwiGLU ? kPlanNoSplit | kPlanGateUp | (M > 128 ? kPlanNoSwap : 0u)
-                                                 : kPlanNoStage;
+                           : epi == kEpiI8SwiGLU ? kPlanGateUp | kPlanI8 | (M > 128 ? kPlanNoSplit : 0u)
+                                                 : kPlanI8;
     bw_plan q = {};
     int rc = make_plan(M, N, (K + 127) / 128 * 64, sms, sms / 2, 0, &q, flags);
     if (rc) return rc;
@@ -65,6 +65,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     p.row_scale = a_scale;
     p.col_scale = b_scale;
     p.out_bf16 = out_type == BW_TYPE_BF16;
+    p.early_weights = M % 2;  // (both orders of the first loads)
     rc = dispatch_i8(q, mx, my, p, epi);
     if (status) std::memcpy(status, g_status, sizeof g_status);
     if (dirty) *dirty = (int)std::count_if(counters.begin(), counters.begin() + q.counters, [](int v) { return v != 0; });

@@ -652,15 +652,16 @@ inline void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, b
     }
 }
 
-// tcgen05.ld 32x32b.x16: lane = the address's lane + the thread's lane in its warp, 16 columns
-inline void tmem_ld(uint32_t taddr, uint32_t (&r)[16])
+// tcgen05.ld 32x32b.x16 (x8): lane = the address's lane + the thread's lane in its warp, 16 (8) columns
+template <int NC>
+inline void tmem_ld(uint32_t taddr, uint32_t (&r)[NC])
 {
     if (g_ld_delay_us > 0) {
         thread_local std::minstd_rand rng((unsigned)(t_tid * 7919 + 17));
         std::this_thread::sleep_for(std::chrono::microseconds(rng() % (unsigned)(g_ld_delay_us + 1)));
     }
     const uint32_t lane = (taddr >> 16) + (uint32_t)(t_tid & 31), col = taddr & 0xFFFFu;
-    if (lane >= (uint32_t)kTmemLanes || col + 16 > (uint32_t)t_cta->tmem_cols) {
+    if (lane >= (uint32_t)kTmemLanes || col + NC > (uint32_t)t_cta->tmem_cols) {
         finding("tcgen05.ld of lane %u column %u outside the allocation", lane, col);
         std::memset(r, 0, sizeof r);
         return;

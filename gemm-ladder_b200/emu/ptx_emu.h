@@ -259,6 +259,7 @@ inline void mma_commit(uint64_t* bar)
     c->tc.post([=] { emu::mb_arrive(c, off, 0); });
 }
 inline void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) { emu::tmem_ld(taddr, r); }
+inline void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) { emu::tmem_ld(taddr, r); }
 inline void tmem_wait_ld() {}
 
 // ------------------------------------------------------------------ descriptors (the same encodings as ptx.cuh)

@@ -19,7 +19,7 @@ def emu(tmp_path_factory):
     if not os.path.isdir(CUDA_INCLUDE):
         pytest.skip("no CUDA headers")
     lib = str(tmp_path_factory.mktemp("emu_moe") / "libbwemu_moe.so")
-    subprocess.check_call(["g++", "-std=c++20", "-O2", "-pthread", "-DBW_EMULATE", "-DBW_EMU_THREADS=224", "-fPIC",
+    subprocess.check_call(["g++", "-std=c++20", "-O2", "-pthread", "-DBW_EMULATE", "-DBW_EMU_THREADS=352", "-fPIC",
                            "-shared", "-w", f"-I{CUDA_INCLUDE}", f"-I{os.path.join(ROOT, 'include')}",
                            f"-I{os.path.join(PKG, 'csrc')}", os.path.join(PKG, "emu", "emu_moe.cpp"), "-o", lib])
     return ctypes.CDLL(lib)
