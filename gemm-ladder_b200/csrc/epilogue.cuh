@@ -21,30 +21,53 @@ __device__ __forceinline__ float i8_value(float bits, float row_scale, float col
 {
     return (float)__float_as_int(bits) * row_scale * col_scale;
 }
-// NC columns n .. n + NC - 1 (inside C) of row m: the scaled values; a row past M (never stored) gets scale 0.
-template <int NC>
-__device__ __forceinline__ void i8_row_values(const Params& p, int m, int n, const float (&s)[NC], float (&v)[NC])
+// TILE and PAIR keep the scales of a tile in shared memory (in the place of the swap-AB transpose buffers, `cst`): its BN
+// column scales, then the block's 128 row scales, loaded while the tile's MMAs run (0 outside C).
+__device__ __forceinline__ const float* i8_scales(const __half* cst) { return reinterpret_cast<const float*>(cst); }
+template <int BN>
+__device__ __forceinline__ void i8_load_scales(const Params& p, __half* cst, int m0, int n0)
 {
-    const float rs = m < p.s.M ? __ldg(p.row_scale + m) : 0.f;
+    float* to = reinterpret_cast<float*>(cst);
+    const int t = threadIdx.x - kEpiThread0;
+#pragma unroll
+    for (int i = 0; i < BN; i += 128) to[i + t] = n0 + i + t < p.s.N ? __ldg(p.col_scale + n0 + i + t) : 0.f;
+    to[BN + t] = m0 + t < p.s.M ? __ldg(p.row_scale + m0 + t) : 0.f;
+}
+// NC columns of a row: the scaled values (cs: their column scales, 16-byte aligned).
+template <int NC>
+__device__ __forceinline__ void i8_row_values(float rs, const float* cs4, const float (&s)[NC], float (&v)[NC])
+{
 #pragma unroll
     for (int j = 0; j < NC; j += 4) {
-        const float4 cs = *reinterpret_cast<const float4*>(p.col_scale + n + j);  // one address per warp: a broadcast
+        const float4 cs = *reinterpret_cast<const float4*>(cs4 + j);  // one address per warp: a broadcast
         v[j] = i8_value(s[j], rs, cs.x);
         v[j + 1] = i8_value(s[j + 1], rs, cs.y);
         v[j + 2] = i8_value(s[j + 2], rs, cs.z);
         v[j + 3] = i8_value(s[j + 3], rs, cs.w);
     }
 }
-// Two values of C in its 16-bit type, the first in the low half.
-template <int EPI>
-__device__ __forceinline__ uint32_t pack2(const Params& p, float a, float b)
+// Two values of C in its 16-bit type, the first in the low half; NP of them (one test of the type for all: a test per pair
+// keeps the conversions from overlapping).
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
 {
-    if (epi_i8(EPI) && p.out_bf16) {
+    if (BF16) {
         const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&y);
     }
     const __half2 x = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&x);
+}
+template <int EPI, int NP>
+__device__ __forceinline__ void pack_pairs(const Params& p, const float (&v)[2 * NP], uint32_t (&h)[NP])
+{
+    if (epi_i8(EPI) && p.out_bf16) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) h[j] = pack2<true>(v[2 * j], v[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) h[j] = pack2<false>(v[2 * j], v[2 * j + 1]);
+    }
 }
 template <int EPI>
 __device__ __forceinline__ __half half_bits(const Params& p, float a)  // one value, as the 16 bits of a __half
@@ -63,6 +86,7 @@ __device__ __forceinline__ __half half_bits(const Params& p, float a)  // one va
 // 16 x 128 fp16 buffers, alternating by chunk), so that C is written by 16-byte stores, a warp covering two rows of
 // 256 contiguous bytes, instead of 16 scattered 2-byte stores per thread.  One named barrier per chunk; the buffer of
 // chunk i + 2 is written only after every thread has passed the barrier of chunk i + 1, so after it read chunk i.
+// Integer sums (kEpiI8*), not swapped: the values scaled from `cst` (BT: the tile's columns), then as the others.
 template <bool SWAP, int EPI = kEpiF16, int BT = 0>
 __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int lane, int c0, const float (&v)[16],
                                             __half* cst)
@@ -72,15 +96,14 @@ __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int
         const int m = m0 + lane, n = n0 + c0;
         if (m >= s.M || n >= s.N) return;
         float w[16];
-        i8_row_values(p, m, n, v, w);
+        i8_row_values(i8_scales(cst)[BT + lane], i8_scales(cst) + c0, v, w);
         if (EPI == kEpiI8F32) {
             float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.C) + (size_t)m * s.N + n);
 #pragma unroll
             for (int q = 0; q < 4; ++q) dst[q] = make_float4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
         } else {
             uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = pack2<EPI>(p, w[2 * j], w[2 * j + 1]);
+            pack_pairs<EPI, 8>(p, w, h);
             uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.C) + (size_t)m * s.N + n);
             dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
             dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
@@ -173,16 +196,19 @@ __device__ __forceinline__ void store_lines64(const Params& p, int r0, int n, in
     constexpr int P = kF32 ? 16 : 8;
     const Sched& s = p.s;
     uint32_t x[P][4];
+    if constexpr (kF32) {
 #pragma unroll
-    for (int i = 0; i < P; ++i)
+        for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            if (kF32) {
-                x[i][w] = __float_as_uint(v[4 * i + w]);
-            } else {
-                x[i][w] = pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w + 1]);
-            }
-        }
+            for (int w = 0; w < 4; ++w) x[i][w] = __float_as_uint(v[4 * i + w]);
+    } else {
+        uint32_t h[32];
+        pack_pairs<EPI, 32>(p, v, h);
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) x[i][w] = h[4 * i + w];
+    }
     transpose_pieces<P>(x, lane);
     const int q = lane & (P - 1), g = lane / P;
     if (n >= s.N) return;  // N % 64 == 0: the 64 columns are all in C or all outside
@@ -207,11 +233,12 @@ __device__ __forceinline__ void store_rows64(const Params& p, int r0, int n, int
 
 // The 64 columns' integer sums (kEpiI8, kEpiI8F32), scaled, the same way.
 template <int EPI>
-__device__ __forceinline__ void store_rows64_i8(const Params& p, int r0, int n, int lane, const float (&sum)[64])
+__device__ __forceinline__ void store_rows64_i8(const Params& p, int r0, int n, int lane, const float (&sum)[64],
+                                                float rs, const float* cs)
 {
     if (n >= p.s.N) return;  // N % 64 == 0: the 64 columns are all in C or all outside
     float v[64];
-    i8_row_values(p, r0 + lane, n, sum, v);
+    i8_row_values(rs, cs, sum, v);
     store_lines64<EPI>(p, r0, n, lane, v);
 }
 
@@ -271,12 +298,13 @@ __device__ __forceinline__ void i8_swiglu_store16(const Params& p, const float (
 }
 
 template <bool SWAP, int BN>
-__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row)
+__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row, const __half* cst)
 {
     const Sched& s = p.s;
     if constexpr (!SWAP) {
         const int m = m0 + row;
-        const float rs = m < s.M ? __ldg(p.row_scale + m) : 0.f;
+        const float* cs = i8_scales(cst);
+        const float rs = cs[BN + row];
 #pragma unroll 1
         for (int c0 = 0; c0 < 128; c0 += 16) {
             uint32_t gr[16], ur[16];
@@ -284,18 +312,13 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
             tmem_ld16(tbase + (uint32_t)(128 + c0), ur);
             tmem_wait_ld();
             if (m >= s.M || n0 >= s.N) continue;
+            float a[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                a[j] = silu_mul(i8_value(__uint_as_float(gr[j]), rs, cs[c0 + j]),
+                                i8_value(__uint_as_float(ur[j]), rs, cs[128 + c0 + j]));
             uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float a[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c = c0 + 2 * j + e;
-                    a[e] = silu_mul(i8_value(__uint_as_float(gr[2 * j + e]), rs, __ldg(p.col_scale + n0 + c)),
-                                    i8_value(__uint_as_float(ur[2 * j + e]), rs, __ldg(p.col_scale + n0 + 128 + c)));
-                }
-                h[j] = pack2<kEpiI8SwiGLU>(p, a[0], a[1]);
-            }
+            pack_pairs<kEpiI8SwiGLU, 8>(p, a, h);
             uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(p.C) + (size_t)m * (s.N / 2) + n0 / 2 + c0);
             dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
             dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
@@ -505,7 +528,8 @@ __device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, 
                 }
             }
             if constexpr (epi_i8(EPI))
-                store_rows64_i8<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v);
+                store_rows64_i8<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v, i8_scales(cst)[BN + row],
+                                     i8_scales(cst) + c0);
             else
                 store_rows64<EPI>(p, m0 + (row & ~31), n0 + c0, row & 31, v);
         }

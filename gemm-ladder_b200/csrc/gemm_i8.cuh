@@ -34,7 +34,7 @@ int i8_plan(DeviceState& d, int M, int N, int K, int epi, bw_plan* q)
         *q = at.q;
         return BW_OK;
     }
-    const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap
+    const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap | kPlanI8
                            : epi == kEpiI8SwiGLU ? kPlanGateUp | kPlanI8 | (M > 128 ? kPlanNoSplit : 0u)
                                                  : kPlanI8;
     if ((rc = make_plan(M, N, (K + 127) / 128 * 64, d.sms, d.pairs, 0, q, flags, held_of(d)))) return rc;
@@ -111,6 +111,8 @@ int i8_dispatch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const C
 #endif
         return i8_launch<256, false, true, kEpiI8>(d, q, mx, my, p, st, pdl);
     }
+    if (q.kernel == BW_KERNEL_TILE && q.bn == 128 && epi == kEpiI8)
+        return i8_launch<128, false, false, kEpiI8>(d, q, mx, my, p, st, pdl);
     if (q.kernel != BW_KERNEL_SWAP) {
         snprintf(g_errbuf, sizeof g_errbuf, "this device holds no pairs of SMs");
         return BW_ERR_LAUNCH;

@@ -475,6 +475,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         for (;;) {
             if (!s.dyn && !it.next(s, P, sg)) break;
+            if constexpr (epi_i8(EPI) && !SWAP) {  // the tile's scales, while its MMAs run
+                int tm, tn;
+                tile_coords(s, sg.tile, tm, tn);
+                named_bar_sync(1, 128);  // the previous tile's have been read
+                i8_load_scales<BN>(p, cst, tm * G::kTileM + rank * 128, tn * BN);
+            }
             // one thread waits (bounded); a named barrier hands its outcome to the other 127, so that an abort
             // takes the whole group out together and no thread is left at a later barrier.  s.dyn: that thread first
             // takes the segment's unit from the queue (go 2: none left)
@@ -526,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release_all(acc);
             } else if (EPI == kEpiI8SwiGLU && sg.k0 == 0 && sg.k1 == s.kblocks) {
                 if constexpr (EPI == kEpiI8SwiGLU) {
-                    i8_swiglu_tile<SWAP, BN>(p, tbase, m0, n0, row);
+                    i8_swiglu_tile<SWAP, BN>(p, tbase, m0, n0, row, cst);
                     release_all(acc);
                 }
             } else if (EPI == kEpiSwiGLU) {
@@ -731,7 +737,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j / 16][j % 16]);
                         if constexpr (epi_i8(EPI))
-                            store_rows64_i8<EPI>(p, m0 + q * 32, n0 + c0, lane, v);
+                            store_rows64_i8<EPI>(p, m0 + q * 32, n0 + c0, lane, v, i8_scales(cst)[BN + row],
+                                                 i8_scales(cst) + c0);
                         else
                             store_rows64<EPI == kEpiF32 ? kEpiF32 : kEpiF16>(p, m0 + q * 32, n0 + c0, lane, v);
                     } else {

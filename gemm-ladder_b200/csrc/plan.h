@@ -197,7 +197,7 @@ inline const char* variant_name(int v)
 // The kernels' geometry, as gemm_kernel.cuh's Geom computes it (checked against it at launch in bwgemm.cu): the ring
 // takes what the 227 KB leave after the alignment slack, the barriers and the swap-AB epilogue's transpose buffers.
 inline int plan_stage_bytes(int bn, int ranks, int wm = 1) { return 128 * wm * 64 * 2 + (bn / ranks) * 64 * 2; }
-inline int plan_cstage_bytes(bool swap) { return swap ? 2 * 16 * 128 * 2 : 0; }
+inline int plan_cstage_bytes(bool swap, int i8_bn = 0) { return swap ? 2 * 16 * 128 * 2 : i8_bn ? (i8_bn + 128) * 4 : 0; }
 // The fused reduce-scatter's window (two 32 KB buffers) for the owner's partials, after the stage ring.
 constexpr int kPlanRsWindowBytes = 2 * 32768;
 // The TMA-store epilogue's staging (BW_EPI_TMA): two buffers of 128 rows x 64 fp16 columns, after the stage ring.
@@ -205,9 +205,9 @@ constexpr int kPlanEpiStageBytes = 2 * 16384;
 // Entries of a block's queue of units (BW_DYN_UNITS: its producer takes units and passes them to the MMA issuer and the
 // epilogue), each with a full and an empty barrier.
 constexpr int kPlanUnitQ = 4;
-inline int plan_stages(int bn, int ranks, bool swap, int wm = 1, int reserve = 0)
+inline int plan_stages(int bn, int ranks, bool swap, int wm = 1, int reserve = 0, bool i8 = false)
 {
-    const int s = (BW_SMEM_LIMIT - 1024 - 512 - plan_cstage_bytes(swap) - reserve) / plan_stage_bytes(bn, ranks, wm);
+    const int s = (BW_SMEM_LIMIT - 1024 - 512 - plan_cstage_bytes(swap, i8 ? bn : 0) - reserve) / plan_stage_bytes(bn, ranks, wm);
     return s < BW_MAX_STAGES ? s : BW_MAX_STAGES;
 }
 // Tensor-memory columns for accumulators of acc_n columns: two of them, or one of 512.
@@ -218,12 +218,12 @@ inline int plan_tmem_cols(int acc_n)
     while (c < need) c *= 2;
     return c;
 }
-inline int plan_smem_bytes(int bn, int ranks, bool swap, int wm = 1, int reserve = 0)
+inline int plan_smem_bytes(int bn, int ranks, bool swap, int wm = 1, int reserve = 0, bool i8 = false)
 {
-    const int st = plan_stages(bn, ranks, swap, wm, reserve);
+    const int st = plan_stages(bn, ranks, swap, wm, reserve, i8);
     const int misc = st * plan_stage_bytes(bn, ranks, wm) + reserve + (2 * st + 8 + 2 * kPlanUnitQ) * 8;
     const int cstage = (misc + 64 + 127) / 128 * 128;
-    return 1024 + cstage + plan_cstage_bytes(swap);
+    return 1024 + cstage + plan_cstage_bytes(swap, i8 ? bn : 0);
 }
 
 // A K-split cluster of c blocks (swap-AB): the bytes one block receives into its idle stage ring.  BW_KSPLIT 0: the
@@ -348,13 +348,21 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
         q.bn = variant == 6 ? 64 : variant == 7 ? 128 : 256;
         ranks = pair ? 2 : 1;
         units = pair ? pairs : sms;
+        if ((flags & kPlanI8) && !(flags & (kPlanGateUp | kPlanNoSwap)) && pair && sms > 0 &&
+            (long long)((M + 127) / 128) * ((N + 127) / 128) <= sms) {
+            q.kernel = BW_KERNEL_TILE;
+            q.bn = 128;
+            ranks = 1;
+            units = sms;
+        }
         q.tiles_m = (M + 128 * ranks - 1) / (128 * ranks);
         // pair tiles of 512 columns for the fp16 entries, where their estimated time is 2 % below the 256-column ones'
         // and they make no stream-K schedule (whose partials would be 256 KB per block)
         const int tw = q.tiles_m * ((N + 511) / 512);
         const bool wide_sk = (BW_SK_ONE_WAVE && tw > units && tw < 2 * units) ||
                              (BW_SK_PART_WAVE && 2 * tw > units && tw < units);
-        if (BW_PAIR_WIDE && pair && (variant == 0 || variant == 3) && !(flags & (kPlanNoSwap | kPlanNarrow)) &&
+        if (BW_PAIR_WIDE && q.kernel == BW_KERNEL_PAIR && (variant == 0 || variant == 3) &&
+            !(flags & (kPlanNoSwap | kPlanNarrow)) &&
             N > 256 && units > 0 && !wide_sk &&
             pair_time(tw, units, q.kblocks, 512) < 0.98 * pair_time(q.tiles_m * ((N + 255) / 256), units, q.kblocks, 256))
             q.bn = 512;
@@ -492,8 +500,9 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     // shared memory after the ring: the fused reduce-scatter's window, or the fp16 TILE / PAIR epilogue's staging
     const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow | kPlanI8));
     const int reserve = (flags & kPlanRsWindow) ? kPlanRsWindowBytes : epi_tma ? kPlanEpiStageBytes : 0;
-    q.stages = plan_stages(q.bn, ranks, swap, q.wm, reserve);
-    q.smem_bytes = plan_smem_bytes(q.bn, ranks, swap, q.wm, reserve);
+    const bool i8 = flags & kPlanI8;
+    q.stages = plan_stages(q.bn, ranks, swap, q.wm, reserve, i8);
+    q.smem_bytes = plan_smem_bytes(q.bn, ranks, swap, q.wm, reserve, i8);
     q.tmem_cols = plan_tmem_cols(q.bn * q.wm);
     q.counters = q.sk_tiles * ranks + (q.dyn ? 2 : 0);  // dyn: the next unit to take, the blocks that finished
     Sched sc = {};

@@ -32,6 +32,7 @@ int dispatch_i8(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, 
         if (q.bn == 512) return launch<512, false, true, kEpiI8, 1>(q, mx, my, mx, p);
         return launch<256, false, true, kEpiI8, 1>(q, mx, my, mx, p);
     }
+    if (q.kernel == BW_KERNEL_TILE) return launch<128, false, false, kEpiI8, 1>(q, mx, my, mx, p);
     if (epi == kEpiI8SwiGLU) return launch_i8_swap<kEpiI8SwiGLU, 2>(q, mx, my, p);
     return q.wm == 2 ? launch_i8_swap<kEpiI8, 2>(q, mx, my, p) : launch_i8_swap<kEpiI8, 1>(q, mx, my, p);
 }
@@ -51,7 +52,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     emu::g_tma_count = 0;
     std::memset(g_status, 0, sizeof g_status);
     const int epi = swiglu ? kEpiI8SwiGLU : out_type == BW_TYPE_F32 ? kEpiI8F32 : kEpiI8;
-    const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap
+    const unsigned flags = epi == kEpiI8F32      ? kPlanNoSwap | kPlanI8
                            : epi == kEpiI8SwiGLU ? kPlanGateUp | kPlanI8 | (M > 128 ? kPlanNoSplit : 0u)
                                                  : kPlanI8;
     bw_plan q = {};

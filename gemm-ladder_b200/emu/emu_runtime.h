@@ -694,6 +694,7 @@ inline float4 __ldcg(const float4* p)
 }
 inline void __stcg(float4* p, float4 v) { *p = v; }
 inline float __expf(float x) { return std::exp(x); }
+inline float __fdividef(float x, float y) { return x / y; }
 inline float __uint_as_float(uint32_t u)
 {
     float f;

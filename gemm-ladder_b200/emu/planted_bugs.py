@@ -247,8 +247,8 @@ MUTATIONS = [
     ("lines_group_rows", EP, "const int q = lane & (P - 1), g = lane / P;", "const int q = lane & (P - 1), g = (lane / P) ^ 1;",
      0, "library"),
     ("lines_row_bound", EP, "if (m < s.M) {", "if (m <= s.M) {", 0, "library"),
-    ("lines_f16_pair_order", EP, "pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w + 1])",
-     "pack2<EPI>(p, v[8 * i + 2 * w], v[8 * i + 2 * w])", 0, "library"),
+    ("lines_f16_pair_order", EP, "h[j] = pack2<false>(v[2 * j], v[2 * j + 1]);",
+     "h[j] = pack2<false>(v[2 * j], v[2 * j]);", 0, "library"),
     ("reduce_column_group", EP, "w[q] = __ldcg(slot_vec<BN>(p, slot, row, chunk * 4 + q));",
      "w[q] = __ldcg(slot_vec<BN>(p, slot, row, chunk * 4 + (q ^ 1)));", 0, "library"),
     ("reduce_reads_own_slot", EP, "const int L = f.nseg - (own_mine ? 1 : 0);  // partials read from memory",
