@@ -259,7 +259,9 @@ def gemm_swiglu(A, B, C=None, stream=None):
 
 # ---------------------------------------------------------------------------------- 8-bit integer products
 # These calls are made once per layer of a decode step, so their host side is kept short: plain comparisons, the raw
-# stream handle, torch's allocator only for what the call needs.
+# stream handle, torch's allocator only for what the call needs.  `stream` (None: the current one) is the stream a call
+# runs on; what it returns belongs to that stream.  Inputs are taken as they are on that stream: a caller whose inputs
+# are still being written on another orders the two, as for any call with a stream.
 _type_codes = {}
 
 
@@ -271,9 +273,10 @@ def _types():
     return _type_codes
 
 
-def _on(device, stream, call):
+def _on(device, stream, call, *tensors):
     """call(stream handle) with `device` current and `stream` (None: the device's current stream) the current stream there,
-    so that memory made inside belongs to the stream the call runs on."""
+    so that memory made inside belongs to the stream the call runs on; the caller's tensors are marked as used by a
+    stream that is not the current one, so that their memory is not handed out again before it is done with them."""
     import torch
 
     if stream is None:
@@ -284,7 +287,12 @@ def _on(device, stream, call):
     if stream.device != device:
         raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
     with torch.cuda.stream(stream):
-        return call(stream.cuda_stream)
+        out = call(stream.cuda_stream)
+        if not torch.cuda.is_current_stream_capturing():
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+    return out
 
 
 def _rows16(X, what):
@@ -361,7 +369,7 @@ def quantize_rows(X, Q=None, scale=None, stream=None):
         check(lib().bw_quant_rows_i8(X.data_ptr(), code, ld, q.data_ptr(), sc.data_ptr(), rows, cols, s))
         return q, sc
 
-    return _on(X.device, stream, call)
+    return _on(X.device, stream, call, X, Q, scale)
 
 
 def _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, swiglu):
@@ -390,7 +398,7 @@ def _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, swiglu):
                 s))
         return out
 
-    return _on(A.device, stream, call)
+    return _on(A.device, stream, call, A, a_scale, B, b_scale, C)
 
 
 def gemm_i8(A, a_scale, B, b_scale, C=None, dtype=None, stream=None):
@@ -421,7 +429,7 @@ def linear_i8(X, B, b_scale, C=None, swiglu=False, stream=None):
                                  work, n, s))
         return out
 
-    return _on(X.device, stream, call)
+    return _on(X.device, stream, call, X, B, b_scale, C)
 
 
 # ---------------------------------------------------------------------------------- mixture of experts
@@ -456,7 +464,7 @@ def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=Non
                                weights.data_ptr() if weights is not None else None, work, n, s))
         return out
 
-    return _on(X.device, stream, call)
+    return _on(X.device, stream, call, X, R, W1, W2, Y, ids, weights)
 
 
 def status():

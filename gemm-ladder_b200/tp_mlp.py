@@ -13,6 +13,10 @@ Megatron-style, one rank per GPU, p ranks:
       or down and the reduce-scatter in one kernel per rank (bwgemm.ReduceScatterGemm: the partial tiles of the other
       ranks' rows pushed into their memory, each rank summing its own rows' partials in rank order), no NCCL call.
 
+In 8 bits (TPMLPI8): the same block with int8 weights (a scale per output channel) and activations quantised by row in
+front of each product (bw_linear_i8; over several ranks down as bw_quant_rows_i8 and bw_gemm_i8 in fp32, then the
+reduce-scatter).
+
 The GEMMs are parameters so that the sharding and the collective can be tested on CPU ranks (gloo) with a CPU matmul
 in their place; on the GPU they are the rung's (bwgemm.gemm, bwgemm.gemm_f32out).
 """
@@ -104,6 +108,43 @@ class TPMLP:
     def flops(M, hidden, f):
         """FLOPs of the whole block (all ranks): the gateup and down GEMMs."""
         return 2.0 * M * hidden * (2 * f) + 2.0 * M * f * hidden
+
+
+def quantize_shards(W1, W2, rank, world, quantize_rows, group=128):
+    """The rank's weights for TPMLPI8 from the block's (W1: hidden x 2F, gate then up; W2: F x hidden; fp16 or bf16):
+    ((W1_r, its scales), (W2_r, its scales)) as quantize_rows gives them, W1_r's rows (2F/world x hidden) in groups of
+    `group` gate rows and the matching up rows, W2_r hidden x F/world."""
+    w1 = shard_gateup_interleaved(W1, rank, world, group).t().contiguous()
+    return quantize_rows(w1), quantize_rows(shard_down(W2, rank, world).t().contiguous())
+
+
+class TPMLPI8:
+    """One rank's part of the block in 8 bits.  W1, W2: (int8 rows, fp32 scales) of quantize_shards.
+    linear(X, rows, scales, swiglu) -> X's product with its rows quantised (bwgemm.linear_i8); over several ranks also
+    quantize_rows(A) -> (int8, scales) and gemm_f32(q, q_scales, rows, scales) -> fp32 (bwgemm.gemm_i8), each rank
+    quantising its own shard of the activation, and reduce_scatter as TPMLP's."""
+
+    def __init__(self, W1, W2, rank, world, linear, quantize_rows=None, gemm_f32=None, reduce_scatter=None):
+        self.W1, self.W2 = W1, W2
+        self.rank, self.world = rank, world
+        self.linear, self.quantize_rows, self.gemm_f32 = linear, quantize_rows, gemm_f32
+        self.reduce_scatter = reduce_scatter
+        if W1[0].shape[0] != 2 * W2[0].shape[1]:
+            raise ValueError("gateup shard and down shard disagree on the MLP width")
+        if world > 1 and (quantize_rows is None or gemm_f32 is None or reduce_scatter is None):
+            raise ValueError("several ranks need quantize_rows, gemm_f32 and reduce_scatter")
+
+    def forward(self, X):
+        M = X.shape[0]
+        if M % self.world:
+            raise ValueError(f"{M} tokens do not split over {self.world} ranks")
+        A = self.linear(X, *self.W1, swiglu=True)                  # M x F/p in X's type
+        if self.world == 1:
+            return self.linear(A, *self.W2, swiglu=False)
+        P = self.gemm_f32(*self.quantize_rows(A), *self.W2)        # M x hidden, fp32 partial sums
+        out = torch.empty((M // self.world, P.shape[1]), dtype=torch.float32, device=P.device)
+        self.reduce_scatter(out, P)
+        return out.to(X.dtype)
 
 
 def nccl_reduce_scatter(out, inp):
