@@ -262,11 +262,15 @@ def gemm_swiglu(A, B, C=None, stream=None):
 # stream handle, torch's allocator only for what the call needs.  `stream` (None: the current one) is the stream a call
 # runs on; what it returns belongs to that stream.  Inputs are taken as they are on that stream: a caller whose inputs
 # are still being written on another orders the two, as for any call with a stream.
+torch = None
 _type_codes = {}
 
 
 def _types():
+    """torch's types by the C ABI's codes; the first call imports torch for the functions below (this module itself is
+    used without it)."""
     if not _type_codes:
+        global torch
         import torch
 
         _type_codes.update({torch.float16: BW_TYPE_F16, torch.bfloat16: BW_TYPE_BF16, torch.float32: BW_TYPE_F32})
@@ -277,8 +281,6 @@ def _on(device, stream, call, *tensors):
     """call(stream handle) with `device` current and `stream` (None: the device's current stream) the current stream there,
     so that memory made inside belongs to the stream the call runs on; the caller's tensors are marked as used by a
     stream that is not the current one, so that their memory is not handed out again before it is done with them."""
-    import torch
-
     if stream is None:
         if torch.cuda.current_device() == device.index:
             return call(torch._C._cuda_getCurrentRawStream(device.index))
@@ -312,8 +314,6 @@ def _rows16(X, what):
 
 
 def _i8_weight(B, b_scale, device):
-    import torch
-
     if B.dtype != torch.int8 or B.dim() != 2 or B.device != device or not B.is_contiguous():
         raise ValueError("B must be a contiguous int8 N x K tensor on A's device")
     if b_scale.dtype != torch.float32 or b_scale.dim() != 1 or b_scale.shape[0] != B.shape[0] or \
@@ -337,8 +337,6 @@ _work_sizes = {}  # (entry, device, sizes ...) -> bytes of workspace: the plan's
 def _work(query, like, *sizes):
     """The call's own workspace from torch's allocator (so of the stream, or the CUDA graph, that the call is part of):
     (tensor or None, address, bytes)."""
-    import torch
-
     key = (query, like.device.index, *sizes)
     n = _work_sizes.get(key)
     if n is None:
@@ -356,8 +354,6 @@ def _work(query, like, *sizes):
 def quantize_rows(X, Q=None, scale=None, stream=None):
     """(Q, scale): the rows of a 2-D fp16 or bf16 CUDA tensor (rows may be strided) as int8 and their fp32 scales,
     scale = max|row| / 127, Q = round-half-even(127 X / max|row|); made if not given.  X's columns: a multiple of 16."""
-    import torch
-
     rows, cols, ld, code = _rows16(X, "X")
     if scale is not None and (scale.dim() != 1 or scale.shape[0] != rows or scale.dtype != torch.float32 or
                               scale.device != X.device or not scale.is_contiguous()):
@@ -373,10 +369,9 @@ def quantize_rows(X, Q=None, scale=None, stream=None):
 
 
 def _gemm_i8(A, a_scale, B, b_scale, C, dtype, stream, swiglu):
-    import torch
-
+    types = _types()
     dtype = torch.float16 if dtype is None else dtype
-    code = _types().get(dtype)
+    code = types.get(dtype)
     if code is None or (swiglu and code == BW_TYPE_F32):
         raise ValueError(f"C cannot be {dtype}")
     if A.dtype != torch.int8 or A.dim() != 2 or not A.is_cuda or not A.is_contiguous():
@@ -441,8 +436,6 @@ def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=Non
     strided), R (E x D) the router, W1 (E x 2F x D) the experts' gate rows then up rows, W2 (E x D x F); each token takes
     its top_k experts by logit (equal ones: the lower index) with softmax weights over them (renormalize) or over all
     experts.  ids (T x top_k int32) and weights (T x top_k fp32), where given, receive the routing."""
-    import torch
-
     T, D, ld, code = _rows16(X, "X")
     for t, what, dim in ((R, "R", 2), (W1, "W1", 3), (W2, "W2", 3)):
         if t.dtype != X.dtype or t.device != X.device or t.dim() != dim or not t.is_contiguous():

@@ -110,8 +110,10 @@ __device__ __forceinline__ uint16_t moe_bits16(float v, int bf16)
     return *reinterpret_cast<const uint16_t*>(&h);
 }
 
-// The other blocks' parts of a split tile added to this block's own (a: the two weight blocks' rows, 8 tokens from c0),
-// all in block order so that the bits do not depend on who is last; up to four parts' loads in flight.
+// The parts of a split tile summed (a: this block's own part, the two weight blocks' rows, 8 tokens from c0), in block
+// order so that the bits do not depend on who is last.  Two parts' loads are in flight at once, unconditional ones (a
+// load under a condition is waited for before the next is issued): this block's own slot, parts past the last and
+// tokens past the last group of four are read from a slot or group that exists and left out of the sum.
 __device__ __forceinline__ void moe_sum_parts(const MoeParams& p, const MoeSeg& g, int c, int row, int c0, int tq,
                                               float (&a)[2][8])
 {
@@ -123,37 +125,31 @@ __device__ __forceinline__ void moe_sum_parts(const MoeParams& p, const MoeSeg& 
             own[w][j] = a[w][j];
             a[w][j] = 0.f;
         }
+    const int g0 = c0 / 4, g1 = min(g0 + 1, tq - 1);  // the groups of four tokens
 #pragma unroll 1
-    for (int b0 = g.first; b0 < g.first + g.nseg; b0 += 4) {
-        float4 v[4][2][2];
+    for (int b0 = g.first; b0 < g.first + g.nseg; b0 += 2) {
+        float4 v[2][2][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int b = b0 + i;
-            if (b >= g.first + g.nseg || b == c) continue;
+        for (int i = 0; i < 2; ++i) {
+            const int b = min(b0 + i, g.first + g.nseg - 1);
             const float4* src = reinterpret_cast<const float4*>(p.partials + (size_t)moe_slot(g, b) * p.slot_floats) + row;
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (c0 + 4 * j < p.T) v[i][w][j] = __ldcg(src + (size_t)(w * tq + c0 / 4 + j) * 128);
+            for (int w = 0; w < 2; ++w) {
+                v[i][w][0] = __ldcg(src + (size_t)(w * tq + g0) * 128);
+                v[i][w][1] = __ldcg(src + (size_t)(w * tq + g1) * 128);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const int b = b0 + i;
-            if (b >= g.first + g.nseg) break;
+            const bool in = b < g.first + g.nseg, mine = b == c;
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    if (b == c) {
+                    const float u[4] = {v[i][w][j].x, v[i][w][j].y, v[i][w][j].z, v[i][w][j].w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[w][4 * j + e] += own[w][4 * j + e];
-                    } else if (c0 + 4 * j < p.T) {
-                        a[w][4 * j] += v[i][w][j].x;
-                        a[w][4 * j + 1] += v[i][w][j].y;
-                        a[w][4 * j + 2] += v[i][w][j].z;
-                        a[w][4 * j + 3] += v[i][w][j].w;
-                    }
+                    for (int e = 0; e < 4; ++e) a[w][4 * j + e] += mine ? own[w][4 * j + e] : in ? u[e] : 0.f;
                 }
         }
     }
@@ -200,14 +196,24 @@ __device__ __noinline__ void moe_sum_down(const MoeParams& p, const MoeSeg& g, i
         const int x = base + lane % per;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (x < i1) {
-#pragma unroll 16
-            for (int b = g.first + sub; b < g.first + g.nseg; b += 1 << ls) {
-                const float4 u =
-                    __ldcg(reinterpret_cast<const float4*>(p.partials + (size_t)moe_slot(g, b) * p.slot_floats) + x);
-                v.x += u.x;
-                v.y += u.y;
-                v.z += u.z;
-                v.w += u.w;
+            // eight parts' loads in flight: unconditional ones (past the last part, the last again), since a load
+            // under a condition is waited for before the next is issued
+#pragma unroll 1
+            for (int b0 = g.first + sub; b0 < g.first + g.nseg; b0 += 8 << ls) {
+                float4 u[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int b = min(b0 + (j << ls), g.first + g.nseg - 1);
+                    u[j] = __ldcg(reinterpret_cast<const float4*>(p.partials + (size_t)moe_slot(g, b) * p.slot_floats) + x);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool in = b0 + (j << ls) < g.first + g.nseg;
+                    v.x += in ? u[j].x : 0.f;
+                    v.y += in ? u[j].y : 0.f;
+                    v.z += in ? u[j].z : 0.f;
+                    v.w += in ? u[j].w : 0.f;
+                }
             }
         }
         for (int m = 16; m >= per; m >>= 1) {

@@ -692,6 +692,7 @@ inline float4 __ldcg(const float4* p)
     std::atomic_thread_fence(std::memory_order_acquire);
     return *p;
 }
+inline int min(int a, int b) { return a < b ? a : b; }
 inline void __stcg(float4* p, float4 v) { *p = v; }
 inline float __expf(float x) { return std::exp(x); }
 inline float __fdividef(float x, float y) { return x / y; }
