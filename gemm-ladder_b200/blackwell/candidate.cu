@@ -1,7 +1,7 @@
 // candidate.cu -- the Blackwell rung as the reference's candidate: the one .cu file the reference's judge, probe and
 // verif link with (judge/judge.cu:5-10,73; probe/probe.cu:38-40; hopper/verif.cu:35-41).
 //
-// The whole rung is compiled into this translation unit (kernels, host dispatch and the C ABI of include/bwgemm.h),
+// The rung's fp16 side is compiled into this translation unit (kernels, host dispatch and its C ABI of bwgemm.h),
 // so the candidate needs no library at run time, as the judge's launcher requires (judge/modal_judge.py:66-72).  It
 // defines the reference's C++ symbols over the C ABI:
 //   candidate_gemm   -> bw_gemm_f16_variant(..., g_var) under the reference's shape rule (M % 16, N % 64, K % 64);
@@ -18,6 +18,7 @@
 #include <cstdlib>
 
 #define BW_API extern "C"
+#define BW_FP16_ONLY  // the reference's candidate is the fp16 product: without the 8-bit and expert entries
 #include "../csrc/bwgemm.cu"
 
 int g_var = 0;

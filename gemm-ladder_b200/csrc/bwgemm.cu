@@ -581,7 +581,7 @@ BW_API const char* bw_status_string(int status)
     case BW_ERR_TIMEOUT: return "a bounded wait on a barrier gave up (see bw_gemm_status)";
     case BW_ERR_ARG: return "bad argument (null or misaligned pointer, unknown variant)";
     case BW_ERR_DEVICE: return "the current device is not an sm_100 GPU";
-    case BW_ERR_SCRATCH: return "the call needs more scratch than the no-allocation entry's fixed array holds";
+    case BW_ERR_SCRATCH: return "the call needs more scratch than it has (the no-allocation entry's fixed array, or the caller's workspace)";
     default: return "unknown status";
     }
 }
@@ -669,11 +669,13 @@ BW_API int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw
     return bw::make_plan(M, N, K, d->sms, d->pairs, variant, out, 0u, bw::held_of(*d));
 }
 
+#ifndef BW_FP16_ONLY  // (candidate.cu: the reference's candidate is the fp16 product alone)
 // ------------------------------------------------------------------ the 8-bit integer entries
 #include "gemm_i8.cuh"
 
 // ------------------------------------------------------------------ the mixture-of-experts layer
 #include "moe_mlp.cuh"
+#endif
 
 #ifdef BW_TRACE
 // The timeline of the last launch (a -DBW_TRACE build only; not part of the C ABI of bwgemm.h).

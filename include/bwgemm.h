@@ -28,7 +28,8 @@ extern "C" {
 #define BW_ERR_TIMEOUT 3   /* a kernel's bounded wait on a barrier gave up; see bw_gemm_status */
 #define BW_ERR_ARG 4       /* null or misaligned pointer, unknown variant */
 #define BW_ERR_DEVICE 5    /* the current device is not an sm_100 (B200-class) GPU */
-#define BW_ERR_SCRATCH 6   /* bw_gemm_f16_noalloc: no plan's scratch fits its fixed array (whole tiles always do) */
+#define BW_ERR_SCRATCH 6   /* bw_gemm_f16_noalloc: no plan's scratch fits its fixed array (whole tiles always do);
+                              the 8-bit and expert entries: the caller's workspace is too small */
 
 /* Kernels of the rule (bw_plan.kernel). */
 #define BW_KERNEL_TILE 0   /* 128 x bn tiles of C, A as the MMA's A operand */
