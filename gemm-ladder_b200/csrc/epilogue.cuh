@@ -24,6 +24,8 @@ __device__ __forceinline__ float i8_value(float bits, float row_scale, float col
 // TILE and PAIR keep the scales of a tile in shared memory (in the place of the swap-AB transpose buffers, `cst`): its BN
 // column scales, then the block's 128 row scales, loaded while the tile's MMAs run (0 outside C).
 __device__ __forceinline__ const float* i8_scales(const __half* cst) { return reinterpret_cast<const float*>(cst); }
+// Swap-AB: the tokens' scales, after the transpose buffers.
+__device__ __forceinline__ float* i8_token_scales(__half* cst) { return reinterpret_cast<float*>(cst + 2 * 16 * 128); }
 template <int BN>
 __device__ __forceinline__ void i8_load_scales(const Params& p, __half* cst, int m0, int n0)
 {
@@ -135,11 +137,9 @@ __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int
         if constexpr (epi_i8(EPI)) {  // the lane's column scale, the chunk's 16 row scales
             const int wb = BT ? c0 / BT : 0, tok = c0 - wb * BT, n = n0 + wb * 128 + lane;
             const float cs = n < s.N ? __ldg(p.col_scale + n) : 0.f;
+            const float* rs = i8_token_scales(cst) + tok;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float rs = tok + j < s.M ? __ldg(p.row_scale + tok + j) : 0.f;
-                buf[j * 128 + lane] = half_bits<EPI>(p, i8_value(v[j], rs, cs));
-            }
+            for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = half_bits<EPI>(p, i8_value(v[j], rs[j], cs));
         } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = __float2half_rn(v[j]);
@@ -285,20 +285,22 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 // 16 tokens' activations of output column n0 / 2 + row (swap-AB), from the gate and up sums: a warp's 32 lanes write 64
 // contiguous bytes of each token's row.
 __device__ __forceinline__ void i8_swiglu_store16(const Params& p, const float (&g)[16], const float (&u)[16], int c0,
-                                                  int n0, int row, float gs, float us)
+                                                  int n0, int row, const float* rs, float gs, float us)
 {
     __half* C = static_cast<__half*>(p.C) + (size_t)c0 * (p.s.N / 2) + n0 / 2 + row;
+    __half h[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        if (c0 + j >= p.s.M) break;
-        const float rs = __ldg(p.row_scale + c0 + j);
-        C[(size_t)j * (p.s.N / 2)] =
-            half_bits<kEpiI8SwiGLU>(p, silu_mul(i8_value(g[j], rs, gs), i8_value(u[j], rs, us)));
-    }
+    for (int j = 0; j < 16; ++j)
+        h[j] = half_bits<kEpiI8SwiGLU>(p, silu_mul(i8_value(g[j], rs[c0 + j], gs), i8_value(u[j], rs[c0 + j], us)));
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (c0 + j < p.s.M) C[(size_t)j * (p.s.N / 2)] = h[j];
 }
 
+// gs, us (SWAP): the scales of the lane's gate and up columns.
 template <bool SWAP, int BN>
-__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row, const __half* cst)
+__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row, __half* cst,
+                                               float gs, float us)
 {
     const Sched& s = p.s;
     if constexpr (!SWAP) {
@@ -325,7 +327,6 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
         }
     } else {
         const bool in = n0 < s.N;  // N % 256 == 0: a tile is in C or outside
-        const float gs = in ? __ldg(p.col_scale + n0 + row) : 0.f, us = in ? __ldg(p.col_scale + n0 + 128 + row) : 0.f;
 #pragma unroll 1
         for (int c0 = 0; c0 < BN; c0 += 16) {
             uint32_t gr[16], ur[16];
@@ -338,7 +339,7 @@ __device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, 
                 g[j] = __uint_as_float(gr[j]);
                 u[j] = __uint_as_float(ur[j]);
             }
-            if (in) i8_swiglu_store16(p, g, u, c0, n0, row, gs, us);
+            if (in) i8_swiglu_store16(p, g, u, c0, n0, row, i8_token_scales(cst), gs, us);
         }
     }
 }
@@ -557,11 +558,10 @@ __device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, 
 // block's own from tensor memory when own_mine), exact in any order, then the activation.
 template <int BN>
 __device__ __noinline__ void i8_swiglu_reduce(const Params& p, int P, int tile, Fixup f, bool own_mine, uint32_t tbase,
-                                              int n0, int row)
+                                              int n0, int row, __half* cst, float gs, float us)
 {
     const Sched& s = p.s;
     if (n0 >= s.N) return;
-    const float gs = __ldg(p.col_scale + n0 + row), us = __ldg(p.col_scale + n0 + 128 + row);
 #pragma unroll 1
     for (int c0 = 0; c0 < BN; c0 += 16) {
         if (c0 >= s.M) break;  // the last group's padding
@@ -600,7 +600,7 @@ __device__ __noinline__ void i8_swiglu_reduce(const Params& p, int P, int tile, 
                     a[w][4 * j + 3] = part_add<kEpiI8>(a[w][4 * j + 3], v[w][j].w);
                 }
         }
-        i8_swiglu_store16(p, a[0], a[1], c0, n0, row, gs, us);
+        i8_swiglu_store16(p, a[0], a[1], c0, n0, row, i8_token_scales(cst), gs, us);
     }
 }
 

@@ -121,6 +121,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         *reduce_flag = 0;
         epi_go[0] = epi_go[1] = 0;
         *recv_flag = 0;
+        if constexpr (kKsplitBuf<BN, SWAP, EPI>) {
+            // the parts this block will receive into its own buffer, expected before any other block can send
+            if (kp && plan_ksplit_recv_bytes(BN, WM, s.ksplit) <= kPlanI8RecvBytes) {
+                const int n = ksplit_run(kr + 1, AN / 16, s.ksplit) - ksplit_run(kr, AN / 16, s.ksplit);
+                if (n) mbar_arrive_expect_tx(krecv, (uint32_t)((s.ksplit - 1) * n) * 8192u);
+            }
+        }
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0) {
@@ -473,8 +480,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release_acc(a);
             }
         };
+        if constexpr (epi_i8(EPI) && SWAP) {  // the tokens' scales, for every tile (read after the loop's barrier)
+            const int t = threadIdx.x - kEpiThread0;
+            i8_token_scales(cst)[t] = t < s.M ? __ldg(p.row_scale + t) : 0.f;
+        }
         for (;;) {
             if (!s.dyn && !it.next(s, P, sg)) break;
+            float col_scale[2] = {0.f, 0.f};  // swap-AB: this lane's columns of the tile's weight blocks
+            if constexpr (epi_i8(EPI) && SWAP) {
+#pragma unroll
+                for (int w = 0; w < WM; ++w) {
+                    const int n = (sg.tile * WM + w) * 128 + row;
+                    if (n < s.N) col_scale[w] = __ldg(p.col_scale + n);
+                }
+            }
             if constexpr (epi_i8(EPI) && !SWAP) {  // the tile's scales, while its MMAs run
                 int tm, tn;
                 tile_coords(s, sg.tile, tm, tn);
@@ -532,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release_all(acc);
             } else if (EPI == kEpiI8SwiGLU && sg.k0 == 0 && sg.k1 == s.kblocks) {
                 if constexpr (EPI == kEpiI8SwiGLU) {
-                    i8_swiglu_tile<SWAP, BN>(p, tbase, m0, n0, row, cst);
+                    i8_swiglu_tile<SWAP, BN>(p, tbase, m0, n0, row, cst, col_scale[0], col_scale[1]);
                     release_all(acc);
                 }
             } else if (EPI == kEpiSwiGLU) {
@@ -575,7 +594,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int kc = s.ksplit;
                 const int own0 = ksplit_run(kr, kChunks, kc), own1 = ksplit_run(kr + 1, kChunks, kc);
                 const uint32_t recv_bytes = (uint32_t)((kc - 1) * (own1 - own0)) * 8192u;
-                if (threadIdx.x == kEpiThread0) {
+                // a buffer of its own (kKsplitBuf): expected at the start, free from the start, so nothing to agree on
+                const bool buf = kKsplitBuf<BN, SWAP, EPI> && plan_ksplit_recv_bytes(BN, WM, kc) <= kPlanI8RecvBytes;
+                const uint32_t recv_off = buf ? (uint32_t)G::kWindowOffset : 0u;
+                if (buf) {
+                } else if (threadIdx.x == kEpiThread0) {
                     if (recv_bytes) mbar_arrive_expect_tx(krecv, recv_bytes);
                     for (int o = 0; o < kc; ++o)
                         if (o != kr) mbar_arrive_cluster(mapa_shared(smem_u32(kgo), (uint32_t)o));
@@ -583,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (ok) fence_acq_rel_cluster();  // after the others' arrivals (release, cluster scope)
                     *reduce_flag = ok ? 1 : 0;
                 }
-                named_bar_sync(1, 128);
-                const bool go = *reduce_flag != 0;
+                if (!buf) named_bar_sync(1, 128);
+                const bool go = buf || *reduce_flag != 0;
                 if (threadIdx.x == kEpiThread0) {
                     BW_TRACE_AT(7);  // the others' rings are idle
                     BW_TRACE_VAL(8, 4 | kc << 8);
@@ -596,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const int o = ksplit_owner(ch, kChunks, kc);
                         const int r0 = ksplit_run(o, kChunks, kc), len = ksplit_run(o + 1, kChunks, kc) - r0;
                         const int piece = (kr < o ? kr : kr - 1) * len + (ch - r0);
-                        const uint32_t dst = mapa_shared(smem_u32(smem), (uint32_t)o) + (uint32_t)piece * 8192u +
+                        const uint32_t dst = mapa_shared(smem_u32(smem + recv_off), (uint32_t)o) + (uint32_t)piece * 8192u +
                                              (uint32_t)row * 16u;
                         const uint32_t bar = mapa_shared(smem_u32(krecv), (uint32_t)o);
                         uint32_t r[16];
@@ -623,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (threadIdx.x == kEpiThread0) BW_TRACE_AT(10);  // the others' parts of this block's chunks are in
                 if (have) {
-                    const float4* ring = reinterpret_cast<const float4*>(smem) + row;  // [piece][col / 4][row][4]
+                    const float4* ring = reinterpret_cast<const float4*>(smem + recv_off) + row;  // [piece][col / 4][row][4]
 #pragma unroll 1
                     for (int ch = own0; ch < own1; ++ch) {
                         float v[16];
@@ -777,7 +800,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (fast == 2) {
                     if constexpr (EPI == kEpiI8SwiGLU && SWAP)
-                        i8_swiglu_reduce<BN>(p, P, sg.tile, f, true, tbase, n0, row);
+                        i8_swiglu_reduce<BN>(p, P, sg.tile, f, true, tbase, n0, row, cst, col_scale[0],
+                                             col_scale[1]);
                     else if (bulk)
                         reduce_tile_bulk<AN, SWAP, R, G::kMaxSum, EPI, BN>(p, P, sg.tile, rank, f, true, tbase, row, m0, n0,
                                                                   cst, smem, rbar, abort_flag, seg);
@@ -816,7 +840,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             BW_TRACE_VAL(8, 1 | f.nseg << 8 | seg << 16);
                         }
                         if constexpr (EPI == kEpiI8SwiGLU && SWAP)
-                            i8_swiglu_reduce<BN>(p, P, sg.tile, f, last_seg, tbase, n0, row);
+                            i8_swiglu_reduce<BN>(p, P, sg.tile, f, last_seg, tbase, n0, row, cst, col_scale[0],
+                                                 col_scale[1]);
                         else if (bulk)
                             reduce_tile_bulk<AN, SWAP, R, G::kMaxSum, EPI, BN>(p, P, sg.tile, rank, f, true, tbase, row, m0, n0,
                                                                       cst, smem, rbar, abort_flag, seg);

@@ -91,7 +91,7 @@ __device__ unsigned long long g_trace[1024 * kTraceSlots];
 #endif
 
 // RSV: bytes of shared memory reserved after the stage ring (the fused reduce-scatter's window).
-// I8: an 8-bit entry (TILE and PAIR stage a tile's column scales and the block's row scales for the epilogue).
+// I8: an 8-bit entry (its epilogue's scales are staged in shared memory).
 template <int BN, bool SWAP, bool PAIR, int WM = 1, int RSV = 0, bool I8 = false>
 struct Geom {
     static constexpr int kRanks = PAIR ? 2 : 1;
@@ -104,8 +104,9 @@ struct Geom {
     static constexpr int kXBytes = 128 * WM * kBK * 2;       // this block's MMA-A operand: 128 (x WM) rows x 64 K
     static constexpr int kYBytes = (BN / kRanks) * kBK * 2;  // this block's MMA-B operand: BN (PAIR: BN / 2) x 64 K
     static constexpr int kStageBytes = kXBytes + kYBytes;
-    // swap-AB epilogue transpose buffers; the 8-bit TILE / PAIR epilogue's scales
-    static constexpr int kCStageBytes = SWAP ? 2 * 16 * 128 * 2 : I8 ? (BN + 128) * 4 : 0;
+    // swap-AB epilogue transpose buffers; the 8-bit epilogue's scales (of the tokens; TILE and PAIR: and of the columns)
+    static constexpr int kTransposeBytes = SWAP ? 2 * 16 * 128 * 2 : 0;
+    static constexpr int kCStageBytes = kTransposeBytes + (I8 ? (SWAP ? 128 : BN + 128) * 4 : 0);
     static constexpr int kRingFit = (BW_SMEM_LIMIT - 1024 - 512 - kCStageBytes - RSV) / kStageBytes;
     static constexpr int kStages = kRingFit < BW_MAX_STAGES ? kRingFit : BW_MAX_STAGES;
     static constexpr int kAccBufs = 2 * kAccN <= 512 ? 2 : 1;  // two accumulators, or one of 512 columns
@@ -139,9 +140,16 @@ struct Geom {
 // staging buffers for TMA stores of C (BW_EPI_TMA).
 template <int BN, bool SWAP, bool PAIR, int EPI>
 constexpr bool kEpiTma = BW_EPI_TMA && !SWAP && EPI == kEpiF16;
+// The 8-bit swap-AB instance of up to 16 tokens keeps a buffer for its cluster's parts (K split) beside the ring, so that
+// they can be sent without asking whether the ring is idle.
+template <int BN, bool SWAP, int EPI>
+constexpr bool kKsplitBuf = BW_KSPLIT && SWAP && BN == 16 && EPI == kEpiI8;
 template <int BN, bool SWAP, bool PAIR, int EPI, int WM = 1>
 using KGeom = Geom<BN, SWAP, PAIR, WM,
-                   EPI == kEpiRS ? kPlanRsWindowBytes : kEpiTma<BN, SWAP, PAIR, EPI> ? kPlanEpiStageBytes : 0,
+                   EPI == kEpiRS                         ? kPlanRsWindowBytes
+                   : kEpiTma<BN, SWAP, PAIR, EPI>        ? kPlanEpiStageBytes
+                   : kKsplitBuf<BN, SWAP, EPI>           ? kPlanI8RecvBytes
+                                                         : 0,
                    epi_i8(EPI)>;
 
 // The 3-D form for the MN-major operand (BW_TMA3D): `n64` is the first 64-column block; the map's box holds the

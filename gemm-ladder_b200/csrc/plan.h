@@ -197,11 +197,17 @@ inline const char* variant_name(int v)
 // The kernels' geometry, as gemm_kernel.cuh's Geom computes it (checked against it at launch in bwgemm.cu): the ring
 // takes what the 227 KB leave after the alignment slack, the barriers and the swap-AB epilogue's transpose buffers.
 inline int plan_stage_bytes(int bn, int ranks, int wm = 1) { return 128 * wm * 64 * 2 + (bn / ranks) * 64 * 2; }
-inline int plan_cstage_bytes(bool swap, int i8_bn = 0) { return swap ? 2 * 16 * 128 * 2 : i8_bn ? (i8_bn + 128) * 4 : 0; }
+inline int plan_cstage_bytes(bool swap, int i8_bn = 0)
+{
+    return (swap ? 2 * 16 * 128 * 2 : 0) + (i8_bn ? (swap ? 128 : i8_bn + 128) * 4 : 0);
+}
 // The fused reduce-scatter's window (two 32 KB buffers) for the owner's partials, after the stage ring.
 constexpr int kPlanRsWindowBytes = 2 * 32768;
 // The TMA-store epilogue's staging (BW_EPI_TMA): two buffers of 128 rows x 64 fp16 columns, after the stage ring.
 constexpr int kPlanEpiStageBytes = 2 * 16384;
+// The 8-bit swap-AB kernel of up to 16 tokens: the buffer for the parts of a K-split cluster (of up to 5 blocks; larger
+// clusters use the idle ring).
+constexpr int kPlanI8RecvBytes = 4 * 8192;
 // Entries of a block's queue of units (BW_DYN_UNITS: its producer takes units and passes them to the MMA issuer and the
 // epilogue), each with a full and an empty barrier.
 constexpr int kPlanUnitQ = 4;
@@ -229,7 +235,7 @@ inline int plan_smem_bytes(int bn, int ranks, bool swap, int wm = 1, int reserve
 // A K-split cluster of c blocks (swap-AB): the bytes one block receives into its idle stage ring.  BW_KSPLIT 0: the
 // second block's whole accumulator (128 x bn x wm fp32) at the first.  BW_KSPLIT 1: the other c - 1 blocks' parts
 // of the longest run of 16-column chunks (8 KB each) that one block owns (runs of floor or ceil(chunks / c)).
-inline int plan_ksplit_recv_bytes(int bn, int wm, int c)
+BW_HD inline int plan_ksplit_recv_bytes(int bn, int wm, int c)
 {
     if (!BW_KSPLIT) return 128 * bn * wm * 4;
     const int chunks = bn * wm / 16;
@@ -408,6 +414,8 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
         ks = ks_wm ? 2 : 0;
 #endif
     }
+    const bool i8 = flags & kPlanI8;
+    const int i8_recv = i8 && BW_KSPLIT && swap && q.bn == 16 && !(flags & kPlanGateUp) ? kPlanI8RecvBytes : 0;
     if (ks) {
         q.ksplit = ks;
         q.wm = ks_wm;
@@ -417,8 +425,8 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
         q.sk_tiles = q.tiles;
         q.splits = ks;
         q.grid = ks * q.tiles;
-        q.stages = plan_stages(q.bn, 1, true, q.wm);
-        q.smem_bytes = plan_smem_bytes(q.bn, 1, true, q.wm);
+        q.stages = plan_stages(q.bn, 1, true, q.wm, i8_recv, i8);
+        q.smem_bytes = plan_smem_bytes(q.bn, 1, true, q.wm, i8_recv, i8);
         q.tmem_cols = plan_tmem_cols(q.bn * q.wm);
         *p = q;
         return BW_OK;
@@ -452,7 +460,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     const size_t dyn_split_bytes = (size_t)q.tiles * 128 * q.bn * q.wm * sizeof(float);  // one partial of every tile
     int dyn_splits = (q.kblocks + BW_DYN_UNIT_KB - 1) / BW_DYN_UNIT_KB;
     if ((size_t)dyn_splits * dyn_split_bytes > BW_DYN_MAX_BYTES) dyn_splits = (int)(BW_DYN_MAX_BYTES / dyn_split_bytes);
-    const bool dyn = BW_DYN_UNITS && swap && stream_k && q.kernel == BW_KERNEL_SWAP && (variant == 0 || variant == 3) &&
+    const bool dyn = BW_DYN_UNITS && !i8 && swap && stream_k && q.kernel == BW_KERNEL_SWAP && (variant == 0 || variant == 3) &&
                      q.bn * q.wm <= BW_DYN_MAX_COLS && dyn_splits >= 2 && q.tiles % units != 0 &&
                      (!work_cap || dyn_splits * dyn_split_bytes <= work_cap);
     if (variant == 1 || q.tiles % units == 0) {
@@ -499,8 +507,7 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
     q.grid = P * ranks;
     // shared memory after the ring: the fused reduce-scatter's window, or the fp16 TILE / PAIR epilogue's staging
     const bool epi_tma = BW_EPI_TMA && !swap && !(flags & (kPlanNoSwap | kPlanRsWindow | kPlanI8));
-    const int reserve = (flags & kPlanRsWindow) ? kPlanRsWindowBytes : epi_tma ? kPlanEpiStageBytes : 0;
-    const bool i8 = flags & kPlanI8;
+    const int reserve = (flags & kPlanRsWindow) ? kPlanRsWindowBytes : epi_tma ? kPlanEpiStageBytes : i8_recv;
     q.stages = plan_stages(q.bn, ranks, swap, q.wm, reserve, i8);
     q.smem_bytes = plan_smem_bytes(q.bn, ranks, swap, q.wm, reserve, i8);
     q.tmem_cols = plan_tmem_cols(q.bn * q.wm);

@@ -142,3 +142,25 @@ def test_python_refuses_tensors_it_cannot_pass_on():
                  lambda: bwgemm.gemm_i8(w, s, w, s, dtype=torch.float64)):
         with pytest.raises(ValueError):  # host tensors, types
             call()
+
+
+@pytest.mark.parametrize("late", [0, 1])
+@pytest.mark.parametrize("force", [2 * 16 + 1, 3 * 16 + 2, 5 * 16 + 1, 6 * 16 + 2, 8 * 16 + 1])
+def test_emulated_k_split_into_the_buffer_or_the_ring(emu, force, late):
+    """Clusters of up to 5 blocks send their parts into a buffer that is expected from the start; larger ones into the idle
+    ring, once it is.  late: the first block of every cluster starts late, so that the others' parts are sent before it
+    runs."""
+    c, wm = force // 16, force % 16
+    rng = np.random.default_rng(force)
+    M, N, K = 11, 256 * wm, 4096
+    A = rng.integers(-127, 128, (M, K), dtype=np.int8)
+    B = rng.integers(-127, 128, (N, K), dtype=np.int8)
+    sa, sb = np.full(M, 1e-2, np.float32), np.full(N, 1e-3, np.float32)
+    emu.bw_emu_set(b"force_ksplit", ctypes.c_longlong(force))
+    emu.bw_emu_set(b"lead_skew_us", ctypes.c_longlong(200000 * late))
+    try:
+        got = emulate_i8(emu, A, sa, B, sb, 2 * c, F16, 0)
+    finally:
+        emu.bw_emu_set(b"force_ksplit", ctypes.c_longlong(0))
+        emu.bw_emu_set(b"lead_skew_us", ctypes.c_longlong(0))
+    assert len(i8_ref.outside(got, i8_ref.product(A, sa, B, sb), "fp16")) == 0
