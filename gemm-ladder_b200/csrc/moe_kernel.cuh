@@ -519,9 +519,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 }
                 named_bar_sync(1, kMoeEpiThreads);  // every thread's part is written (and epi_sum read)
                 if (threadIdx.x == kMoeEpiThread0) {
-                    __threadfence();  // cumulative: the other threads' stores, ordered before by the barrier, too
-                    const int old = atomicAdd(counter, 1);
-                    __threadfence();
+                    const int old = atom_add_acq_rel_gpu(counter, 1);  // after every thread's stores (the barrier)
                     epi_sum[seg & 1] = sg.phase == 0 && old == sg.nseg - 1 ? 1 : 0;
                 }
                 if (sg.phase == 0) {  // the last block of a split gate/up tile sums it
@@ -567,8 +565,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 if (sg.phase == 0) {
                     named_bar_sync(1, kMoeEpiThreads);
                     if (threadIdx.x == kMoeEpiThread0) {
-                        __threadfence();  // h before the count
-                        atomicAdd(p.ready + sl, 1);
+                        red_add_release_gpu(p.ready + sl, 1);  // h before the count
                         BW_TRACE_AT(8);  // this block's last gate/up tile is done
                     }
                 }

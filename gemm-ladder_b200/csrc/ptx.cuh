@@ -431,6 +431,19 @@ __device__ __forceinline__ int ld_acquire_gpu(const int* p)
     return v;
 }
 
+// Adds at gpu scope that order this thread's earlier accesses -- and, by cumulativity, those of the threads it has met at a
+// barrier -- before the add (release), and the add before its later ones (acquire); the red form returns nothing.
+__device__ __forceinline__ int atom_add_acq_rel_gpu(int* p, int v)
+{
+    int old;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
+}
+__device__ __forceinline__ void red_add_release_gpu(int* p, int v)
+{
+    asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
 // ------------------------------------------------------------------ system scope: flags in another GPU's memory
 // (reached through a CUDA IPC mapping over NVLink) or in this GPU's memory written by another GPU
 __device__ __forceinline__ unsigned ld_acquire_sys(const unsigned* p)

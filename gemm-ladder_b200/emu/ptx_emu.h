@@ -281,6 +281,8 @@ constexpr uint32_t idesc_i8_s32(int m, int n)
 
 // ------------------------------------------------------------------ global memory ordering, named barriers
 inline int ld_acquire_gpu(const int* p) { return __atomic_load_n(p, __ATOMIC_ACQUIRE); }
+inline int atom_add_acq_rel_gpu(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_ACQ_REL); }
+inline void red_add_release_gpu(int* p, int v) { __atomic_fetch_add(p, v, __ATOMIC_RELEASE); }
 inline void named_bar_sync(uint32_t id, uint32_t count) { emu::named_sync((int)id, (int)count); }
 
 }  // namespace bw
