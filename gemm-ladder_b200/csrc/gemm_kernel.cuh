@@ -826,12 +826,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // at the last segment the accumulator stays (no later MMA needs it): the reduction reads this
                     // block's own partial from tensor memory
                     if (!last_seg) release_all(acc);
-                    __threadfence();
+                    // (kEpiI8*: one release / acquire add, ordered after every thread's stores by the barrier, in place
+                    // of fences that each wait behind the loads in flight)
+                    if constexpr (!epi_i8(EPI)) __threadfence();
                     named_bar_sync(1, 128);
                     if (threadIdx.x == kEpiThread0) {
-                        const int old = atomicAdd(counter, 1);
-                        if (old == f.nseg - 1) __threadfence();
-                        *reduce_flag = old == f.nseg - 1 ? 1 : 0;
+                        if constexpr (epi_i8(EPI)) {
+                            *reduce_flag = atom_add_acq_rel_gpu(counter, 1) == f.nseg - 1 ? 1 : 0;
+                        } else {
+                            const int old = atomicAdd(counter, 1);
+                            if (old == f.nseg - 1) __threadfence();
+                            *reduce_flag = old == f.nseg - 1 ? 1 : 0;
+                        }
                     }
                     named_bar_sync(1, 128);
                     if (*reduce_flag == 1) {
