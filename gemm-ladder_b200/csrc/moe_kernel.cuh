@@ -16,7 +16,7 @@
 //   - both products are cut evenly over the blocks by K-blocks (moe_sched.h); split tiles are summed in block order
 //     (the same bits on every run).
 //   - between the products a block waits for the activations it needs, by active expert, but only its token-side loads
-//     do: the weights of W2 are already on their way into the ring (up to 200 KB per SM, 30 MB in all), so the wait
+//     do: the weights of W2 are already on their way into the ring (up to 175 KB per SM, 26 MB in all), so the wait
 //     costs no memory time.
 // Roles: one thread of warp 0 the weights' producer, one of warp 10 the tokens', one of warp 1 the MMA issuer, warps 2-9
 // the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
@@ -36,7 +36,8 @@ namespace bw {
 constexpr int kMoeThreads = 352;  // 11 warps
 constexpr int kMoeEpiThreads = 256;
 constexpr int kMoeXBytes = 32768; // a stage's weights: 256 rows x 64 values
-constexpr int kMoeMaxStages = 6;
+constexpr int kMoeMaxStages = 5;  // as fast as 6 or 1 % faster from 1 to 16 tokens (3: up to 5 % slower): deeper rings make
+                                   // the counts and partials queue behind more weights in flight
 constexpr int kMoeEpiThread0 = 64;
 
 struct MoeParams {
@@ -57,12 +58,13 @@ struct MoeParams {
 
 // Shared memory after the ring (offsets from its end).
 struct MoeSmem {
-    static constexpr int kBars = 0;  // weights in, tokens in, empty (6 each), tfull, tempty (2 each), drain
-    static constexpr int kMisc = kBars + (3 * kMoeMaxStages + 5) * 8 + 8;  // tmem slot, flags
+    static constexpr int kBars = 0;  // weights in, tokens in, empty (5 each), tfull, tempty (2 each), drain
+    static constexpr int kMisc = (kBars + (3 * kMoeMaxStages + 5) * 8 + 15) / 16 * 16;  // tmem slot, flags
     static constexpr int kMask = kMisc + 64;                       // a bit per expert
     static constexpr int kExpert = kMask + kMoeMaxExperts / 8;     // the active experts, 16 bits each
     static constexpr int kGate = kExpert + 2 * kMoeMaxExperts;     // p of every token for the epilogue's expert (on 16 bytes)
     static constexpr int kBytes = kGate + 4 * kMoeMaxTokens;
+    static_assert(kGate % 16 == 0, "read by 16 bytes");
 };
 __host__ __device__ constexpr int moe_stage_bytes(int tp) { return kMoeXBytes + tp * 128; }
 __host__ __device__ constexpr int moe_stages(int tp)
