@@ -354,8 +354,14 @@ inline int make_plan(int M, int N, int K, int sms, int pairs, int variant, bw_pl
         q.bn = variant == 6 ? 64 : variant == 7 ? 128 : 256;
         ranks = pair ? 2 : 1;
         units = pair ? pairs : sms;
+        // 8 bits: 128 x 128 tiles on single SMs where one wave holds them all.  The pair tiles they replace leave half
+        // the GPU idle or split K (measured at 1001 x 2304: 11.5 against 14.0 us at K = 1104, 29 against 37 at 8192, 50
+        // against 51 at 16384), except for a long K that the pair tiles, split in two, fill the pairs with (82 against 68
+        // us at 1001 x 2304 x 28672; 640 x 3584 x 28672, whose pair tiles do not fit twice: 81 against 127)
+        const int t2 = (M + 255) / 256 * ((N + 255) / 256);
         if ((flags & kPlanI8) && !(flags & (kPlanGateUp | kPlanNoSwap)) && pair && sms > 0 &&
-            (long long)((M + 127) / 128) * ((N + 127) / 128) <= sms) {
+            (long long)((M + 127) / 128) * ((N + 127) / 128) <= sms &&
+            !(q.kblocks > 128 && 2 * t2 <= units && 8 * t2 >= 3 * units)) {
             q.kernel = BW_KERNEL_TILE;
             q.bn = 128;
             ranks = 1;
