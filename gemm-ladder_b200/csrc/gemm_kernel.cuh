@@ -47,7 +47,7 @@ namespace bw {
 template <int BN, bool SWAP, bool PAIR, int EPI = kEpiF16, int WM = 1>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy,
-                const __grid_constant__ CUtensorMap tmc, const Params p)
+                const __grid_constant__ CUtensorMap tmc, const KParams<EPI> p)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     constexpr int AN = G::kAccN;  // accumulator columns (TMEM)

@@ -65,12 +65,35 @@ struct Params {
                                       // than wait_ns: the ranks' processes reach their first call out of step
     int tn;                      // 1: B is N x K row-major (K-major for the tensor core, like A); 0: K x N
     const RsTable* rs;           // kEpiRS only: the ranks' regions
-    const float* row_scale;      // kEpiI8*: M scales of A's rows
-    const float* col_scale;      // kEpiI8*: N scales of B's rows (C's columns)
-    int out_bf16;                // kEpiI8, kEpiI8SwiGLU: C in bf16 (0: fp16)
-    int early_weights;           // kEpiI8* swap-AB: the weights were complete before the kernel this one waits for
-                                 // (griddep_wait) began, so their first loads need not wait for it
 };
+
+// What the 8-bit kernels take besides.  A type of its own: 24 bytes more in Params made the fp16 kernels 2 to 5 % slower
+// (the copy that their out-of-line reductions read grows with it).
+struct ParamsI8 : Params {
+    const float* row_scale;      // M scales of A's rows
+    const float* col_scale;      // N scales of B's rows (C's columns)
+    int out_bf16;                // kEpiI8, kEpiI8SwiGLU: C in bf16 (0: fp16)
+    int early_weights;           // swap-AB: the weights were complete before the kernel this one waits for (griddep_wait)
+                                 // began, so their first loads need not wait for it
+};
+template <int EPI>
+struct ParamsOf {
+    using type = Params;
+};
+template <>
+struct ParamsOf<kEpiI8> {
+    using type = ParamsI8;
+};
+template <>
+struct ParamsOf<kEpiI8F32> {
+    using type = ParamsI8;
+};
+template <>
+struct ParamsOf<kEpiI8SwiGLU> {
+    using type = ParamsI8;
+};
+template <int EPI>
+using KParams = typename ParamsOf<EPI>::type;
 
 __host__ __device__ constexpr int pow2_at_least(int v, int p) { return p >= v ? p : pow2_at_least(v, 2 * p); }
 

@@ -9,7 +9,7 @@ namespace bw {
 namespace {
 
 template <int EPI, int WM>
-int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p)
+int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p)
 {
     switch (q.bn) {
     case 16: return launch<16, true, false, EPI, WM>(q, mx, my, mx, p);
@@ -24,7 +24,7 @@ int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& m
     }
 }
 
-int dispatch_i8(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p, int epi)
+int dispatch_i8(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p, int epi)
 {
     if (q.kernel == BW_KERNEL_PAIR) {
         if (epi == kEpiI8F32) return launch<256, false, true, kEpiI8F32, 1>(q, mx, my, mx, p);
@@ -62,7 +62,8 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     std::vector<int> counters((size_t)q.counters + 1, 0);
     CUtensorMap mx, my;
     make_maps(q, A, B, M, N, K / 2, &mx, &my, true);
-    Params p = make_params(q, M, N, q.kblocks * 64, C, work.data(), counters.data(), true);
+    ParamsI8 p = {};
+    static_cast<Params&>(p) = make_params(q, M, N, q.kblocks * 64, C, work.data(), counters.data(), true);
     p.row_scale = a_scale;
     p.col_scale = b_scale;
     p.out_bf16 = out_type == BW_TYPE_BF16;
