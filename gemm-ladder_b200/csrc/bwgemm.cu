@@ -256,7 +256,7 @@ const int* held_of(const DeviceState& d) { return BW_KSPLIT ? d.held : nullptr; 
 
 template <int BN, bool SWAP, bool PAIR, int EPI = kEpiF16, int WM = 1>
 int launch_kernel(DeviceState& d, unsigned long long bit, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my,
-                  const CUtensorMap& mc, const KParams<EPI>& p, cudaStream_t st, bool pdl = false)
+                  const CUtensorMap& mc, const Params& p, cudaStream_t st, bool pdl = false)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     // K split: what a block receives from the others of its cluster lands in its idle stage ring

@@ -27,13 +27,13 @@ __device__ __forceinline__ const float* i8_scales(const __half* cst) { return re
 // Swap-AB: the tokens' scales, after the transpose buffers.
 __device__ __forceinline__ float* i8_token_scales(__half* cst) { return reinterpret_cast<float*>(cst + 2 * 16 * 128); }
 template <int BN>
-__device__ __forceinline__ void i8_load_scales(const ParamsI8& p, __half* cst, int m0, int n0)
+__device__ __forceinline__ void i8_load_scales(const Params& p, __half* cst, int m0, int n0)
 {
     float* to = reinterpret_cast<float*>(cst);
     const int t = threadIdx.x - kEpiThread0;
 #pragma unroll
-    for (int i = 0; i < BN; i += 128) to[i + t] = n0 + i + t < p.s.N ? __ldg(p.col_scale + n0 + i + t) : 0.f;
-    to[BN + t] = m0 + t < p.s.M ? __ldg(p.row_scale + m0 + t) : 0.f;
+    for (int i = 0; i < BN; i += 128) to[i + t] = n0 + i + t < p.s.N ? __ldg(i8_col_scale(p) + n0 + i + t) : 0.f;
+    to[BN + t] = m0 + t < p.s.M ? __ldg(i8_row_scale(p) + m0 + t) : 0.f;
 }
 // NC columns of a row: the scaled values (cs: their column scales, 16-byte aligned).
 template <int NC>
@@ -61,13 +61,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b)
     return *reinterpret_cast<const uint32_t*>(&x);
 }
 template <int EPI>
-__device__ __forceinline__ bool i8_bf16(const KParams<EPI>& p)
+__device__ __forceinline__ bool i8_bf16(const Params& p)
 {
-    if constexpr (epi_i8(EPI)) return p.out_bf16 != 0;
-    return false;
+    return epi_i8(EPI) && (p.tn & kI8OutBf16);
 }
 template <int EPI, int NP>
-__device__ __forceinline__ void pack_pairs(const KParams<EPI>& p, const float (&v)[2 * NP], uint32_t (&h)[NP])
+__device__ __forceinline__ void pack_pairs(const Params& p, const float (&v)[2 * NP], uint32_t (&h)[NP])
 {
     if (i8_bf16<EPI>(p)) {
 #pragma unroll
@@ -78,7 +77,7 @@ __device__ __forceinline__ void pack_pairs(const KParams<EPI>& p, const float (&
     }
 }
 template <int EPI>
-__device__ __forceinline__ __half half_bits(const KParams<EPI>& p, float a)  // one value, as the 16 bits of a __half
+__device__ __forceinline__ __half half_bits(const Params& p, float a)  // one value, as the 16 bits of a __half
 {
     if (i8_bf16<EPI>(p)) {
         const __nv_bfloat16 y = __float2bfloat16_rn(a);
@@ -96,7 +95,7 @@ __device__ __forceinline__ __half half_bits(const KParams<EPI>& p, float a)  // 
 // chunk i + 2 is written only after every thread has passed the barrier of chunk i + 1, so after it read chunk i.
 // Integer sums (kEpiI8*), not swapped: the values scaled from `cst` (BT: the tile's columns), then as the others.
 template <bool SWAP, int EPI = kEpiF16, int BT = 0>
-__device__ __forceinline__ void store_chunk(const KParams<EPI>& p, int m0, int n0, int lane, int c0, const float (&v)[16],
+__device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int lane, int c0, const float (&v)[16],
                                             __half* cst)
 {
     const Sched& s = p.s;
@@ -142,7 +141,7 @@ __device__ __forceinline__ void store_chunk(const KParams<EPI>& p, int m0, int n
         __half* buf = cst + ((c0 >> 4) & 1) * (16 * 128);
         if constexpr (epi_i8(EPI)) {  // the lane's column scale, the chunk's 16 row scales
             const int wb = BT ? c0 / BT : 0, tok = c0 - wb * BT, n = n0 + wb * 128 + lane;
-            const float cs = n < s.N ? __ldg(p.col_scale + n) : 0.f;
+            const float cs = n < s.N ? __ldg(i8_col_scale(p) + n) : 0.f;
             const float* rs = i8_token_scales(cst) + tok;
 #pragma unroll
             for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = half_bits<EPI>(p, i8_value(v[j], rs[j], cs));
@@ -196,7 +195,7 @@ __device__ __forceinline__ void transpose_pieces(uint32_t (&x)[P][4], int lane)
 }
 
 template <int EPI>
-__device__ __forceinline__ void store_lines64(const KParams<EPI>& p, int r0, int n, int lane, const float (&v)[64])
+__device__ __forceinline__ void store_lines64(const Params& p, int r0, int n, int lane, const float (&v)[64])
 {
     constexpr bool kF32 = EPI == kEpiF32 || EPI == kEpiI8F32;
     constexpr int P = kF32 ? 16 : 8;
@@ -231,7 +230,7 @@ __device__ __forceinline__ void store_lines64(const KParams<EPI>& p, int r0, int
 }
 
 template <int EPI>
-__device__ __forceinline__ void store_rows64(const KParams<EPI>& p, int r0, int n, int lane, const float (&v)[64])
+__device__ __forceinline__ void store_rows64(const Params& p, int r0, int n, int lane, const float (&v)[64])
 {
     static_assert(EPI == kEpiF16 || EPI == kEpiF32, "fp16 or fp32 C");
     store_lines64<EPI>(p, r0, n, lane, v);
@@ -239,7 +238,7 @@ __device__ __forceinline__ void store_rows64(const KParams<EPI>& p, int r0, int 
 
 // The 64 columns' integer sums (kEpiI8, kEpiI8F32), scaled, the same way.
 template <int EPI>
-__device__ __forceinline__ void store_rows64_i8(const KParams<EPI>& p, int r0, int n, int lane, const float (&sum)[64],
+__device__ __forceinline__ void store_rows64_i8(const Params& p, int r0, int n, int lane, const float (&sum)[64],
                                                 float rs, const float* cs)
 {
     if (n >= p.s.N) return;  // N % 64 == 0: the 64 columns are all in C or all outside
@@ -290,7 +289,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 
 // 16 tokens' activations of output column n0 / 2 + row (swap-AB), from the gate and up sums: a warp's 32 lanes write 64
 // contiguous bytes of each token's row.
-__device__ __forceinline__ void i8_swiglu_store16(const ParamsI8& p, const float (&g)[16], const float (&u)[16], int c0,
+__device__ __forceinline__ void i8_swiglu_store16(const Params& p, const float (&g)[16], const float (&u)[16], int c0,
                                                   int n0, int row, const float* rs, float gs, float us)
 {
     __half* C = static_cast<__half*>(p.C) + (size_t)c0 * (p.s.N / 2) + n0 / 2 + row;
@@ -305,7 +304,7 @@ __device__ __forceinline__ void i8_swiglu_store16(const ParamsI8& p, const float
 
 // gs, us (SWAP): the scales of the lane's gate and up columns.
 template <bool SWAP, int BN>
-__device__ __forceinline__ void i8_swiglu_tile(const ParamsI8& p, uint32_t tbase, int m0, int n0, int row, __half* cst,
+__device__ __forceinline__ void i8_swiglu_tile(const Params& p, uint32_t tbase, int m0, int n0, int row, __half* cst,
                                                float gs, float us)
 {
     const Sched& s = p.s;
@@ -367,7 +366,7 @@ __device__ __forceinline__ float4* slot_vec(const Params& p, long long slot, int
 // The loads from memory are a stream of (16-column chunk, partial) pairs in chunk order, kept kWin deep in flight:
 // with one partial in memory four chunks are on their way at once, instead of one L2 round trip per chunk.
 template <int BN, bool SWAP, int RANKS, int EPI, int BT = 0>
-__device__ __noinline__ void reduce_tile(const KParams<EPI>& p, int P, int tile, int rank, Fixup f, bool own_mine,
+__device__ __noinline__ void reduce_tile(const Params& p, int P, int tile, int rank, Fixup f, bool own_mine,
                                             uint32_t tbase, int row, int m0, int n0, __half* cst)
 {
     constexpr int kWin = 4;
@@ -450,7 +449,7 @@ __device__ __noinline__ void reduce_tile(const KParams<EPI>& p, int P, int tile,
 // shared memory.  The sum runs over at most kMaxSum partials, unrolled and predicated, so that everything stays in
 // registers.  Returns false if the copy did not complete within the wait limit (the block's abort flag is up).
 template <int BN, bool SWAP, int RANKS, int kMaxSum, int EPI, int BT = 0>
-__device__ __noinline__ bool reduce_tile_bulk(const KParams<EPI>& p, int P, int tile, int rank, Fixup f, bool own_mine,
+__device__ __noinline__ bool reduce_tile_bulk(const Params& p, int P, int tile, int rank, Fixup f, bool own_mine,
                                               uint32_t tbase, int row, int m0, int n0, __half* cst, uint8_t* ring,
                                               uint64_t* rbar, volatile int* abort_flag, int seg)
 {
@@ -563,7 +562,7 @@ __device__ __noinline__ bool reduce_tile_bulk(const KParams<EPI>& p, int P, int 
 // A split swap-AB tile of kEpiI8SwiGLU, by its last block: the gate and up sums of 16 tokens over the tile's partials (this
 // block's own from tensor memory when own_mine), exact in any order, then the activation.
 template <int BN>
-__device__ __noinline__ void i8_swiglu_reduce(const ParamsI8& p, int P, int tile, Fixup f, bool own_mine, uint32_t tbase,
+__device__ __noinline__ void i8_swiglu_reduce(const Params& p, int P, int tile, Fixup f, bool own_mine, uint32_t tbase,
                                               int n0, int row, __half* cst, float gs, float us)
 {
     const Sched& s = p.s;

@@ -65,7 +65,7 @@ I8Work i8_work(const bw_plan& q, int M, int K, bool linear)
 }
 
 template <int BN, bool SWAP, bool PAIR, int EPI, int WM = 1>
-int i8_launch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p,
+int i8_launch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p,
               cudaStream_t st, bool pdl)
 {
     // the instance's shared-memory limit, set once per device (an atomic flag: calls may come from several threads)
@@ -84,7 +84,7 @@ int i8_launch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUt
 }
 
 template <int EPI, int WM>
-int i8_launch_swap(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p,
+int i8_launch_swap(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p,
                    cudaStream_t st, bool pdl)
 {
     switch (q.bn) {
@@ -100,7 +100,7 @@ int i8_launch_swap(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, cons
     }
 }
 
-int i8_dispatch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p,
+int i8_dispatch(DeviceState& d, const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p,
                 cudaStream_t st, int epi, bool pdl)
 {
     if (q.kernel == BW_KERNEL_PAIR) {
@@ -138,13 +138,9 @@ int i8_product(DeviceState& d, const bw_plan& q, const I8Work& w, const void* A,
         snprintf(g_errbuf, sizeof g_errbuf, "cuTensorMapEncodeTiled failed");
         return BW_ERR_LAUNCH;
     }
-    ParamsI8 p = {};
-    static_cast<Params&>(p) =
+    Params p =
         make_params(q, M, N, q.kblocks * 64, C, reinterpret_cast<float*>(work + w.partial_off), counters, true);
-    p.row_scale = a_scale;
-    p.col_scale = b_scale;
-    p.out_bf16 = bf16 ? 1 : 0;
-    p.early_weights = zeroed ? 1 : 0;
+    i8_params(p, a_scale, b_scale, bf16, zeroed);
     return i8_dispatch(d, q, mx, my, p, st, epi, zeroed);
 }
 

@@ -47,7 +47,7 @@ namespace bw {
 template <int BN, bool SWAP, bool PAIR, int EPI = kEpiF16, int WM = 1>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmy,
-                const __grid_constant__ CUtensorMap tmc, const KParams<EPI> p)
+                const __grid_constant__ CUtensorMap tmc, const Params p)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     constexpr int AN = G::kAccN;  // accumulator columns (TMEM)
@@ -152,11 +152,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    // kEpiI8*: the weights may be complete already (early_weights); their first stages are then on their way before the
+    // kEpiI8*: the weights may be complete already (kI8EarlyWeights); their first stages are then on their way before the
     // wait, while the kernel ahead quantises the tokens
     int early = 0;
     if constexpr (epi_i8(EPI) && SWAP) {
-        if (p.early_weights && threadIdx.x == 0) {
+        if ((p.tn & kI8EarlyWeights) && threadIdx.x == 0) {
             SegIter it(s, c, P);
             Seg sg;
             const uint64_t pol_sb = BW_SWAP_HINT_B ? l2_policy(BW_SWAP_HINT_B) : 0ull;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if constexpr (epi_i8(EPI) && SWAP) {  // the tokens' scales, for every tile (read after the loop's barrier)
             const int t = threadIdx.x - kEpiThread0;
-            i8_token_scales(cst)[t] = t < s.M ? __ldg(p.row_scale + t) : 0.f;
+            i8_token_scales(cst)[t] = t < s.M ? __ldg(i8_row_scale(p) + t) : 0.f;
         }
         for (;;) {
             if (!s.dyn && !it.next(s, P, sg)) break;
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int w = 0; w < WM; ++w) {
                     const int n = (sg.tile * WM + w) * 128 + row;
-                    if (n < s.N) col_scale[w] = __ldg(p.col_scale + n);
+                    if (n < s.N) col_scale[w] = __ldg(i8_col_scale(p) + n);
                 }
             }
             if constexpr (epi_i8(EPI) && !SWAP) {  // the tile's scales, while its MMAs run

@@ -24,7 +24,7 @@ enum : int {
     kEpiRS = 3,      // the fused reduce-scatter: C (fp16, this rank's M / world rows) = the sum over the ranks of
                      // their A_r B_r, the partials exchanged tile by tile through the ranks' memory (RsTable)
     // A (M x K) and B (N x K) in 8-bit signed integers, 32-bit integer sums s, a scale per row of A and per row of B:
-    kEpiI8 = 4,        // C = row_scale[m] col_scale[n] s in fp16 or bf16 (Params.out_bf16)
+    kEpiI8 = 4,        // C = row_scale[m] col_scale[n] s in fp16 or bf16 (kI8OutBf16)
     kEpiI8F32 = 5,     // the same in fp32
     kEpiI8SwiGLU = 6,  // the activation of kEpiSwiGLU from the scaled sums, fp16 or bf16
 };
@@ -67,33 +67,29 @@ struct Params {
     const RsTable* rs;           // kEpiRS only: the ranks' regions
 };
 
-// What the 8-bit kernels take besides.  A type of its own: 24 bytes more in Params made the fp16 kernels 2 to 5 % slower
-// (the copy that their out-of-line reductions read grows with it).
-struct ParamsI8 : Params {
-    const float* row_scale;      // M scales of A's rows
-    const float* col_scale;      // N scales of B's rows (C's columns)
-    int out_bf16;                // kEpiI8, kEpiI8SwiGLU: C in bf16 (0: fp16)
-    int early_weights;           // swap-AB: the weights were complete before the kernel this one waits for (griddep_wait)
-                                 // began, so their first loads need not wait for it
+// What the 8-bit kernels take besides, in the fields that only the reduce-scatter reads.  A kernel whose parameters (with
+// the three maps) exceed 512 bytes loses 2 to 5 % here: 24 bytes more did, at 16 to 2048 tokens in fp16.
+__host__ __device__ __forceinline__ const float* i8_row_scale(const Params& p)  // M scales of A's rows
+{
+    return reinterpret_cast<const float*>(p.rs);
+}
+__host__ __device__ __forceinline__ const float* i8_col_scale(const Params& p)  // N scales of B's rows (C's columns)
+{
+    return reinterpret_cast<const float*>(p.rank_wait_ns);
+}
+enum : int {  // Params.tn
+    kI8Rows = 1,          // B is N x K
+    kI8OutBf16 = 2,       // kEpiI8, kEpiI8SwiGLU: C in bf16 (else fp16)
+    kI8EarlyWeights = 4,  // swap-AB: the weights were complete before the kernel this one waits for (griddep_wait) began,
+                          // so their first loads need not wait for it
 };
-template <int EPI>
-struct ParamsOf {
-    using type = Params;
-};
-template <>
-struct ParamsOf<kEpiI8> {
-    using type = ParamsI8;
-};
-template <>
-struct ParamsOf<kEpiI8F32> {
-    using type = ParamsI8;
-};
-template <>
-struct ParamsOf<kEpiI8SwiGLU> {
-    using type = ParamsI8;
-};
-template <int EPI>
-using KParams = typename ParamsOf<EPI>::type;
+inline void i8_params(Params& p, const float* row_scale, const float* col_scale, bool bf16, bool early)
+{
+    p.rs = reinterpret_cast<const RsTable*>(row_scale);
+    p.rank_wait_ns = reinterpret_cast<unsigned long long>(col_scale);
+    p.tn = kI8Rows | (bf16 ? kI8OutBf16 : 0) | (early ? kI8EarlyWeights : 0);
+}
+static_assert(3 * sizeof(CUtensorMap) + sizeof(Params) <= 512, "kernel parameters");
 
 __host__ __device__ constexpr int pow2_at_least(int v, int p) { return p >= v ? p : pow2_at_least(v, 2 * p); }
 

@@ -117,7 +117,7 @@ inline bool g_dry_run = false;  // dispatch and check a plan's instance and geom
 inline long long g_noalloc_cap = -1;  // >= 0: bw_emu_gemm plans as bw_gemm_f16_noalloc does, with this many bytes
 
 template <int BN, bool SWAP, bool PAIR, int EPI, int WM>
-int launch(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const CUtensorMap& mc, const KParams<EPI>& p)
+int launch(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const CUtensorMap& mc, const Params& p)
 {
     using G = KGeom<BN, SWAP, PAIR, EPI, WM>;
     if (q.smem_bytes != G::kSmemBytes || q.stages != G::kStages || q.tmem_cols != G::kTmemCols || q.wm != WM) {

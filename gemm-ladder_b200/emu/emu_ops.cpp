@@ -9,7 +9,7 @@ namespace bw {
 namespace {
 
 template <int EPI, int WM>
-int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p)
+int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p)
 {
     switch (q.bn) {
     case 16: return launch<16, true, false, EPI, WM>(q, mx, my, mx, p);
@@ -24,7 +24,7 @@ int launch_i8_swap(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& m
     }
 }
 
-int dispatch_i8(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const ParamsI8& p, int epi)
+int dispatch_i8(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const Params& p, int epi)
 {
     if (q.kernel == BW_KERNEL_PAIR) {
         if (epi == kEpiI8F32) return launch<256, false, true, kEpiI8F32, 1>(q, mx, my, mx, p);
@@ -62,12 +62,8 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     std::vector<int> counters((size_t)q.counters + 1, 0);
     CUtensorMap mx, my;
     make_maps(q, A, B, M, N, K / 2, &mx, &my, true);
-    ParamsI8 p = {};
-    static_cast<Params&>(p) = make_params(q, M, N, q.kblocks * 64, C, work.data(), counters.data(), true);
-    p.row_scale = a_scale;
-    p.col_scale = b_scale;
-    p.out_bf16 = out_type == BW_TYPE_BF16;
-    p.early_weights = M % 2;  // (both orders of the first loads)
+    Params p = make_params(q, M, N, q.kblocks * 64, C, work.data(), counters.data(), true);
+    i8_params(p, a_scale, b_scale, out_type == BW_TYPE_BF16, M % 2 != 0);  // (both orders of the first loads)
     rc = dispatch_i8(q, mx, my, p, epi);
     if (status) std::memcpy(status, g_status, sizeof g_status);
     if (dirty) *dirty = (int)std::count_if(counters.begin(), counters.begin() + q.counters, [](int v) { return v != 0; });
