@@ -47,7 +47,8 @@ struct MoeParams {
     int stages, stage_bytes;
     const int* ids;     // T x top_k
     const float* weights;
-    uint16_t* H;        // [active expert][T][F]
+    const uint8_t* X;   // the tokens, by K-blocks (moe_token_bytes)
+    uint8_t* H;         // the activations of each active expert, likewise
     uint16_t* Y;        // T x D
     float* partials;
     long long slot_floats;
@@ -242,10 +243,9 @@ __device__ __forceinline__ uint32_t moe_idesc(int n, int bf16)
 }
 
 // tmw1: W1 as {D, F, 2 E} (gate and up halves of an expert are two planes), boxes of 64 x 128; tmw2: W2 as {F, D, E},
-// boxes of 64 x 256; tmx: X as {D, T}, tmh: H as {F, T, slots}, boxes of 64 x Tp.  Zeros outside all of them.
+// boxes of 64 x 256.  Zeros outside both.
 __global__ void __launch_bounds__(kMoeThreads, 1)
     moe_experts_kernel(const __grid_constant__ CUtensorMap tmw1, const __grid_constant__ CUtensorMap tmw2,
-                       const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmh,
                        const MoeParams p)
 {
 #ifdef BW_EMULATE
@@ -295,8 +295,6 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&tmw1);
         prefetch_tmap(&tmw2);
-        prefetch_tmap(&tmx);
-        prefetch_tmap(&tmh);
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, (uint32_t)tmem_cols);
@@ -387,11 +385,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         seen = sl;
                     }
                     uint8_t* dst = smem + (size_t)stage * p.stage_bytes + kMoeXBytes;
-                    mbar_arrive_expect_tx(&xfull[stage], (uint32_t)Tp * 128u);
-                    if (sg.phase == 0)
-                        tma_load_2d(dst, &tmx, kb * 64, 0, &xfull[stage]);
-                    else
-                        tma_load_3d(dst, &tmh, (kb - sl * s.kbf) * 64, 0, sl, &xfull[stage]);
+                    // the T rows of the K-block (what the MMA reads past them only fills accumulator columns past T)
+                    const uint32_t bytes = (uint32_t)p.T * 128u;
+                    mbar_arrive_expect_tx(&xfull[stage], bytes);
+                    bulk_load(dst, (sg.phase == 0 ? p.X : p.H) + (size_t)kb * bytes, bytes, &xfull[stage]);
                     ++issued;
                     if (++stage == S) {
                         stage = 0;
@@ -549,10 +546,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     if (sg.phase == 0) {
                         uint16_t h[8];
                         moe_activation(a, gate + c0, p.bf16, h);
-                        uint16_t* dst = p.H + ((size_t)sl * p.T + c0) * p.F + f;
+                        // row c0 + j (c0 a multiple of 8), value f % 64 of K-block f / 64: a warp fills 64 bytes of a row
+                        uint8_t* dst = p.H + moe_token_bytes(p.T, sl * s.kbf + (f >> 6), c0, 0) + (f & 7) * 2;
+                        const int chunk = f >> 3 & 7;
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            if (c0 + j < p.T && f < p.F) dst[(size_t)j * p.F] = h[j];
+                            if (c0 + j < p.T && f < p.F)
+                                *reinterpret_cast<uint16_t*>(dst + j * 128 + ((chunk ^ j) << 4)) = h[j];
                     } else {
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {

@@ -21,19 +21,6 @@ bool moe_map(CUtensorMap* m, const void* base, int bf16, uint64_t d0, uint64_t d
                dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-bool moe_map2(CUtensorMap* m, const void* base, int bf16, uint64_t d0, uint64_t d1, uint64_t ld1, uint32_t rows)
-{
-    EncodeTiled enc = encoder();
-    if (!enc) return false;
-    const cuuint64_t dims[2] = {d0, d1};
-    const cuuint64_t strides[1] = {ld1 * 2};
-    const cuuint32_t box[2] = {64, rows};
-    const cuuint32_t elem[2] = {1, 1};
-    return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
-               dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int moe_shape(int T, int E, int top_k, int D, int F)
 {
     if (T < 0 || T > kMoeMaxTokens || E < 1 || E > kMoeMaxExperts || top_k < 1 || top_k > kMoeMaxTopK || top_k > E)
@@ -81,7 +68,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     DeviceState* d = nullptr;
     if ((rc = device_state(&d))) return rc;
     const int grid = moe_grid(*d);
-    const MoeWork w = moe_work(T, E, top_k, F, grid);
+    const MoeWork w = moe_work(T, E, top_k, D, F, grid);
     if ((size_t)w.bytes > work_bytes) return scratch_fail((size_t)w.bytes, work_bytes);
     uint8_t* ws = static_cast<uint8_t*>(work);
     if (!ids) ids = reinterpret_cast<int*>(ws + w.ids);
@@ -99,7 +86,8 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     p.stage_bytes = moe_stage_bytes(p.Tp);
     p.ids = ids;
     p.weights = weights;
-    p.H = reinterpret_cast<uint16_t*>(ws + w.h);
+    p.X = ws + w.x;
+    p.H = ws + w.h;
     p.Y = static_cast<uint16_t*>(Y);
     p.partials = reinterpret_cast<float*>(ws + w.partials);
     p.slot_floats = w.slot_floats;
@@ -107,11 +95,9 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     p.counters = p.ready + w.slots;
     p.wait_ns = g_wait_ns;
 
-    CUtensorMap m1, m2, mx, mh;
+    CUtensorMap m1, m2;
     if (!moe_map(&m1, W1, p.bf16, D, F, 2 * (uint64_t)E, D, (uint64_t)F * D, 128) ||
-        !moe_map(&m2, W2, p.bf16, F, D, E, F, (uint64_t)F * D, 256) ||
-        !moe_map2(&mx, X, p.bf16, D, T, (uint64_t)ldx, (uint32_t)p.Tp) ||
-        !moe_map(&mh, p.H, p.bf16, F, T, w.slots, F, (uint64_t)T * F, (uint32_t)p.Tp)) {
+        !moe_map(&m2, W2, p.bf16, F, D, E, F, (uint64_t)F * D, 256)) {
         snprintf(g_errbuf, sizeof g_errbuf, "cuTensorMapEncodeTiled failed");
         return BW_ERR_LAUNCH;
     }
@@ -125,7 +111,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     }
 
     RouterParams r = {static_cast<const uint16_t*>(X), ldx, static_cast<const uint16_t*>(R), T, E, top_k, D,
-                      router_ranges(E), renormalize, ids, weights, p.ready, w.zero_words};
+                      router_ranges(E), renormalize, ws + w.x, ids, weights, p.ready, w.zero_words};
     e = p.bf16 ? router_launch<true>(r, st) : router_launch<false>(r, st);
     if (e != cudaSuccess) return cuda_fail(e, "kernel launch (router)");
 
@@ -142,7 +128,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     attr[0].val.cooperative = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, moe_experts_kernel, m1, m2, mx, mh, p);
+    e = cudaLaunchKernelEx(&cfg, moe_experts_kernel, m1, m2, p);
     if (e != cudaSuccess) return cuda_fail(e, "kernel launch (experts)");
     return BW_OK;
 }
@@ -159,7 +145,7 @@ BW_API int bw_moe_work_bytes(int T, int E, int top_k, int D, int F, size_t* byte
     if (rc || T == 0) return rc;
     DeviceState* d = nullptr;
     if ((rc = device_state(&d))) return rc;
-    *bytes = (size_t)moe_work(T, E, top_k, F, moe_grid(*d)).bytes;
+    *bytes = (size_t)moe_work(T, E, top_k, D, F, moe_grid(*d)).bytes;
     return BW_OK;
 }
 

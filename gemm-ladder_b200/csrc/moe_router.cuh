@@ -10,7 +10,7 @@
 // The sums are chains of fp32 additions of products that are exact in fp32 (22 bits), short ones (D / (32 ds)), then a
 // tree: the choice between two experts can differ from the exact one only where their logits agree to about 2^-21 of
 // the products' magnitude.
-// It also clears the words that the experts kernel counts on.
+// It also clears the words that the experts kernel counts on, and lays the tokens out for its copies.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,6 +28,7 @@ struct RouterParams {
     int T, E, top_k, D;
     int ranges;         // router_ranges(E)
     int renormalize;    // 1: the weights' sum over the chosen experts is 1; 0: the softmax is over all experts
+    uint8_t* XT;        // the tokens as the experts' MMAs read them (moe_token_bytes)
     int* ids;           // T x top_k, by falling logit
     float* weights;
     int* zero;
@@ -71,6 +72,12 @@ __global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterT
     constexpr int TE = kRouterTE, NV = TE * TG;
     __shared__ float part[kRouterWarps][NV];  // the warps' sums
     const int ds = p.ranges, gpb = kRouterWarps / ds;  // ranges of D; groups of experts per block
+    for (int i = rank * kRouterThreads + threadIdx.x; i < TG * (p.D / 8); i += kRouterBlocks * kRouterThreads) {
+        const int t = t0 + i / (p.D / 8), c = i % (p.D / 8);
+        if (t < p.T)
+            *reinterpret_cast<uint4*>(p.XT + moe_token_bytes(p.T, c >> 3, t, c & 7)) =
+                reinterpret_cast<const uint4*>(p.X + (size_t)t * p.ldx)[c];
+    }
     const int nv = p.D / 8, v0 = nv * (warp % ds) / ds, v1 = nv * (warp % ds + 1) / ds;
     for (int g0 = 0; g0 * TE < p.E; g0 += kRouterBlocks * gpb) {
         const int e0 = (g0 + rank * gpb + warp / ds) * TE;

@@ -138,23 +138,29 @@ BW_MOE_HD inline int moe_slot(const MoeSeg& seg, int c) { return 4 * c + 2 * seg
 // The counter of a split tile: a block is the first of at most one split tile in each product.
 BW_MOE_HD inline int moe_counter(const MoeSeg& seg) { return 2 * seg.first + seg.phase; }
 
-// The workspace of a call on `grid` blocks (offsets in bytes): the chosen experts and their weights, the activations of
-// the active experts, the partials, then the words that start at zero (a count of finished gate/up tiles per active
+// The token-side operands of both products (X, and the activations h of each active expert) lie in the workspace as the
+// MMA reads them: by K-blocks of 64 values, T rows of 128 bytes each, a row's 16-byte chunk c at c ^ (t % 8) (the 128-byte
+// swizzle of the shared-memory descriptors), so that a stage's rows are one contiguous copy.
+BW_MOE_HD inline long long moe_token_bytes(int T, int kb, int t, int chunk) { return ((long long)kb * T + t) * 128 + ((chunk ^ (t & 7)) << 4); }
+
+// The workspace of a call on `grid` blocks (offsets in bytes): the chosen experts and their weights, X and the
+// activations of the active experts, the partials, then the words that start at zero (a count of finished gate/up tiles per active
 // expert, the split tiles' counters).
 struct MoeWork {
-    long long ids, weights, h, partials, zero, bytes;
+    long long ids, weights, x, h, partials, zero, bytes;
     int slots, zero_words;
     long long slot_floats;
 };
 BW_MOE_HD inline long long moe_up(long long v) { return (v + 255) / 256 * 256; }
-BW_MOE_HD inline MoeWork moe_work(int T, int E, int k, int F, int grid)
+BW_MOE_HD inline MoeWork moe_work(int T, int E, int k, int D, int F, int grid)
 {
     MoeWork w;
     w.slots = T * k < E ? T * k : E;
     w.slot_floats = 256LL * ((T + 3) / 4 * 4);
     w.ids = 0;
     w.weights = moe_up(w.ids + 4LL * T * k);
-    w.h = moe_up(w.weights + 4LL * T * k);
+    w.x = moe_up(w.weights + 4LL * T * k);
+    w.h = moe_up(w.x + 2LL * T * D);
     w.partials = moe_up(w.h + 2LL * w.slots * T * F);
     w.zero = moe_up(w.partials + 4LL * 4 * grid * w.slot_floats);
     w.zero_words = w.slots + 2 * grid;

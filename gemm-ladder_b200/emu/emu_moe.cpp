@@ -50,7 +50,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     emu::g_first_finding[0] = 0;
     emu::g_tma_count = 0;
     std::memset(g_status, 0, sizeof g_status);
-    const MoeWork w = moe_work(T, E, top_k, F, grid);
+    const MoeWork w = moe_work(T, E, top_k, D, F, grid);
     std::vector<uint8_t> work((size_t)w.bytes + 256, 0xFF);  // NaN: what the kernel does not write shows
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(work.data()) + 255) & ~uintptr_t(255));
     std::memset(base + w.zero, 0, 4 * (size_t)w.zero_words);
@@ -58,19 +58,16 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     p.T = T, p.Tp = (T + 15) / 16 * 16, p.E = E, p.top_k = top_k, p.D = D, p.F = F, p.bf16 = bf16;
     p.stages = moe_stages(p.Tp), p.stage_bytes = moe_stage_bytes(p.Tp);
     p.ids = ids, p.weights = weights;
-    p.H = reinterpret_cast<uint16_t*>(base + w.h), p.Y = Y;
+    p.X = base + w.x, p.H = base + w.h, p.Y = Y;
+    for (int t = 0; t < T; ++t)  // the router's layout of the tokens
+        for (int c = 0; c < D / 8; ++c)
+            std::memcpy(base + w.x + moe_token_bytes(T, c >> 3, t, c & 7), X + t * ldx + 8 * c, 16);
     p.partials = reinterpret_cast<float*>(base + w.partials), p.slot_floats = w.slot_floats;
     p.ready = reinterpret_cast<int*>(base + w.zero), p.counters = p.ready + w.slots;
     p.wait_ns = emu::g_wait_ns;
-    CUtensorMap m1, m2, mx, mh;
+    CUtensorMap m1, m2;
     map3(&m1, W1, D, F, 2 * (uint64_t)E, D, (uint64_t)F * D, 128);
     map3(&m2, W2, F, D, E, F, (uint64_t)F * D, 256);
-    {
-        const uint64_t dims[2] = {(uint64_t)D, (uint64_t)T}, strides[2] = {2, (uint64_t)ldx * 2};
-        const uint32_t box[2] = {64, (uint32_t)p.Tp};
-        emu::make_map(&mx, X, 2, dims, strides, box);
-    }
-    map3(&mh, p.H, F, T, w.slots, F, (uint64_t)T * F, (uint32_t)p.Tp);
     emu::g_smem_limit = moe_smem_bytes(p.Tp) - 1024;
     const unsigned seq = emu::g_launch_seq++;
     std::vector<std::unique_ptr<emu::Cta>> ctas;
@@ -91,7 +88,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
                 emu::start_jitter((unsigned)b, seq);
                 if (emu::g_block_ramp_us > 0)
                     std::this_thread::sleep_for(std::chrono::microseconds((long long)emu::g_block_ramp_us * b));
-                moe_experts_kernel(m1, m2, mx, mh, p);
+                moe_experts_kernel(m1, m2, p);
             });
     gate.set_value();
     for (auto& th : threads) th.join();
