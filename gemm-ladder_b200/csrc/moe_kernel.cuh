@@ -22,7 +22,8 @@
 // the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
 // resident); every wait is bounded (ptx.cuh).
 //
-// Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32), y once at the end; sums in fp32.
+// Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32; up to 8 tokens as two values,
+// kMoeSplitTokens), y once at the end; sums in fp32.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -48,7 +49,8 @@ struct MoeParams {
     const int* ids;     // T x top_k
     const float* weights;
     const uint8_t* X;   // the tokens, by K-blocks (moe_token_bytes)
-    uint8_t* H;         // the activations of each active expert, likewise
+    uint8_t* H;         // the activations of each active expert, likewise (T <= kMoeSplitTokens: two planes)
+    long long plane;
     uint16_t* Y;        // T x D
     float* partials;
     long long slot_floats;
@@ -161,9 +163,8 @@ __device__ __forceinline__ void moe_sum_parts(const MoeParams& p, const MoeSeg& 
 // h = p silu(g) u of 8 tokens, without a branch so that their chains overlap (the last whole gate/up tile's epilogue is
 // what the down product waits for).  The fast exponential and division are within (2 + 1.16 |g|) 2^-23 and 2^-22.  A
 // token that did not choose the expert (p = 0) contributes nothing, whatever its products.
-__device__ __forceinline__ void moe_activation(const float (&a)[2][8], const float* gate, int bf16, uint16_t (&h)[8])
+__device__ __forceinline__ void moe_activation(const float (&a)[2][8], const float* gate, float (&v)[8])
 {
-    float v[8];
     const float4 p0 = *reinterpret_cast<const float4*>(gate), p1 = *reinterpret_cast<const float4*>(gate + 4);
     const float pr[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
 #pragma unroll
@@ -171,6 +172,11 @@ __device__ __forceinline__ void moe_activation(const float (&a)[2][8], const flo
         v[j] = pr[j] * (__fdividef(a[0][j], 1.0f + __expf(-a[0][j])) * a[1][j]);
         v[j] = pr[j] == 0.f ? 0.f : v[j];
     }
+}
+
+// 8 values in the tokens' type (one test of it for all).
+__device__ __forceinline__ void moe_bits8(const float (&v)[8], int bf16, uint16_t (&h)[8])
+{
     if (bf16) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = moe_bits16(v[j], 1);
@@ -178,6 +184,37 @@ __device__ __forceinline__ void moe_activation(const float (&a)[2][8], const flo
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] = moe_bits16(v[j], 0);
     }
+}
+// What rounding v to h left (exact in fp32), 0 where h is an infinity.
+__device__ __forceinline__ float moe_left(float v, uint16_t h, int bf16)
+{
+    float r;
+    if (bf16) {
+        r = __uint_as_float((uint32_t)h << 16);
+    } else {
+        __half x;
+        *reinterpret_cast<uint16_t*>(&x) = h;
+        r = __half2float(x);
+    }
+    return (h & 0x7FFFu) == (bf16 ? 0x7F80u : 0x7C00u) ? 0.f : v - r;
+}
+
+// 8 tokens' sums from c0 of both weight blocks (tbase: the lane's accumulator, Tp columns per block); two: the columns of
+// the second plane, 8 on, added.
+__device__ __forceinline__ void moe_load8(uint32_t tbase, int Tp, int c0, bool two, uint32_t (&r)[2][8])
+{
+    tmem_ld8(tbase + (uint32_t)c0, r[0]);
+    tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
+    tmem_wait_ld();
+    if (!two) return;
+    uint32_t x[2][8];
+    tmem_ld8(tbase + 8u, x[0]);
+    tmem_ld8(tbase + (uint32_t)(Tp + 8), x[1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[w][j] = __float_as_uint(__uint_as_float(r[w][j]) + __uint_as_float(x[w][j]));
 }
 
 __device__ __forceinline__ float moe_shfl_xor(float v, int m)
@@ -272,6 +309,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
     const int S = p.stages, Tp = p.Tp;
+    const bool split = p.T <= kMoeSplitTokens;
     int tmem_cols = 32;
     while (tmem_cols < 4 * Tp) tmem_cols *= 2;
 
@@ -387,8 +425,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     uint8_t* dst = smem + (size_t)stage * p.stage_bytes + kMoeXBytes;
                     // the T rows of the K-block (what the MMA reads past them only fills accumulator columns past T)
                     const uint32_t bytes = (uint32_t)p.T * 128u;
-                    mbar_arrive_expect_tx(&xfull[stage], bytes);
+                    const bool both = sg.phase && split;
+                    mbar_arrive_expect_tx(&xfull[stage], both ? 2 * bytes : bytes);
                     bulk_load(dst, (sg.phase == 0 ? p.X : p.H) + (size_t)kb * bytes, bytes, &xfull[stage]);
+                    if (both) bulk_load(dst + 1024, p.H + p.plane + (size_t)kb * bytes, bytes, &xfull[stage]);
                     ++issued;
                     if (++stage == S) {
                         stage = 0;
@@ -504,9 +544,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 #pragma unroll 1
                 for (int c0 = 8 * half; c0 < p.T; c0 += 16) {
                     uint32_t r[2][8];
-                    tmem_ld8(tbase + (uint32_t)c0, r[0]);
-                    tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
-                    tmem_wait_ld();
+                    moe_load8(tbase, Tp, c0, sg.phase && split, r);
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -534,9 +572,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     float a[2][8];
                     {
                         uint32_t r[2][8];
-                        tmem_ld8(tbase + (uint32_t)c0, r[0]);
-                        tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
-                        tmem_wait_ld();
+                        moe_load8(tbase, Tp, c0, sg.phase && split, r);
 #pragma unroll
                         for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -544,8 +580,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     }
                     if (sg.nseg > 1) moe_sum_parts(p, sg, c, row, c0, tq, a);
                     if (sg.phase == 0) {
+                        float v[8];
                         uint16_t h[8];
-                        moe_activation(a, gate + c0, p.bf16, h);
+                        moe_activation(a, gate + c0, v);
+                        moe_bits8(v, p.bf16, h);
                         // row c0 + j (c0 a multiple of 8), value f % 64 of K-block f / 64: a warp fills 64 bytes of a row
                         uint8_t* dst = p.H + moe_token_bytes(p.T, sl * s.kbf + (f >> 6), c0, 0) + (f & 7) * 2;
                         const int chunk = f >> 3 & 7;
@@ -553,6 +591,15 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         for (int j = 0; j < 8; ++j)
                             if (c0 + j < p.T && f < p.F)
                                 *reinterpret_cast<uint16_t*>(dst + j * 128 + ((chunk ^ j) << 4)) = h[j];
+                        if (split) {  // what the rounding left, to the second plane
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = moe_left(v[j], h[j], p.bf16);
+                            moe_bits8(v, p.bf16, h);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (c0 + j < p.T && f < p.F)
+                                    *reinterpret_cast<uint16_t*>(dst + p.plane + j * 128 + ((chunk ^ j) << 4)) = h[j];
+                        }
                     } else {
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {

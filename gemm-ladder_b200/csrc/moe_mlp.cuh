@@ -88,6 +88,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     p.weights = weights;
     p.X = ws + w.x;
     p.H = ws + w.h;
+    p.plane = w.plane;
     p.Y = static_cast<uint16_t*>(Y);
     p.partials = reinterpret_cast<float*>(ws + w.partials);
     p.slot_floats = w.slot_floats;

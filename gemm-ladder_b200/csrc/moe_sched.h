@@ -143,11 +143,18 @@ BW_MOE_HD inline int moe_counter(const MoeSeg& seg) { return 2 * seg.first + seg
 // swizzle of the shared-memory descriptors), so that a stage's rows are one contiguous copy.
 BW_MOE_HD inline long long moe_token_bytes(int T, int kb, int t, int chunk) { return ((long long)kb * T + t) * 128 + ((chunk ^ (t & 7)) << 4); }
 
+// Up to this many tokens h goes to the down product as two values of the tokens' type, h rounded and what the rounding left
+// (a second plane of the same layout): the MMA's N is 16 anyway, so rows 8 .. 8 + T - 1 of the operand are free, and the
+// layer's error is that of its one rounding of Y.  With more tokens h is rounded once (the layer's error is then about
+// 1.4 times that of rounding Y alone).
+constexpr int kMoeSplitTokens = 8;
+
 // The workspace of a call on `grid` blocks (offsets in bytes): the chosen experts and their weights, X and the
 // activations of the active experts, the partials, then the words that start at zero (a count of finished gate/up tiles per active
 // expert, the split tiles' counters).
 struct MoeWork {
     long long ids, weights, x, h, partials, zero, bytes;
+    long long plane;  // bytes of one plane of h
     int slots, zero_words;
     long long slot_floats;
 };
@@ -161,7 +168,8 @@ BW_MOE_HD inline MoeWork moe_work(int T, int E, int k, int D, int F, int grid)
     w.weights = moe_up(w.ids + 4LL * T * k);
     w.x = moe_up(w.weights + 4LL * T * k);
     w.h = moe_up(w.x + 2LL * T * D);
-    w.partials = moe_up(w.h + 2LL * w.slots * T * F);
+    w.plane = 2LL * w.slots * T * F;
+    w.partials = moe_up(w.h + (T <= kMoeSplitTokens ? 2 : 1) * w.plane);
     w.zero = moe_up(w.partials + 4LL * 4 * grid * w.slot_floats);
     w.zero_words = w.slots + 2 * grid;
     w.bytes = moe_up(w.zero + 4LL * w.zero_words);

@@ -58,7 +58,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     p.T = T, p.Tp = (T + 15) / 16 * 16, p.E = E, p.top_k = top_k, p.D = D, p.F = F, p.bf16 = bf16;
     p.stages = moe_stages(p.Tp), p.stage_bytes = moe_stage_bytes(p.Tp);
     p.ids = ids, p.weights = weights;
-    p.X = base + w.x, p.H = base + w.h, p.Y = Y;
+    p.X = base + w.x, p.H = base + w.h, p.plane = w.plane, p.Y = Y;
     for (int t = 0; t < T; ++t)  // the router's layout of the tokens
         for (int c = 0; c < D / 8; ++c)
             std::memcpy(base + w.x + moe_token_bytes(T, c >> 3, t, c & 7), X + t * ldx + 8 * c, 16);

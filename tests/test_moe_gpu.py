@@ -214,3 +214,16 @@ def test_refused_tensors():
     rc = L.bw_moe_mlp(X.data_ptr(), 128, R.data_ptr(), W1.data_ptr(), W2.data_ptr(), X.data_ptr(), 4, 8, 2, 128, 64, 0, 1,
                       None, None, w.data_ptr(), n.value - 1, None)
     assert rc == bwgemm.BW_ERR_SCRATCH
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,D,F", [(1, 8, 2, 512, 1024), (3, 256, 8, 1152, 576), (8, 32, 8, 1024, 704)])
+def test_few_tokens_are_as_exact_as_one_rounding(T, E, k, D, F, dtype):
+    """Up to 8 tokens h is kept as two values, to 2^-16 (bf16) or 2^-22 (fp16) of it: what is left beside the rounding of Y
+    is that (for bf16 1 / 128 of Y's own rounding, added in quadrature) and fp32 sums, 2^-20 of Y's norm at these sizes."""
+    a = inputs(T, E, D, F, dtype, seed=77)
+    Y = bwgemm.moe_mlp(*a, k)
+    ids, weights, err = moe_ref.route(a[0], a[1], k)
+    y, _ = moe_ref.layer(a[0], ids, weights, err, a[2], a[3])
+    rounded = (y.to(dtype).double() - y).norm()
+    assert (Y.double() - y).norm() <= 1.02 * rounded + 2.0 ** -18 * y.norm()
