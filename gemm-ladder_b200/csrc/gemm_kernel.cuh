@@ -36,6 +36,8 @@
 // where it holds 64 fp16, and an MMA's 32-byte slice 32 where it holds 16, so to everything but the MMA and the
 // epilogue an int8 row of K is an fp16 row of K / 2: the maps, stages, descriptors, schedules and partials are the fp16
 // ones (the maps' zero fill past K adds zeros), the MMA is kind::i8 and the sums are 32-bit integers (epilogue.cuh).
+// Measured: 8192^3 in 374 us (2.94 POP/s, under the power cap), 2048 x 10240 x 8192 in 130 to 150 us, whose 256 x 256
+// pair tiles wait for operands (tensor pipe active 63 % of the cycles); 16 x 57344 x 8192 at 7.1 TB/s of weights.
 // Every wait on a barrier is bounded (ptx.cuh, wait_bounded): a stalled pipeline ends the kernel with an error status
 // instead of hanging the GPU.
 #pragma once

@@ -10,6 +10,7 @@
 // The sums are chains of fp32 additions of products that are exact in fp32 (22 bits), short ones (D / (32 ds)), then a
 // tree: the choice between two experts can differ from the exact one only where their logits agree to about 2^-21 of
 // the products' magnitude.
+// Measured: 3.0 us at one token over 64 experts of 2048, 4.6 us at 8 over 128 of 4096, 8 us at 64.
 // It also clears the words that the experts kernel counts on, and lays the tokens out for its copies.
 #pragma once
 #include <cuda_bf16.h>
