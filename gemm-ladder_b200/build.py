@@ -21,7 +21,7 @@ NEXT_DEFINES = ["-DBW_KSPLIT=1", "-DBW_EPI_TMA=1"]
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "--split-compile=0", *ARCH, "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
+NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", *ARCH, "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
               f"-I{INCLUDE}", f"-I{CSRC}"]
 
 

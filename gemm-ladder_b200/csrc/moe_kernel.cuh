@@ -22,9 +22,9 @@
 // the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
 // resident); every wait is bounded (ptx.cuh).
 //
-// Measured on a B200, router included: 33 tokens over 8 experts of 4096 x 14336 (2.8 GB of weights, bf16) 426 to 460 us,
-// 6.9 TB/s in the streams; 8 tokens over 128 of 4096 x 1344 (51 active, 1.7 GB) 270 us; 64 tokens over 128 of 4096 x 1280
-// 630 to 670 us; 128 tokens over 32 of 2880 x 2880 319 to 355 us, where the SMs take in 59 GB/s each of weights and tokens;
+// Measured on a B200, router included: 33 tokens over 8 experts of 4096 x 14336 (2.8 GB of weights, bf16) 431 us,
+// 6.9 TB/s in the streams; 8 tokens over 128 of 4096 x 1344 (51 active, 1.7 GB) 269 us; 64 tokens over 128 of 4096 x 1280
+// 634 us; 128 tokens over 32 of 2880 x 2880 329 us, where the SMs take in 59 GB/s each of weights and tokens;
 // one token, top 8 of 64 of 2048 x 1024 (100 MB) 42 us, of which the stream is 15.
 //
 // Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32; up to 8 tokens as two values,
