@@ -1,7 +1,7 @@
 """The 8-bit integer operators on a B200, through the public entry points, against the definition in 64 bits
 (tests/i8_ref.py derives how far a result may be from it): every plan form, ragged tokens, K that ends inside a stage,
 strided rows, rows of zeros, infinities and NaN, half-way quotients; streams, CUDA graphs that overlap, the largest
-magnitudes; a quantised gated MLP run end to end."""
+magnitudes."""
 import numpy as np
 import pytest
 
