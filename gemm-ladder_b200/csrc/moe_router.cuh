@@ -58,20 +58,36 @@ __device__ __forceinline__ uint32_t router_key(float v)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A block's shared memory: NV sums of each warp; the logits of the token the block chooses for.
+template <int NV, int EMAX>
+struct RouterSmem {
+    float part[kRouterWarps][NV];
+    float logits[EMAX];
+};
+
 // TG tokens per cluster; up to 32 PER experts.
 template <bool BF16, int TG, int PER>
 __global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterThreads, 2)
     moe_router_kernel(const RouterParams p)
 {
-    __shared__ float logits[32 * PER];  // of the token this block chooses for
+    constexpr int TE = kRouterTE, NV = TE * TG;
+    using Smem = RouterSmem<NV, 32 * PER>;
+#ifdef BW_EMULATE
+    Smem& sm = *reinterpret_cast<Smem*>(emu::cta_smem());
+#else
+    __shared__ Smem sm;
+#endif
+    auto& part = sm.part;
+    auto& logits = sm.logits;
+    // Another block's shared memory may be written once that block has started: the first stores wait below, behind the
+    // dot products.
+    cluster_arrive();
     if (threadIdx.x == 0) BW_TRACE_AT(12);
     for (int i = blockIdx.x * kRouterThreads + threadIdx.x; i < p.zero_words; i += gridDim.x * kRouterThreads)
         p.zero[i] = 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     const int t0 = blockIdx.x / kRouterBlocks * TG;
-    constexpr int TE = kRouterTE, NV = TE * TG;
-    __shared__ float part[kRouterWarps][NV];  // the warps' sums
     const int ds = p.ranges, gpb = kRouterWarps / ds;  // ranges of D; groups of experts per block
     for (int i = rank * kRouterThreads + threadIdx.x; i < TG * (p.D / 8); i += kRouterBlocks * kRouterThreads) {
         const int t = t0 + i / (p.D / 8), c = i % (p.D / 8);
@@ -126,14 +142,14 @@ __global__ void __cluster_dims__(kRouterBlocks, 1, 1) __launch_bounds__(kRouterT
                 if (lane == (i * TG + t) % 32) part[warp][i * TG + t] = v;
             }
         __syncthreads();
+        if (g0 == 0) cluster_wait();
         // a logit per thread: its ranges in order, to the block that chooses for its token
         for (int n = threadIdx.x; n < gpb * NV; n += kRouterThreads) {
             const int g = n / NV, i = n % NV / TG, t = n % TG, e = (g0 + rank * gpb + g) * TE + i;
             float v = 0.f;
             for (int r = 0; r < ds; ++r) v += part[g * ds + r][i * TG + t];
             if (e < p.E) {
-                const uint32_t dst = mapa_shared(smem_u32(&logits[e]), (uint32_t)t);
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+                st_cluster_f32(mapa_shared(smem_u32(&logits[e]), (uint32_t)t), v);
             }
         }
         if ((g0 + kRouterBlocks * gpb) * TE < p.E) __syncthreads();  // the sums are read before the next ones

@@ -242,6 +242,16 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The same in two halves, for work that needs no other block in between.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// A float into a shared::cluster address (mapa_shared).
+__device__ __forceinline__ void st_cluster_f32(uint32_t dst, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(v) : "memory");
+}
+
 // One arrival on a barrier of another block of the cluster (a shared::cluster address from mapa_shared).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {

@@ -91,6 +91,28 @@ struct Barrier {
             cv.notify_all();
         }
     }
+    // The two halves of sync: an arrival, which gives the generation to wait for the end of.
+    unsigned arrive(int count)
+    {
+        std::unique_lock<std::mutex> l(m);
+        const unsigned g = gen;
+        if (++arrived >= count) {
+            arrived = 0;
+            ++gen;
+            cv.notify_all();
+        }
+        return g;
+    }
+    void wait(unsigned g)
+    {
+        std::unique_lock<std::mutex> l(m);
+        if (!cv.wait_for(l, std::chrono::milliseconds(g_barrier_limit_ms), [&] { return gen != g; })) {
+            finding("a cluster barrier that %d threads reached (a deadlock in the kernel's control flow)", arrived);
+            arrived = 0;
+            ++gen;
+            cv.notify_all();
+        }
+    }
 };
 
 // a TMA or bulk completion that the drop_tma knob takes away (its bytes never arrive: a stall, made on purpose)
@@ -340,9 +362,30 @@ inline void named_sync(int id, int count)
     }
     t_cta->named[id].sync(count);
 }
+// Whether this thread has been through a cluster barrier: until then nothing says that the other blocks of its cluster
+// have started, and another block's shared memory may not be touched.
+inline thread_local bool t_met = false;
+inline void met(uint32_t addr, const char* what)
+{
+    if (!t_met && cta_of(addr) != t_cta)
+        finding("%s in another block's shared memory before the blocks of the cluster have met", what);
+}
+inline thread_local unsigned t_arrived = 0;
+inline void cluster_arrive()
+{
+    Cluster* cl = t_cta->cluster;
+    t_arrived = (cl ? cl->all : t_cta->named[0]).arrive(kCtaThreads * (cl ? cl->size : 1));
+}
+inline void cluster_wait()
+{
+    Cluster* cl = t_cta->cluster;
+    (cl ? cl->all : t_cta->named[0]).wait(t_arrived);
+    t_met = true;
+}
 inline void cluster_sync()
 {
     Cluster* cl = t_cta->cluster;
+    t_met = true;  // (past the barrier, as far as this thread goes on)
     if (!cl) {
         t_cta->named[0].sync(kCtaThreads);
         return;
@@ -686,6 +729,47 @@ inline uint32_t __shfl_xor_sync(unsigned, uint32_t v, int m)
     c->warp[w].sync(32);
     return r;
 }
+inline float __shfl_xor_sync(unsigned mask, float v, int m)
+{
+    uint32_t u;
+    std::memcpy(&u, &v, 4);
+    u = __shfl_xor_sync(mask, u, m);
+    std::memcpy(&v, &u, 4);
+    return v;
+}
+inline uint32_t __shfl_sync(unsigned, uint32_t v, int src)
+{
+    bw::emu::Cta* c = bw::emu::t_cta;
+    const int w = bw::emu::t_tid >> 5, lane = bw::emu::t_tid & 31;
+    c->shfl[w][lane] = v;
+    c->warp[w].sync(32);
+    const uint32_t r = c->shfl[w][src & 31];
+    c->warp[w].sync(32);
+    return r;
+}
+inline uint32_t __reduce_max_sync(unsigned mask, uint32_t v)
+{
+    for (int m = 16; m >= 1; m >>= 1) {
+        const uint32_t o = __shfl_xor_sync(mask, v, m);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+inline uint32_t __reduce_min_sync(unsigned mask, uint32_t v) { return ~__reduce_max_sync(mask, ~v); }
+inline uint32_t __vmaxu2(uint32_t a, uint32_t b)
+{
+    const uint32_t lo = (a & 0xFFFFu) > (b & 0xFFFFu) ? a & 0xFFFFu : b & 0xFFFFu;
+    return ((a >> 16) > (b >> 16) ? a & 0xFFFF0000u : b & 0xFFFF0000u) | lo;
+}
+inline uint32_t __byte_perm(uint32_t a, uint32_t b, uint32_t s)
+{
+    uint32_t r = 0;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t k = s >> (4 * i) & 7u;
+        r |= ((k < 4 ? a >> (8 * k) : b >> (8 * (k - 4))) & 0xFFu) << (8 * i);
+    }
+    return r;
+}
 inline void __threadfence() { std::atomic_thread_fence(std::memory_order_seq_cst); }
 inline float4 __ldcg(const float4* p)
 {
@@ -693,6 +777,7 @@ inline float4 __ldcg(const float4* p)
     return *p;
 }
 inline int min(int a, int b) { return a < b ? a : b; }
+inline uint32_t max(uint32_t a, uint32_t b) { return a > b ? a : b; }
 inline void __stcg(float4* p, float4 v) { *p = v; }
 inline float __expf(float x) { return std::exp(x); }
 inline float __fdividef(float x, float y) { return x / y; }
@@ -738,4 +823,7 @@ inline unsigned atomicCAS(unsigned* p, unsigned cmp, unsigned val)
 #endif
 #ifndef __launch_bounds__
 #define __launch_bounds__(...)
+#endif
+#ifndef __cluster_dims__
+#define __cluster_dims__(...)
 #endif

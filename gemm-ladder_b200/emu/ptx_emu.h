@@ -176,11 +176,25 @@ inline void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
 inline uint32_t cluster_ctarank() { return (uint32_t)emu::t_cta->rank; }
 inline uint32_t mapa_shared(uint32_t saddr, uint32_t rank) { return emu::mapa(saddr, rank); }
 inline void cluster_sync() { emu::cluster_sync(); }
-inline void mbar_arrive_cluster(uint32_t cluster_addr) { emu::mb_arrive(emu::cta_of(cluster_addr), emu::off_of(cluster_addr), 0); }
+inline void cluster_arrive() { emu::cluster_arrive(); }
+inline void cluster_wait() { emu::cluster_wait(); }
+inline void st_cluster_f32(uint32_t dst, float v)
+{
+    emu::met(dst, "a store");
+    uint32_t u;
+    std::memcpy(&u, &v, 4);
+    emu::remote_store(dst, &u, 4);
+}
+inline void mbar_arrive_cluster(uint32_t cluster_addr)
+{
+    emu::met(cluster_addr, "an arrival");
+    emu::mb_arrive(emu::cta_of(cluster_addr), emu::off_of(cluster_addr), 0);
+}
 // st.async: the 16 bytes land in the other block later (queued to this block's TMA engine, standing for the path
 // between the blocks), then complete on that block's barrier.
 inline void st_async_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar)
 {
+    emu::met(dst, "an st.async");
     emu::t_cta->tma.post([=] {
         const uint32_t v[4] = {a, b, c, d};
         emu::remote_store(dst, v, 16);
