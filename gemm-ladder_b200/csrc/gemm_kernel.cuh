@@ -880,6 +880,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        if constexpr (kKsplitBuf<BN, SWAP, EPI>) {
+            // a block that gave up before the hand-over: the parts that the others send into its buffer all the same
+            // (expected at the start, nothing asked) land before it leaves
+            if (kp && seg == 0 && threadIdx.x == kEpiThread0 &&
+                plan_ksplit_recv_bytes(BN, WM, s.ksplit) <= kPlanI8RecvBytes &&
+                ksplit_run(kr, AN / 16, s.ksplit) != ksplit_run(kr + 1, AN / 16, s.ksplit))
+                wait_drain(krecv, 0, p.wait_ns);
+        }
         // the TMA stores of C complete before the block leaves (their sources are this block's shared memory)
         if (kEpiTma<BN, SWAP, PAIR, EPI> && lane == 0) bulk_wait<0>();
         if (threadIdx.x == kEpiThread0) BW_TRACE_AT(4);

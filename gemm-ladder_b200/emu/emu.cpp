@@ -174,6 +174,7 @@ int launch(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, const
                     if (emu::g_block_ramp_us > 0)
                         std::this_thread::sleep_for(std::chrono::microseconds((long long)emu::g_block_ramp_us * blk));
                     gemm_kernel<BN, SWAP, PAIR, EPI, WM>(mx, my, mc, p);
+                    ++emu::t_cta->left;
                 });
         gate.set_value();
         for (auto& th : threads) th.join();
@@ -255,7 +256,8 @@ int dispatch(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, con
 
 // Sets a knob of the emulator: "wait_ns" (the kernel's limit of one bounded wait), "rank_wait_ns" (the limit of a wait
 // for another rank's flag; 0: wait_ns), "drop_tma" (the n-th TMA / bulk
-// completion of each launch never arrives, -1 none), "barrier_limit_ms" (a thread barrier never completed: a finding
+// completion of each launch never arrives, -1 none), "drop_block" (>= 0: the n-th of this block's), "drop_commit" (from now on
+// the n-th tcgen05.commit of block drop_block arrives nowhere), "barrier_limit_ms" (a thread barrier never completed: a finding
 // after this long), "cluster_batch" (clusters run at once; 0: as many as the host's cores take), "noalloc_cap"
 // (>= 0: fp16 calls of variant 0 plan as bw_gemm_f16_noalloc does, its array this many bytes; -1: the rule),
 // "ld_delay_us" (a random pause of up to this long before each tensor-memory load), "start_jitter_us" (each block starts
@@ -271,6 +273,8 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_set(const char* nam
     else if (n == "rank_wait_ns") g_rank_wait_ns = (unsigned long long)value;
     else if (n == "cluster_batch") bw::g_cluster_batch = value;
     else if (n == "drop_tma") g_drop_tma = value;
+    else if (n == "drop_block") g_drop_block = (int)value;
+    else if (n == "drop_commit") g_drop_commit = value, g_commit_count = 0;
     else if (n == "barrier_limit_ms") g_barrier_limit_ms = value;
     else if (n == "noalloc_cap") bw::g_noalloc_cap = value;
     else if (n == "ld_delay_us") g_ld_delay_us = (int)value;

@@ -66,6 +66,9 @@ inline void finding(const char* fmt, ...)
 inline long long g_barrier_limit_ms = 120000;  // a thread barrier that never completes: a finding, then on
 inline long long g_drop_tma = -1;              // the n-th TMA / bulk completion of a launch is dropped (-1: none)
 inline std::atomic<long long> g_tma_count{0};
+inline int g_drop_block = -1;                  // >= 0: of this block's completions alone
+inline long long g_drop_commit = -1;           // the n-th tcgen05.commit of block g_drop_block is dropped (-1: none)
+inline std::atomic<long long> g_commit_count{0};
 
 // ------------------------------------------------------------------ barriers between host threads
 // A thread barrier the kernel's threads never all reach (a deadlock in the kernel's own control flow) ends with a
@@ -116,7 +119,15 @@ struct Barrier {
 };
 
 // a TMA or bulk completion that the drop_tma knob takes away (its bytes never arrive: a stall, made on purpose)
-inline bool keep_completion() { return g_tma_count.fetch_add(1) != g_drop_tma; }
+inline bool keep_completion()
+{
+    if (g_drop_block >= 0 && (int)blockIdx.x != g_drop_block) return true;
+    return g_tma_count.fetch_add(1) != g_drop_tma;
+}
+inline bool keep_commit()
+{
+    return g_drop_commit < 0 || (int)blockIdx.x != g_drop_block || g_commit_count.fetch_add(1) != g_drop_commit;
+}
 inline unsigned long long g_wait_ns = 60ull * 1000000000ull;  // the kernel's limit of one bounded wait
 inline unsigned long long g_rank_wait_ns = 0;  // the limit of a wait for another rank's flag (0: g_wait_ns)
 
@@ -183,6 +194,7 @@ struct Cta {
     Barrier warp[kCtaThreads / 32];
     uint32_t shfl[kCtaThreads / 32][32];
     int tmem_cols = 0;  // allocated columns (0: none)
+    std::atomic<int> left{0};  // threads that have returned from the kernel
     Engine tma, tc;     // the TMA engine (tiled loads, bulk copies) and the tensor core (MMAs, their commits)
     Cta() : raw(new uint8_t[kSmemBytes + 1024]), tmem((size_t)kTmemLanes * kTmemCols, 0u)
     {
@@ -529,6 +541,7 @@ inline void remote_store(uint32_t dst, const uint32_t* v, uint32_t bytes)
 {
     Cta* c = cta_of(dst);
     const uint32_t off = off_of(dst);
+    if (c->left.load() == kCtaThreads) finding("bytes into the shared memory of a block that has left");
     if (off + bytes > (uint32_t)g_smem_limit || off % bytes || over_mbar(c, off, bytes)) {
         finding("an st.async outside the destination block's shared memory, unaligned or over an mbarrier");
         return;

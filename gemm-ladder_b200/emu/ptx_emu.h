@@ -268,6 +268,7 @@ inline void mma_commit_pair(uint32_t bar)
 }
 inline void mma_commit(uint64_t* bar)
 {
+    if (!emu::keep_commit()) return;
     const uint32_t off = emu::offset_of(bar);
     emu::Cta* c = emu::t_cta;
     c->tc.post([=] { emu::mb_arrive(c, off, 0); });

@@ -164,3 +164,32 @@ def test_emulated_k_split_into_the_buffer_or_the_ring(emu, force, late):
         emu.bw_emu_set(b"force_ksplit", ctypes.c_longlong(0))
         emu.bw_emu_set(b"lead_skew_us", ctypes.c_longlong(0))
     assert len(i8_ref.outside(got, i8_ref.product(A, sa, B, sb), "fp16")) == 0
+
+
+@pytest.mark.parametrize("force", [2 * 16 + 1, 3 * 16 + 2, 5 * 16 + 1])
+def test_a_block_that_gives_up_leaves_after_the_parts_sent_to_it(emu, force):
+    """The last block of a cluster owns a run of the tile's columns; its accumulator's completion never arrives, so
+    its epilogue gives up, while the other blocks' parts of those columns are on their way into
+    its buffer (expected from the start, so nobody asks).  They land before it leaves."""
+    c, wm = force // 16, force % 16
+    rng = np.random.default_rng(force)
+    M, N, K = 11, 256 * wm, 128 * 4 * c  # 4 stages a block: commits 0 to 3 free them, 4 is the accumulator's
+    A = rng.integers(-127, 128, (M, K), dtype=np.int8)
+    B = rng.integers(-127, 128, (N, K), dtype=np.int8)
+    C = np.zeros((M, N), np.uint16)
+    sa, sb = np.ones(M, np.float32), np.ones(N, np.float32)
+    st, dirty, nf = (ctypes.c_uint * 4)(), ctypes.c_int(), ctypes.c_int()
+    msg, vp = ctypes.create_string_buffer(512), ctypes.c_void_p
+    # a part takes about half a second to cross; the wait gives up after 0.3 s, the drain after 1 s more
+    knobs = dict(force_ksplit=force, wait_ns=300_000_000, engine_delay_us=2000, drop_block=c - 1, drop_commit=4)
+    for name, value in knobs.items():
+        assert emu.bw_emu_set(name.encode(), ctypes.c_longlong(value)) == 0
+    try:
+        emu.bw_emu_gemm_i8(vp(A.ctypes.data), vp(sa.ctypes.data), vp(B.ctypes.data), vp(sb.ctypes.data), vp(C.ctypes.data),
+                           M, N, K, 2 * c, F16, 0, st, ctypes.byref(dirty), ctypes.byref(nf), msg, 512)
+    finally:
+        for name, value in dict(force_ksplit=0, wait_ns=60_000_000_000, engine_delay_us=20, drop_block=-1,
+                                drop_commit=-1).items():
+            emu.bw_emu_set(name.encode(), ctypes.c_longlong(value))
+    assert st[0] == 3, "no wait gave up"
+    assert nf.value == 0, msg.value.decode()
