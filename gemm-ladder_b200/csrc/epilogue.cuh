@@ -26,14 +26,17 @@ __device__ __forceinline__ float i8_value(float bits, float row_scale, float col
 __device__ __forceinline__ const float* i8_scales(const __half* cst) { return reinterpret_cast<const float*>(cst); }
 // Swap-AB: the tokens' scales, after the transpose buffers.
 __device__ __forceinline__ float* i8_token_scales(__half* cst) { return reinterpret_cast<float*>(cst + 2 * 16 * 128); }
+// The scales' loads are plain ones, not __ldg: the kernel ahead (the quantiser; with BWGEMM_PDL=1 any) may be writing them
+// when this one starts, so they are no constants of it.
+__device__ __forceinline__ float i8_load_scale(const float* p) { return *p; }
 template <int BN>
 __device__ __forceinline__ void i8_load_scales(const Params& p, __half* cst, int m0, int n0)
 {
     float* to = reinterpret_cast<float*>(cst);
     const int t = threadIdx.x - kEpiThread0;
 #pragma unroll
-    for (int i = 0; i < BN; i += 128) to[i + t] = n0 + i + t < p.s.N ? __ldg(i8_col_scale(p) + n0 + i + t) : 0.f;
-    to[BN + t] = m0 + t < p.s.M ? __ldg(i8_row_scale(p) + m0 + t) : 0.f;
+    for (int i = 0; i < BN; i += 128) to[i + t] = n0 + i + t < p.s.N ? i8_load_scale(i8_col_scale(p) + n0 + i + t) : 0.f;
+    to[BN + t] = m0 + t < p.s.M ? i8_load_scale(i8_row_scale(p) + m0 + t) : 0.f;
 }
 // NC columns of a row: the scaled values (cs: their column scales, 16-byte aligned).
 template <int NC>
@@ -141,7 +144,7 @@ __device__ __forceinline__ void store_chunk(const Params& p, int m0, int n0, int
         __half* buf = cst + ((c0 >> 4) & 1) * (16 * 128);
         if constexpr (epi_i8(EPI)) {  // the lane's column scale, the chunk's 16 row scales
             const int wb = BT ? c0 / BT : 0, tok = c0 - wb * BT, n = n0 + wb * 128 + lane;
-            const float cs = n < s.N ? __ldg(i8_col_scale(p) + n) : 0.f;
+            const float cs = n < s.N ? i8_load_scale(i8_col_scale(p) + n) : 0.f;
             const float* rs = i8_token_scales(cst) + tok;
 #pragma unroll
             for (int j = 0; j < 16; ++j) buf[j * 128 + lane] = half_bits<EPI>(p, i8_value(v[j], rs[j], cs));

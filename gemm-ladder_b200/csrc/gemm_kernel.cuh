@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if constexpr (epi_i8(EPI) && SWAP) {  // the tokens' scales, for every tile (read after the loop's barrier)
             const int t = threadIdx.x - kEpiThread0;
-            i8_token_scales(cst)[t] = t < s.M ? __ldg(i8_row_scale(p) + t) : 0.f;
+            i8_token_scales(cst)[t] = t < s.M ? i8_load_scale(i8_row_scale(p) + t) : 0.f;
         }
         for (;;) {
             if (!s.dyn && !it.next(s, P, sg)) break;
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int w = 0; w < WM; ++w) {
                     const int n = (sg.tile * WM + w) * 128 + row;
-                    if (n < s.N) col_scale[w] = __ldg(i8_col_scale(p) + n);
+                    if (n < s.N) col_scale[w] = i8_load_scale(i8_col_scale(p) + n);
                 }
             }
             if constexpr (epi_i8(EPI) && !SWAP) {  // the tile's scales, while its MMAs run

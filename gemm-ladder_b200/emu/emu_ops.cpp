@@ -64,6 +64,9 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_gemm_i8(const void*
     make_maps(q, A, B, M, N, K / 2, &mx, &my, true);
     Params p = make_params(q, M, N, q.kblocks * 64, C, work.data(), counters.data(), true);
     i8_params(p, a_scale, b_scale, out_type == BW_TYPE_BF16, M % 2 != 0);  // (both orders of the first loads)
+    // bw_linear_i8: the quantiser writes the row scales; with BWGEMM_PDL=1 one ahead of bw_gemm_i8 may write either
+    emu::g_ahead[0][0] = a_scale, emu::g_ahead[0][1] = a_scale + M;
+    emu::g_ahead[1][0] = b_scale, emu::g_ahead[1][1] = b_scale + N;
     rc = dispatch_i8(q, mx, my, p, epi);
     if (status) std::memcpy(status, g_status, sizeof g_status);
     if (dirty) *dirty = (int)std::count_if(counters.begin(), counters.begin() + q.counters, [](int v) { return v != 0; });

@@ -812,7 +812,19 @@ inline float __int_as_float(int u)
     std::memcpy(&f, &u, 4);
     return f;
 }
-inline float __ldg(const float* p) { return *p; }
+// Memory that the kernel ahead may still be writing when this one starts (programmatic launch): no constant of this one,
+// so not for the non-coherent path.
+namespace bw {
+namespace emu {
+inline const float* g_ahead[2][2] = {};  // [range][begin, end]
+}
+}  // namespace bw
+inline float __ldg(const float* p)
+{
+    for (const auto& r : bw::emu::g_ahead)
+        if (p >= r[0] && p < r[1]) bw::emu::finding("a non-coherent load of memory that the kernel ahead writes");
+    return *p;
+}
 inline uint32_t __float_as_uint(float f)
 {
     uint32_t u;

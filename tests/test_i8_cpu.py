@@ -193,3 +193,15 @@ def test_a_block_that_gives_up_leaves_after_the_parts_sent_to_it(emu, force):
             emu.bw_emu_set(name.encode(), ctypes.c_longlong(value))
     assert st[0] == 3, "no wait gave up"
     assert nf.value == 0, msg.value.decode()
+
+
+@pytest.mark.parametrize("M,N,K,sms,out_type,swiglu", [(9, 256, 256, 4, F16, 0), (20, 512, 256, 4, BF16, 1),
+                                                       (130, 512, 256, 8, F16, 0), (130, 256, 256, 4, F32, 0)])
+def test_the_scales_are_no_constants_of_the_product(emu, M, N, K, sms, out_type, swiglu):
+    """In the linear layer's one call the product starts while the quantiser still writes the row scales, and with
+    BWGEMM_PDL=1 so may a product whose column scales a kernel ahead writes: neither may be read through the non-coherent
+    path (the emulator reports such a load)."""
+    A, B = np.ones((M, K), np.int8), np.ones((N, K), np.int8)
+    s = np.ones(max(M, N), np.float32)
+    got = emulate_i8(emu, A, s[:M].copy(), B, s[:N].copy(), sms, out_type, swiglu)
+    assert (got == (K * K if swiglu else K)).all()
