@@ -27,8 +27,8 @@
 // 634 us; 128 tokens over 32 of 2880 x 2880 329 us, where the SMs take in 59 GB/s each of weights and tokens;
 // one token, top 8 of 64 of 2048 x 1024 (100 MB) 42 us, of which the stream is 15.
 //
-// Roundings: h to the tokens' type (the MMA's operand; p is folded in before, in fp32; up to 8 tokens as two values,
-// kMoeSplitTokens), y once at the end; sums in fp32.
+// Roundings: h to two values of the tokens' type (the MMA's operand; moe_plane_rows of moe_sched.h; p is folded in before, in
+// fp32), y once at the end; sums in fp32.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -41,20 +41,21 @@ namespace bw {
 
 constexpr int kMoeThreads = 352;  // 11 warps
 constexpr int kMoeEpiThreads = 256;
-constexpr int kMoeXBytes = 32768; // a stage's weights: 256 rows x 64 values
-constexpr int kMoeMaxStages = 5;  // as fast as 6 or 1 % faster from 1 to 16 tokens (3: up to 5 % slower): deeper rings make
-                                   // the counts and partials queue behind more weights in flight
+constexpr int kMoeXBytes = 32768; // a stage of the weights' ring: 256 rows x 64 values
+constexpr int kMoeMaxStages = 5;  // as fast as 6 or 1 % faster from 1 to 16 tokens (3: up to 5 % slower, 8 % at 128): deeper
+                                   // rings make the counts and partials queue behind more weights in flight
 constexpr int kMoeEpiThread0 = 64;
 
 struct MoeParams {
-    int T, Tp;          // tokens; rounded up to 16 (the MMA's N, the rows of a token box)
+    int T, Tp;          // tokens; rounded up to 16 (the gate/up MMA's N)
     int E, top_k, D, F;
     int bf16;           // the tokens', weights' and results' type: 1 bf16, 0 fp16
-    int stages, stage_bytes;
+    int stages, slots;  // of the weights' ring and of the tokens'
+    int slot_bytes;
     const int* ids;     // T x top_k
     const float* weights;
     const uint8_t* X;   // the tokens, by K-blocks (moe_token_bytes)
-    uint8_t* H;         // the activations of each active expert, likewise (T <= kMoeSplitTokens: two planes)
+    uint8_t* H;         // the activations of each active expert, likewise, two planes
     long long plane;
     uint16_t* Y;        // T x D
     float* partials;
@@ -66,24 +67,49 @@ struct MoeParams {
 
 // Shared memory after the ring (offsets from its end).
 struct MoeSmem {
-    static constexpr int kBars = 0;  // weights in, tokens in, empty (5 each), tfull, tempty (2 each), drain
-    static constexpr int kMisc = (kBars + (3 * kMoeMaxStages + 5) * 8 + 15) / 16 * 16;  // tmem slot, flags
+    static constexpr int kBars = 0;  // weights in and out, tokens in and out (5 each), tfull, tempty (2 each), drain
+    static constexpr int kMisc = (kBars + (4 * kMoeMaxStages + 5) * 8 + 15) / 16 * 16;  // tmem slot, flags
     static constexpr int kMask = kMisc + 64;                       // a bit per expert
     static constexpr int kExpert = kMask + kMoeMaxExperts / 8;     // the active experts, 16 bits each
     static constexpr int kGate = kExpert + 2 * kMoeMaxExperts;     // p of every token for the epilogue's expert (on 16 bytes)
     static constexpr int kBytes = kGate + 4 * kMoeMaxTokens;
     static_assert(kGate % 16 == 0, "read by 16 bytes");
 };
-__host__ __device__ constexpr int moe_stage_bytes(int tp) { return kMoeXBytes + tp * 128; }
-__host__ __device__ constexpr int moe_stages(int tp)
+// The weights and the tokens have rings of their own: a slot of tokens holds both planes of a K-block of h, and beyond 96
+// tokens 4 stages of weights fit beside 3 such slots (from L2, so soon there) where only 3 stages of both would.
+__host__ __device__ inline int moe_slot_bytes(int T) { return 2 * moe_plane_rows(T) * 128; }
+inline void moe_rings(int T, int* stages, int* slots)
 {
-    const int fit = (BW_SMEM_LIMIT - 1024 - MoeSmem::kBytes) / moe_stage_bytes(tp);
-    return fit < kMoeMaxStages ? fit : kMoeMaxStages;
+    const int room = BW_SMEM_LIMIT - 1024 - MoeSmem::kBytes;
+    for (int s = kMoeMaxStages;; --s) {
+        const int fit = (room - s * kMoeXBytes) / moe_slot_bytes(T);
+        *stages = s;
+        *slots = fit < s ? fit : s;
+        if (fit >= s - 1) return;  // (at 4 stages always)
+    }
 }
-__host__ __device__ constexpr int moe_smem_bytes(int tp)
+inline int moe_smem_bytes(const MoeParams& p)
 {
-    return 1024 + moe_stages(tp) * moe_stage_bytes(tp) + MoeSmem::kBytes;
+    return 1024 + p.stages * kMoeXBytes + p.slots * p.slot_bytes + MoeSmem::kBytes;
 }
+
+// The accumulators in tensor memory: two buffers of `cols` columns, each of both weight blocks, `n` columns apart (the
+// MMA's N).  A down product of more than 64 tokens takes both buffers as one (2 x 2 x 2 Tp columns are not there).
+struct MoeAcc {
+    int n0, n1;  // gate/up, down
+    int cols;
+    bool both;   // the down product takes both buffers
+    __device__ explicit MoeAcc(int T)
+    {
+        n0 = moe_padded(T);
+        n1 = 2 * moe_plane_rows(T);
+        both = n0 > 64;
+        cols = both ? 2 * n0 : 2 * n1;
+    }
+    __device__ __forceinline__ int n(int phase) const { return phase ? n1 : n0; }
+    __device__ __forceinline__ bool joint(int phase) const { return phase && both; }
+    __device__ __forceinline__ uint32_t base(int phase, int acc) const { return joint(phase) ? 0u : (uint32_t)(acc * cols); }
+};
 
 // Spins until the counter at p reaches `want`, the abort flag rises or the limit passes.  One thread calls it.
 __device__ __noinline__ bool moe_wait_count(const int* p, int want, volatile int* abort_flag, uint64_t limit_ns,
@@ -190,36 +216,33 @@ __device__ __forceinline__ void moe_bits8(const float (&v)[8], int bf16, uint16_
         for (int j = 0; j < 8; ++j) h[j] = moe_bits16(v[j], 0);
     }
 }
-// What rounding v to h left (exact in fp32), 0 where h is an infinity.
+// What rounding v (scaled) to h left, at the second plane's scale (exact in fp32), 0 where h is an infinity.
 __device__ __forceinline__ float moe_left(float v, uint16_t h, int bf16)
 {
-    float r;
-    if (bf16) {
-        r = __uint_as_float((uint32_t)h << 16);
-    } else {
-        __half x;
-        *reinterpret_cast<uint16_t*>(&x) = h;
-        r = __half2float(x);
-    }
-    return (h & 0x7FFFu) == (bf16 ? 0x7F80u : 0x7C00u) ? 0.f : v - r;
+    if (bf16) return (h & 0x7FFFu) == 0x7F80u ? 0.f : v - __uint_as_float((uint32_t)h << 16);
+    __half x;
+    *reinterpret_cast<uint16_t*>(&x) = h;
+    return (h & 0x7FFFu) == 0x7C00u ? 0.f : (v - __half2float(x)) * (kMoeLoScale / kMoeHiScale);
 }
 
-// 8 tokens' sums from c0 of both weight blocks (tbase: the lane's accumulator, Tp columns per block); two: the columns of
-// the second plane, 8 on, added.
-__device__ __forceinline__ void moe_load8(uint32_t tbase, int Tp, int c0, bool two, uint32_t (&r)[2][8])
+// 8 tokens' sums from c0 of both weight blocks (tbase: the lane's accumulator, n columns per block); lo: the columns from
+// the first plane of h to the second (0: there is one plane), both brought to scale and added.
+__device__ __forceinline__ void moe_load8(uint32_t tbase, int n, int c0, int lo, int bf16, uint32_t (&r)[2][8])
 {
     tmem_ld8(tbase + (uint32_t)c0, r[0]);
-    tmem_ld8(tbase + (uint32_t)(Tp + c0), r[1]);
+    tmem_ld8(tbase + (uint32_t)(n + c0), r[1]);
     tmem_wait_ld();
-    if (!two) return;
+    if (!lo) return;
     uint32_t x[2][8];
-    tmem_ld8(tbase + 8u, x[0]);
-    tmem_ld8(tbase + (uint32_t)(Tp + 8), x[1]);
+    tmem_ld8(tbase + (uint32_t)(lo + c0), x[0]);
+    tmem_ld8(tbase + (uint32_t)(n + lo + c0), x[1]);
     tmem_wait_ld();
+    const float sh = bf16 ? 1.f : 1.f / kMoeHiScale, sl = bf16 ? 1.f : 1.f / kMoeLoScale;
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[w][j] = __float_as_uint(__uint_as_float(r[w][j]) + __uint_as_float(x[w][j]));
+        for (int j = 0; j < 8; ++j)
+            r[w][j] = __float_as_uint(fmaf(__uint_as_float(x[w][j]), sl, __uint_as_float(r[w][j]) * sh));
 }
 
 __device__ __forceinline__ float moe_shfl_xor(float v, int m)
@@ -296,11 +319,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     extern __shared__ uint8_t smem_raw[];
 #endif
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* misc = smem + (size_t)p.stages * p.stage_bytes;
+    uint8_t* ring_x = smem + (size_t)p.stages * kMoeXBytes;
+    uint8_t* misc = ring_x + (size_t)p.slots * p.slot_bytes;
     uint64_t* wfull = reinterpret_cast<uint64_t*>(misc + MoeSmem::kBars);  // a barrier per stage and producer, so that
-    uint64_t* xfull = wfull + kMoeMaxStages;                               // each can drain its own loads
-    uint64_t* empty = xfull + kMoeMaxStages;
-    uint64_t* tfull = empty + kMoeMaxStages;
+    uint64_t* wempty = wfull + kMoeMaxStages;                              // each can drain its own loads
+    uint64_t* xfull = wempty + kMoeMaxStages;
+    uint64_t* xempty = xfull + kMoeMaxStages;
+    uint64_t* tfull = xempty + kMoeMaxStages;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMisc);
@@ -314,17 +339,21 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
     const int S = p.stages, Tp = p.Tp;
-    const bool split = p.T <= kMoeSplitTokens;
+    const MoeAcc A(p.T);
+    const int lo_rows = moe_plane_rows(p.T);  // from h's first plane to its second
     int tmem_cols = 32;
-    while (tmem_cols < 4 * Tp) tmem_cols *= 2;
+    while (tmem_cols < 2 * A.cols) tmem_cols *= 2;
 
     if (threadIdx.x == 0) {
         for (int i = 1; i < 12; ++i) BW_TRACE_VAL(i, 0);  // (12 to 15 are the router's)
         BW_TRACE_AT(0);
         for (int i = 0; i < S; ++i) {
-            mbar_init(&wfull[i], 1);  // the producer's arrive.expect_tx
+            mbar_init(&wfull[i], 1);   // the producer's arrive.expect_tx
+            mbar_init(&wempty[i], 1);  // one tcgen05.commit
+        }
+        for (int i = 0; i < p.slots; ++i) {
             mbar_init(&xfull[i], 1);
-            mbar_init(&empty[i], 1);  // one tcgen05.commit
+            mbar_init(&xempty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&tfull[i], 1);
@@ -379,11 +408,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             bool ok = true;
             while (ok && it.next(s, sg)) {
                 for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
+                    if (!wait_bounded(&wempty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
                         ok = false;
                         break;
                     }
-                    uint8_t* dst = smem + (size_t)stage * p.stage_bytes;
+                    uint8_t* dst = smem + (size_t)stage * kMoeXBytes;
                     mbar_arrive_expect_tx(&wfull[stage], kMoeXBytes);
                     if (sg.phase == 0) {
                         const int e = expert[sg.tile / s.f_tiles], f0 = sg.tile % s.f_tiles * 128;
@@ -409,12 +438,12 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         if (lane == 0) {
             MoeIter it(s, c);
             MoeSeg sg;
-            int stage = 0, seg = 0, seen = -1, issued = 0;
+            int slot = 0, seg = 0, seen = -1, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
             while (ok && it.next(s, sg)) {
                 for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(3, 1, stage), seg)) {
+                    if (!wait_bounded(&xempty[slot], ph ^ 1u, abort_flag, p.wait_ns, site(3, 1, slot), seg)) {
                         ok = false;
                         break;
                     }
@@ -427,42 +456,45 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         fence_proxy_async_global();
                         seen = sl;
                     }
-                    uint8_t* dst = smem + (size_t)stage * p.stage_bytes + kMoeXBytes;
+                    uint8_t* dst = ring_x + (size_t)slot * p.slot_bytes;
                     // the T rows of the K-block (what the MMA reads past them only fills accumulator columns past T)
                     const uint32_t bytes = (uint32_t)p.T * 128u;
-                    const bool both = sg.phase && split;
-                    mbar_arrive_expect_tx(&xfull[stage], both ? 2 * bytes : bytes);
-                    bulk_load(dst, (sg.phase == 0 ? p.X : p.H) + (size_t)kb * bytes, bytes, &xfull[stage]);
-                    if (both) bulk_load(dst + 1024, p.H + p.plane + (size_t)kb * bytes, bytes, &xfull[stage]);
+                    mbar_arrive_expect_tx(&xfull[slot], sg.phase ? 2 * bytes : bytes);
+                    bulk_load(dst, (sg.phase == 0 ? p.X : p.H) + (size_t)kb * bytes, bytes, &xfull[slot]);
+                    if (sg.phase) bulk_load(dst + lo_rows * 128, p.H + p.plane + (size_t)kb * bytes, bytes, &xfull[slot]);
                     ++issued;
-                    if (++stage == S) {
-                        stage = 0;
+                    if (++slot == p.slots) {
+                        slot = 0;
                         ph ^= 1u;
                     }
                 }
                 ++seg;
             }
-            moe_drain(xfull, issued, S, p.wait_ns);
+            moe_drain(xfull, issued, p.slots, p.wait_ns);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------- the MMA issuer
         if (lane == 0) {
-            const uint32_t idesc = moe_idesc(Tp, p.bf16);
 #ifdef BW_TRACE
             bool in_down = false;
 #endif
             MoeIter it(s, c);
             MoeSeg sg;
-            int stage = 0, acc = 0, seg = 0;
-            uint32_t ph = 0, aph = 0;
+            int stage = 0, slot = 0, acc = 0, seg = 0;
+            uint32_t ph = 0, xph = 0, aph = 0;
             bool ok = true;
             while (ok && it.next(s, sg)) {
+                const int n = A.n(sg.phase);
+                const bool joint = A.joint(sg.phase);
                 if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) break;
+                if (joint && !wait_bounded(&tempty[acc ^ 1], aph ^ (uint32_t)acc ^ 1u, abort_flag, p.wait_ns,
+                                           site(1, 3, acc ^ 1), seg))
+                    break;
                 tc_fence_after();
-                const uint32_t d = tmem_base + (uint32_t)(acc * 2 * Tp);
+                const uint32_t d = tmem_base + A.base(sg.phase, acc), idesc = moe_idesc(n, p.bf16);
                 for (int kb = sg.k0; kb < sg.k1; ++kb) {
                     if (!wait_bounded(&wfull[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg) ||
-                        !wait_bounded(&xfull[stage], ph, abort_flag, p.wait_ns, site(1, 12, stage), seg)) {
+                        !wait_bounded(&xfull[slot], xph, abort_flag, p.wait_ns, site(1, 12, slot), seg)) {
                         ok = false;
                         break;
                     }
@@ -474,14 +506,20 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     else BW_TRACE_AT(7);                             // the last down stage
 #endif
                     tc_fence_after();
-                    const uint32_t sx = smem_u32(smem + (size_t)stage * p.stage_bytes), sy = sx + kMoeXBytes;
+                    const uint32_t sx = smem_u32(smem + (size_t)stage * kMoeXBytes);
+                    const uint32_t sy = smem_u32(ring_x + (size_t)slot * p.slot_bytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t accumulate = (kb > sg.k0 || k > 0) ? 1u : 0u;
                         mma_f16(d, desc_kmajor(sx, k), desc_kmajor(sy, k), idesc, accumulate);
-                        mma_f16(d + (uint32_t)Tp, desc_kmajor(sx + kMoeXBytes / 2, k), desc_kmajor(sy, k), idesc, accumulate);
+                        mma_f16(d + (uint32_t)n, desc_kmajor(sx + kMoeXBytes / 2, k), desc_kmajor(sy, k), idesc, accumulate);
                     }
-                    mma_commit(&empty[stage]);
+                    mma_commit(&wempty[stage]);
+                    mma_commit(&xempty[slot]);
+                    if (++slot == p.slots) {
+                        slot = 0;
+                        xph ^= 1u;
+                    }
                     if (++stage == S) {
                         stage = 0;
                         ph ^= 1u;
@@ -489,7 +527,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 }
                 if (!ok) break;
                 mma_commit(&tfull[acc]);
-                if (++acc == 2) {
+                if (joint) {  // (acc as before, in the next phase)
+                    mma_commit(&tfull[acc ^ 1]);
+                    aph ^= 1u;
+                } else if (++acc == 2) {
                     acc = 0;
                     aph ^= 1u;
                 }
@@ -532,7 +573,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 gate_slot = sl;
             }
             if (threadIdx.x == kMoeEpiThread0) {
-                epi_go[seg & 1] = wait_bounded(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, acc), seg) ? 1 : 0;
+                bool in = wait_bounded(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, acc), seg);
+                if (in && A.joint(sg.phase))
+                    in = wait_bounded(&tfull[acc ^ 1], aph ^ (uint32_t)acc, abort_flag, p.wait_ns, site(2, 2, acc ^ 1), seg);
+                epi_go[seg & 1] = in ? 1 : 0;
                 // a split gate/up tile whose other parts are all there is summed here, without writing this one
                 epi_sum[seg & 1] = sg.nseg == 1 || (sg.phase == 0 && ld_acquire_gpu(counter) == sg.nseg - 1) ? 1 : 0;
             }
@@ -542,14 +586,15 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 break;
             }
             tc_fence_after();
-            const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 2 * Tp);
+            const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + A.base(sg.phase, acc);
+            const int n = A.n(sg.phase), lo = sg.phase ? lo_rows : 0;
             bool sum_here = epi_sum[seg & 1] != 0;
             if (!sum_here) {
                 float4* dst = slot_of(c, sg) + row;
 #pragma unroll 1
                 for (int c0 = 8 * half; c0 < p.T; c0 += 16) {
                     uint32_t r[2][8];
-                    moe_load8(tbase, Tp, c0, sg.phase && split, r);
+                    moe_load8(tbase, n, c0, lo, p.bf16, r);
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -577,7 +622,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                     float a[2][8];
                     {
                         uint32_t r[2][8];
-                        moe_load8(tbase, Tp, c0, sg.phase && split, r);
+                        moe_load8(tbase, n, c0, lo, p.bf16, r);
 #pragma unroll
                         for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -588,6 +633,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         float v[8];
                         uint16_t h[8];
                         moe_activation(a, gate + c0, v);
+                        if (!p.bf16) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] *= kMoeHiScale;
+                        }
                         moe_bits8(v, p.bf16, h);
                         // row c0 + j (c0 a multiple of 8), value f % 64 of K-block f / 64: a warp fills 64 bytes of a row
                         uint8_t* dst = p.H + moe_token_bytes(p.T, sl * s.kbf + (f >> 6), c0, 0) + (f & 7) * 2;
@@ -596,15 +645,14 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                         for (int j = 0; j < 8; ++j)
                             if (c0 + j < p.T && f < p.F)
                                 *reinterpret_cast<uint16_t*>(dst + j * 128 + ((chunk ^ j) << 4)) = h[j];
-                        if (split) {  // what the rounding left, to the second plane
+                        // what the rounding left, to the second plane
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = moe_left(v[j], h[j], p.bf16);
-                            moe_bits8(v, p.bf16, h);
+                        for (int j = 0; j < 8; ++j) v[j] = moe_left(v[j], h[j], p.bf16);
+                        moe_bits8(v, p.bf16, h);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                if (c0 + j < p.T && f < p.F)
-                                    *reinterpret_cast<uint16_t*>(dst + p.plane + j * 128 + ((chunk ^ j) << 4)) = h[j];
-                        }
+                        for (int j = 0; j < 8; ++j)
+                            if (c0 + j < p.T && f < p.F)
+                                *reinterpret_cast<uint16_t*>(dst + p.plane + j * 128 + ((chunk ^ j) << 4)) = h[j];
                     } else {
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
@@ -627,7 +675,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[acc]);  // the accumulator is read
-            if (++acc == 2) {
+            if (A.joint(sg.phase)) {
+                if (lane == 0) mbar_arrive(&tempty[acc ^ 1]);
+                aph ^= 1u;
+            } else if (++acc == 2) {
                 acc = 0;
                 aph ^= 1u;
             }

@@ -76,14 +76,14 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
 
     MoeParams p = {};
     p.T = T;
-    p.Tp = (T + 15) / 16 * 16;
+    p.Tp = moe_padded(T);
     p.E = E;
     p.top_k = top_k;
     p.D = D;
     p.F = F;
     p.bf16 = type == BW_TYPE_BF16;
-    p.stages = moe_stages(p.Tp);
-    p.stage_bytes = moe_stage_bytes(p.Tp);
+    moe_rings(T, &p.stages, &p.slots);
+    p.slot_bytes = moe_slot_bytes(T);
     p.ids = ids;
     p.weights = weights;
     p.X = ws + w.x;
@@ -119,7 +119,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kMoeThreads);
-    cfg.dynamicSmemBytes = (size_t)moe_smem_bytes(p.Tp);
+    cfg.dynamicSmemBytes = (size_t)moe_smem_bytes(p);
     cfg.stream = st;
     // the blocks wait for one another, so all of them have to be resident.  (A cooperative launch does not overlap the
     // router's end: measured, programmatic serialisation has no effect on it; without the cooperative attribute it saves

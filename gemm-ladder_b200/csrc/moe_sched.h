@@ -143,11 +143,18 @@ BW_MOE_HD inline int moe_counter(const MoeSeg& seg) { return 2 * seg.first + seg
 // swizzle of the shared-memory descriptors), so that a stage's rows are one contiguous copy.
 BW_MOE_HD inline long long moe_token_bytes(int T, int kb, int t, int chunk) { return ((long long)kb * T + t) * 128 + ((chunk ^ (t & 7)) << 4); }
 
-// Up to this many tokens h goes to the down product as two values of the tokens' type, h rounded and what the rounding left
-// (a second plane of the same layout): the MMA's N is 16 anyway, so rows 8 .. 8 + T - 1 of the operand are free, and the
-// layer's error is that of its one rounding of Y.  With more tokens h is rounded once (the layer's error is then about
-// 1.4 times that of rounding Y alone).
-constexpr int kMoeSplitTokens = 8;
+// h goes to the down product as two values of the tokens' type, h rounded and what the rounding left, in two planes of the
+// same layout, so that the layer's error is that of its one rounding of Y (rounded once, h would make it 1.4 times that).
+// The planes are rows of one operand, each with accumulator columns of its own, so in fp16 they carry scales that keep h
+// within its range: the first holds 2^-8 h (|h| up to 1.6e7), the second 2^3 times what that left (at most 2^12, so below
+// 2^15), which leaves h off by 2^-23 of it or 2^-28, the larger.  bf16 has fp32's range: no scales, 2^-17 of h.
+//   up to 8 tokens  the planes are rows 0 and 8 of the 16 that the MMA takes anyway: free
+//   more            rows 0 and Tp (T rounded up to 16) of 2 Tp, one MMA of N = 2 Tp.  The tokens' intake of the down product
+//                   doubles: 1 % at 16 tokens, 3 % at 33 and 64, 8 % at 128 against one value.  (Two MMAs of N = Tp in its
+//                   place read the weights twice from shared memory: 13 to 18 % against one value.)
+BW_MOE_HD inline int moe_padded(int T) { return (T + 15) / 16 * 16; }
+BW_MOE_HD inline int moe_plane_rows(int T) { return T <= 8 ? 8 : moe_padded(T); }
+constexpr float kMoeHiScale = 0.00390625f, kMoeLoScale = 8.0f;  // fp16
 
 // The workspace of a call on `grid` blocks (offsets in bytes): the chosen experts and their weights, X and the
 // activations of the active experts, the partials, then the words that start at zero (a count of finished gate/up tiles per active
@@ -169,7 +176,7 @@ BW_MOE_HD inline MoeWork moe_work(int T, int E, int k, int D, int F, int grid)
     w.x = moe_up(w.weights + 4LL * T * k);
     w.h = moe_up(w.x + 2LL * T * D);
     w.plane = 2LL * w.slots * T * F;
-    w.partials = moe_up(w.h + (T <= kMoeSplitTokens ? 2 : 1) * w.plane);
+    w.partials = moe_up(w.h + 2 * w.plane);
     w.zero = moe_up(w.partials + 4LL * 4 * grid * w.slot_floats);
     w.zero_words = w.slots + 2 * grid;
     w.bytes = moe_up(w.zero + 4LL * w.zero_words);

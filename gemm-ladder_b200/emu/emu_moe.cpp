@@ -55,8 +55,9 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(work.data()) + 255) & ~uintptr_t(255));
     std::memset(base + w.zero, 0, 4 * (size_t)w.zero_words);
     MoeParams p = {};
-    p.T = T, p.Tp = (T + 15) / 16 * 16, p.E = E, p.top_k = top_k, p.D = D, p.F = F, p.bf16 = bf16;
-    p.stages = moe_stages(p.Tp), p.stage_bytes = moe_stage_bytes(p.Tp);
+    p.T = T, p.Tp = moe_padded(T), p.E = E, p.top_k = top_k, p.D = D, p.F = F, p.bf16 = bf16;
+    moe_rings(T, &p.stages, &p.slots);
+    p.slot_bytes = moe_slot_bytes(T);
     p.ids = ids, p.weights = weights;
     p.X = base + w.x, p.H = base + w.h, p.plane = w.plane, p.Y = Y;
     for (int t = 0; t < T; ++t)  // the router's layout of the tokens
@@ -68,7 +69,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     CUtensorMap m1, m2;
     map3(&m1, W1, D, F, 2 * (uint64_t)E, D, (uint64_t)F * D, 128);
     map3(&m2, W2, F, D, E, F, (uint64_t)F * D, 256);
-    emu::g_smem_limit = moe_smem_bytes(p.Tp) - 1024;
+    emu::g_smem_limit = moe_smem_bytes(p) - 1024;
     const unsigned seq = emu::g_launch_seq++;
     std::vector<std::unique_ptr<emu::Cta>> ctas;
     for (int b = 0; b < grid; ++b) ctas.emplace_back(new emu::Cta());

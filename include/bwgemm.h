@@ -128,8 +128,8 @@ int bw_linear_i8(const void* X, int x_type, long long ld, const void* B, const v
  *   logits l = X R^T (fp32); S_t = the top_k experts of token t by logit (equal logits: the lower index);
  *   p_te = softmax over S_t (renormalize 1) or over all experts (0);
  *   Y_t = sum over S_t of p_te (silu(X_t G_e^T) * (X_t U_e^T)) W2_e^T
- * in fp32 sums; p_te silu * up is rounded to the type before the down product (up to 8 tokens kept as two values, so to
- * twice its precision), Y once.  D % 64 == 0, F % 64 == 0,
+ * in fp32 sums; p_te silu * up goes to the down product as two values of the type, to twice its precision (in fp16 scaled, so
+ * that it may reach 1.6e7), and Y is rounded once.  D % 64 == 0, F % 64 == 0,
  * E <= 512, top_k <= min(E, 32), ldx >= D, ldx % 8 == 0; X, R, W1 and W2 16-byte aligned.
  * The down products of all active experts are one product for all tokens (with p = 0 where a token did not choose an
  * expert), so a W2 that holds an infinity or a NaN reaches every token of a call in which any token chose its expert;

@@ -221,3 +221,46 @@ def test_no_tokens_and_the_workspace_query():
     assert bwgemm.lib().bw_moe_work_bytes(0, 8, 2, 128, 64, ctypes.byref(n)) == bwgemm.BW_OK and n.value == 0
     assert bwgemm.lib().bw_moe_work_bytes(4, 8, 9, 128, 64, ctypes.byref(n)) == bwgemm.BW_ERR_SHAPE
     assert bwgemm.lib().bw_moe_work_bytes(4, 8, 2, 128, 64, None) == bwgemm.BW_ERR_ARG
+
+
+# ------------------------------------------------------------------ what of h reaches the down product
+def close_to_one_rounding(Y, X, ids, weights, err, W1, W2):
+    """h = p silu(g) u goes to the down product as two values of the type, together within 2^-16 (bf16) or 2^-22 (fp16) of it
+    and, in fp16, at worst 2^-28 off (half the second value's smallest step, its scale counted): independent errors, whose
+    sum over an expert's F has at most 2^-28 / sqrt(3) of the norm of W2's row as its standard deviation.  The sums are fp32
+    (2^-20 of Y's norm at these sizes).  Beside Y's own rounding that is (for bf16 1 / 128 of the rounding, added in quadrature)."""
+    y, _ = moe_ref.layer(X, ids, weights, err, W1, W2)
+    rounded = (y.to(X.dtype).double() - y).norm()
+    tiny = torch.zeros_like(y)
+    if X.dtype == torch.float16:
+        for t in range(X.shape[0]):
+            for e in ids[t].tolist():
+                tiny[t] += (2.0 ** -28 * W2[e].double().norm(dim=1)) ** 2
+    assert torch.isfinite(Y.double()).all()
+    got = (Y.double() - y).norm()
+    assert got <= 1.02 * rounded + 2.0 ** -18 * y.norm() + tiny.sum().sqrt(), float(got / rounded)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,D,F,grid", [(8, 4, 2, 128, 128, 4), (9, 4, 2, 128, 192, 3), (40, 3, 3, 128, 128, 7),
+                                            (64, 2, 1, 64, 128, 2), (65, 2, 1, 320, 64, 3), (128, 2, 2, 64, 192, 2)])
+def test_emulated_layer_is_as_exact_as_one_rounding(emu, T, E, k, D, F, grid, dtype):
+    X, R, W1, W2 = inputs(T, E, D, F, dtype, T + F)
+    ids, weights, err = moe_ref.route(X, R, k)
+    Y, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, grid)
+    assert findings == 0 and st[0] == 0, (msg, st)
+    assert torch.isnan(Y[T:]).all()
+    close_to_one_rounding(Y[:T], X, ids, weights, err, W1, W2)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 8, 2.0 ** -9])
+@pytest.mark.parametrize("T", [3, 20, 80])
+def test_emulated_activations_beyond_the_range_of_fp16(emu, T, scale):
+    """h up to some 2^20 with small W2, where fp16 ends at 65504; h around 2^-19, below its smallest normal, with large W2."""
+    D, F = 128, 128
+    X, R, W1, W2 = inputs(T, 4, D, F, torch.float16, T)
+    W1, W2 = (W1.float() * scale).half(), (W2.float() / scale ** 1.5).half()
+    ids, weights, err = moe_ref.route(X, R, 2)
+    Y, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, 4)
+    assert findings == 0 and st[0] == 0, (msg, st)
+    close_to_one_rounding(Y[:T], X, ids, weights, err, W1, W2)

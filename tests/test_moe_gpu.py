@@ -227,3 +227,35 @@ def test_few_tokens_are_as_exact_as_one_rounding(T, E, k, D, F, dtype):
     y, _ = moe_ref.layer(a[0], ids, weights, err, a[2], a[3])
     rounded = (y.to(dtype).double() - y).norm()
     assert (Y.double() - y).norm() <= 1.02 * rounded + 2.0 ** -18 * y.norm()
+
+
+def close_to_one_rounding(Y, X, R, W1, W2, k):
+    """As test_moe_cpu.close_to_one_rounding derives it: h is off by 2^-16 (bf16) or 2^-22 (fp16) of itself or, in fp16, by up
+    to 2^-28 (independent errors, whose sum has at most 2^-28 / sqrt(3) of the norm of W2's row as its standard deviation);
+    the sums are fp32, 2^-20 of Y's norm at these sizes."""
+    ids, weights, err = moe_ref.route(X, R, k)
+    y, _ = moe_ref.layer(X, ids, weights, err, W1, W2)
+    rounded = (y.to(X.dtype).double() - y).norm()
+    tiny = 0.0
+    if X.dtype == torch.float16:
+        rows = torch.stack([w.double().norm() for w in W2])  # over an expert's D rows
+        tiny = 2.0 ** -28 * float(rows[ids].norm())
+    assert torch.isfinite(Y).all()
+    assert (Y.double() - y).norm() <= 1.02 * rounded + 2.0 ** -18 * y.norm() + tiny
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,D,F", [(9, 16, 4, 512, 704), (17, 8, 2, 2112, 320), (48, 32, 4, 256, 512), (64, 8, 2, 1024, 576),
+                                       (65, 8, 2, 512, 1344), (96, 4, 1, 320, 64), (128, 32, 4, 1472, 704)])
+def test_any_number_of_tokens_is_as_exact_as_one_rounding(T, E, k, D, F, dtype):
+    a = inputs(T, E, D, F, dtype, seed=T)
+    close_to_one_rounding(bwgemm.moe_mlp(*a, k), *a, k)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 8, 2.0 ** -9])
+@pytest.mark.parametrize("T", [3, 20, 80])
+def test_activations_beyond_the_range_of_fp16(T, scale):
+    """h up to some 2^20 with small W2, where fp16 ends at 65504; h around 2^-19, below its smallest normal, with large W2."""
+    X, R, W1, W2 = inputs(T, 8, 256, 512, torch.float16, T)
+    W1, W2 = (W1.float() * scale).half(), (W2.float() / scale ** 1.5).half()
+    close_to_one_rounding(bwgemm.moe_mlp(X, R, W1, W2, 2), X, R, W1, W2, 2)
