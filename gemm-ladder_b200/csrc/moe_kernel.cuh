@@ -54,6 +54,7 @@ struct MoeParams {
     int slot_bytes;
     const int* ids;     // T x top_k
     const float* weights;
+    const uint16_t* W2; // (the tensor maps hold the weights' addresses otherwise)
     const uint8_t* X;   // the tokens, by K-blocks (moe_token_bytes)
     uint8_t* H;         // the activations of each active expert, likewise, two planes
     long long plane;
@@ -245,18 +246,28 @@ __device__ __forceinline__ void moe_load8(uint32_t tbase, int n, int c0, int lo,
             r[w][j] = __float_as_uint(fmaf(__uint_as_float(x[w][j]), sl, __uint_as_float(r[w][j]) * sh));
 }
 
+__device__ __forceinline__ bool moe_finite(float v) { return fabsf(v) <= 3.4028235e38f; }
 __device__ __forceinline__ float moe_shfl_xor(float v, int m)
 {
     return __uint_as_float(__shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(v), m));
 }
 
-// This block's part of the sum of a split down tile: items (four tokens of one column) [n mine / nseg, n (mine + 1) /
-// nseg) of the tile's n.  With few tokens there are fewer items than threads: 2^ls lanes then share an item, each
-// adding every 2^ls-th part in block order, and their sums meet in a tree (ls depends on the sizes alone).
-__device__ __noinline__ void moe_sum_down(const MoeParams& p, const MoeSeg& g, int c, int tq, int tid, int lane)
+// This block's part of a down tile's results: of the tile's n items (four tokens of one column) [n mine / nseg, n (mine + 1) /
+// nseg).
+__device__ __forceinline__ void moe_down_items(const MoeSeg& g, int c, int tq, int& i0, int& i1)
 {
     const int items = 2 * tq * 128, mine = c - g.first;
-    const int i0 = (int)((long long)items * mine / g.nseg), i1 = (int)((long long)items * (mine + 1) / g.nseg);
+    i0 = (int)((long long)items * mine / g.nseg);
+    i1 = (int)((long long)items * (mine + 1) / g.nseg);
+}
+
+// Its sum over a split tile's parts; true if all of it is finite.  With few tokens there are fewer items than threads: 2^ls lanes then share an item, each
+// adding every 2^ls-th part in block order, and their sums meet in a tree (ls depends on the sizes alone).
+__device__ __noinline__ bool moe_sum_down(const MoeParams& p, const MoeSeg& g, int c, int tq, int tid, int lane)
+{
+    int i0, i1;
+    moe_down_items(g, c, tq, i0, i1);
+    bool fine = true;
     int ls = 0;
     while (ls < 5 && (1 << ls) < g.nseg && ((i1 - i0) << (ls + 1)) <= kMoeEpiThreads) ++ls;
     const int per = 32 >> ls, sub = lane / per;  // items per warp; this lane's share of its item
@@ -298,6 +309,68 @@ __device__ __noinline__ void moe_sum_down(const MoeParams& p, const MoeSeg& g, i
         if (t0 + 1 < p.T) dst[(size_t)p.D] = moe_bits16(v.y, p.bf16);
         if (t0 + 2 < p.T) dst[2 * (size_t)p.D] = moe_bits16(v.z, p.bf16);
         if (t0 + 3 < p.T) dst[3 * (size_t)p.D] = moe_bits16(v.w, p.bf16);
+        fine &= moe_finite(v.x) && (t0 + 1 >= p.T || moe_finite(v.y)) && (t0 + 2 >= p.T || moe_finite(v.z)) &&
+                (t0 + 3 >= p.T || moe_finite(v.w));
+    }
+    return fine;
+}
+
+__device__ __forceinline__ float moe_value(uint32_t bits, int bf16)
+{
+    if (bf16) return __uint_as_float(bits << 16);
+    __half h;
+    *reinterpret_cast<uint16_t*>(&h) = (uint16_t)bits;
+    return __half2float(h);
+}
+// This block's results that are no finite numbers, again: each as the sum over its own token's experts alone, h put
+// together before it is multiplied.  In the shared accumulators the zeros of tokens that did not choose an expert meet an
+// infinity or a NaN of its W2 (0 x inf), and h's second value meets it with a sign of its own.  A warp per element, for
+// results that were no numbers anyway: ordinary calls pay a flag.
+__device__ __noinline__ void moe_redo(const MoeParams& p, const MoeSched& s, const uint32_t* mask, int c, int tq, int tid,
+                                      int lane)
+{
+    MoeIter it(s, c);
+    MoeSeg g;
+    const uint16_t inf = p.bf16 ? 0x7F80u : 0x7C00u;
+    const float sh = p.bf16 ? 1.f : 1.f / kMoeHiScale, sl = p.bf16 ? 1.f : 1.f / kMoeLoScale;
+    while (it.next(s, g)) {
+        if (!g.phase) continue;
+        int i0, i1;
+        moe_down_items(g, c, tq, i0, i1);
+        for (int x = i0 + (tid >> 5); x < i1; x += kMoeEpiThreads / 32) {
+            const int w = x / (tq * 128), t0 = (x - w * tq * 128) / 128 * 4;
+            const int d = g.tile * 256 + w * 128 + (x & 127);
+            for (int t = t0; d < p.D && t < t0 + 4 && t < p.T; ++t) {
+                uint16_t* y = p.Y + (size_t)t * p.D + d;
+                if ((*y & 0x7FFFu) < inf) continue;
+                float v = 0.f;
+                for (int j = 0; j < p.top_k; ++j) {
+                    const int e = p.ids[t * p.top_k + j];
+                    int at = __popc(mask[e >> 5] & ((1u << (e & 31)) - 1u));
+                    for (int i = 0; i < e >> 5; ++i) at += __popc(mask[i]);
+                    ld_acquire_gpu(p.ready + at);  // (complete: h is in)
+                    const uint16_t* w2 = p.W2 + ((size_t)e * p.D + d) * p.F;
+                    for (int f = 8 * lane; f < p.F; f += 256) {
+                        const uint8_t* h = p.H + moe_token_bytes(p.T, at * s.kbf + (f >> 6), t, f >> 3 & 7);
+                        const uint4 a = __ldcg(reinterpret_cast<const uint4*>(h));
+                        const uint4 b = __ldcg(reinterpret_cast<const uint4*>(h + p.plane));
+                        const uint4 m = __ldcg(reinterpret_cast<const uint4*>(w2 + f));
+                        const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+                        const uint32_t mv[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = (i & 1) * 16;
+                            const float hi = moe_value(av[i / 2] >> r & 0xFFFFu, p.bf16);
+                            const float lo = moe_value(bv[i / 2] >> r & 0xFFFFu, p.bf16);
+                            v = fmaf(fmaf(lo, sl, hi * sh), moe_value(mv[i / 2] >> r & 0xFFFFu, p.bf16), v);
+                        }
+                    }
+                }
+                for (int m = 16; m >= 1; m >>= 1) v += moe_shfl_xor(v, m);
+                __syncwarp();  // every lane has read what was there
+                if (lane == 0) *y = moe_bits16(v, p.bf16);
+            }
+        }
     }
 }
 
@@ -333,6 +406,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     volatile int* epi_go = abort_flag + 1;    // two slots, alternating by segment
     volatile int* epi_sum = abort_flag + 3;   // two slots: this block sums the segment's tile
     volatile int* epi_pend = abort_flag + 5;  // two slots: a split down tile's parts are all there
+    volatile int* epi_odd = abort_flag + 7;   // a result of this block is not finite
     uint32_t* mask = reinterpret_cast<uint32_t*>(misc + MoeSmem::kMask);
     uint16_t* expert = reinterpret_cast<uint16_t*>(misc + MoeSmem::kExpert);
     float* gate = reinterpret_cast<float*>(misc + MoeSmem::kGate);
@@ -361,6 +435,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
+        *epi_odd = 0;
         fence_barrier_init();
     }
     if (threadIdx.x < kMoeMaxExperts / 32) mask[threadIdx.x] = 0u;
@@ -551,7 +626,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         MoeSeg sg, pend[2];
         int acc = 0, seg = 0, n_pend = 0, gate_slot = -1;
         uint32_t aph = 0;
-        bool ok = true;
+        bool ok = true, fine = true;  // fine: this thread's results are finite so far
         // a partial: [block w of 2][group of 4 tokens][row][4]
         auto slot_of = [&](int blk, const MoeSeg& g) {
             return reinterpret_cast<float4*>(p.partials + (size_t)moe_slot(g, blk) * p.slot_floats);
@@ -660,7 +735,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                             if (d >= p.D) continue;
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                if (c0 + j < p.T) p.Y[(size_t)(c0 + j) * p.D + d] = moe_bits16(a[w][j], p.bf16);
+                                if (c0 + j < p.T) {
+                                    p.Y[(size_t)(c0 + j) * p.D + d] = moe_bits16(a[w][j], p.bf16);
+                                    fine &= moe_finite(a[w][j]);
+                                }
                         }
                     }
                 }
@@ -697,8 +775,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             named_bar_sync(1, kMoeEpiThreads);
             ok = epi_pend[i] != 0;
             if (threadIdx.x == kMoeEpiThread0) BW_TRACE_AT(10);  // the others' partials are in
-            if (ok) moe_sum_down(p, g, c, tq, tid, lane);
+            if (ok) fine &= moe_sum_down(p, g, c, tq, tid, lane);
         }
+        if (!fine) *epi_odd = 1;
+        named_bar_sync(1, kMoeEpiThreads);  // (also: this block's results are written)
+        if (ok && *epi_odd) moe_redo(p, s, mask, c, tq, tid, lane);
     }
 
     __syncwarp();

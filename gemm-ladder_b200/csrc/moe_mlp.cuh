@@ -86,6 +86,7 @@ int moe_mlp(const void* X, long long ldx, const void* R, const void* W1, const v
     p.slot_bytes = moe_slot_bytes(T);
     p.ids = ids;
     p.weights = weights;
+    p.W2 = static_cast<const uint16_t*>(W2);
     p.X = ws + w.x;
     p.H = ws + w.h;
     p.plane = w.plane;

@@ -59,6 +59,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe(const uint16_t*
     moe_rings(T, &p.stages, &p.slots);
     p.slot_bytes = moe_slot_bytes(T);
     p.ids = ids, p.weights = weights;
+    p.W2 = W2;
     p.X = base + w.x, p.H = base + w.h, p.plane = w.plane, p.Y = Y;
     for (int t = 0; t < T; ++t)  // the router's layout of the tokens
         for (int c = 0; c < D / 8; ++c)

@@ -789,6 +789,11 @@ inline float4 __ldcg(const float4* p)
     std::atomic_thread_fence(std::memory_order_acquire);
     return *p;
 }
+inline uint4 __ldcg(const uint4* p)
+{
+    std::atomic_thread_fence(std::memory_order_acquire);
+    return *p;
+}
 inline int min(int a, int b) { return a < b ? a : b; }
 inline uint32_t max(uint32_t a, uint32_t b) { return a > b ? a : b; }
 inline void __stcg(float4* p, float4 v) { *p = v; }

@@ -131,9 +131,8 @@ int bw_linear_i8(const void* X, int x_type, long long ld, const void* B, const v
  * in fp32 sums; p_te silu * up goes to the down product as two values of the type, to twice its precision (in fp16 scaled, so
  * that it may reach 1.6e7), and Y is rounded once.  D % 64 == 0, F % 64 == 0,
  * E <= 512, top_k <= min(E, 32), ldx >= D, ldx % 8 == 0; X, R, W1 and W2 16-byte aligned.
- * The down products of all active experts are one product for all tokens (with p = 0 where a token did not choose an
- * expert), so a W2 that holds an infinity or a NaN reaches every token of a call in which any token chose its expert;
- * an infinity or a NaN anywhere else stays with the tokens that meet it.
+ * An infinity or a NaN in X or in the weights reaches the elements of Y whose sums hold it and no others (elements that are
+ * not finite are summed a second time, so a call with many of them takes longer).
  * ids (T x top_k int32, by falling logit) and weights (T x top_k fp32) receive the routing where not null.
  * `work`: as for the 8-bit entries, at least bw_moe_work_bytes (T, E, top_k, D, F) bytes, 256-byte aligned.  The experts
  * kernel is a cooperative launch of one block per SM.  T == 0 is a call that does nothing.  No reference counterpart.

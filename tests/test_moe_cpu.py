@@ -264,3 +264,35 @@ def test_emulated_activations_beyond_the_range_of_fp16(emu, T, scale):
     Y, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, 4)
     assert findings == 0 and st[0] == 0, (msg, st)
     close_to_one_rounding(Y[:T], X, ids, weights, err, W1, W2)
+
+
+# ------------------------------------------------------------------ infinities and NaN in the weights
+def check_w2(Y, clean, X, ids, weights, err, W1, W2, cols):
+    """An infinity or a NaN of W2 reaches, in its own column, the tokens that chose its expert, as the definition has it;
+    every other element is what it is without (in those columns up to the order of its sum)."""
+    y, _ = moe_ref.layer(X, ids, weights, err, W1, W2)
+    y0, tol = moe_ref.layer(X, ids, weights, err, W1, torch.nan_to_num(W2, 0.0, 0.0, 0.0))
+    Y, fine = Y.double(), torch.isfinite(y)
+    assert (~fine).any() and fine[:, cols].any(), "the case shows nothing"
+    rest = [c for c in range(Y.shape[1]) if c not in cols]
+    assert torch.equal(Y[:, rest], clean.double()[:, rest])
+    assert torch.isfinite(Y[fine]).all()
+    assert ((Y - y0).abs() <= tol)[fine].all()
+    assert torch.equal(torch.isnan(Y), torch.isnan(y)) and torch.equal(Y[torch.isinf(y)], y[torch.isinf(y)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,D,F,grid", [(2, 8, 2, 256, 128, 4), (5, 4, 1, 576, 64, 2), (12, 6, 2, 320, 192, 3),
+                                            (70, 4, 1, 64, 64, 2)])
+def test_emulated_infinity_or_nan_in_w2_reaches_the_tokens_of_its_expert(emu, T, E, k, D, F, grid, dtype):
+    X, R, W1, W2 = inputs(T, E, D, F, dtype, T + 11)
+    ids, weights, err = moe_ref.route(X, R, k)
+    clean, _, _, _ = emulate(emu, X, W1, W2, ids, weights, grid)
+    e = int(ids[0, 0])
+    W2[e, 3, F // 2] = float("inf")
+    W2[e, D - 1, 0] = float("nan")
+    W2[e, 17, 5], W2[e, 17, 40] = float("inf"), float("-inf")
+    Y, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, grid)
+    assert findings == 0 and st[0] == 0, (msg, st)
+    assert torch.isnan(Y[T:]).all()
+    check_w2(Y[:T], clean[:T], X, ids, weights, err, W1, W2, [3, D - 1, 17])

@@ -259,3 +259,38 @@ def test_activations_beyond_the_range_of_fp16(T, scale):
     X, R, W1, W2 = inputs(T, 8, 256, 512, torch.float16, T)
     W1, W2 = (W1.float() * scale).half(), (W2.float() / scale ** 1.5).half()
     close_to_one_rounding(bwgemm.moe_mlp(X, R, W1, W2, 2), X, R, W1, W2, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,D,F", [(1, 8, 2, 256, 128), (7, 16, 4, 512, 704), (33, 8, 2, 1024, 1792), (128, 32, 4, 1472, 704),
+                                       (20, 2, 1, 64, 64)])
+def test_infinity_or_nan_in_w2_reaches_the_tokens_of_its_expert(T, E, k, D, F, dtype):
+    """As test_moe_cpu.check_w2: in its own column, the tokens that chose its expert; every other element is what it is
+    without (in those columns up to the order of its sum)."""
+    X, R, W1, W2 = inputs(T, E, D, F, dtype, seed=T + 9)
+    clean = bwgemm.moe_mlp(X, R, W1, W2, k)
+    ids, weights, err = moe_ref.route(X, R, k)
+    e, cols = int(ids[0, 0]), [3, D - 1, 17]
+    W2[e, 3, F // 2] = float("inf")
+    W2[e, D - 1, 0] = float("nan")
+    W2[e, 17, 5], W2[e, 17, 40] = float("inf"), float("-inf")
+    Y = bwgemm.moe_mlp(X, R, W1, W2, k)
+    y, _ = moe_ref.layer(X, ids, weights, err, W1, W2)
+    y0, tol = moe_ref.layer(X, ids, weights, err, W1, torch.nan_to_num(W2, 0.0, 0.0, 0.0))
+    rest = [c for c in range(D) if c not in cols]
+    assert torch.equal(Y[:, rest], clean[:, rest])
+    Y, fine = Y.double(), torch.isfinite(y)
+    assert not fine[0, cols].any()
+    assert ((Y - y0).abs() <= tol)[fine].all() and torch.isfinite(Y[fine]).all()
+    assert torch.equal(torch.isnan(Y), torch.isnan(y)) and torch.equal(Y[torch.isinf(y)], y[torch.isinf(y)])
+
+
+def test_a_weight_tensor_full_of_nan():
+    """Every result is summed again: slower, and still the definition's (an expert that nobody chose is not met)."""
+    X, R, W1, W2 = inputs(64, 8, 512, 1024, torch.bfloat16, 51)
+    ids, _, _ = moe_ref.route(X, R, 2)
+    bwgemm.moe_mlp(X, R, W1, W2, 2)
+    W2[:] = float("nan")
+    assert torch.isnan(bwgemm.moe_mlp(X, R, W1, W2, 2)).all()
+    torch.cuda.synchronize()
+    assert bwgemm.status()[0] == 0
