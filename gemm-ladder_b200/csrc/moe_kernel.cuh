@@ -10,7 +10,7 @@
 // weights without a pause from the first to the last byte:
 //   - as in the swap-AB GEMM the weights fill the MMA's 128 rows (two MMAs per stage: gate and up rows, or 256 rows of
 //     W2) and the tokens its N.  All T tokens are multiplied with every active expert (the tensor core idles anyway);
-//     a token that did not choose the expert gets p = 0, so no rows are gathered or sorted.
+//     a token that did not choose the expert gets h = 0, so no rows are gathered or sorted.
 //   - the router's weights are folded into h, so that the down product of all experts is one product whose K is the
 //     active experts' F one after the other: the sum over the experts happens in the accumulator.
 //   - both products are cut evenly over the blocks by K-blocks (moe_sched.h); split tiles are summed in block order
@@ -192,9 +192,12 @@ __device__ __forceinline__ void moe_sum_parts(const MoeParams& p, const MoeSeg& 
     }
 }
 
+constexpr float kMoeNotChosen = -1.f;  // in the place of p, which is no negative number (0 where it underflowed)
+
 // h = p silu(g) u of 8 tokens, without a branch so that their chains overlap (the last whole gate/up tile's epilogue is
-// what the down product waits for).  The fast exponential and division are within (2 + 1.16 |g|) 2^-23 and 2^-22.  A
-// token that did not choose the expert (p = 0) contributes nothing, whatever its products.
+// what the down product waits for).  The fast exponential and division are within (2 + 1.16 |g|) 2^-23 and 2^-22 (below
+// g = -87.3, where 1 + exp(-g) passes 2^126, the division gives 0 for up to 2^-119 |u|).  A token that did not choose the
+// expert (kMoeNotChosen) contributes nothing, whatever its products.
 __device__ __forceinline__ void moe_activation(const float (&a)[2][8], const float* gate, float (&v)[8])
 {
     const float4 p0 = *reinterpret_cast<const float4*>(gate), p1 = *reinterpret_cast<const float4*>(gate + 4);
@@ -202,7 +205,7 @@ __device__ __forceinline__ void moe_activation(const float (&a)[2][8], const flo
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         v[j] = pr[j] * (__fdividef(a[0][j], 1.0f + __expf(-a[0][j])) * a[1][j]);
-        v[j] = pr[j] == 0.f ? 0.f : v[j];
+        v[j] = pr[j] == kMoeNotChosen ? 0.f : v[j];
     }
 }
 
@@ -638,7 +641,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                 named_bar_sync(1, kMoeEpiThreads);   // the previous expert's have been read
                 if (tid < Tp) {  // (a group of 8 tokens reads 8)
                     const int e = expert[sl];
-                    float v = 0.f;
+                    float v = kMoeNotChosen;
                     for (int j = 0; tid < p.T && j < p.top_k; ++j) {
                         const float pr = p.weights[tid * p.top_k + j];
                         if (p.ids[tid * p.top_k + j] == e) v = pr;

@@ -296,3 +296,15 @@ def test_emulated_infinity_or_nan_in_w2_reaches_the_tokens_of_its_expert(emu, T,
     assert findings == 0 and st[0] == 0, (msg, st)
     assert torch.isnan(Y[T:]).all()
     check_w2(Y[:T], clean[:T], X, ids, weights, err, W1, W2, [3, D - 1, 17])
+
+
+def test_a_chosen_expert_whose_weight_underflowed_still_passes_nan_on(emu):
+    """p = 0 of an expert that was chosen (a softmax weight below fp32) is a factor, 0 x NaN; of one that was not, no term."""
+    X, R, W1, W2 = inputs(5, 4, 128, 64, torch.bfloat16, 15)
+    ids = torch.tensor([[0, 1], [0, 2], [1, 2], [3, 2], [2, 0]])
+    weights = torch.tensor([[1.0, 0.0], [1.0, 0.0], [0.5, 0.5], [1.0, 0.0], [0.25, 0.75]])
+    want, _, _, _ = emulate(emu, X, W1, W2, ids, weights, 3)
+    W1[1, 7] = float("nan")
+    Y, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, 3)
+    assert findings == 0 and st[0] == 0, (msg, st)
+    assert torch.isnan(Y[[0, 2]]).all() and torch.equal(Y[[1, 3, 4]], want[[1, 3, 4]])
