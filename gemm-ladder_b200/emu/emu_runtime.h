@@ -128,6 +128,12 @@ inline bool keep_commit()
 {
     return g_drop_commit < 0 || (int)blockIdx.x != g_drop_block || g_commit_count.fetch_add(1) != g_drop_commit;
 }
+// Stalls of the experts kernel, made on purpose: the n-th (of a launch; -1: none) bulk completion, count of a finished
+// gate/up tile, count of a split tile's part goes missing.
+enum { kDropBulk, kDropRed, kDropAtom, kDrops };
+inline long long g_drop_nth[kDrops] = {-1, -1, -1};
+inline std::atomic<long long> g_drop_count[kDrops];
+inline bool kept(int kind) { return g_drop_nth[kind] < 0 || g_drop_count[kind].fetch_add(1) != g_drop_nth[kind]; }
 inline unsigned long long g_wait_ns = 60ull * 1000000000ull;  // the kernel's limit of one bounded wait
 inline unsigned long long g_rank_wait_ns = 0;  // the limit of a wait for another rank's flag (0: g_wait_ns)
 

@@ -164,7 +164,7 @@ inline uint64_t policy_evict_last() { return 0; }
 inline void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
 {
     emu::Cta* c = emu::t_cta;
-    const bool keep = emu::keep_completion();
+    const bool keep = emu::keep_completion() & emu::kept(emu::kDropBulk);
     const uint32_t boff = emu::offset_of(bar);
     c->tma.post([=] {
         emu::bulk_copy(dst, src, bytes);
@@ -296,8 +296,14 @@ constexpr uint32_t idesc_i8_s32(int m, int n)
 
 // ------------------------------------------------------------------ global memory ordering, named barriers
 inline int ld_acquire_gpu(const int* p) { return __atomic_load_n(p, __ATOMIC_ACQUIRE); }
-inline int atom_add_acq_rel_gpu(int* p, int v) { return __atomic_fetch_add(p, v, __ATOMIC_ACQ_REL); }
-inline void red_add_release_gpu(int* p, int v) { __atomic_fetch_add(p, v, __ATOMIC_RELEASE); }
+inline int atom_add_acq_rel_gpu(int* p, int v)
+{
+    return __atomic_fetch_add(p, emu::kept(emu::kDropAtom) ? v : 0, __ATOMIC_ACQ_REL);
+}
+inline void red_add_release_gpu(int* p, int v)
+{
+    if (emu::kept(emu::kDropRed)) __atomic_fetch_add(p, v, __ATOMIC_RELEASE);
+}
 inline void named_bar_sync(uint32_t id, uint32_t count) { emu::named_sync((int)id, (int)count); }
 
 }  // namespace bw

@@ -294,3 +294,20 @@ def test_a_weight_tensor_full_of_nan():
     assert torch.isnan(bwgemm.moe_mlp(X, R, W1, W2, 2)).all()
     torch.cuda.synchronize()
     assert bwgemm.status()[0] == 0
+
+
+def test_a_stalls_status_stays_until_it_is_cleared():
+    """A wait that ran out elsewhere (the library's own check) is still in the status word after a call of the layer, whose
+    result does not depend on it."""
+    a = inputs(5, 16, 256, 128, torch.float16, 61)
+    want = bwgemm.moe_mlp(*a, 4)
+    try:
+        assert bwgemm.wait_selftest(50_000_000) == bwgemm.BW_ERR_TIMEOUT
+        before = bwgemm.status()
+        assert before[0] == bwgemm.BW_ERR_TIMEOUT
+        assert torch.equal(bwgemm.moe_mlp(*a, 4), want)
+        torch.cuda.synchronize()
+        assert bwgemm.status() == before
+    finally:
+        bwgemm.clear_status()
+    assert bwgemm.status()[0] == 0
