@@ -257,7 +257,8 @@ int dispatch(const bw_plan& q, const CUtensorMap& mx, const CUtensorMap& my, con
 // Sets a knob of the emulator: "wait_ns" (the kernel's limit of one bounded wait), "rank_wait_ns" (the limit of a wait
 // for another rank's flag; 0: wait_ns), "drop_tma" (the n-th TMA / bulk
 // completion of each launch never arrives, -1 none), "drop_block" (>= 0: the n-th of this block's), "drop_commit" (from now on
-// the n-th tcgen05.commit of block drop_block arrives nowhere), "barrier_limit_ms" (a thread barrier never completed: a finding
+// the n-th tcgen05.commit of block drop_block arrives nowhere), "short_kind" (>= 0: waits on barriers
+// of this kind of the status word give up after a tenth of the limit), "barrier_limit_ms" (a thread barrier never completed: a finding
 // after this long), "cluster_batch" (clusters run at once; 0: as many as the host's cores take), "noalloc_cap"
 // (>= 0: fp16 calls of variant 0 plan as bw_gemm_f16_noalloc does, its array this many bytes; -1: the rule),
 // "ld_delay_us" (a random pause of up to this long before each tensor-memory load), "start_jitter_us" (each block starts
@@ -274,6 +275,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_set(const char* nam
     else if (n == "cluster_batch") bw::g_cluster_batch = value;
     else if (n == "drop_tma") g_drop_tma = value;
     else if (n == "drop_block") g_drop_block = (int)value;
+    else if (n == "short_kind") g_short_kind = (int)value;
     else if (n == "drop_commit") g_drop_commit = value, g_commit_count = 0;
     else if (n == "barrier_limit_ms") g_barrier_limit_ms = value;
     else if (n == "noalloc_cap") bw::g_noalloc_cap = value;

@@ -4,7 +4,7 @@
 //
 // C entry:
 //   bw_emu_moe(X, ldx, W1, W2, Y, ids, weights, T, E, top_k, D, F, grid, bf16, status[4], &findings, finding, len)
-//   bw_emu_moe_set(name, value): wait_ns, drop_tma, drop_bulk, drop_red, drop_atom (emu_runtime.h), engine_delay_us, start_jitter_us, block_ramp_us, ld_delay_us
+//   bw_emu_moe_set(name, value): wait_ns, drop_tma, drop_bulk, drop_red, drop_atom, first_kind (emu_runtime.h), engine_delay_us, start_jitter_us, block_ramp_us, ld_delay_us
 #include <future>
 #include <string>
 #include <thread>
@@ -35,6 +35,7 @@ extern "C" __attribute__((visibility("default"))) int bw_emu_moe_set(const char*
     else if (n == "start_jitter_us") g_start_jitter_us = (int)value;
     else if (n == "block_ramp_us") g_block_ramp_us = (int)value;
     else if (n == "ld_delay_us") g_ld_delay_us = (int)value;
+    else if (n == "first_kind") g_first_kind = (int)value;
     else if (n == "drop_bulk") g_drop_nth[kDropBulk] = value, g_drop_count[kDropBulk] = 0;
     else if (n == "drop_red") g_drop_nth[kDropRed] = value, g_drop_count[kDropRed] = 0;
     else if (n == "drop_atom") g_drop_nth[kDropAtom] = value, g_drop_count[kDropAtom] = 0;

@@ -128,6 +128,10 @@ inline bool keep_commit()
 {
     return g_drop_commit < 0 || (int)blockIdx.x != g_drop_block || g_commit_count.fetch_add(1) != g_drop_commit;
 }
+// Barrier waits of other kinds than g_first_kind (>= 0; site's kind) wait 5 times as long: which of the waits that a stall
+// holds up gives up first is then no matter of chance.
+inline int g_first_kind = -1;
+inline int g_short_kind = -1;  // barrier waits of this kind (>= 0) wait a tenth as long
 // Stalls of the experts kernel, made on purpose: the n-th (of a launch; -1: none) bulk completion, count of a finished
 // gate/up tile, count of a split tile's part goes missing.
 enum { kDropBulk, kDropRed, kDropAtom, kDrops };

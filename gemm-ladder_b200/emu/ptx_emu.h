@@ -74,6 +74,8 @@ inline void spin_pause(uint32_t i)
 inline bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns, uint32_t where, int seg)
 {
     const uint64_t t0 = globaltimer_ns();
+    if (emu::g_first_kind >= 0 && (int)(where >> 8 & 0xFFu) != emu::g_first_kind) limit_ns *= 5;
+    if (emu::g_short_kind >= 0 && (int)(where >> 8 & 0xFFu) == emu::g_short_kind) limit_ns /= 10;
     for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         spin_pause(i);

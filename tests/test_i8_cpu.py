@@ -180,15 +180,15 @@ def test_a_block_that_gives_up_leaves_after_the_parts_sent_to_it(emu, force):
     sa, sb = np.ones(M, np.float32), np.ones(N, np.float32)
     st, dirty, nf = (ctypes.c_uint * 4)(), ctypes.c_int(), ctypes.c_int()
     msg, vp = ctypes.create_string_buffer(512), ctypes.c_void_p
-    # a part takes about half a second to cross; the wait gives up after 0.3 s, the drain after 1 s more
-    knobs = dict(force_ksplit=force, wait_ns=300_000_000, engine_delay_us=2000, drop_block=c - 1, drop_commit=4)
+    # a part takes about half a second to cross; the accumulator's wait (kind 2) gives up after 0.3 s, others after 3
+    knobs = dict(force_ksplit=force, wait_ns=3_000_000_000, short_kind=2, engine_delay_us=2000, drop_block=c - 1, drop_commit=4)
     for name, value in knobs.items():
         assert emu.bw_emu_set(name.encode(), ctypes.c_longlong(value)) == 0
     try:
         emu.bw_emu_gemm_i8(vp(A.ctypes.data), vp(sa.ctypes.data), vp(B.ctypes.data), vp(sb.ctypes.data), vp(C.ctypes.data),
                            M, N, K, 2 * c, F16, 0, st, ctypes.byref(dirty), ctypes.byref(nf), msg, 512)
     finally:
-        for name, value in dict(force_ksplit=0, wait_ns=60_000_000_000, engine_delay_us=20, drop_block=-1,
+        for name, value in dict(force_ksplit=0, wait_ns=60_000_000_000, short_kind=-1, engine_delay_us=20, drop_block=-1,
                                 drop_commit=-1).items():
             emu.bw_emu_set(name.encode(), ctypes.c_longlong(value))
     assert st[0] == 3, "no wait gave up"

@@ -310,17 +310,21 @@ def test_a_chosen_expert_whose_weight_underflowed_still_passes_nan_on(emu):
     assert torch.isnan(Y[[0, 2]]).all() and torch.equal(Y[[1, 3, 4]], want[[1, 3, 4]])
 
 
-@pytest.mark.parametrize("what,role,kind", [("drop_bulk", 1, 12), ("drop_red", 3, 10), ("drop_atom", 2, 11)])
-def test_a_stall_is_recorded_where_it_was_seen(emu, what, role, kind):
-    """A stage's tokens that never land, a gate/up tile that is never counted, a part of a split down tile that is never
-    counted (D = 64: no gate/up tile is split): the wait that gave up is in the status word, and every block leaves."""
-    X, R, W1, W2 = inputs(2, 4, 64, 256, torch.float16, 16)
+@pytest.mark.parametrize("what,D,grid,role,kind", [("drop_bulk", 512, 1, 1, 12), ("drop_red", 64, 4, 3, 10),
+                                                   ("drop_atom", 64, 4, 2, 11)])
+def test_a_stall_is_recorded_where_it_was_seen(emu, what, D, grid, role, kind):
+    """A stage's tokens that never land (one block, more stages than its ring holds), a gate/up tile that is never counted, a
+    part of a split down tile that is never counted (D = 64: no gate/up tile is split): the wait that gave up first is in the
+    status word, and every block leaves."""
+    X, R, W1, W2 = inputs(2, 4, D, 256, torch.float16, 16)
     ids, weights, _ = moe_ref.route(X, R, 2)
-    emu.bw_emu_moe_set(b"wait_ns", ctypes.c_longlong(300_000_000))
+    emu.bw_emu_moe_set(b"first_kind", ctypes.c_longlong(kind))
+    emu.bw_emu_moe_set(b"wait_ns", ctypes.c_longlong(1_000_000_000))
     emu.bw_emu_moe_set(what.encode(), ctypes.c_longlong(1))
     try:
-        _, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, 4)
+        _, st, findings, msg = emulate(emu, X, W1, W2, ids, weights, grid)
     finally:
+        emu.bw_emu_moe_set(b"first_kind", ctypes.c_longlong(-1))
         emu.bw_emu_moe_set(b"wait_ns", ctypes.c_longlong(60_000_000_000))
         emu.bw_emu_moe_set(what.encode(), ctypes.c_longlong(-1))
     assert findings == 0, msg
