@@ -312,8 +312,8 @@ __device__ __noinline__ bool moe_sum_down(const MoeParams& p, const MoeSeg& g, i
         if (t0 + 1 < p.T) dst[(size_t)p.D] = moe_bits16(v.y, p.bf16);
         if (t0 + 2 < p.T) dst[2 * (size_t)p.D] = moe_bits16(v.z, p.bf16);
         if (t0 + 3 < p.T) dst[3 * (size_t)p.D] = moe_bits16(v.w, p.bf16);
-        fine &= moe_finite(v.x) && (t0 + 1 >= p.T || moe_finite(v.y)) && (t0 + 2 >= p.T || moe_finite(v.z)) &&
-                (t0 + 3 >= p.T || moe_finite(v.w));
+        fine &= moe_finite(v.x) & (moe_finite(v.y) | (t0 + 1 >= p.T)) & (moe_finite(v.z) | (t0 + 2 >= p.T)) &
+                (moe_finite(v.w) | (t0 + 3 >= p.T));
     }
     return fine;
 }
@@ -329,9 +329,10 @@ __device__ __forceinline__ float moe_value(uint32_t bits, int bf16)
 // together before it is multiplied.  In the shared accumulators the zeros of tokens that did not choose an expert meet an
 // infinity or a NaN of its W2 (0 x inf), and h's second value meets it with a sign of its own.  A warp per element, for
 // results that were no numbers anyway: ordinary calls pay a flag.
-__device__ __noinline__ void moe_redo(const MoeParams& p, const MoeSched& s, const uint32_t* mask, int c, int tq, int tid,
-                                      int lane)
+__device__ __noinline__ void moe_redo(const MoeParams& p, const uint32_t* mask, int active, int tid, int lane)
 {
+    const MoeSched s = moe_sched(p.T, p.D, p.F, active, gridDim.x);
+    const int c = blockIdx.x, tq = (p.T + 3) / 4;
     MoeIter it(s, c);
     MoeSeg g;
     const uint16_t inf = p.bf16 ? 0x7F80u : 0x7C00u;
@@ -780,14 +781,14 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             if (threadIdx.x == kMoeEpiThread0) BW_TRACE_AT(10);  // the others' partials are in
             if (ok) fine &= moe_sum_down(p, g, c, tq, tid, lane);
         }
-        if (!fine) *epi_odd = 1;
-        named_bar_sync(1, kMoeEpiThreads);  // (also: this block's results are written)
-        if (ok && *epi_odd) moe_redo(p, s, mask, c, tq, tid, lane);
+        if (ok && !fine) *epi_odd = 1;
     }
 
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (warp >= 2 && warp < 10 && *epi_odd)  // (this block's results are written: the barrier)
+        moe_redo(p, mask, active, threadIdx.x - kMoeEpiThread0, lane);
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
