@@ -16,16 +16,16 @@
 //   - both products are cut evenly over the blocks by K-blocks (moe_sched.h); split tiles are summed in block order
 //     (the same bits on every run).
 //   - between the products a block waits for the activations it needs, by active expert, but only its token-side loads
-//     do: the weights of W2 are already on their way into the ring (up to 175 KB per SM, 26 MB in all), so the wait
+//     do: the weights of W2 are already on their way into the ring (up to 160 KB per SM, 24 MB in all), so the wait
 //     costs no memory time.
 // Roles: one thread of warp 0 the weights' producer, one of warp 10 the tokens', one of warp 1 the MMA issuer, warps 2-9
 // the epilogue.  The blocks wait for one another, so the launch is cooperative (all blocks
 // resident); every wait is bounded (ptx.cuh).
 //
-// Measured on a B200, router included: 33 tokens over 8 experts of 4096 x 14336 (2.8 GB of weights, bf16) 431 us,
-// 6.9 TB/s in the streams; 8 tokens over 128 of 4096 x 1344 (51 active, 1.7 GB) 269 us; 64 tokens over 128 of 4096 x 1280
-// 634 us; 128 tokens over 32 of 2880 x 2880 329 us, where the SMs take in 59 GB/s each of weights and tokens;
-// one token, top 8 of 64 of 2048 x 1024 (100 MB) 42 us, of which the stream is 15.
+// Measured on a B200, router included, under load: 33 tokens over 8 experts of 4096 x 14336 (2.8 GB of weights, bf16) 466 us,
+// 6.4 TB/s in the streams; 8 tokens over 128 of 4096 x 1344 (51 active, 1.7 GB) 272 us; 64 tokens over 128 of 4096 x 1280
+// 686 us; 128 tokens over 32 of 2880 x 2880 380 us, where the SMs take in 58 to 75 GB/s each of weights and tokens;
+// one token, top 8 of 64 of 2048 x 1024 (100 MB) 44 us, of which the stream is 15.
 //
 // Roundings: h to two values of the tokens' type (the MMA's operand; moe_plane_rows of moe_sched.h; p is folded in before, in
 // fp32), y once at the end; sums in fp32.

@@ -7,9 +7,10 @@
 // products and a warp's loads are all in flight at once.  The ranges are summed in shared memory, the logits go to the
 // block of the cluster that chooses for the token through distributed shared memory, and one warp per token picks: no
 // counters, no second kernel.
-// The sums are chains of fp32 additions of products that are exact in fp32 (22 bits), short ones (D / (32 ds)), then a
-// tree: the choice between two experts can differ from the exact one only where their logits agree to about 2^-21 of
-// the products' magnitude.
+// A logit is a chain of D / (32 ds) fp32 additions per lane (of products that are exact in fp32), a tree of five and a chain
+// over the ds ranges, so within (D / (32 ds) + 5 + ds) 2^-24 of the sum of its products' magnitudes: 2^-19.6 at 64 experts of
+// 2048 (ds 8), 2^-18.6 at 128 of 4096 (ds 4), 2^-17 at 256 of 8192 (ds 2).  The choice between two experts can differ from
+// the exact one only where their logits agree that far.
 // Measured: 3.0 us at one token over 64 experts of 2048, 4.6 us at 8 over 128 of 4096, 8 us at 64.
 // It also clears the words that the experts kernel counts on, and lays the tokens out for its copies.
 #pragma once

@@ -150,8 +150,8 @@ BW_MOE_HD inline long long moe_token_bytes(int T, int kb, int t, int chunk) { re
 // 2^15), which leaves h off by 2^-23 of it or 2^-28, the larger.  bf16 has fp32's range: no scales, 2^-17 of h.
 //   up to 8 tokens  the planes are rows 0 and 8 of the 16 that the MMA takes anyway: free
 //   more            rows 0 and Tp (T rounded up to 16) of 2 Tp, one MMA of N = 2 Tp.  The tokens' intake of the down product
-//                   doubles: 1 % at 16 tokens, 3 % at 33 and 64, 8 % at 128 against one value.  (Two MMAs of N = Tp in its
-//                   place read the weights twice from shared memory: 13 to 18 % against one value.)
+//                   doubles: 1 % of the layer's time at 16 tokens, 3 % at 33 and 64, 8 % at 128 against one value (under the
+//                   power cap 4, 5 and 10 %).  (Two MMAs of N = Tp in its place: 13 to 18 %.)
 BW_MOE_HD inline int moe_padded(int T) { return (T + 15) / 16 * 16; }
 BW_MOE_HD inline int moe_plane_rows(int T) { return T <= 8 ? 8 : moe_padded(T); }
 constexpr float kMoeHiScale = 0.00390625f, kMoeLoScale = 8.0f;  // fp16

@@ -82,7 +82,9 @@ int bw_gemm_f16_swiglu(const void* A, const void* B, void* C, int M, int N, int 
  * 8-bit integer products with a scale per token and per channel.  A (M x K) and B (N x K, a linear layer's weight
  * layout) are row-major int8; a_scale[m] and b_scale[n] (fp32) are the scales of their rows; the sums are exact 32-bit
  * integers:
- *   C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k]      rounded once to C's type (out_type, BW_TYPE_*).
+ *   C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k]
+ * computed in fp32 as (float(sum) * a_scale[m]) * b_scale[n], in this order (three roundings; a product beyond fp32's range is
+ * an infinity or 0), then rounded to C's type (out_type, BW_TYPE_*).
  * N % 64 == 0, K % 16 == 0, 16 <= K <= 131056 (where the sum of K products of magnitude 2^14 stays below 2^31), any M;
  * A, B, C and b_scale 16-byte aligned, a_scale 4-byte aligned.  The same rule and plans as the fp16 entries, an int8 row
  * of K taking the place of an fp16 row of K / 2 (out_type BW_TYPE_F32: SM-pair tiles at every M).
