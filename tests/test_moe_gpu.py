@@ -311,3 +311,29 @@ def test_a_stalls_status_stays_until_it_is_cleared():
     finally:
         bwgemm.clear_status()
     assert bwgemm.status()[0] == 0
+
+
+def test_weights_whose_offsets_pass_32_bits():
+    """W1 of 2.35e9 elements; the chosen experts are the last ones, and an infinity in the last one's W2 takes the second
+    summation there."""
+    E, D, F = 160, 4096, 1792
+    X, R, _, _ = inputs(2, E, D, 64, torch.bfloat16, 71)
+    W1 = torch.zeros((E, 2 * F, D), dtype=torch.bfloat16, device="cuda")
+    W2 = torch.zeros((E, D, F), dtype=torch.bfloat16, device="cuda")
+    assert W1.numel() > 2 ** 31
+    g = torch.Generator(device="cuda")
+    g.manual_seed(72)
+    for e in (E - 2, E - 1):
+        W1[e] = torch.randn((2 * F, D), generator=g, device="cuda") / D ** 0.5
+        W2[e] = torch.randn((D, F), generator=g, device="cuda") * (2 / F ** 0.5)
+    R[:] = 0
+    R[E - 1], R[E - 2] = X[0] / D, X[1] / D  # token 0: the last expert, token 1: the one before
+    Y = bwgemm.moe_mlp(X, R, W1, W2, 1)
+    ids, _, _ = check(Y, X, R, W1, W2, 1)
+    assert ids.flatten().tolist() == [E - 1, E - 2]
+    W2[E - 1, D - 1, F - 1] = float("inf")
+    got = bwgemm.moe_mlp(X, R, W1, W2, 1)
+    assert torch.isinf(got[0, D - 1])
+    assert torch.equal(got[1], Y[1]) or ((got[1, D - 1] - Y[1, D - 1]).abs() <= 2.0 ** -7 * Y[1, D - 1].abs() and
+                                         torch.equal(got[1, :-1], Y[1, :-1]))
+    assert torch.equal(got[0, :-1], Y[0, :-1])
