@@ -20,6 +20,7 @@ BW_OK, BW_ERR_SHAPE, BW_ERR_LAUNCH, BW_ERR_TIMEOUT, BW_ERR_ARG, BW_ERR_DEVICE = 
 BW_ERR_SCRATCH = 6
 BW_KERNEL_TILE, BW_KERNEL_SWAP, BW_KERNEL_PAIR = 0, 1, 2
 BW_TYPE_F16, BW_TYPE_BF16, BW_TYPE_F32 = 0, 1, 2
+BW_LAYOUT_KN, BW_LAYOUT_NK = 0, 1
 
 
 class Plan(ctypes.Structure):
@@ -125,6 +126,20 @@ def lib():
         L.bw_moe_work_bytes.restype = i
         L.bw_moe_mlp.argtypes = [vp, ll, vp, vp, vp, vp, i, i, i, i, i, i, i, vp, vp, vp, sz, vp]
         L.bw_moe_mlp.restype = i
+        L.bw_gemm_grouped_work_bytes.argtypes = [i, i, i, i, i, i, ctypes.POINTER(sz)]
+        L.bw_gemm_grouped_work_bytes.restype = i
+        L.bw_gemm_grouped.argtypes = [vp, ll, vp, vp, vp, i, i, i, i, i, i, i, vp, sz, vp]
+        L.bw_gemm_grouped.restype = i
+        L.bw_quant_f8.argtypes = [vp, i, ll, vp, vp, ll, i, i, vp]
+        L.bw_quant_f8.restype = i
+        L.bw_quant_blocks_f8.argtypes = [vp, i, vp, vp, i, i, i, vp]
+        L.bw_quant_blocks_f8.restype = i
+        L.bw_gemm_f8_work_bytes.argtypes = [i, i, i, i, i, i, i, ctypes.POINTER(sz)]
+        L.bw_gemm_f8_work_bytes.restype = i
+        L.bw_gemm_f8.argtypes = [vp, vp, ll, vp, vp, vp, i, vp, i, i, i, i, i, vp, sz, vp]
+        L.bw_gemm_f8.restype = i
+        L.bw_linear_f8.argtypes = [vp, i, ll, vp, vp, vp, i, vp, i, i, i, i, vp, sz, vp]
+        L.bw_linear_f8.restype = i
         L.bw_status_string.argtypes = [i]
         L.bw_status_string.restype = ctypes.c_char_p
         L.bw_last_error_string.argtypes = []
@@ -458,6 +473,179 @@ def moe_mlp(X, R, W1, W2, top_k, renormalize=True, Y=None, ids=None, weights=Non
         return out
 
     return _on(X.device, stream, call, X, R, W1, W2, Y, ids, weights)
+
+
+# ---------------------------------------------------------------------------------- products grouped by expert
+GROUP_MAX_EXPERTS = 1024
+
+
+def _offsets(offsets, device, E):
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.device != device or \
+            not offsets.is_contiguous():
+        raise ValueError("offsets must be a contiguous int32 tensor of E + 1 row numbers on X's device")
+
+
+def _gemm_grouped(X, B, offsets, C, stream, layout, swiglu):
+    M, K, ld, code = _rows16(X, "X")
+    if B.dtype != X.dtype or B.dim() != 3 or B.device != X.device or not B.is_contiguous():
+        raise ValueError("B must be a contiguous 3-D tensor of X's type on X's device")
+    E, N, K2 = B.shape if layout == BW_LAYOUT_NK else (B.shape[0], B.shape[2], B.shape[1])
+    if K2 != K:
+        raise ValueError(f"X is {M} x {K} but B is {tuple(B.shape)}")
+    _offsets(offsets, X.device, E)
+
+    def call(s):
+        out = _out(C, X, M, N // 2 if swiglu else N, X.dtype)
+        _t, work, n = _work("bw_gemm_grouped_work_bytes", X, E, M, N, K, layout, swiglu)
+        check(lib().bw_gemm_grouped(X.data_ptr(), ld, B.data_ptr(), offsets.data_ptr(), out.data_ptr(), E, M, N, K, code,
+                                    layout, swiglu, work, n, s))
+        return out
+
+    return _on(X.device, stream, call, X, B, offsets, C)
+
+
+def gemm_grouped(X, B, offsets, C=None, stream=None):
+    """C (M x N) = X B_e for the rows of each expert e, offsets[e] .. offsets[e + 1] - 1 of X (M x K, fp16 or bf16, rows may be
+    strided), B: E x K x N; offsets: E + 1 ascending int32 on the device.  Rows of no expert are not written.  The input's
+    gradient of gemm_grouped_tn."""
+    return _gemm_grouped(X, B, offsets, C, stream, BW_LAYOUT_KN, 0)
+
+
+def gemm_grouped_tn(X, Bt, offsets, C=None, swiglu=False, stream=None):
+    """The same with Bt: E x N x K, C = X Bt_e^T; swiglu: C (M x N/2) = silu(gate) * up, Bt_e's first N/2 rows gate, its last
+    up (moe_mlp's W1)."""
+    return _gemm_grouped(X, Bt, offsets, C, stream, BW_LAYOUT_NK, 1 if swiglu else 0)
+
+
+# ---------------------------------------------------------------------------------- 8-bit floating point
+F8_BLOCK = 128
+
+
+def _f8(t, what, dim, device):
+    if t.dtype != torch.float8_e4m3fn or t.dim() != dim or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dim}-D float8_e4m3fn tensor on one device with the others")
+
+
+def _f8_scales(rows, cols, like):
+    """Scales of rows x cols stored column by column, each column on 16 bytes."""
+    blocks = -(-cols // F8_BLOCK)
+    return like.new_empty((blocks, (rows + 3) // 4 * 4), dtype=torch.float32)[:, :rows].t()
+
+
+def _f8_scale_ld(scale, rows, cols, device, what):
+    """Elements from column to column of a rows x blocks scale tensor stored column by column."""
+    blocks = -(-cols // F8_BLOCK)
+    if scale.dtype != torch.float32 or tuple(scale.shape) != (rows, blocks) or scale.device != device:
+        raise ValueError(f"{what} must be an fp32 tensor of {rows} x {blocks} scales on one device with the others")
+    ld = scale.stride(1) if blocks > 1 else rows
+    if (scale.stride(0) != 1 and rows > 1) or ld < rows:
+        raise ValueError(f"{what} must be stored column by column, as quantize_f8 returns it")
+    return ld
+
+
+def quantize_f8(X, Q=None, scale=None, stream=None):
+    """(Q, scale): the rows of a 2-D fp16 or bf16 CUDA tensor (rows may be strided) as float8_e4m3fn and, for each group of 128
+    columns, an fp32 scale (M x ceil(K / 128), stored column by column): scale = fl(a / 448) with a the group's largest
+    magnitude, Q = e4m3(fl(x fl(448 / a))); made if not given.  X's columns: a multiple of 16."""
+    rows, cols, ld, code = _rows16(X, "X")
+    lds = None if scale is None else _f8_scale_ld(scale, rows, cols, X.device, "scale")
+    if Q is not None:
+        _out(Q, X, rows, cols, torch.float8_e4m3fn, "Q")
+
+    def call(s):
+        q = _out(Q, X, rows, cols, torch.float8_e4m3fn, "Q")
+        sc = _f8_scales(rows, cols, X) if scale is None else scale
+        n = _f8_scale_ld(sc, rows, cols, X.device, "scale") if lds is None else lds
+        check(lib().bw_quant_f8(X.data_ptr(), code, ld, q.data_ptr(), sc.data_ptr(), n, rows, cols, s))
+        return q, sc
+
+    return _on(X.device, stream, call, X, Q, scale)
+
+
+def quantize_blocks_f8(W, Q=None, scale=None, stream=None):
+    """(Q, scale): a contiguous fp16 or bf16 matrix W (N x K, or E x N x K) as float8_e4m3fn with an fp32 scale for each block of
+    128 x 128 ([E x] ceil(N / 128) x ceil(K / 128)), by quantize_f8's formula; made if not given.  K: a multiple of 16."""
+    code = _types().get(W.dtype)
+    if code is None or code == BW_TYPE_F32 or not W.is_cuda or W.dim() not in (2, 3) or not W.is_contiguous():
+        raise ValueError("W must be a contiguous 2-D or 3-D fp16 or bf16 CUDA tensor")
+    N, K = W.shape[-2:]
+    shape = (*W.shape[:-2], -(-N // F8_BLOCK), -(-K // F8_BLOCK))
+    if Q is not None and (Q.dtype != torch.float8_e4m3fn or Q.shape != W.shape or Q.device != W.device or
+                          not Q.is_contiguous()):
+        raise ValueError("Q must be a contiguous float8_e4m3fn tensor of W's shape on W's device")
+    if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != shape or scale.device != W.device or
+                              not scale.is_contiguous()):
+        raise ValueError(f"scale must be a contiguous fp32 tensor of {shape} on W's device")
+
+    def call(s):
+        q = W.new_empty(W.shape, dtype=torch.float8_e4m3fn) if Q is None else Q
+        sc = W.new_empty(shape, dtype=torch.float32) if scale is None else scale
+        check(lib().bw_quant_blocks_f8(W.data_ptr(), code, q.data_ptr(), sc.data_ptr(), W.shape[0] if W.dim() == 3 else 1, N, K,
+                                       s))
+        return q, sc
+
+    return _on(W.device, stream, call, W, Q, scale)
+
+
+def _f8_weight(B, b_scale, offsets, K, device):
+    """(E, N) of a weight: E 0 without offsets."""
+    _f8(B, "B", 2 if offsets is None else 3, device)
+    if B.shape[-1] != K:
+        raise ValueError(f"A's rows have {K} columns but B is {tuple(B.shape)}")
+    N = B.shape[-2]
+    shape = (*B.shape[:-2], -(-N // F8_BLOCK), -(-K // F8_BLOCK))
+    if b_scale.dtype != torch.float32 or tuple(b_scale.shape) != shape or b_scale.device != device or \
+            not b_scale.is_contiguous():
+        raise ValueError(f"b_scale must be a contiguous fp32 tensor of {shape} on B's device")
+    if offsets is None:
+        return 0, N
+    _offsets(offsets, device, B.shape[0])
+    return B.shape[0], N
+
+
+def gemm_f8(A, a_scale, B, b_scale, offsets=None, C=None, dtype=None, swiglu=False, stream=None):
+    """C (M x N) = A B^T of float8_e4m3fn CUDA tensors A (M x K, scales as quantize_f8 gives them) and B (N x K, scales as
+    quantize_blocks_f8 gives them), the scaled sums of 128 products each added in fp32, in `dtype` (fp16 by default, bf16 or
+    fp32).  offsets: grouped by expert as gemm_grouped_tn is, B: E x N x K.  swiglu: silu(gate) * up, M x N/2; B's rows in
+    groups of 128 gate then 128 up, with offsets the first N/2 rows gate, the last up."""
+    types = _types()
+    dtype = torch.float16 if dtype is None else dtype
+    code = types.get(dtype)
+    if code is None:
+        raise ValueError(f"C cannot be {dtype}")
+    if not A.is_cuda:
+        raise ValueError("A must be a CUDA tensor")
+    _f8(A, "A", 2, A.device)
+    M, K = A.shape
+    lds = _f8_scale_ld(a_scale, M, K, A.device, "a_scale")
+    E, N = _f8_weight(B, b_scale, offsets, K, A.device)
+    swiglu = 1 if swiglu else 0
+
+    def call(s):
+        out = _out(C, A, M, N // 2 if swiglu else N, dtype)
+        _t, work, n = _work("bw_gemm_f8_work_bytes", A, E, M, N, K, code, swiglu, 0)
+        check(lib().bw_gemm_f8(A.data_ptr(), a_scale.data_ptr(), lds, B.data_ptr(), b_scale.data_ptr(),
+                               offsets.data_ptr() if E else None, E, out.data_ptr(), M, N, K, code, swiglu, work, n, s))
+        return out
+
+    return _on(A.device, stream, call, A, a_scale, B, b_scale, offsets, C)
+
+
+def linear_f8(X, B, b_scale, offsets=None, C=None, swiglu=False, stream=None):
+    """C = X B^T in X's type (fp16 or bf16): X (M x K, rows may be strided) quantised by quantize_f8 on the way; B, b_scale,
+    offsets and swiglu as gemm_f8 takes them."""
+    M, K, ld, code = _rows16(X, "X")
+    E, N = _f8_weight(B, b_scale, offsets, K, X.device)
+    swiglu = 1 if swiglu else 0
+
+    def call(s):
+        out = _out(C, X, M, N // 2 if swiglu else N, X.dtype)
+        _t, work, n = _work("bw_gemm_f8_work_bytes", X, E, M, N, K, code, swiglu, 1)
+        check(lib().bw_linear_f8(X.data_ptr(), code, ld, B.data_ptr(), b_scale.data_ptr(), offsets.data_ptr() if E else None,
+                                 E, out.data_ptr(), M, N, K, swiglu, work, n, s))
+        return out
+
+    return _on(X.device, stream, call, X, B, b_scale, offsets, C)
 
 
 def status():

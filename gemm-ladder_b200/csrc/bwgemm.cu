@@ -675,6 +675,7 @@ BW_API int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw
 
 // ------------------------------------------------------------------ the mixture-of-experts layer
 #include "moe_mlp.cuh"
+#include "grouped.cuh"
 #endif
 
 #ifdef BW_TRACE

@@ -1,0 +1,640 @@
+// grouped_kernel.cuh -- products grouped by expert with ragged numbers of rows, and products in 8-bit floating point with
+// a scale per block of 128: one kernel.
+//
+//   Y[t, n] = sum_k X[t, k] W_e[n, k]     t in the rows of expert e, n < N            (KIND 0: fp16 or bf16)
+//   Y[t, n] = sum_b xs[t, b] ws_e[n / 128, b] sum_{k in block b} X[t, k] W_e[n, k]    (KIND 1: e4m3, blocks of 128 of K)
+// or W as E x K x N (KIND 0), or silu(gate) * up of two of W's rows per output column.  One expert and no offsets: a plain
+// product.
+//
+// A pair of SMs (cta_group::2) holds a tile of 256 weight rows x up to 256 tokens: each block loads its 128 weight rows
+// and half of the tokens, the leader issues the MMA over both blocks' shared memory.  The weights are the MMA's M, so the
+// ragged dimension is its N, set per tile (grouped_sched.h).  Roles of a block's 11 warps:
+//   warp 0      TMA producer: a ring of stages of 128 bytes of K (64 16-bit values or 128 e4m3).
+//   warp 1      tensor memory; one thread of the leader issues the MMAs into one of two accumulators.
+//   warps 2-9   epilogue: TMEM lanes 32 (warp % 4) .. + 31 (weight rows), the first or second half of the columns (tokens).
+//   warp 10     KIND 1: the products xs ws of a K-block, one per token, into a ring in shared memory.
+// KIND 1: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers (128 per
+// thread); the MMAs of the next K-block run into the other accumulator meanwhile.  The scales differ from block to block, so
+// no MMA may run across two.  Per K-block and SM 128 x 256 multiply-adds (256 cycles of its 128 lanes) stand beside 512
+// cycles of MMA at the e4m3 rate.
+// Every wait is bounded (ptx.cuh); after one that gave up the epilogue walks its segments to the end without waiting,
+// reading or writing, so that all threads meet at every barrier.
+#pragma once
+#include "grouped_sched.h"
+#include "kernel_common.cuh"
+
+namespace bw {
+
+constexpr int kGxThreads = 352;
+constexpr int kGxEpi0 = 64;          // the first epilogue thread
+constexpr int kGxEpiThreads = 256;
+constexpr int kGxXBytes = 128 * 128;  // a block's weight rows of a stage
+constexpr int kGxMaxStages = 12;
+constexpr int kGxScales = 4;          // K-blocks of scale products held
+constexpr int kGxBufBytes = 8 * 16 * 32 * 4;                    // per epilogue warp 16 tokens x 32 columns of C
+constexpr int kGxScaleBytes = kGxScales * 2 * 256 * 4;          // [K-block][gate, up][token]
+constexpr int kGxBars = 2 * kGxMaxStages + 4 + 2 * kGxScales + 1;
+
+// What silu * up pairs: nothing; rows 256 g + i with 256 g + 128 + i; rows f with N / 2 + f.
+enum : int { kGxPlain = 0, kGxGluBlocks = 1, kGxGluHalves = 2 };
+
+struct GxParams {
+    const int* offsets;    // E + 1 ascending row numbers; null: one expert with all T rows
+    int E, T;              // experts, rows of X
+    int N, Nout;           // weight rows per expert; columns of C
+    int nt, kblocks;       // weight tiles per expert, K-blocks
+    int cap, box;          // the most tokens of a tile; rows of one TMA box of X
+    int stages, stage_bytes, ring_bytes;
+    int mn_major;          // W is E x K x N
+    int glu, out;          // kGx*; BW_TYPE_* (0 fp16, 1 bf16, 2 fp32)
+    uint32_t idesc;        // without N
+    void* C;               // T x Nout, contiguous
+    const float* xs;       // KIND 1: scale of token t, K-block b at xs[b * xs_ld + t]
+    long long xs_ld;
+    const float* ws;       // KIND 1: [e][block of 128 rows][K-block]
+    int ws_rows;           // blocks of 128 rows per expert
+    float* work;           // parts of split tiles: slots of 2 x 128 x cap
+    int* counters;         // two per split tile, zero at the start of a call
+    unsigned long long wait_ns;
+};
+
+// Offsets in shared memory of what follows the stage ring.
+struct GxSmem {
+    int buf, scales, bars, misc, tables, bytes;
+};
+__host__ __device__ inline GxSmem gx_smem(int ring_bytes, int E)
+{
+    GxSmem m;
+    m.buf = ring_bytes;
+    m.scales = m.buf + kGxBufBytes;
+    m.bars = m.scales + kGxScaleBytes;
+    m.misc = m.bars + kGxBars * 8;
+    m.tables = m.misc + 64;
+    m.bytes = m.tables + 2 * (E + 1) * 4;
+    return m;
+}
+
+// A tile's rows of X and weight rows.
+struct GxTile {
+    int e, n;     // expert, weight tile
+    int t0;       // its first token (may lie before lo: rounded down to 4 rows for the scales)
+    int lo, hi;   // the tokens of C it writes: [lo, hi)
+    int N;        // MMA N: a multiple of 32
+};
+
+// Follows ascending tile indices through the experts.
+struct GxFind {
+    int e = 0;
+    template <bool F8>
+    __device__ __forceinline__ GxTile at(const GxParams& p, const int* off, const int* cum, int tile)
+    {
+        while (cum[e + 1] * p.nt <= tile) ++e;
+        GxTile t;
+        t.e = e;
+        const int runs = cum[e + 1] - cum[e], a = off[e], b = off[e + 1], s = F8 ? a & ~3 : a;
+        int m;
+        group_place(tile - cum[e] * p.nt, p.nt, runs, m, t.n);
+        const int rows = group_run_rows(s, b, runs);
+        t.t0 = s + m * rows;
+        const int end = t.t0 + rows < b ? t.t0 + rows : b;
+        t.lo = t.t0 < a ? a : t.t0;
+        t.hi = end;
+        t.N = (end - t.t0 + 31) / 32 * 32;
+        return t;
+    }
+};
+
+// Warp-uniform bounded wait: all lanes see the phase complete (and what it orders), or none goes on.
+__device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                             uint32_t where, int seg)
+{
+    const uint32_t b = smem_u32(bar);
+    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(b, parity))) return true;
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = wait_slow(b, parity, abort_flag, limit_ns, where, seg) ? 1u : 0u;
+    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+    if (ok) mbar_try_wait(b, parity);  // complete: this lane acquires too
+    return ok != 0;
+}
+
+// 16 tokens x 32 columns of C: v[j] is token tb + j, column f + lane.  Through the warp's buffer, so that a token's 32
+// columns leave as 16-byte pieces; only tokens [lo, hi) and columns below Nout (a multiple of 8) are written.
+__device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[16], void* buf, int tb, int lo, int hi, int f,
+                                           int lane, bool write)
+{
+    if (p.out == 2) {
+        float* b = static_cast<float*>(buf);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) b[j * 32 + lane] = v[j];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = tb + i * 4 + (lane >> 3), c = f + (lane & 7) * 4;
+            if (write && t >= lo && t < hi && c < p.Nout)
+                *reinterpret_cast<float4*>(static_cast<float*>(p.C) + (size_t)t * p.Nout + c) =
+                    *reinterpret_cast<const float4*>(b + (i * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
+        }
+    } else {
+        uint16_t* b = static_cast<uint16_t*>(buf);
+        if (p.out == 1) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const __nv_bfloat16 h = __float2bfloat16_rn(v[j]);
+                b[j * 32 + lane] = *reinterpret_cast<const uint16_t*>(&h);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const __half h = __float2half_rn(v[j]);
+                b[j * 32 + lane] = *reinterpret_cast<const uint16_t*>(&h);
+            }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = tb + i * 8 + (lane >> 2), c = f + (lane & 3) * 8;
+            if (write && t >= lo && t < hi && c < p.Nout)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.C) + (size_t)t * p.Nout + c) =
+                    *reinterpret_cast<const uint4*>(b + (i * 8 + (lane >> 2)) * 32 + (lane & 3) * 8);
+        }
+    }
+    __syncwarp();
+}
+
+// 16 tokens of a finished sum to C.  With the activation a warp of gate rows (quarters 0 and 1) takes the up rows' sums
+// from the warp of the same columns two quarters on, through that warp's buffer; the two meet twice.
+__device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], uint8_t* bufs, int ew, int q, int h, int tb,
+                                            const GxTile& t, int f, int lane, bool write)
+{
+    uint8_t* mine = bufs + ew * 2048;
+    if (p.glu == kGxPlain) {
+        gx_store16(p, v, mine, tb, t.lo, t.hi, f, lane, write);
+        return;
+    }
+    const uint32_t bar = 2u + (uint32_t)(h * 2 + (q & 1));
+    if (q >= 2) {
+        float* b = reinterpret_cast<float*>(mine);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) b[j * 32 + lane] = v[j];
+        named_bar_sync(bar, 64);
+        named_bar_sync(bar, 64);
+    } else {
+        named_bar_sync(bar, 64);
+        // the up rows' warp: the same half, quarter q + 2 (warps 2 .. 9 have quarters 2, 3, 0, 1, 2, 3, 0, 1)
+        const float* b = reinterpret_cast<const float*>(bufs + (ew - 2) * 2048);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * b[j * 32 + lane];
+        named_bar_sync(bar, 64);
+        gx_store16(p, v, mine, tb, t.lo, t.hi, f, lane, write);
+    }
+}
+
+// Part `slot` of a split tile: 128 x cap fp32 of this block's rows as [token / 4][row][4].
+__device__ __forceinline__ float4* gx_slot(const GxParams& p, int slot, int rank, int row, int c4)
+{
+    return reinterpret_cast<float4*>(p.work) + ((size_t)(slot * 2 + rank) * (p.cap / 4) + c4) * 128 + row;
+}
+
+// acc[j] += v[j] s[j]
+__device__ __forceinline__ void gx_fma16(float (&acc)[16], const uint32_t (&r)[16], const float* s)
+{
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(s + j);  // one address per warp: a broadcast
+        acc[j] = fmaf(__uint_as_float(r[j]), x.x, acc[j]);
+        acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), x.y, acc[j + 1]);
+        acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), x.z, acc[j + 2]);
+        acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), x.w, acc[j + 3]);
+    }
+}
+
+// The experts' rows and their running number of runs, in shared memory: off[e], cum[e].  Row numbers are clamped to
+// ascend within [0, T], so that no value of the caller's leads outside X or C.  By the first warp.
+template <bool F8>
+__device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum, int lane)
+{
+    if (!p.offsets) {
+        if (lane == 0) {
+            off[0] = 0;
+            off[1] = p.T;
+            cum[0] = 0;
+            cum[1] = group_runs(0, p.T, p.cap);
+        }
+        return;
+    }
+    const int per = (p.E + 32) / 32;  // E + 1 numbers
+    const int i0 = lane * per, i1 = i0 + per < p.E + 1 ? i0 + per : p.E + 1;
+    int top = 0;
+    for (int i = i0; i < i1; ++i) {
+        int v = p.offsets[i];
+        v = v < 0 ? 0 : v > p.T ? p.T : v;
+        top = v > top ? v : top;
+        off[i] = top;
+    }
+    int run = top;
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = (int)__shfl_sync(0xFFFFFFFFu, (uint32_t)run, (lane - d) & 31);
+        if (lane >= d && o > run) run = o;
+    }
+    int before = (int)__shfl_sync(0xFFFFFFFFu, (uint32_t)run, (lane - 1) & 31);
+    if (lane == 0) before = 0;
+    for (int i = i0; i < i1; ++i)
+        if (off[i] < before) off[i] = before;
+    __syncwarp();
+    int n = 0;
+    for (int i = i0; i < i1 && i < p.E; ++i) {
+        const int a = F8 ? off[i] & ~3 : off[i];
+        n += off[i + 1] > off[i] ? group_runs(a, off[i + 1], p.cap) : 0;
+    }
+    int sum = n;
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = (int)__shfl_sync(0xFFFFFFFFu, (uint32_t)sum, (lane - d) & 31);
+        if (lane >= d) sum += o;
+    }
+    n = sum - n;
+    for (int i = i0; i < i1; ++i) {
+        cum[i] = n;
+        if (i < p.E) {
+            const int a = F8 ? off[i] & ~3 : off[i];
+            n += off[i + 1] > off[i] ? group_runs(a, off[i + 1], p.cap) : 0;
+        }
+    }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kGxThreads, 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const GxParams p)
+{
+    constexpr bool F8 = KIND == 1;
+    constexpr int kRowElems = 64;  // a 128-byte row of a stage in the maps' 16-bit elements
+#ifdef BW_EMULATE
+    uint8_t* smem_raw = emu::cta_smem();
+#else
+    extern __shared__ uint8_t smem_raw[];
+#endif
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const GxSmem L = gx_smem(p.ring_bytes, p.E);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
+    uint64_t* empty = full + kGxMaxStages;
+    uint64_t* tfull = empty + kGxMaxStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* sfull = tempty + 2;
+    uint64_t* sempty = sfull + kGxScales;
+    uint64_t* drain = sempty + kGxScales;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* reduce_flag = abort_flag + 1;
+    float* scales = reinterpret_cast<float*>(smem + L.scales);
+    int* off = reinterpret_cast<int*>(smem + L.tables);
+    int* cum = off + p.E + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
+    const int S = p.stages;
+    const int tmem_cols = 2 * p.cap;  // a power of two, 64 .. 512
+
+    griddep_launch();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 16);  // the epilogue warps of both blocks
+        }
+        for (int i = 0; i < kGxScales; ++i) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sempty[i], 8);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        *reduce_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tmw);
+        prefetch_tmap(&tmx);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, (uint32_t)tmem_cols);
+        tmem_relinquish_pair();
+    }
+    griddep_wait();  // what the kernel ahead wrote (the offsets, X, its scales, the counters) is visible from here on
+    if (warp == 2) gx_tables<F8>(p, off, cum, lane);
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // barriers, tables and tensor memory of both blocks are there
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+    GroupWalk walk(s, c);
+    GroupSeg sg;
+    GxFind find;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            int stage = 0, issued = 0, seg = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            while (ok && walk.next(s, sg)) {
+                const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+                const int boxes = (t.N / 2 + p.box - 1) / p.box;
+                const uint32_t bytes = 2u * (kGxXBytes + (uint32_t)(boxes * p.box) * 128u);
+                const int tok = t.t0 + rank * (t.N / 2);
+                // this block's weight rows: 128 in a row, or 64 gate and 64 up rows
+                const int w0 = p.glu == kGxPlain ? t.n * 256 + rank * 128
+                               : p.glu == kGxGluBlocks ? t.n * 256 + rank * 64
+                                                       : t.n * 128 + rank * 64;
+                const int w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sx = smem + stage * p.stage_bytes;
+                    uint8_t* sy = sx + kGxXBytes;
+                    const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);  // both blocks complete the leader's
+                    if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
+                    if (p.mn_major) {
+                        tma_load_3d_pair(sx, &tmw, w0, kb * 64, t.e, bar);
+                        tma_load_3d_pair(sx + 8192, &tmw, w0 + 64, kb * 64, t.e, bar);
+                    } else if (p.glu == kGxPlain) {
+                        tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
+                    } else {
+                        tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
+                        tma_load_3d_pair(sx + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
+                    }
+                    for (int i = 0; i < boxes; ++i)
+                        tma_load_3d_pair(sy + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
+                    ++issued;
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                ++seg;
+            }
+            if (leader) {  // loads in flight land before the blocks may leave (after an abort; else they have landed)
+                const int n = issued < S ? issued : S;
+                for (int i = 1; i <= n; ++i) {
+                    const int q = issued - i;
+                    wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------- MMA issuer
+        if (lane == 0 && leader) {
+            int stage = 0, acc = 0, seg = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            auto next_acc = [&] {
+                mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 0));
+                mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 1));
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
+            };
+            while (ok && walk.next(s, sg)) {
+                const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+                const uint32_t idesc = p.idesc | (uint32_t)(t.N >> 3) << 17;
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (F8 || kb == sg.k0) {
+                        if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    if (!wait_bounded(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sx = smem_u32(smem + stage * p.stage_bytes), sy = sx + kGxXBytes;
+                    const uint32_t d = tmem_base + (uint32_t)(acc * p.cap);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t accumulate = ((!F8 && kb > sg.k0) || k > 0) ? 1u : 0u;
+                        const uint64_t ad = !F8 && p.mn_major ? desc_mnmajor(sx, k) : desc_kmajor(sx, k);
+                        const uint64_t bd = desc_kmajor(sy, k);
+                        if constexpr (F8)
+                            mma_f8_pair(d, ad, bd, idesc, accumulate);
+                        else
+                            mma_f16_pair(d, ad, bd, idesc, accumulate);
+                    }
+                    mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 0));
+                    mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 1));
+                    if (F8) next_acc();
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if (!F8) next_acc();
+                ++seg;
+            }
+            // the MMAs in flight finish before the tensor memory is freed
+            mma_commit_pair(mapa_shared(smem_u32(drain), 0));
+            wait_drain(drain, 0, p.wait_ns);
+        }
+        __syncwarp();
+    } else if (warp < 10) {
+        // ---------------------------------------------------------- epilogue
+        const int ew = warp - 2, q = warp & 3, h = ew >> 2;
+        const int row = q * 32 + lane;
+        const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
+        uint8_t* bufs = smem + L.buf;
+        int acc = 0, seg = 0, si = 0;
+        uint32_t aph = 0, sph = 0;
+        bool alive = true;
+        const float* sc_base = scales + (p.glu != kGxPlain && q >= 2 ? 256 : 0);
+        auto release = [&](int a) {
+            tc_fence_before();
+            __syncwarp();
+            if (alive && lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)a);
+        };
+        while (walk.next(s, sg)) {
+            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+            const int nc = t.N / 2, c0 = h * nc;  // this warp's columns
+            const int tb = t.t0 + c0;
+            const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
+            const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
+            float sum[F8 ? 8 : 1][16];
+            if constexpr (F8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
+                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    if (alive)
+                        alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), seg) &&
+                                gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                    if (alive) {
+                        tc_fence_after();
+                        const float* sc = sc_base + si * 512 + c0;
+                        const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if (i * 16 >= nc) break;
+                            uint32_t r[16];
+                            tmem_ld16(tm + (uint32_t)(i * 16), r);
+                            tmem_wait_ld();
+                            gx_fma16(sum[i], r, sc + i * 16);
+                        }
+                    }
+                    release(acc);
+                    if (alive && lane == 0) mbar_arrive(&sempty[si]);
+                    acc ^= 1;
+                    if (acc == 0) aph ^= 1u;
+                    if (++si == kGxScales) {
+                        si = 0;
+                        sph ^= 1u;
+                    }
+                }
+            } else {
+                if (alive)
+                    alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                tc_fence_after();
+            }
+            const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
+            // this segment's sum of 16 columns
+            auto own = [&](int i, float(&v)[16]) {
+                if constexpr (F8) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = sum[i][j];
+                } else {
+                    uint32_t r[16];
+                    tmem_ld16(tm + (uint32_t)(i * 16), r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                }
+            };
+            if (sg.k0 == 0 && sg.k1 == s.kb) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (i * 16 >= nc) break;
+                    float v[16];
+                    own(i, v);
+                    gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
+                }
+            } else {
+                // a part of a split tile: the last block to finish sums all parts in the order of K
+                const int first = tile_first_part(s, sg.tile), last = tile_last_part(s, sg.tile);
+                const int nseg = last - first + 1;
+                int* counter = p.counters + sg.tile * 2 + rank;
+                named_bar_sync(1, kGxEpiThreads);  // the flag of an earlier tile has been read
+                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == nseg - 1 ? 1 : 0;
+                named_bar_sync(1, kGxEpiThreads);
+                int go = *reduce_flag;
+                if (!go) {
+                    const int slot = part_slot(s, c, sg.tile);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (i * 16 >= nc) break;
+                        float v[16];
+                        own(i, v);
+                        if (alive) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                __stcg(gx_slot(p, slot, rank, row, c0 / 4 + i * 4 + j),
+                                       make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                        }
+                    }
+                    named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
+                    if (threadIdx.x == kGxEpi0)
+                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == nseg - 1 ? 1 : 0;
+                    named_bar_sync(1, kGxEpiThreads);
+                    go = *reduce_flag;
+                }
+                if (go) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (i * 16 >= nc) break;
+                        float v[16], mine[16];
+                        own(i, mine);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                        for (int part = first; part <= last; ++part) {
+                            if (part == c) {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] += mine[j];
+                                continue;
+                            }
+                            const int slot = part_slot(s, part, sg.tile);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 x = __ldcg(gx_slot(p, slot, rank, row, c0 / 4 + i * 4 + j));
+                                v[4 * j] += x.x;
+                                v[4 * j + 1] += x.y;
+                                v[4 * j + 2] += x.z;
+                                v[4 * j + 3] += x.w;
+                            }
+                        }
+                        gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
+                    }
+                }
+            }
+            if constexpr (!F8) {
+                release(acc);
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
+            }
+            ++seg;
+        }
+    } else if (F8) {
+        // ---------------------------------------------------------- scale products
+        int si = 0, seg = 0;
+        uint32_t sph = 0;
+        bool alive = true;
+        while (alive && walk.next(s, sg)) {
+            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+            // the scale blocks of this block's weight rows (gate and up: of each)
+            const int r0 = p.glu == kGxGluHalves ? t.n : p.glu == kGxGluBlocks ? 2 * t.n : 2 * t.n + rank;
+            const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : 2 * t.n + 1;
+            const float* w0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
+            const float* w1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
+            for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                float x[8];
+                const float* xs = p.xs + kb * p.xs_ld + t.t0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = i * 32 + lane;
+                    x[i] = k < t.hi - t.t0 ? xs[k] : 0.f;
+                }
+                const float a = w0[kb], b = p.glu != kGxPlain ? w1[kb] : 0.f;
+                alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), seg);
+                if (!alive) break;
+                float* to = scales + si * 512;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (i * 32 >= t.N) break;
+                    to[i * 32 + lane] = x[i] * a;
+                    if (p.glu != kGxPlain) to[256 + i * 32 + lane] = x[i] * b;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfull[si]);
+                if (++si == kGxScales) {
+                    si = 0;
+                    sph ^= 1u;
+                }
+            }
+            ++seg;
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // neither block leaves while the other may still read its memory or arrive on its barriers
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, (uint32_t)tmem_cols);
+    }
+}
+
+}  // namespace bw

@@ -1,0 +1,67 @@
+// grouped_plan.h -- host side arithmetic of the grouped kernels, shared by the library and the emulator: the token tile,
+// the stage ring, the workspace, the tensor maps' sizes.
+#pragma once
+#include "grouped_kernel.cuh"
+
+namespace bw {
+
+// The most tokens of a tile for an average of `rows` per expert.  A tile's MMA is as wide as the tokens it has, so a large
+// cap costs little computing; a small one leaves shared memory for more stages of weights, which is what few tokens want.
+inline int gx_cap(int T, int E, bool grouped)
+{
+    const long long rows = grouped ? ((long long)T + E - 1) / E : T;
+    // (experts' numbers of rows spread around the average: twice it, so that most take one run)
+    const long long want = grouped ? 2 * rows : rows;
+    return want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
+}
+
+// Everything of a call but its addresses.  cap 0: the rule's.
+inline GxParams gx_params(int E, int T, int N, int K, bool f8, bool bf16, bool mn_major, int glu, int out, int cap)
+{
+    GxParams p = {};
+    p.E = E;
+    p.T = T;
+    p.N = N;
+    p.Nout = glu == kGxPlain ? N : N / 2;
+    p.nt = glu == kGxGluHalves ? (N / 2 + 127) / 128 : (N + 255) / 256;
+    p.kblocks = f8 ? (K + 127) / 128 : (K + 63) / 64;
+    p.cap = cap;
+    p.box = p.cap == 32 ? 16 : 32;
+    p.stage_bytes = kGxXBytes + p.cap / 2 * 128;
+    const int fixed = gx_smem(0, E).bytes + 1024;
+    p.stages = (BW_SMEM_LIMIT - fixed) / p.stage_bytes;
+    if (p.stages > kGxMaxStages) p.stages = kGxMaxStages;
+    p.ring_bytes = p.stages * p.stage_bytes;
+    p.mn_major = mn_major ? 1 : 0;
+    p.glu = glu;
+    p.out = out;
+    p.idesc = f8 ? idesc_e4m3_f32_m(256) : idesc_16_f32_m(256, bf16, mn_major, false);
+    p.ws_rows = (N + 127) / 128;
+    return p;
+}
+
+// Parts of split tiles: two slots per pair, each of both blocks' 128 rows x cap fp32.
+inline size_t gx_work_bytes(int pairs, int cap) { return (size_t)pairs * 2 * 2 * 128 * (size_t)cap * 4; }
+
+// The tensor maps in 16-bit elements (two e4m3 each): {d0, d1, d2, row stride, plane stride, box rows}, boxes of 64 x rows.
+struct GxMaps {
+    uint64_t w[6], x[6];
+};
+inline GxMaps gx_maps(const GxParams& p, int K, long long ldx, bool f8)
+{
+    const uint64_t k = f8 ? (uint64_t)K / 2 : (uint64_t)K, ld = f8 ? (uint64_t)ldx / 2 : (uint64_t)ldx;
+    GxMaps m;
+    const uint64_t n = (uint64_t)p.N, e = (uint64_t)p.E;
+    if (p.mn_major) {
+        const uint64_t w[6] = {n, k, e, n, n * k, 64};
+        for (int i = 0; i < 6; ++i) m.w[i] = w[i];
+    } else {
+        const uint64_t w[6] = {k, n, e, k, n * k, p.glu == kGxPlain ? 128u : 64u};
+        for (int i = 0; i < 6; ++i) m.w[i] = w[i];
+    }
+    const uint64_t x[6] = {k, (uint64_t)p.T, 1, ld, ld * (uint64_t)p.T, (uint64_t)p.box};
+    for (int i = 0; i < 6; ++i) m.x[i] = x[i];
+    return m;
+}
+
+}  // namespace bw

@@ -1,0 +1,121 @@
+// grouped_sched.h -- how the products grouped by expert are cut into tiles and how the tiles are dealt out, on the device
+// (the experts' numbers of rows are device data) and, for the tests, on the host.
+//
+// Expert e owns rows offsets[e] .. offsets[e + 1] - 1.  Its rows are cut evenly into runs of at most `cap` (a multiple of
+// 32), its weight rows into tiles of 256 (a pair of SMs, 128 each).  The weights are the MMA's 256-row operand and the
+// tokens its N, which a tile sets to its own number of tokens rounded up to 32: an expert's odd number of rows costs at
+// most 31 columns, where a 256-row token tile would cost up to 255.
+//
+// Order: expert by expert; within one, weight tile by weight tile with up to 8 of its runs of tokens in turn, so that the
+// runs share a weight tile while it is in L2 and the weight tiles a run of tokens.
+//
+// Dealing: with `tiles` tiles on P pairs, the first tiles % P are split along K over all pairs (the K-blocks of those
+// tiles cut into P even ranges), then every pair takes the same number of whole tiles.  The parts of a split tile are
+// summed by the last pair to finish it, in the order of K, so results repeat bit for bit.
+#pragma once
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define BW_GS __host__ __device__ __forceinline__
+#else
+#define BW_GS inline
+#endif
+
+namespace bw {
+
+constexpr int kGroupMax = 1024;      // experts
+constexpr int kGroupRowTiles = 8;    // runs of tokens that share a weight tile in turn
+constexpr int kGroupMinUnits = 4;    // K-blocks: the shortest range a split tile is cut into
+
+struct GroupSched {
+    int nt;        // weight tiles per expert
+    int kb;        // K-blocks per tile
+    int pairs;     // pairs of SMs
+    int tiles;     // all tiles
+    int split;     // the first tiles, split along K
+    int parts;     // pairs that take a range of them
+};
+
+BW_GS GroupSched group_sched(int nt, int kb, int pairs, int runs)
+{
+    GroupSched s;
+    s.nt = nt;
+    s.kb = kb;
+    s.pairs = pairs;
+    s.tiles = nt * runs;
+    s.split = s.tiles % pairs;
+    const long long units = (long long)s.split * kb;
+    long long parts = units / kGroupMinUnits;
+    if (parts > pairs) parts = pairs;
+    if (parts < s.split) parts = s.split;
+    s.parts = (int)parts;
+    // a remainder that fills most of a wave is as quick in whole tiles
+    if (s.tiles > pairs && s.split * 8 > pairs * 7) s.parts = s.split;
+    return s;
+}
+
+// The runs of an expert's rows [a, b): their number, and the rows of each but the last (a multiple of 32).
+BW_GS int group_runs(int a, int b, int cap) { return b > a ? (b - a + cap - 1) / cap : 0; }
+BW_GS int group_run_rows(int a, int b, int runs) { return ((b - a + runs - 1) / runs + 31) / 32 * 32; }
+
+// The first K-block (of split tile x kb) of part c, and the part that holds K-block u.
+BW_GS long long part_begin(const GroupSched& s, int c) { return (long long)s.split * s.kb * c / s.parts; }
+BW_GS int part_of(const GroupSched& s, long long u)
+{
+    return (int)(((u + 1) * s.parts - 1) / ((long long)s.split * s.kb));
+}
+
+struct GroupSeg {
+    int tile;    // index in the order above
+    int k0, k1;  // its K-blocks [k0, k1)
+};
+
+// A pair's segments in order: its range of the split tiles, then its whole tiles.
+struct GroupWalk {
+    long long u, uend;
+    int tile;
+    BW_GS GroupWalk(const GroupSched& s, int c)
+    {
+        u = uend = 0;
+        if (s.split && c < s.parts) {
+            u = part_begin(s, c);
+            uend = part_begin(s, c + 1);
+        }
+        tile = s.split + c;
+    }
+    BW_GS bool next(const GroupSched& s, GroupSeg& g)
+    {
+        if (u < uend) {
+            g.tile = (int)(u / s.kb);
+            g.k0 = (int)(u - (long long)g.tile * s.kb);
+            const long long end = (long long)(g.tile + 1) * s.kb;
+            g.k1 = s.kb - (int)(end > uend ? end - uend : 0);
+            u = end > uend ? uend : end;
+            return true;
+        }
+        if (tile >= s.tiles) return false;
+        g.tile = tile;
+        g.k0 = 0;
+        g.k1 = s.kb;
+        tile += s.pairs;
+        return true;
+    }
+};
+
+// The parts of split tile t: [first, last]; part c's slot for it (a part's range touches at most two tiles).
+BW_GS int tile_first_part(const GroupSched& s, int t) { return part_of(s, (long long)t * s.kb); }
+BW_GS int tile_last_part(const GroupSched& s, int t) { return part_of(s, (long long)(t + 1) * s.kb - 1); }
+BW_GS int part_slot(const GroupSched& s, int c, int t) { return 2 * c + (part_begin(s, c) / s.kb == t ? 0 : 1); }
+
+// A tile's place in its expert: weight tile n and run m, of `runs` runs; j counts the expert's tiles.
+BW_GS void group_place(int j, int nt, int runs, int& m, int& n)
+{
+    const int g = j / (kGroupRowTiles * nt);
+    const int left = runs - g * kGroupRowTiles;
+    const int rows = left < kGroupRowTiles ? left : kGroupRowTiles;
+    const int r = j - g * kGroupRowTiles * nt;
+    m = g * kGroupRowTiles + r % rows;
+    n = r / rows;
+}
+
+}  // namespace bw

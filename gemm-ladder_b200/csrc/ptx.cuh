@@ -376,6 +376,19 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t adesc, uin
         : "memory");
 }
 
+// The pair's MMA in 8-bit floating point (e4m3 by the instruction descriptor), kind::f8f6f4: fp32 accumulators, K of 32 per
+// MMA.
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrives once on the barrier at shared::cluster address `bar` (this block's or the other block's of the pair) when
 // every tcgen05 operation the leader has issued so far has completed.  The pair's barriers in both blocks are reached
 // by one such commit each (no multicast form is used anywhere in this library).
@@ -426,6 +439,15 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n, bool a_mn_maj
     return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
 }
+
+// The same for bf16 A and B (formats 1) or fp16, and for kind::f8f6f4 with e4m3 A and B (formats 0, K-major); N is added at
+// run time.
+__host__ __device__ constexpr uint32_t idesc_16_f32_m(int m, bool bf16, bool a_mn_major, bool b_mn_major)
+{
+    return idesc_f16_f32(m, 0, a_mn_major, b_mn_major) | (bf16 ? 1u << 7 | 1u << 10 : 0u);
+}
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32_m(int m) { return (1u << 4) | ((uint32_t)(m >> 4) << 24); }
+__host__ __device__ constexpr uint32_t idesc_n(int n) { return (uint32_t)(n >> 3) << 17; }
 
 // kind::i8: 32-bit signed accumulators (bits [4,6) = 2), signed 8-bit A and B (bits [7,10) and [10,13) = 1), K-major.
 __host__ __device__ constexpr uint32_t idesc_i8_s32(int m, int n)

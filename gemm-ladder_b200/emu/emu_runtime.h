@@ -718,6 +718,59 @@ inline void mma_i8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, b
     }
 }
 
+inline float e4m3_value(uint8_t u)
+{
+    const int e = u >> 3 & 15, m = u & 7;
+    const float v = (u & 0x7F) == 0x7F ? NAN : e ? std::ldexp(8.f + (float)m, e - 10) : std::ldexp((float)m, -9);
+    return u & 0x80 ? -v : v;
+}
+
+// The same in e4m3 (kind::f8f6f4, a pair of blocks): K32 slices, both operands K-major, fp32 accumulators.
+inline void mma_f8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate)
+{
+    for (uint64_t desc : {adesc, bdesc})
+        if ((desc >> 61) != 2u || ((desc >> 46) & 3u) != 1u) finding("a descriptor that is not sm_100 128-byte swizzle");
+    const int N = (int)((idesc >> 17) & 0x3Fu) << 3, M = (int)((idesc >> 24) & 0x1Fu) << 4;
+    if (((idesc >> 4) & 3u) != 1u || (idesc >> 7 & 0x1FFu)) finding("an 8-bit MMA that is not e4m3, K-major, into fp32");
+    if (M != 256 || N < 32 || N > 256 || N % 32 || !t_cta->cluster || t_cta->cluster->size != 2) {
+        finding("an 8-bit MMA of M %d N %d on a pair", M, N);
+        return;
+    }
+    const uint32_t lane0 = d >> 16, col0 = d & 0xFFFFu;
+    if (lane0 != 0 || col0 + (uint32_t)N > (uint32_t)kTmemCols) {
+        finding("an MMA accumulator at lane %u column %u (N %d) outside tensor memory", lane0, col0, N);
+        return;
+    }
+    auto load = [](const Cta* c, uint64_t desc, int row, int k) -> float {
+        const uint32_t start = (uint32_t)(desc & 0x3FFFu) << 4, sbo = (uint32_t)((desc >> 32) & 0x3FFFu) << 4;
+        const uint32_t p = swizzle128(start + (uint32_t)(row >> 3) * sbo + (uint32_t)(row & 7) * 128u + (uint32_t)k);
+        if (p >= (uint32_t)kSmemBytes) {
+            finding("an MMA operand read past the end of shared memory");
+            return 0.f;
+        }
+        return e4m3_value(c->smem[p]);
+    };
+    std::vector<float> b((size_t)N * 32), a(128 * 32);
+    Cta* cta[2] = {t_cta->cluster->cta[0], t_cta->cluster->cta[1]};
+    for (int n = 0; n < N; ++n)
+        for (int k = 0; k < 32; ++k) b[(size_t)n * 32 + k] = load(cta[n / (N / 2)], bdesc, n % (N / 2), k);
+    for (int r = 0; r < 2; ++r) {
+        for (int m = 0; m < 128; ++m)
+            for (int k = 0; k < 32; ++k) a[(size_t)m * 32 + k] = load(cta[r], adesc, m, k);
+        if (cta[r]->tmem_cols < (int)(col0 + N)) finding("an MMA into tensor memory not allocated");
+        for (int m = 0; m < 128; ++m) {
+            uint32_t* row = cta[r]->tmem.data() + (size_t)m * kTmemCols + col0;
+            for (int n = 0; n < N; ++n) {
+                float s = 0.f, acc;
+                for (int k = 0; k < 32; ++k) s += a[(size_t)m * 32 + k] * b[(size_t)n * 32 + k];
+                std::memcpy(&acc, &row[n], 4);
+                acc = accumulate ? acc + s : s;
+                std::memcpy(&row[n], &acc, 4);
+            }
+        }
+    }
+}
+
 // tcgen05.ld 32x32b.x16 (x8): lane = the address's lane + the thread's lane in its warp, 16 (8) columns
 template <int NC>
 inline void tmem_ld(uint32_t taddr, uint32_t (&r)[NC])
@@ -778,6 +831,7 @@ inline uint32_t __reduce_max_sync(unsigned mask, uint32_t v)
     }
     return v;
 }
+inline int __all_sync(unsigned mask, int p) { return __reduce_max_sync(mask, p ? 0u : 1u) == 0u; }
 inline uint32_t __reduce_min_sync(unsigned mask, uint32_t v) { return ~__reduce_max_sync(mask, ~v); }
 inline uint32_t __vmaxu2(uint32_t a, uint32_t b)
 {

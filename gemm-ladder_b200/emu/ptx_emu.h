@@ -264,6 +264,15 @@ inline void mma_i8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_
         --tc.mmas;
     });
 }
+inline void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    emu::Engine& tc = emu::t_cta->tc;
+    ++tc.mmas;
+    tc.post([=, &tc] {
+        emu::mma_f8(d_tmem, adesc, bdesc, idesc, accumulate != 0);
+        --tc.mmas;
+    });
+}
 inline void mma_commit_pair(uint32_t bar)
 {
     emu::t_cta->tc.post([=] { emu::mb_arrive(emu::cta_of(bar), emu::off_of(bar), 0); });
@@ -290,6 +299,13 @@ constexpr uint32_t idesc_f16_f32(int m, int n, bool a_mn_major, bool b_mn_major)
     return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
 }
+
+constexpr uint32_t idesc_16_f32_m(int m, bool bf16, bool a_mn_major, bool b_mn_major)
+{
+    return idesc_f16_f32(m, 0, a_mn_major, b_mn_major) | (bf16 ? 1u << 7 | 1u << 10 : 0u);
+}
+constexpr uint32_t idesc_e4m3_f32_m(int m) { return (1u << 4) | ((uint32_t)(m >> 4) << 24); }
+constexpr uint32_t idesc_n(int n) { return (uint32_t)(n >> 3) << 17; }
 
 constexpr uint32_t idesc_i8_s32(int m, int n)
 {

@@ -144,6 +144,60 @@ int bw_moe_mlp(const void* X, long long ldx, const void* R, const void* W1, cons
                int top_k, int D, int F, int type, int renormalize, void* ids, void* weights, void* work,
                size_t work_bytes, void* stream);
 
+/*
+ * Products grouped by expert: the rows of X (M x K, fp16 or bf16 by `type`, ldx elements from row to row) are sorted by
+ * expert, expert e's being offsets[e] .. offsets[e + 1] - 1 (E + 1 ascending int32 on the device; any number of rows each,
+ * none included).  For the rows of each expert
+ *   layout BW_LAYOUT_KN   C = X B_e,    B: E x K x N
+ *   layout BW_LAYOUT_NK   C = X B_e^T,  B: E x N x K (a linear layer's weight layout)
+ *   BW_LAYOUT_NK, swiglu 1   C (M x N/2) = silu(X G_e^T) * (X U_e^T), B_e's first N/2 rows G_e, its last U_e
+ *                            (the layout of bw_moe_mlp's W1; N % 16 == 0)
+ * with fp32 sums, C in X's type, rounded once.  Rows before offsets[0] and from offsets[E] on are not written.  Row numbers
+ * outside [0, M], or below an earlier one, are taken as the nearest that are not.
+ * N % 8 == 0, K % 8 == 0 (both layouts), ldx >= K, ldx % 8 == 0, 1 <= E <= 1024; X, B and C 16-byte aligned, C contiguous.
+ * `work` (bw_gemm_grouped_work_bytes), overlap and capture: as for the 8-bit entries.  M == 0 is a call that does nothing.
+ * The kernel that reads the offsets runs on `stream`: they may be written by a kernel ahead of the call.
+ * No reference counterpart.
+ */
+#define BW_LAYOUT_KN 0
+#define BW_LAYOUT_NK 1
+int bw_gemm_grouped_work_bytes(int E, int M, int N, int K, int layout, int swiglu, size_t* bytes);
+int bw_gemm_grouped(const void* X, long long ldx, const void* B, const void* offsets, void* C, int E, int M, int N, int K,
+                    int type, int layout, int swiglu, void* work, size_t work_bytes, void* stream);
+
+/*
+ * Products in 8-bit floating point (e4m3) with a scale for each block of 128.
+ *
+ * bw_quant_f8 makes e4m3 rows of fp16 or bf16 (x_type) ones, ld elements from row to row, a scale for each group of 128
+ * columns (the last may be shorter): with a the group's largest magnitude and fl rounding to fp32,
+ *   scale = fl(a / 448),  q = e4m3(fl(x fl(448 / a))), to nearest, ties to even
+ * scale[b * lds + m] is that of row m's group b (lds >= rows).  Q is rows x cols, contiguous.  A group of zeros gets scale 0
+ * and zeros; one that holds an infinity or a NaN gets scale NaN and zeros.  Where 448 / a leaves fp32, a and x are first
+ * scaled by a power of two.
+ * bw_quant_blocks_f8 does the same to E matrices W (N x K, contiguous) by blocks of 128 x 128: scale is
+ * E x ceil(N / 128) x ceil(K / 128), contiguous.
+ *
+ * bw_gemm_f8: C = A B^T with A (M x K) and B (N x K) e4m3, contiguous, a_scale as bw_quant_f8 and b_scale as
+ * bw_quant_blocks_f8 write them:
+ *   C[m][n] = sum_b (a_scale[b][m] b_scale[n / 128][b]) sum_{k in block b} A[m][k] B[n][k]
+ * in fp32, rounded once to out_type (BW_TYPE_*).  offsets null and E 0: one matrix B.  E >= 1: grouped by expert as
+ * bw_gemm_grouped is, B: E x N x K.  swiglu 1: silu(gate) * up of the sums, C M x N/2, N % 256 == 0; E 0: B's rows in groups
+ * of 128 gate then 128 up rows (as bw_gemm_i8_swiglu takes them); E >= 1: B_e's first N/2 rows gate, its last up.
+ * bw_linear_f8 is both in one call: X (fp16 or bf16) quantised as bw_quant_f8 does on the way, C in X's type.
+ *
+ * K % 16 == 0, N % 8 == 0, E <= 1024; X, Q, A, B and C 16-byte aligned, scales 4-byte aligned.
+ * `work` (bw_gemm_f8_work_bytes, linear 1 for bw_linear_f8), overlap and capture: as for the 8-bit integer entries.
+ * M == 0 is a call that does nothing.  No reference counterpart.
+ */
+int bw_quant_f8(const void* X, int x_type, long long ld, void* Q, void* scale, long long lds, int rows, int cols,
+                void* stream);
+int bw_quant_blocks_f8(const void* W, int w_type, void* Q, void* scale, int E, int N, int K, void* stream);
+int bw_gemm_f8_work_bytes(int E, int M, int N, int K, int out_type, int swiglu, int linear, size_t* bytes);
+int bw_gemm_f8(const void* A, const void* a_scale, long long lds, const void* B, const void* b_scale, const void* offsets,
+               int E, void* C, int M, int N, int K, int out_type, int swiglu, void* work, size_t work_bytes, void* stream);
+int bw_linear_f8(const void* X, int x_type, long long ld, const void* B, const void* b_scale, const void* offsets, int E,
+                 void* C, int M, int N, int K, int swiglu, void* work, size_t work_bytes, void* stream);
+
 /* The number of variants.  Replaces: the weak `int g_nvar` (probe/probe.cu:40, hopper/verif.cu:38,
  * hopper/step7.cu:16). */
 int bw_gemm_variant_count(void);
