@@ -130,6 +130,10 @@ def lib():
         L.bw_gemm_grouped_work_bytes.restype = i
         L.bw_gemm_grouped.argtypes = [vp, ll, vp, vp, vp, i, i, i, i, i, i, i, vp, sz, vp]
         L.bw_gemm_grouped.restype = i
+        L.bw_gemm_grouped_dw_work_bytes.argtypes = [i, i, i, i, i, ctypes.POINTER(sz)]
+        L.bw_gemm_grouped_dw_work_bytes.restype = i
+        L.bw_gemm_grouped_dw.argtypes = [vp, ll, vp, ll, vp, vp, i, i, i, i, i, i, vp, sz, vp]
+        L.bw_gemm_grouped_dw.restype = i
         L.bw_quant_f8.argtypes = [vp, i, ll, vp, vp, ll, i, i, vp]
         L.bw_quant_f8.restype = i
         L.bw_quant_blocks_f8.argtypes = [vp, i, vp, vp, i, i, i, vp]
@@ -515,6 +519,38 @@ def gemm_grouped_tn(X, Bt, offsets, C=None, swiglu=False, stream=None):
     """The same with Bt: E x N x K, C = X Bt_e^T; swiglu: C (M x N/2) = silu(gate) * up, Bt_e's first N/2 rows gate, its last
     up (moe_mlp's W1)."""
     return _gemm_grouped(X, Bt, offsets, C, stream, BW_LAYOUT_NK, 1 if swiglu else 0)
+
+
+def gemm_grouped_dw(dY, X, offsets, dW=None, dtype=None, stream=None):
+    """dW (E x N x K) = dY_e^T X_e over each expert's rows of dY (M x N) and X (M x K), both fp16 or both bf16, rows may be
+    strided; in `dtype` (the inputs' by default; fp16, bf16 or fp32); zero for an expert without rows.  The weights' gradient
+    of gemm_grouped_tn; with dY and X exchanged, of gemm_grouped."""
+    types = _types()
+    M, N, ldy, code = _rows16(dY, "dY")
+    M2, K, ldx, code2 = _rows16(X, "X")
+    if M2 != M or code2 != code or X.device != dY.device:
+        raise ValueError(f"dY {tuple(dY.shape)} {dY.dtype} and X {tuple(X.shape)} {X.dtype} must have the same rows, type and "
+                         "device")
+    if offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError("offsets must hold E + 1 row numbers")
+    E = offsets.shape[0] - 1
+    _offsets(offsets, X.device, E)
+    dtype = dY.dtype if dtype is None else dtype
+    out_code = types.get(dtype)
+    if out_code is None:
+        raise ValueError(f"dW cannot be {dtype}")
+    if dW is not None and (dW.dtype != dtype or tuple(dW.shape) != (E, N, K) or dW.device != X.device or
+                           not dW.is_contiguous()):
+        raise ValueError(f"dW must be a contiguous {dtype} tensor of {E} x {N} x {K} on the inputs' device")
+
+    def call(s):
+        out = X.new_empty((E, N, K), dtype=dtype) if dW is None else dW
+        _t, work, n = _work("bw_gemm_grouped_dw_work_bytes", X, E, M, N, K, out_code)
+        check(lib().bw_gemm_grouped_dw(dY.data_ptr(), ldy, X.data_ptr(), ldx, offsets.data_ptr(), out.data_ptr(), E, M, N, K,
+                                       code, out_code, work, n, s))
+        return out
+
+    return _on(X.device, stream, call, dY, X, offsets, dW)
 
 
 # ---------------------------------------------------------------------------------- 8-bit floating point

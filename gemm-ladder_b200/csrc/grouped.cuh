@@ -1,5 +1,5 @@
 // grouped.cuh -- host side of the products grouped by expert and in 8-bit floating point (bw_gemm_grouped,
-// bw_quant_f8, bw_quant_blocks_f8, bw_gemm_f8, bw_linear_f8 of bwgemm.h), included by bwgemm.cu: argument checks, the tensor
+// bw_gemm_grouped_dw, bw_quant_f8, bw_quant_blocks_f8, bw_gemm_f8, bw_linear_f8 of bwgemm.h), included by bwgemm.cu: argument checks, the tensor
 // maps, the caller's workspace, the launches.
 #pragma once
 #include "grouped_plan.h"
@@ -133,6 +133,79 @@ int gemm_grouped(const void* X, long long ldx, const void* B, const int* offsets
     p.offsets = offsets;
     p.C = C;
     return gx_product(*d, p, gx_maps(p, K, ldx, false), X, B, w, static_cast<uint8_t*>(work), pairs, false, false, st);
+}
+
+int dw_check(int E, int M, int N, int K, int out_type)
+{
+    if (out_type < BW_TYPE_F16 || out_type > BW_TYPE_F32) return BW_ERR_ARG;
+    if (!gx_sizes_ok(E, M, N, K) || N % 8 || K % 8) return BW_ERR_SHAPE;
+    // tiles and K-blocks within 32-bit indices
+    const long long per = (long long)((N + 255) / 256) * ((K + 255) / 256);
+    if (per * E >= (1LL << 30) || per * ((long long)M / 64 + E) >= (1LL << 40)) return BW_ERR_SHAPE;
+    return BW_OK;
+}
+
+size_t dw_work(const DwParams& p, int pairs, size_t* counters)
+{
+    *counters = up256(gx_work_bytes(pairs, 256));
+    return *counters + up256((size_t)dw_counters(p, pairs) * sizeof(int));
+}
+
+int gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx, const int* offsets, void* dW, int E, int M,
+                    int N, int K, int type, int out_type, void* work, size_t work_bytes, cudaStream_t st)
+{
+    if (type != BW_TYPE_F16 && type != BW_TYPE_BF16) return BW_ERR_ARG;
+    int rc = dw_check(E, M, N, K, out_type);
+    if (rc) return rc;
+    if (ldy < N || ldy % 8 || ldy > (1LL << 32) || ldx < K || ldx % 8 || ldx > (1LL << 32)) return BW_ERR_SHAPE;
+    if (!aligned(dW, 16)) return BW_ERR_ARG;
+    cudaError_t e;
+    if (M == 0) {  // no rows: every gradient is zero
+        e = cudaMemsetAsync(dW, 0, (size_t)E * N * K * (out_type == BW_TYPE_F32 ? 4 : 2), st);
+        return e == cudaSuccess ? BW_OK : cuda_fail(e, "cudaMemsetAsync (gradient)");
+    }
+    if (!aligned(dY, 16) || !aligned(X, 16) || !aligned(offsets, 4) || !aligned(work, 256)) return BW_ERR_ARG;
+    DeviceState* d = nullptr;
+    int pairs = 0;
+    if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
+    DwParams p = dw_params(E, M, N, K, type == BW_TYPE_BF16, out_type);
+    size_t at = 0;
+    const size_t bytes = dw_work(p, pairs, &at);
+    if (bytes > work_bytes) return scratch_fail(bytes, work_bytes);
+    p.offsets = offsets;
+    p.dW = dW;
+    p.work = static_cast<float*>(work);
+    p.counters = reinterpret_cast<int*>(static_cast<uint8_t*>(work) + at);
+    p.wait_ns = g_wait_ns;
+    e = cudaMemsetAsync(p.counters, 0, (size_t)dw_counters(p, pairs) * sizeof(int), st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync (counters)");
+    CUtensorMap my, mx;
+    if (!moe_map(&my, dY, 0, (uint64_t)N, (uint64_t)M, 1, (uint64_t)ldy, (uint64_t)ldy * M, 64) ||
+        !moe_map(&mx, X, 0, (uint64_t)K, (uint64_t)M, 1, (uint64_t)ldx, (uint64_t)ldx * M, 64)) {
+        snprintf(g_errbuf, sizeof g_errbuf, "cuTensorMapEncodeTiled failed");
+        return BW_ERR_LAUNCH;
+    }
+    static std::atomic<bool> limit_set[kMaxDevices];
+    std::atomic<bool>& done = limit_set[d - g_dev];
+    if (!done.load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(grouped_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BW_SMEM_LIMIT);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+        done.store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(kGxThreads);
+    cfg.dynamicSmemBytes = (size_t)(1024 + dw_smem(p.ring_bytes, E).bytes);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, grouped_dw_kernel, my, mx, p);
+    return e == cudaSuccess ? BW_OK : cuda_fail(e, "kernel launch (grouped gradient)");
 }
 
 int f8_check(int E, int M, int N, int K, int out_type, int swiglu)
@@ -306,4 +379,26 @@ BW_API int bw_gemm_grouped(const void* X, long long ldx, const void* B, const vo
 {
     return bw::gemm_grouped(X, ldx, B, static_cast<const int*>(offsets), C, E, M, N, K, type, layout, swiglu, work, work_bytes,
                             static_cast<cudaStream_t>(stream));
+}
+
+BW_API int bw_gemm_grouped_dw_work_bytes(int E, int M, int N, int K, int out_type, size_t* bytes)
+{
+    using namespace bw;
+    if (!bytes) return BW_ERR_ARG;
+    *bytes = 0;
+    int rc = dw_check(E, M, N, K, out_type);
+    if (rc || M == 0) return rc;
+    DeviceState* d = nullptr;
+    int pairs = 0;
+    if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
+    size_t at = 0;
+    *bytes = dw_work(dw_params(E, M, N, K, false, out_type), pairs, &at);
+    return BW_OK;
+}
+
+BW_API int bw_gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx, const void* offsets, void* dW,
+                              int E, int M, int N, int K, int type, int out_type, void* work, size_t work_bytes, void* stream)
+{
+    return bw::gemm_grouped_dw(dY, ldy, X, ldx, static_cast<const int*>(offsets), dW, E, M, N, K, type, out_type, work,
+                               work_bytes, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,402 @@
+// grouped_dw.cuh -- the weights' gradient of a product grouped by expert:
+//
+//   dW_e[n, k] = sum over expert e's rows t of dY[t, n] X[t, k]          (fp16 or bf16 operands, fp32 sums)
+//
+// The sum runs over the ragged dimension.  A pair of SMs holds a tile of 256 rows x up to 256 columns of dW_e; both operands
+// are MN-major (a row of dY or X is one k of the MMA), in stages of 64 rows.  An expert's last rows end anywhere in a stage:
+// the rows after them are another expert's (perhaps not finite), so they are overwritten with zeros up to the next 16 (an
+// MMA's depth) between the load and the MMAs.  For that each block's loads complete on its own barrier; its warp 10 waits
+// there, clears what has to be cleared and arrives on the leader's barrier, where the MMA issuer waits for both blocks.
+// Roles otherwise as in grouped_kernel.cuh; a TMEM lane is a row of dW, a column a column.
+#pragma once
+#include "grouped_kernel.cuh"
+
+namespace bw {
+
+constexpr int kDwStageBytes = 32768;  // 64 rows x 128 columns of dY, the same of X
+constexpr int kDwMaxStages = 6;
+
+struct DwParams {
+    const int* offsets;
+    int E, T, N, K;
+    int tn, tk;      // tiles along N and K
+    int width;       // columns of a tile but the last (a multiple of 32)
+    int stages, ring_bytes;
+    int out;         // BW_TYPE_*
+    uint32_t idesc;  // without N
+    void* dW;        // E x N x K
+    float* work;     // parts of split tiles
+    int* counters;   // two per split tile, zero at the start of a call
+    unsigned long long wait_ns;
+};
+
+struct DwSmem {
+    int bars, misc, tables, bytes;
+};
+__host__ __device__ inline DwSmem dw_smem(int ring_bytes, int E)
+{
+    DwSmem m;
+    m.bars = ring_bytes;
+    m.misc = m.bars + (3 * kDwMaxStages + 5) * 8;
+    m.misc = (m.misc + 15) / 16 * 16;
+    m.tables = m.misc + 64;
+    m.bytes = m.tables + 2 * (E + 1) * 4;
+    return m;
+}
+
+// Row numbers as gx_tables has them, and the running number of K-blocks of one tile of each expert.  By one warp.
+__device__ __forceinline__ void dw_tables(const DwParams& p, int* off, int* cum, int lane)
+{
+    GxParams g;
+    g.offsets = p.offsets;
+    g.E = p.E;
+    g.T = p.T;
+    g.cap = 64;
+    gx_tables<false>(g, off, cum, lane);  // cum: runs of at most 64, 0 where an expert has no rows
+    __syncwarp();
+    // one more for each expert without rows: added from the end of the table on, each entry by the empty experts before it
+    const int per = (p.E + 32) / 32;
+    const int i0 = lane * per, i1 = i0 + per < p.E + 1 ? i0 + per : p.E + 1;
+    int n = 0;
+    for (int i = i0; i < i1 && i < p.E; ++i) n += off[i + 1] == off[i] ? 1 : 0;
+    int sum = n;
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = (int)__shfl_sync(0xFFFFFFFFu, (uint32_t)sum, (lane - d) & 31);
+        if (lane >= d) sum += o;
+    }
+    n = sum - n;
+    for (int i = i0; i < i1; ++i) {
+        cum[i] += n;
+        if (i < p.E) n += off[i + 1] == off[i] ? 1 : 0;
+    }
+}
+
+// 16 columns of one row of dW.
+__device__ __forceinline__ void dw_store16(const DwParams& p, const float (&v)[16], size_t at, int left)
+{
+    if (p.out == 2) {
+        float* d = static_cast<float*>(p.dW) + at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * j < left) *reinterpret_cast<float4*>(d + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        return;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (p.out == 1) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        } else {
+            const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    }
+    uint16_t* d = static_cast<uint16_t*>(p.dW) + at;
+    if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+__global__ void __launch_bounds__(kGxThreads, 1)
+    grouped_dw_kernel(const __grid_constant__ CUtensorMap tmy, const __grid_constant__ CUtensorMap tmx, const DwParams p)
+{
+#ifdef BW_EMULATE
+    uint8_t* smem_raw = emu::cta_smem();
+#else
+    extern __shared__ uint8_t smem_raw[];
+#endif
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const DwSmem L = dw_smem(p.ring_bytes, p.E);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);  // this block's loads
+    uint64_t* ready = full + kDwMaxStages;                        // the leader's: both blocks' stages may be multiplied
+    uint64_t* empty = ready + kDwMaxStages;
+    uint64_t* tfull = empty + kDwMaxStages;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* drain = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* reduce_flag = abort_flag + 1;
+    int* off = reinterpret_cast<int*>(smem + L.tables);
+    int* cum = off + p.E + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
+    const int S = p.stages;
+
+    griddep_launch();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&ready[i], 2);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 16);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        *reduce_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&tmy);
+        prefetch_tmap(&tmx);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512u);
+        tmem_relinquish_pair();
+    }
+    griddep_wait();
+    if (warp == 2) dw_tables(p, off, cum, lane);
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
+    DwWalk walk(s, c);
+    DwSeg sg;
+    // a tile's place and columns: neighbouring tiles share dY's columns
+    auto place = [&](int& n0, int& k0, int& width) {
+        const int i = sg.tile - sg.e * s.per;
+        n0 = i / p.tk * 256;
+        k0 = i % p.tk * p.width;
+        const int left = p.K - k0;
+        width = left < p.width ? (left + 31) / 32 * 32 : p.width;
+    };
+
+    if (warp == 0) {
+        // ---------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            int stage = 0, issued = 0, seg = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            while (ok && walk.next(s, off, cum, sg)) {
+                int n0, k0, width;
+                place(n0, k0, width);
+                const int t0 = off[sg.e], rows = off[sg.e + 1] - t0;
+                const int boxes = (width / 2 + 63) / 64;
+                for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
+                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sy = smem + stage * kDwStageBytes;
+                    uint8_t* sx = sy + 16384;
+                    mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 + boxes) * 8192u);
+                    const int t = t0 + kb * 64;
+                    tma_load_3d(sy, &tmy, n0 + rank * 128, t, 0, &full[stage]);
+                    tma_load_3d(sy + 8192, &tmy, n0 + rank * 128 + 64, t, 0, &full[stage]);
+                    for (int i = 0; i < boxes; ++i)
+                        tma_load_3d(sx + i * 8192, &tmx, k0 + rank * (width / 2) + 64 * i, t, 0, &full[stage]);
+                    ++issued;
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
+                }
+                ++seg;
+            }
+            const int n = issued < S ? issued : S;
+            for (int i = 1; i <= n; ++i) {
+                const int q = issued - i;
+                wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------- MMA issuer
+        if (lane == 0 && leader) {
+            int stage = 0, acc = 0, seg = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            while (ok && walk.next(s, off, cum, sg)) {
+                int n0, k0, width;
+                place(n0, k0, width);
+                const int rows = off[sg.e + 1] - off[sg.e];
+                if (rows > 0) {
+                    if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) break;
+                    const uint32_t idesc = p.idesc | idesc_n(width);
+                    const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+                    for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                        if (!wait_bounded(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t sy = smem_u32(smem + stage * kDwStageBytes), sx = sy + 16384u;
+                        const int here = rows - kb * 64 < 64 ? rows - kb * 64 : 64;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k * 16 < here)
+                                mma_f16_pair(d, desc_mnmajor(sy, k), desc_mnmajor(sx, k), idesc,
+                                             kb > sg.k0 || k > 0 ? 1u : 0u);
+                        mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 0));
+                        mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 1));
+                        if (++stage == S) {
+                            stage = 0;
+                            ph ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 0));
+                    mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 1));
+                    acc ^= 1;
+                    if (acc == 0) aph ^= 1u;
+                }
+                ++seg;
+            }
+            mma_commit_pair(mapa_shared(smem_u32(drain), 0));
+            wait_drain(drain, 0, p.wait_ns);
+        }
+        __syncwarp();
+    } else if (warp < 10) {
+        // ---------------------------------------------------------- epilogue
+        const int ew = warp - 2, q = warp & 3, h = ew >> 2;
+        const int row = q * 32 + lane;
+        const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
+        int acc = 0, seg = 0;
+        uint32_t aph = 0;
+        bool alive = true;
+        while (walk.next(s, off, cum, sg)) {
+            int n0, k0, width;
+            place(n0, k0, width);
+            const int rows = off[sg.e + 1] - off[sg.e];
+            const int nc = width / 2, c0 = h * nc;
+            const int n = n0 + rank * 128 + row, k = k0 + c0;
+            const size_t at = ((size_t)sg.e * p.N + n) * p.K + k;
+            const bool mine = alive && n < p.N;
+            if (rows == 0) {
+                float z[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) z[j] = 0.f;
+                for (int i = 0; mine && i < nc; i += 16) dw_store16(p, z, at + i, p.K - k - i);
+                ++seg;
+                continue;
+            }
+            if (alive) alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+            tc_fence_after();
+            const bool write = alive && n < p.N;
+            const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256 + c0);
+            auto own = [&](int i, float(&v)[16]) {
+                uint32_t r[16];
+                tmem_ld16(tm + (uint32_t)i, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+            };
+            if (sg.k0 == 0 && sg.k1 == sg.kb) {
+#pragma unroll 1
+                for (int i = 0; i < nc; i += 16) {
+                    float v[16];
+                    own(i, v);
+                    if (write) dw_store16(p, v, at + i, p.K - k - i);
+                }
+            } else {
+                // a part of a split tile: the last block to finish sums all parts in the order of K
+                const int first = dw_part_of(s, sg.u0), last = dw_part_of(s, sg.u0 + sg.kb - 1);
+                const int nseg = last - first + 1;
+                int* counter = p.counters + sg.tile * 2 + rank;
+                auto slot_at = [&](int part, int i) {
+                    return reinterpret_cast<float4*>(p.work) +
+                           ((size_t)(dw_slot(s, part, sg.u0) * 2 + rank) * 64 + (c0 + i) / 4) * 128 + row;
+                };
+                named_bar_sync(1, kGxEpiThreads);
+                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == nseg - 1 ? 1 : 0;
+                named_bar_sync(1, kGxEpiThreads);
+                int go = *reduce_flag;
+                if (!go) {
+#pragma unroll 1
+                    for (int i = 0; i < nc; i += 16) {
+                        float v[16];
+                        own(i, v);
+                        if (alive) {
+                            float4* to = slot_at(c, i);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                __stcg(to + j * 128, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                        }
+                    }
+                    named_bar_sync(1, kGxEpiThreads);
+                    if (threadIdx.x == kGxEpi0)
+                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == nseg - 1 ? 1 : 0;
+                    named_bar_sync(1, kGxEpiThreads);
+                    go = *reduce_flag;
+                }
+                if (go) {
+#pragma unroll 1
+                    for (int i = 0; i < nc; i += 16) {
+                        float v[16], o[16];
+                        own(i, o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                        for (int part = first; part <= last; ++part) {
+                            if (part == c) {
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) v[j] += o[j];
+                                continue;
+                            }
+                            const float4* from = slot_at(part, i);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 x = __ldcg(from + j * 128);
+                                v[4 * j] += x.x;
+                                v[4 * j + 1] += x.y;
+                                v[4 * j + 2] += x.z;
+                                v[4 * j + 3] += x.w;
+                            }
+                        }
+                        if (write) dw_store16(p, v, at + i, p.K - k - i);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (alive && lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)acc);
+            acc ^= 1;
+            if (acc == 0) aph ^= 1u;
+            ++seg;
+        }
+    } else {
+        // ---------------------------------------------------------- stages handed on, an expert's last one cleared behind it
+        const uint32_t ready0 = mapa_shared(smem_u32(&ready[0]), 0);
+        int stage = 0, seg = 0;
+        uint32_t ph = 0;
+        bool alive = true;
+        while (alive && walk.next(s, off, cum, sg)) {
+            const int rows = off[sg.e + 1] - off[sg.e];
+            for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
+                alive = gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(5, 0, (uint32_t)stage), seg);
+                if (!alive) break;
+                const int here = rows - kb * 64;
+                if (here < 64 && here % 16) {
+                    const int r1 = (here + 15) / 16 * 16;
+                    uint4* box = reinterpret_cast<uint4*>(smem + stage * kDwStageBytes);  // 4 boxes of 64 rows of 8 pieces
+                    const int n = (r1 - here) * 8;
+                    for (int i = lane; i < 4 * n; i += 32) box[(i / n) * 512 + here * 8 + i % n] = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_shared();  // the MMAs read what was written, not what was loaded
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive_cluster(ready0 + 8u * (uint32_t)stage);
+                if (++stage == S) {
+                    stage = 0;
+                    ph ^= 1u;
+                }
+            }
+            ++seg;
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512u);
+    }
+}
+
+}  // namespace bw

@@ -1,7 +1,7 @@
 // grouped_plan.h -- host side arithmetic of the grouped kernels, shared by the library and the emulator: the token tile,
 // the stage ring, the workspace, the tensor maps' sizes.
 #pragma once
-#include "grouped_kernel.cuh"
+#include "grouped_dw.cuh"
 
 namespace bw {
 
@@ -62,6 +62,29 @@ inline GxMaps gx_maps(const GxParams& p, int K, long long ldx, bool f8)
     const uint64_t x[6] = {k, (uint64_t)p.T, 1, ld, ld * (uint64_t)p.T, (uint64_t)p.box};
     for (int i = 0; i < 6; ++i) m.x[i] = x[i];
     return m;
+}
+
+// The weights' gradient: everything of a call but its addresses.
+inline DwParams dw_params(int E, int T, int N, int K, bool bf16, int out)
+{
+    DwParams p = {};
+    p.E = E;
+    p.T = T;
+    p.N = N;
+    p.K = K;
+    p.tn = (N + 255) / 256;
+    p.tk = (K + 255) / 256;
+    p.width = ((K + p.tk - 1) / p.tk + 31) / 32 * 32;
+    p.stages = kDwMaxStages;
+    p.ring_bytes = p.stages * kDwStageBytes;
+    p.out = out;
+    p.idesc = idesc_16_f32_m(256, bf16, true, true);
+    return p;
+}
+inline int dw_counters(const DwParams& p, int pairs)
+{
+    const long long tiles = (long long)p.E * p.tn * p.tk;
+    return 2 * (int)(tiles <= kDwFewWaves * pairs ? tiles : tiles % pairs);
 }
 
 }  // namespace bw

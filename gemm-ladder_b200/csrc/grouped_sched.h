@@ -118,4 +118,88 @@ BW_GS void group_place(int j, int nt, int runs, int& m, int& n)
     n = r / rows;
 }
 
+// ------------------------------------------------------------------ the weights' gradient
+// dW_e (N x K) in tiles of 256 rows x up to 256 columns; a tile's K-blocks are runs of 64 of expert e's rows (an expert without
+// rows: one unit that only writes zeros).  Tiles in the order of experts, `per` each.  The experts' lengths differ, so the
+// split tiles are dealt out by units (K-blocks): with few tiles all of them, else the first tiles % pairs; the others whole,
+// one pair after the other, so that the pairs work on the same expert's rows at a time.
+constexpr int kDwFewWaves = 4;
+
+struct DwSched {
+    int per, pairs, tiles, split, parts;
+    long long units;  // of the split tiles
+};
+BW_GS int dw_blocks(int rows) { return rows > 0 ? (rows + 63) / 64 : 1; }
+
+// cum[e]: units of one tile of each expert before e (so tile t of expert e begins at unit per cum[e] + t blocks_e).
+BW_GS long long dw_tile_unit(const int* off, const int* cum, int per, int tile, int E)
+{
+    const int e = tile / per;
+    if (e >= E) return (long long)per * cum[E];
+    return (long long)per * cum[e] + (long long)(tile - e * per) * dw_blocks(off[e + 1] - off[e]);
+}
+BW_GS DwSched dw_sched(const int* off, const int* cum, int E, int per, int pairs)
+{
+    DwSched s;
+    s.per = per;
+    s.pairs = pairs;
+    s.tiles = E * per;
+    s.split = s.tiles <= kDwFewWaves * pairs ? s.tiles : s.tiles % pairs;
+    s.units = dw_tile_unit(off, cum, per, s.split, E);
+    long long parts = s.units / kGroupMinUnits;
+    if (parts > pairs) parts = pairs;
+    if (parts < 1) parts = 1;
+    s.parts = (int)parts;
+    return s;
+}
+BW_GS long long dw_begin(const DwSched& s, int c) { return s.units * c / s.parts; }
+BW_GS int dw_part_of(const DwSched& s, long long u) { return (int)(((u + 1) * s.parts - 1) / s.units); }
+// Part c's slot for a tile that begins at unit u0: a part's range cuts at most its first and its last tile.
+BW_GS int dw_slot(const DwSched& s, int c, long long u0) { return 2 * c + (u0 <= dw_begin(s, c) ? 0 : 1); }
+
+struct DwSeg {
+    int tile, e, k0, k1, kb;  // K-blocks [k0, k1) of kb
+    long long u0;             // the tile's first unit (split tiles)
+};
+struct DwWalk {
+    long long u, uend;
+    int tile, e;
+    BW_GS DwWalk(const DwSched& s, int c)
+    {
+        u = uend = 0;
+        if (s.split && c < s.parts) {
+            u = dw_begin(s, c);
+            uend = dw_begin(s, c + 1);
+        }
+        tile = s.split + c;
+        e = 0;
+    }
+    BW_GS bool next(const DwSched& s, const int* off, const int* cum, DwSeg& g)
+    {
+        if (u < uend) {
+            while ((long long)s.per * cum[e + 1] <= u) ++e;
+            g.e = e;
+            g.kb = dw_blocks(off[e + 1] - off[e]);
+            const long long base = (long long)s.per * cum[e];
+            const int i = (int)((u - base) / g.kb);
+            g.tile = e * s.per + i;
+            g.u0 = base + (long long)i * g.kb;
+            g.k0 = (int)(u - g.u0);
+            const long long end = g.u0 + g.kb;
+            g.k1 = g.kb - (int)(end > uend ? end - uend : 0);
+            u = end > uend ? uend : end;
+            return true;
+        }
+        if (tile >= s.tiles) return false;
+        g.e = tile / s.per;
+        g.kb = dw_blocks(off[g.e + 1] - off[g.e]);
+        g.tile = tile;
+        g.k0 = 0;
+        g.k1 = g.kb;
+        g.u0 = 0;
+        tile += s.pairs;
+        return true;
+    }
+};
+
 }  // namespace bw

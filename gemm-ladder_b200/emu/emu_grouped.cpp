@@ -4,6 +4,7 @@
 // C entries:
 //   bw_emu_grouped(X, ldx, xs, xs_ld, W, ws, offsets, C, E, T, N, K, pairs, kind, bf16, mn_major, glu, out, cap, stages,
 //                  status[4], &dirty, &findings, finding, len)
+//   bw_emu_grouped_dw(dY, ldy, X, ldx, offsets, dW, E, T, N, K, pairs, bf16, out, stages, status[4], &findings, finding, len)
 //   bw_emu_grouped_set(name, value): wait_ns, drop_tma, engine_delay_us, start_jitter_us, lead_skew_us, ld_delay_us
 #include <future>
 #include <string>
@@ -129,6 +130,30 @@ EMU_API int bw_emu_grouped(const void* X, long long ldx, const float* xs, long l
             grouped_kernel<0>(mw, mx, p);
     });
     (void)dirty;
+    end(status, findings, finding, len);
+    return 0;
+}
+
+EMU_API int bw_emu_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx, const int* offsets, void* dW, int E,
+                              int T, int N, int K, int pairs, int bf16, int out, int stages, unsigned* status, int* findings,
+                              char* finding, int len)
+{
+    using namespace bw;
+    begin();
+    DwParams p = dw_params(E, T, N, K, bf16, out);
+    if (stages && stages < p.stages) {
+        p.stages = stages;
+        p.ring_bytes = stages * kDwStageBytes;
+    }
+    p.offsets = offsets, p.dW = dW;
+    std::vector<float> work(gx_work_bytes(pairs, 256) / 4, NAN);
+    std::vector<int> counters((size_t)dw_counters(p, pairs) + 1, 0);
+    p.work = work.data(), p.counters = counters.data();
+    p.wait_ns = emu::g_wait_ns;
+    CUtensorMap my, mx;
+    map3(&my, dY, (uint64_t)N, (uint64_t)T, 1, (uint64_t)ldy, (uint64_t)ldy * T, 64);
+    map3(&mx, X, (uint64_t)K, (uint64_t)T, 1, (uint64_t)ldx, (uint64_t)ldx * T, 64);
+    launch_pairs(pairs, dw_smem(p.ring_bytes, p.E).bytes, [&] { grouped_dw_kernel(my, mx, p); });
     end(status, findings, finding, len);
     return 0;
 }

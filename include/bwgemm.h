@@ -166,6 +166,18 @@ int bw_gemm_grouped(const void* X, long long ldx, const void* B, const void* off
                     int type, int layout, int swiglu, void* work, size_t work_bytes, void* stream);
 
 /*
+ * The weights' gradient of such a product: dW_e = dY_e^T X_e over expert e's rows of dY (M x N) and X (M x K), ldy and ldx
+ * elements from row to row, offsets as above; dW is E x N x K, contiguous, in out_type (BW_TYPE_*), rounded once from fp32
+ * sums; zero for an expert without rows (so all of it where M == 0).  For a weight laid out as E x K x N exchange dY and X.
+ * (The input's gradient is bw_gemm_grouped with the other layout.)  Rows of no expert reach no gradient, whatever they hold.
+ * N % 8 == 0, K % 8 == 0, ldy % 8 == 0, ldx % 8 == 0; dY, X and dW 16-byte aligned.  `work`
+ * (bw_gemm_grouped_dw_work_bytes) as above.
+ */
+int bw_gemm_grouped_dw_work_bytes(int E, int M, int N, int K, int out_type, size_t* bytes);
+int bw_gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx, const void* offsets, void* dW, int E,
+                       int M, int N, int K, int type, int out_type, void* work, size_t work_bytes, void* stream);
+
+/*
  * Products in 8-bit floating point (e4m3) with a scale for each block of 128.
  *
  * bw_quant_f8 makes e4m3 rows of fp16 or bf16 (x_type) ones, ld elements from row to row, a scale for each group of 128

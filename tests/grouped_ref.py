@@ -108,6 +108,19 @@ def grouped(x, off, weight, n, product):
     return y, err, covered
 
 
+def weight_gradient(dY, X, off):
+    """(dW, error bound): E x N x K."""
+    o = off.tolist()
+    E = len(o) - 1
+    y = torch.zeros((E, dY.shape[1], X.shape[1]), dtype=torch.float64, device=X.device)
+    err = torch.zeros_like(y)
+    for e in range(E):
+        r = slice(o[e], o[e + 1])
+        if o[e] < o[e + 1]:
+            y[e], err[e] = product16(dY[r].t(), X[r].t())
+    return y, err
+
+
 def close(got, y, err):
     """Whether every element is within the bound (NaN where the definition is NaN)."""
     tol = err + (y.abs() + err) * HALF_STEP[got.dtype] + FLOOR[got.dtype]

@@ -124,3 +124,38 @@ def test_emulated_f8(emu, case):
     ok, worst = ref.close(C[:T][rows], y[rows], err[rows])
     assert ok, worst
     assert torch.isnan(C[:T][~rows].float()).all() and torch.isnan(C[T:].float()).all(), "rows of no expert were written"
+
+
+CASES_DW = [  # counts, N, K, pairs, type, out
+    ([5], 64, 64, 1, torch.float16, torch.float16),
+    ([0, 7, 0, 64, 81], 136, 200, 2, torch.bfloat16, torch.float32),    # empty experts, one whole stage, a tail of 1
+    ([3, 66, 16, 0], 264, 72, 3, torch.float16, torch.float16),
+    ([300, 0], 256, 328, 3, torch.bfloat16, torch.bfloat16),            # split tiles
+    ([1] * 7 + [130], 72, 296, 1, torch.bfloat16, torch.bfloat16),      # more tiles than a pair splits
+]
+
+
+@pytest.mark.parametrize("case", CASES_DW, ids=lambda c: "-".join(map(str, c[0])) + "x%dx%d" % (c[1], c[2]))
+def test_emulated_weight_gradient(emu, case):
+    counts, N, K, pairs, dtype, out = case
+    g = gen(N + K)
+    first, tail = 2, 3
+    T = first + sum(counts) + tail
+    dY, X = (torch.randn((T, n + 8), generator=g).to(dtype)[:, :n] for n in (N, K))
+    off = ref.offsets_of(counts, first)
+    # rows of no expert hold infinities and NaN: they reach nothing
+    for v in (dY, X):
+        v[:first] = float("nan")
+        v[T - tail:] = float("inf")
+    E = len(counts)
+    dW = torch.full((E + 1, N, K), float("nan"), dtype=out)
+    st, nf, msg = (ctypes.c_uint * 4)(), i32(), ctypes.create_string_buffer(512)
+    emu.bw_emu_grouped_dw(vp(dY.data_ptr()), ll(dY.stride(0)), vp(X.data_ptr()), ll(X.stride(0)), vp(off.data_ptr()),
+                          vp(dW.data_ptr()), E, T, N, K, pairs, int(dtype == torch.bfloat16), OUT[out], 0, st,
+                          ctypes.byref(nf), msg, 512)
+    assert nf.value == 0, msg.value.decode()
+    assert st[0] == 0, list(st)
+    y, err = ref.weight_gradient(dY, X, off)
+    ok, worst = ref.close(dW[:E], y, err)
+    assert ok, worst
+    assert torch.isnan(dW[E]).all()

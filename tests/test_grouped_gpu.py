@@ -73,6 +73,22 @@ def test_grouped(form, dtype, counts):
         assert torch.isnan(C[~covered]).all(), "rows of no expert were written"
 
 
+@pytest.mark.parametrize("out", [None, F32])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("counts", COUNTS + [[9000]], ids=lambda c: "-".join(map(str, c[:6])))
+def test_weight_gradient(dtype, out, counts):
+    for N, K in SIZES:
+        T, E = sum(counts) + 5, len(counts)
+        dY, X = rows(T, N, dtype, N + T, pad=8), rows(T, K, dtype, K + T + 1, pad=16)
+        off = ref.offsets_of(counts, 2, "cuda")
+        for v in (dY, X):  # rows of no expert reach no gradient
+            v[:2] = float("nan")
+            v[T - 3:] = float("inf")
+        dW = torch.full((E, N, K), float("nan"), dtype=out or dtype, device="cuda")
+        assert bwgemm.gemm_grouped_dw(dY, X, off, dW, dtype=out) is dW
+        check(dW, *ref.weight_gradient(dY, X, off))
+
+
 def f8_operands(T, E, N, K, dtype, seed):
     X = rows(T, K, dtype, seed)
     W = weights(max(1, E), N, K, dtype, seed + 1)
