@@ -5,7 +5,7 @@
 // The sum runs over the ragged dimension.  A pair of SMs holds a tile of 256 rows x up to 256 columns of dW_e; both operands
 // are MN-major (a row of dY or X is one k of the MMA), in stages of 64 rows.  An expert's last rows end anywhere in a stage:
 // the rows after them are another expert's (perhaps not finite), so they are overwritten with zeros up to the next 16 (an
-// MMA's depth) between the load and the MMAs.  For that each block's loads complete on its own barrier; its warp 10 waits
+// MMA's depth) between the load and the MMAs.  For that each block's loads complete on its own barrier; its warp 2 waits
 // there, clears what has to be cleared and arrives on the leader's barrier, where the MMA issuer waits for both blocks.
 // Roles otherwise as in grouped_kernel.cuh; a TMEM lane is a row of dW, a column a column.
 #pragma once
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_relinquish_pair();
     }
     griddep_wait();
-    if (warp == 2) dw_tables(p, off, cum, lane);
+    if (warp == 4) dw_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
     cluster_sync();
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
     DwWalk walk(s, c);
-    DwSeg sg;
+    DwSeg sg = {};
     // a tile's place and columns: neighbouring tiles share dY's columns
     auto place = [&](int& n0, int& k0, int& width) {
         const int i = sg.tile - sg.e * s.per;
@@ -252,9 +252,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             wait_drain(drain, 0, p.wait_ns);
         }
         __syncwarp();
-    } else if (warp < 10) {
+    } else if (warp >= 4) {
         // ---------------------------------------------------------- epilogue
-        const int ew = warp - 2, q = warp & 3, h = ew >> 2;
+        const int ew = warp - 4, q = warp & 3, h = ew >> 2;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
         int acc = 0, seg = 0;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             if (acc == 0) aph ^= 1u;
             ++seg;
         }
-    } else {
+    } else if (warp == 2) {
         // ---------------------------------------------------------- stages handed on, an expert's last one cleared behind it
         const uint32_t ready0 = mapa_shared(smem_u32(&ready[0]), 0);
         int stage = 0, seg = 0;

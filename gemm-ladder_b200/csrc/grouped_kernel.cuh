@@ -8,11 +8,11 @@
 //
 // A pair of SMs (cta_group::2) holds a tile of 256 weight rows x up to 256 tokens: each block loads its 128 weight rows
 // and half of the tokens, the leader issues the MMA over both blocks' shared memory.  The weights are the MMA's M, so the
-// ragged dimension is its N, set per tile (grouped_sched.h).  Roles of a block's 11 warps:
+// ragged dimension is its N, set per tile (grouped_sched.h).  Roles of a block's 12 warps:
 //   warp 0      TMA producer: a ring of stages of 128 bytes of K (64 16-bit values or 128 e4m3).
 //   warp 1      tensor memory; one thread of the leader issues the MMAs into one of two accumulators.
-//   warps 2-9   epilogue: TMEM lanes 32 (warp % 4) .. + 31 (weight rows), the first or second half of the columns (tokens).
-//   warp 10     KIND 1: the products xs ws of a K-block, one per token, into a ring in shared memory.
+//   warps 2, 3  KIND 1: the products xs ws of a K-block, one per token (a warp 128 of them), into a ring in shared memory.
+//   warps 4-11  epilogue: TMEM lanes 32 (warp % 4) .. + 31 (weight rows), the first or second half of the columns (tokens).
 // KIND 1: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers (128 per
 // thread); the MMAs of the next K-block run into the other accumulator meanwhile.  The scales differ from block to block, so
 // no MMA may run across two.  Per K-block and SM 128 x 256 multiply-adds (256 cycles of its 128 lanes) stand beside 512
@@ -25,12 +25,21 @@
 
 namespace bw {
 
-constexpr int kGxThreads = 352;
-constexpr int kGxEpi0 = 64;          // the first epilogue thread
+#ifdef BW_TRACE
+#define GX_CLOCK(...) __VA_ARGS__
+#else
+#define GX_CLOCK(...)
+#endif
+
+constexpr int kGxThreads = 384;
+constexpr int kGxEpi0 = 128;         // the first epilogue thread
 constexpr int kGxEpiThreads = 256;
 constexpr int kGxXBytes = 128 * 128;  // a block's weight rows of a stage
 constexpr int kGxMaxStages = 12;
 constexpr int kGxScales = 4;          // K-blocks of scale products held
+constexpr int kGxOtherRegs = 72, kGxEpiRegs = 216;
+static_assert(128 * kGxOtherRegs + 256 * kGxEpiRegs <= kGxThreads * 168, "registers moved within what the launch holds");
+constexpr int kGxAhead = 4;           // K-blocks whose scales are on their way
 constexpr int kGxBufBytes = 8 * 16 * 32 * 4;                    // per epilogue warp 16 tokens x 32 columns of C
 constexpr int kGxScaleBytes = kGxScales * 2 * 256 * 4;          // [K-block][gate, up][token]
 constexpr int kGxBars = 2 * kGxMaxStages + 4 + 2 * kGxScales + 1;
@@ -111,7 +120,7 @@ __device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, vol
     const uint32_t b = smem_u32(bar);
     if (__all_sync(0xFFFFFFFFu, mbar_try_wait(b, parity))) return true;
     uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = wait_slow(b, parity, abort_flag, limit_ns, where, seg) ? 1u : 0u;
+    if ((threadIdx.x & 31) == 0) ok = wait_spin(b, parity, abort_flag, limit_ns, where, seg) ? 1u : 0u;
     ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
     if (ok) mbar_try_wait(b, parity);  // complete: this lane acquires too
     return ok != 0;
@@ -180,8 +189,8 @@ __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], u
         named_bar_sync(bar, 64);
     } else {
         named_bar_sync(bar, 64);
-        // the up rows' warp: the same half, quarter q + 2 (warps 2 .. 9 have quarters 2, 3, 0, 1, 2, 3, 0, 1)
-        const float* b = reinterpret_cast<const float*>(bufs + (ew - 2) * 2048);
+        // the up rows' warp: the same half, quarter q + 2
+        const float* b = reinterpret_cast<const float*>(bufs + (ew + 2) * 2048);
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * b[j * 32 + lane];
         named_bar_sync(bar, 64);
@@ -195,16 +204,14 @@ __device__ __forceinline__ float4* gx_slot(const GxParams& p, int slot, int rank
     return reinterpret_cast<float4*>(p.work) + ((size_t)(slot * 2 + rank) * (p.cap / 4) + c4) * 128 + row;
 }
 
-// acc[j] += v[j] s[j]
-__device__ __forceinline__ void gx_fma16(float (&acc)[16], const uint32_t (&r)[16], const float* s)
+// acc[j] += v[j] s[j] for 16 columns, as pairs.
+__device__ __forceinline__ void gx_fma16(uint64_t (&acc)[8], const uint32_t (&r)[16], const float* s)
 {
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(s + j);  // one address per warp: a broadcast
-        acc[j] = fmaf(__uint_as_float(r[j]), x.x, acc[j]);
-        acc[j + 1] = fmaf(__uint_as_float(r[j + 1]), x.y, acc[j + 1]);
-        acc[j + 2] = fmaf(__uint_as_float(r[j + 2]), x.z, acc[j + 2]);
-        acc[j + 3] = fmaf(__uint_as_float(r[j + 3]), x.w, acc[j + 3]);
+    for (int j = 0; j < 4; ++j) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(s + 4 * j);  // one address per warp: a broadcast
+        acc[2 * j] = fma_f32x2(pair_f32(r[4 * j], r[4 * j + 1]), x.x, acc[2 * j]);
+        acc[2 * j + 1] = fma_f32x2(pair_f32(r[4 * j + 2], r[4 * j + 3]), x.y, acc[2 * j + 1]);
     }
 }
 
@@ -288,13 +295,17 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     int* off = reinterpret_cast<int*>(smem + L.tables);
     int* cum = off + p.E + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
     const int S = p.stages;
     const int tmem_cols = 2 * p.cap;  // a power of two, 64 .. 512
 
+    if (threadIdx.x == 0) {
+        BW_TRACE_CLEAR();
+        BW_TRACE_AT(0);
+    }
     griddep_launch();
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
@@ -306,7 +317,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&tempty[i], 16);  // the epilogue warps of both blocks
         }
         for (int i = 0; i < kGxScales; ++i) {
-            mbar_init(&sfull[i], 1);
+            mbar_init(&sfull[i], 2);
             mbar_init(&sempty[i], 8);
         }
         mbar_init(drain, 1);
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_relinquish_pair();
     }
     griddep_wait();  // what the kernel ahead wrote (the offsets, X, its scales, the counters) is visible from here on
-    if (warp == 2) gx_tables<F8>(p, off, cum, lane);
+    if (warp == 4) gx_tables<F8>(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // barriers, tables and tensor memory of both blocks are there
@@ -333,118 +344,131 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     GroupWalk walk(s, c);
     GroupSeg sg;
     GxFind find;
+    // KIND 1 holds 128 sums in registers: the epilogue's 8 warps take registers from the other 4 (384 threads are launched
+    // with 168 each: 128 x 72 + 256 x 216 <= 384 x 168)
+    if (F8 && warp < 4) reg_dec<kGxOtherRegs>();
 
     if (warp == 0) {
         // ---------------------------------------------------------- TMA producer
-        if (lane == 0) {
-            int stage = 0, issued = 0, seg = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            while (ok && walk.next(s, sg)) {
-                const GxTile t = find.at<F8>(p, off, cum, sg.tile);
-                const int boxes = (t.N / 2 + p.box - 1) / p.box;
-                const uint32_t bytes = 2u * (kGxXBytes + (uint32_t)(boxes * p.box) * 128u);
-                const int tok = t.t0 + rank * (t.N / 2);
-                // this block's weight rows: 128 in a row, or 64 gate and 64 up rows
-                const int w0 = p.glu == kGxPlain ? t.n * 256 + rank * 128
-                               : p.glu == kGxGluBlocks ? t.n * 256 + rank * 64
-                                                       : t.n * 128 + rank * 64;
-                const int w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
-                for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* sx = smem + stage * p.stage_bytes;
-                    uint8_t* sy = sx + kGxXBytes;
-                    const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);  // both blocks complete the leader's
+        const uint32_t full0 = mapa_shared(smem_u32(full), 0);  // both blocks complete the leader's barriers
+        int stage = 0, issued = 0, seg = 0;
+        uint32_t ph = 0;
+        bool alive = true;
+        while (alive && walk.next(s, sg)) {
+            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+            const int boxes = (t.N / 2 + p.box - 1) / p.box;
+            const uint32_t bytes = 2u * (kGxXBytes + (uint32_t)(boxes * p.box) * 128u);
+            const int tok = t.t0 + rank * (t.N / 2);
+            // this block's weight rows: 128 in a row, or 64 gate and 64 up rows
+            const int w0 = p.glu == kGxPlain ? t.n * 256 + rank * 128
+                           : p.glu == kGxGluBlocks ? t.n * 256 + rank * 64
+                                                   : t.n * 128 + rank * 64;
+            const int w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
+            for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg);
+                if (!alive) break;
+                uint8_t* sx = smem + stage * p.stage_bytes;
+                const uint32_t bar = full0 + 8u * (uint32_t)stage;
+                if (elect_one()) {
                     if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
                     if (p.mn_major) {
                         tma_load_3d_pair(sx, &tmw, w0, kb * 64, t.e, bar);
                         tma_load_3d_pair(sx + 8192, &tmw, w0 + 64, kb * 64, t.e, bar);
-                    } else if (p.glu == kGxPlain) {
-                        tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
                     } else {
                         tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
-                        tma_load_3d_pair(sx + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
+                        if (p.glu != kGxPlain) tma_load_3d_pair(sx + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
                     }
                     for (int i = 0; i < boxes; ++i)
-                        tma_load_3d_pair(sy + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
-                    ++issued;
-                    if (++stage == S) {
-                        stage = 0;
-                        ph ^= 1u;
-                    }
+                        tma_load_3d_pair(sx + kGxXBytes + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
                 }
-                ++seg;
+                ++issued;
+                if (++stage == S) {
+                    stage = 0;
+                    ph ^= 1u;
+                }
             }
-            if (leader) {  // loads in flight land before the blocks may leave (after an abort; else they have landed)
-                const int n = issued < S ? issued : S;
-                for (int i = 1; i <= n; ++i) {
-                    const int q = issued - i;
-                    wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
-                }
+            ++seg;
+        }
+        if (leader && lane == 0) {  // loads in flight land before the blocks may leave (after an abort; else they have landed)
+            const int n = issued < S ? issued : S;
+            for (int i = 1; i <= n; ++i) {
+                const int q = issued - i;
+                wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
             }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA issuer
-        if (lane == 0 && leader) {
+        if (leader) {
+            const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
+            const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
+            // the descriptors' low words (a 16-byte step of the address is a step of 1) and their constant high words
+            const uint64_t dx = !F8 && p.mn_major ? desc_mnmajor(smem_u32(smem), 0) : desc_kmajor(smem_u32(smem), 0);
+            const uint64_t dy = desc_kmajor(smem_u32(smem) + kGxXBytes, 0);
+            const uint32_t step = (uint32_t)p.stage_bytes >> 4, kx = !F8 && p.mn_major ? 128u : 2u;
             int stage = 0, acc = 0, seg = 0;
             uint32_t ph = 0, aph = 0;
-            bool ok = true;
-            auto next_acc = [&] {
-                mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 0));
-                mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 1));
-                acc ^= 1;
-                if (acc == 0) aph ^= 1u;
-            };
-            while (ok && walk.next(s, sg)) {
+            bool alive = true;
+            GX_CLOCK(long long w_full = 0, w_acc = 0, n_kb = 0, t_at = 0);
+            while (alive && walk.next(s, sg)) {
                 const GxTile t = find.at<F8>(p, off, cum, sg.tile);
-                const uint32_t idesc = p.idesc | (uint32_t)(t.N >> 3) << 17;
+                const uint32_t idesc = p.idesc | idesc_n(t.N);
                 for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                    if (F8 || kb == sg.k0) {
-                        if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) {
-                            ok = false;
-                            break;
+                    GX_CLOCK(t_at = clock64());
+                    if (F8 || kb == sg.k0)
+                        alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg);
+                    GX_CLOCK(w_acc += clock64() - t_at; t_at = clock64());
+                    alive = alive && gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg);
+                    if (!alive) break;
+                    GX_CLOCK(w_full += clock64() - t_at; if (n_kb++ == 0 && lane == 0) BW_TRACE_AT(2));
+                    tc_fence_after();
+                    const uint64_t ad = dx + (uint64_t)(step * (uint32_t)stage), bd = dy + (uint64_t)(step * (uint32_t)stage);
+                    const uint32_t d = tmem_base + (uint32_t)(acc * p.cap);
+                    const bool last = F8 || kb + 1 == sg.k1;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t accumulate = ((!F8 && kb > sg.k0) || k > 0) ? 1u : 0u;
+                            if constexpr (F8)
+                                mma_f8_pair(d, ad + kx * k, bd + 2 * k, idesc, accumulate);
+                            else
+                                mma_f16_pair(d, ad + kx * k, bd + 2 * k, idesc, accumulate);
+                        }
+                        mma_commit_pair(empty0[0] + 8u * (uint32_t)stage);
+                        mma_commit_pair(empty0[1] + 8u * (uint32_t)stage);
+                        if (last) {
+                            mma_commit_pair(tfull0[0] + 8u * (uint32_t)acc);
+                            mma_commit_pair(tfull0[1] + 8u * (uint32_t)acc);
                         }
                     }
-                    if (!wait_bounded(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg)) {
-                        ok = false;
-                        break;
+                    __syncwarp();
+                    if (last) {
+                        acc ^= 1;
+                        if (acc == 0) aph ^= 1u;
                     }
-                    tc_fence_after();
-                    const uint32_t sx = smem_u32(smem + stage * p.stage_bytes), sy = sx + kGxXBytes;
-                    const uint32_t d = tmem_base + (uint32_t)(acc * p.cap);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t accumulate = ((!F8 && kb > sg.k0) || k > 0) ? 1u : 0u;
-                        const uint64_t ad = !F8 && p.mn_major ? desc_mnmajor(sx, k) : desc_kmajor(sx, k);
-                        const uint64_t bd = desc_kmajor(sy, k);
-                        if constexpr (F8)
-                            mma_f8_pair(d, ad, bd, idesc, accumulate);
-                        else
-                            mma_f16_pair(d, ad, bd, idesc, accumulate);
-                    }
-                    mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 0));
-                    mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 1));
-                    if (F8) next_acc();
                     if (++stage == S) {
                         stage = 0;
                         ph ^= 1u;
                     }
                 }
-                if (!ok) break;
-                if (!F8) next_acc();
                 ++seg;
             }
+            if (lane == 0) {
+                BW_TRACE_AT(3);
+                BW_TRACE_VAL(12, w_full);
+                BW_TRACE_VAL(13, w_acc);
+                BW_TRACE_VAL(14, n_kb);
+            }
             // the MMAs in flight finish before the tensor memory is freed
-            mma_commit_pair(mapa_shared(smem_u32(drain), 0));
-            wait_drain(drain, 0, p.wait_ns);
+            if (elect_one()) {
+                mma_commit_pair(mapa_shared(smem_u32(drain), 0));
+                wait_drain(drain, 0, p.wait_ns);
+            }
         }
         __syncwarp();
-    } else if (warp < 10) {
+    } else if (warp >= 4) {
         // ---------------------------------------------------------- epilogue
-        const int ew = warp - 2, q = warp & 3, h = ew >> 2;
+        if (F8) reg_inc<kGxEpiRegs>();
+        const int ew = warp - 4, q = warp & 3, h = ew >> 2;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
         uint8_t* bufs = smem + L.buf;
@@ -463,13 +487,13 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const int tb = t.t0 + c0;
             const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
             const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
-            float sum[F8 ? 8 : 1][16];
             if constexpr (F8) {
+                uint64_t sum[8][8];  // 128 columns as pairs
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
-                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                    for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
+                for (int kb = sg.k0;;) {
                     if (alive)
                         alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), seg) &&
                                 gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
@@ -477,24 +501,39 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         tc_fence_after();
                         const float* sc = sc_base + si * 512 + c0;
                         const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
+                        // the next 16 columns leave tensor memory while these are added
+                        uint32_t r[2][16];
+                        tmem_ld16(tm, r[0]);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             if (i * 16 >= nc) break;
-                            uint32_t r[16];
-                            tmem_ld16(tm + (uint32_t)(i * 16), r);
                             tmem_wait_ld();
-                            gx_fma16(sum[i], r, sc + i * 16);
+                            if (i < 7 && (i + 1) * 16 < nc) tmem_ld16(tm + (uint32_t)(i * 16 + 16), r[(i + 1) & 1]);
+                            gx_fma16(sum[i], r[i & 1], sc + i * 16);
                         }
                     }
-                    release(acc);
+                    __syncwarp();  // every lane has read the scales
                     if (alive && lane == 0) mbar_arrive(&sempty[si]);
-                    acc ^= 1;
-                    if (acc == 0) aph ^= 1u;
                     if (++si == kGxScales) {
                         si = 0;
                         sph ^= 1u;
                     }
+                    if (++kb == sg.k1) break;
+                    release(acc);
+                    acc ^= 1;
+                    if (acc == 0) aph ^= 1u;
                 }
+                // the sums go back into the last accumulator, where the code below takes them for both kinds
+                const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (i * 16 >= nc) break;
+                    uint32_t r[16];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
+                    tmem_st16(tm + (uint32_t)(i * 16), r);
+                }
+                tmem_wait_st();
             } else {
                 if (alive)
                     alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
@@ -503,21 +542,15 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
             // this segment's sum of 16 columns
             auto own = [&](int i, float(&v)[16]) {
-                if constexpr (F8) {
+                uint32_t r[16];
+                tmem_ld16(tm + (uint32_t)(i * 16), r);
+                tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = sum[i][j];
-                } else {
-                    uint32_t r[16];
-                    tmem_ld16(tm + (uint32_t)(i * 16), r);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-                }
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
             };
             if (sg.k0 == 0 && sg.k1 == s.kb) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (i * 16 >= nc) break;
+#pragma unroll 1
+                for (int i = 0; i * 16 < nc; ++i) {
                     float v[16];
                     own(i, v);
                     gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
@@ -533,9 +566,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 int go = *reduce_flag;
                 if (!go) {
                     const int slot = part_slot(s, c, sg.tile);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (i * 16 >= nc) break;
+#pragma unroll 1
+                    for (int i = 0; i * 16 < nc; ++i) {
                         float v[16];
                         own(i, v);
                         if (alive) {
@@ -552,9 +584,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     go = *reduce_flag;
                 }
                 if (go) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (i * 16 >= nc) break;
+#pragma unroll 1
+                    for (int i = 0; i * 16 < nc; ++i) {
                         float v[16], mine[16];
                         own(i, mine);
 #pragma unroll
@@ -579,15 +610,15 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     }
                 }
             }
-            if constexpr (!F8) {
-                release(acc);
-                acc ^= 1;
-                if (acc == 0) aph ^= 1u;
-            }
+            release(acc);
+            acc ^= 1;
+            if (acc == 0) aph ^= 1u;
             ++seg;
         }
+        if (threadIdx.x == kGxEpi0) BW_TRACE_AT(4);
     } else if (F8) {
         // ---------------------------------------------------------- scale products
+        const int t00 = (warp - 2) * 128 + lane;  // this lane's first token of a tile
         int si = 0, seg = 0;
         uint32_t sph = 0;
         bool alive = true;
@@ -598,29 +629,39 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : 2 * t.n + 1;
             const float* w0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
             const float* w1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
-            for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                float x[8];
+            const int have = t.hi - t.t0;
+            // loaded kGxAhead K-blocks ahead: a load takes as long as several K-blocks of MMAs
+            float x[kGxAhead][4], a[kGxAhead], b[kGxAhead];
+            auto load = [&](int kb, float(&x)[4], float& a, float& b) {
+                if (kb >= sg.k1) return;
                 const float* xs = p.xs + kb * p.xs_ld + t.t0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int k = i * 32 + lane;
-                    x[i] = k < t.hi - t.t0 ? xs[k] : 0.f;
-                }
-                const float a = w0[kb], b = p.glu != kGxPlain ? w1[kb] : 0.f;
-                alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), seg);
-                if (!alive) break;
-                float* to = scales + si * 512;
+                for (int i = 0; i < 4; ++i) x[i] = t00 + i * 32 < have ? xs[t00 + i * 32] : 0.f;
+                a = w0[kb];
+                b = p.glu != kGxPlain ? w1[kb] : 0.f;
+            };
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (i * 32 >= t.N) break;
-                    to[i * 32 + lane] = x[i] * a;
-                    if (p.glu != kGxPlain) to[256 + i * 32 + lane] = x[i] * b;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sfull[si]);
-                if (++si == kGxScales) {
-                    si = 0;
-                    sph ^= 1u;
+            for (int d = 0; d < kGxAhead; ++d) load(sg.k0 + d, x[d], a[d], b[d]);
+            for (int kb = sg.k0; alive && kb < sg.k1; kb += kGxAhead) {
+#pragma unroll
+                for (int d = 0; d < kGxAhead; ++d) {
+                    if (kb + d >= sg.k1) break;
+                    alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), seg);
+                    if (!alive) break;
+                    float* to = scales + si * 512;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (t00 + i * 32 >= t.N) break;
+                        to[t00 + i * 32] = x[d][i] * a[d];
+                        if (p.glu != kGxPlain) to[256 + t00 + i * 32] = x[d][i] * b[d];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[si]);
+                    if (++si == kGxScales) {
+                        si = 0;
+                        sph ^= 1u;
+                    }
+                    load(kb + d + kGxAhead, x[d], a[d], b[d]);
                 }
             }
             ++seg;
@@ -635,6 +676,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, (uint32_t)tmem_cols);
     }
+    if (threadIdx.x == 0) BW_TRACE_AT(5);
 }
 
 }  // namespace bw

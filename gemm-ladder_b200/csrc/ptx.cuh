@@ -83,9 +83,10 @@ __device__ __forceinline__ void record_timeout(volatile int* abort_flag, uint32_
 }
 
 // Spins on (bar, parity) until the phase completes, the block's abort flag rises, or `limit_ns` pass. On a timeout it
-// records `where` and raises the abort flag; returns false on timeout or abort.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
-                                       uint32_t where, int seg)
+// records `where` and raises the abort flag; returns false on timeout or abort.  (wait_spin in place: for kernels that move
+// registers between warpgroups, which may not call functions.)
+__device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                          uint32_t where, int seg)
 {
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t i = 1;; ++i) {
@@ -98,6 +99,11 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile i
             }
         }
     }
+}
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                       uint32_t where, int seg)
+{
+    return wait_spin(bar, parity, abort_flag, limit_ns, where, seg);
 }
 
 __device__ __forceinline__ bool wait_bounded(uint64_t* barp, uint32_t parity, volatile int* abort_flag,
@@ -421,7 +427,60 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
+// The other way: each thread's 16 values into its lane; tmem_wait_st before they are read.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ------------------------------------------------------------------ one lane of a warp that stays together
+// True in one lane, the same one each time: the warp runs a loop as a whole, so that its values are the same in all lanes and
+// the compiler keeps them in uniform registers, which TMA and MMA instructions take their operands from.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A value that is the same in all lanes, as one the compiler knows to be.
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+
+// ------------------------------------------------------------------ registers moved between warpgroups
+// Each warp of a warpgroup executes it; the increases wait until the decreases have made room.
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ------------------------------------------------------------------ two fp32 operations at once
+// A pair of floats in a 64-bit register: (a.lo b.lo + c.lo, a.hi b.hi + c.hi), each rounded once.
+__device__ __forceinline__ uint64_t pair_f32(uint32_t lo, uint32_t hi)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair_f32(uint64_t v, uint32_t& lo, uint32_t& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
 
 // ------------------------------------------------------------------ descriptors
 // Shared-memory matrix descriptor (sm_100 layout): start >> 4 in bits [0,14), leading byte offset >> 4 in [16,30),

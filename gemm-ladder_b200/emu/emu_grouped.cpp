@@ -1,5 +1,5 @@
 // emu_grouped.cpp -- the host emulator over the grouped kernels (test infrastructure; a build of its own with
-// -DBW_EMU_THREADS=352, the kernels' block).
+// -DBW_EMU_THREADS=384, the kernels' block).
 //
 // C entries:
 //   bw_emu_grouped(X, ldx, xs, xs_ld, W, ws, offsets, C, E, T, N, K, pairs, kind, bf16, mn_major, glu, out, cap, stages,

@@ -789,6 +789,19 @@ inline void tmem_ld(uint32_t taddr, uint32_t (&r)[NC])
     std::memcpy(r, t_cta->tmem.data() + (size_t)lane * kTmemCols + col, sizeof r);
 }
 
+// tcgen05.st 32x32b.x16: the way back
+template <int NC>
+inline void tmem_st(uint32_t taddr, const uint32_t (&r)[NC])
+{
+    const uint32_t lane = (taddr >> 16) + (uint32_t)(t_tid & 31), col = taddr & 0xFFFFu;
+    if (lane >= (uint32_t)kTmemLanes || col + NC > (uint32_t)t_cta->tmem_cols) {
+        finding("tcgen05.st of lane %u column %u outside the allocation", lane, col);
+        return;
+    }
+    if (((uint32_t)(t_tid >> 5) & 3u) != ((taddr >> 16) >> 5)) finding("a warp writing a TMEM lane quarter not its own");
+    std::memcpy(t_cta->tmem.data() + (size_t)lane * kTmemCols + col, r, sizeof r);
+}
+
 }  // namespace emu
 }  // namespace bw
 

@@ -89,6 +89,11 @@ inline bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, u
     }
 }
 
+inline bool wait_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns, uint32_t where, int seg)
+{
+    return wait_slow(bar, parity, abort_flag, limit_ns, where, seg);
+}
+
 // ------------------------------------------------------------------ system scope (the emulated GPUs of one process)
 inline unsigned ld_acquire_sys(const unsigned* p) { return __atomic_load_n(p, __ATOMIC_ACQUIRE); }
 inline void st_release_sys(unsigned* p, unsigned v) { __atomic_store_n(p, v, __ATOMIC_RELEASE); }
@@ -287,6 +292,29 @@ inline void mma_commit(uint64_t* bar)
 inline void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) { emu::tmem_ld(taddr, r); }
 inline void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) { emu::tmem_ld(taddr, r); }
 inline void tmem_wait_ld() {}
+inline void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) { emu::tmem_st(taddr, r); }
+inline void tmem_wait_st() {}
+
+inline bool elect_one() { return (emu::t_tid & 31) == 0; }
+inline int warp_uniform(int v) { return v; }
+template <int N>
+inline void reg_inc() {}
+template <int N>
+inline void reg_dec() {}
+
+inline uint64_t pair_f32(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
+inline void unpair_f32(uint64_t v, uint32_t& lo, uint32_t& hi)
+{
+    lo = (uint32_t)v;
+    hi = (uint32_t)(v >> 32);
+}
+inline uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    const float lo = std::fma(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)b), __uint_as_float((uint32_t)c));
+    const float hi = std::fma(__uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)(b >> 32)),
+                              __uint_as_float((uint32_t)(c >> 32)));
+    return pair_f32(__float_as_uint(lo), __float_as_uint(hi));
+}
 
 // ------------------------------------------------------------------ descriptors (the same encodings as ptx.cuh)
 inline uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo)

@@ -18,7 +18,7 @@ def emu(tmp_path_factory):
     if not os.path.isdir(CUDA_INCLUDE):
         pytest.skip("no CUDA headers")
     lib = str(tmp_path_factory.mktemp("emu_grouped") / "libbwemu_grouped.so")
-    subprocess.check_call(["g++", "-std=c++20", "-O2", "-pthread", "-DBW_EMULATE", "-DBW_EMU_THREADS=352", "-fPIC",
+    subprocess.check_call(["g++", "-std=c++20", "-O2", "-pthread", "-DBW_EMULATE", "-DBW_EMU_THREADS=384", "-fPIC",
                            "-shared", "-w", f"-I{CUDA_INCLUDE}", f"-I{os.path.join(ROOT, 'include')}",
                            f"-I{os.path.join(PKG, 'csrc')}", os.path.join(PKG, "emu", "emu_grouped.cpp"), "-o", lib])
     return ctypes.CDLL(lib)
