@@ -85,8 +85,8 @@ int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CU
 
 // The product of p (its addresses but C's workspace filled in); zeroed: the counters are zero already, by a kernel that the
 // launch may overlap.
-int gx_product(DeviceState& d, GxParams& p, const GxMaps& m, const void* X, const void* W, const GxWork& w, uint8_t* work,
-               int pairs, bool f8, bool zeroed, cudaStream_t st)
+int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m, const void* X, const void* W, const GxWork& w, uint8_t* work,
+               int pairs, bool zeroed, cudaStream_t st)
 {
     p.work = reinterpret_cast<float*>(work + w.parts);
     p.counters = reinterpret_cast<int*>(work + w.counters);
@@ -101,7 +101,11 @@ int gx_product(DeviceState& d, GxParams& p, const GxMaps& m, const void* X, cons
         snprintf(g_errbuf, sizeof g_errbuf, "cuTensorMapEncodeTiled failed");
         return BW_ERR_LAUNCH;
     }
-    return f8 ? gx_launch<1>(d, p, mw, mx, pairs, zeroed, st) : gx_launch<0>(d, p, mw, mx, pairs, zeroed, st);
+    switch (form.kind) {
+    case kGxF8Tokens: return gx_launch<kGxF8Tokens>(d, p, mw, mx, pairs, zeroed, st);
+    case kGxF8Weights: return gx_launch<kGxF8Weights>(d, p, mw, mx, pairs, zeroed, st);
+    default: return gx_launch<kGx16>(d, p, mw, mx, pairs, zeroed, st);
+    }
 }
 
 int grouped_check(int E, int M, int N, int K, int layout, int swiglu)
@@ -125,14 +129,13 @@ int gemm_grouped(const void* X, long long ldx, const void* B, const int* offsets
     DeviceState* d = nullptr;
     int pairs = 0;
     if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
-    const int cap = gx_cap(M, E, true);
-    const GxWork w = gx_work(M, K, cap, pairs, false);
+    const GxForm form = gx_form(M, E, true, false);
+    const GxWork w = gx_work(M, K, form.cap, pairs, false);
     if (w.bytes > work_bytes) return scratch_fail(w.bytes, work_bytes);
-    GxParams p = gx_params(E, M, N, K, false, type == BW_TYPE_BF16, layout == BW_LAYOUT_KN,
-                           swiglu ? kGxGluHalves : kGxPlain, type, cap);
+    GxParams p = gx_params(E, M, N, K, form, type == BW_TYPE_BF16, layout == BW_LAYOUT_KN, swiglu ? kGxGluHalves : kGxPlain, type);
     p.offsets = offsets;
     p.C = C;
-    return gx_product(*d, p, gx_maps(p, K, ldx, false), X, B, w, static_cast<uint8_t*>(work), pairs, false, false, st);
+    return gx_product(*d, p, form, gx_maps(p, K, ldx, false), X, B, w, static_cast<uint8_t*>(work), pairs, false, st);
 }
 
 int dw_check(int E, int M, int N, int K, int out_type)
@@ -216,18 +219,18 @@ int f8_check(int E, int M, int N, int K, int out_type, int swiglu)
 }
 
 // C = A B^T of e4m3 operands; E 0: one matrix, all rows.
-int f8_product(DeviceState& d, int pairs, int cap, const GxWork& w, const void* A, const float* a_scale, long long lds,
+int f8_product(DeviceState& d, int pairs, const GxForm& form, const GxWork& w, const void* A, const float* a_scale, long long lds,
                const void* B, const float* b_scale, const int* offsets, int E, void* C, int M, int N, int K, int out_type,
                int swiglu, uint8_t* work, bool zeroed, cudaStream_t st)
 {
-    GxParams p = gx_params(E ? E : 1, M, N, K, true, false, false,
-                           !swiglu ? kGxPlain : E ? kGxGluHalves : kGxGluBlocks, out_type, cap);
+    GxParams p = gx_params(E ? E : 1, M, N, K, form, false, false, !swiglu ? kGxPlain : E ? kGxGluHalves : kGxGluBlocks,
+                           out_type);
     p.offsets = E ? offsets : nullptr;
     p.C = C;
     p.xs = a_scale;
     p.xs_ld = lds;
     p.ws = b_scale;
-    return gx_product(d, p, gx_maps(p, K, K, true), A, B, w, work, pairs, true, zeroed, st);
+    return gx_product(d, p, form, gx_maps(p, K, K, true), A, B, w, work, pairs, zeroed, st);
 }
 
 int gemm_f8(const void* A, const void* a_scale, long long lds, const void* B, const void* b_scale, const int* offsets, int E,
@@ -243,10 +246,10 @@ int gemm_f8(const void* A, const void* a_scale, long long lds, const void* B, co
     DeviceState* d = nullptr;
     int pairs = 0;
     if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
-    const int cap = gx_cap(M, E ? E : 1, E > 0);
-    const GxWork w = gx_work(M, K, cap, pairs, false);
+    const GxForm form = gx_form(M, E ? E : 1, E > 0, true);
+    const GxWork w = gx_work(M, K, form.cap, pairs, false);
     if (w.bytes > work_bytes) return scratch_fail(w.bytes, work_bytes);
-    return f8_product(*d, pairs, cap, w, A, static_cast<const float*>(a_scale), lds, B, static_cast<const float*>(b_scale),
+    return f8_product(*d, pairs, form, w, A, static_cast<const float*>(a_scale), lds, B, static_cast<const float*>(b_scale),
                       offsets, E, C, M, N, K, out_type, swiglu, static_cast<uint8_t*>(work), false, st);
 }
 
@@ -323,7 +326,7 @@ BW_API int bw_gemm_f8_work_bytes(int E, int M, int N, int K, int out_type, int s
     DeviceState* d = nullptr;
     int pairs = 0;
     if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
-    *bytes = gx_work(M, K, gx_cap(M, E ? E : 1, E > 0), pairs, linear != 0).bytes;
+    *bytes = gx_work(M, K, gx_form(M, E ? E : 1, E > 0, true).cap, pairs, linear != 0).bytes;
     return BW_OK;
 }
 
@@ -347,8 +350,8 @@ BW_API int bw_linear_f8(const void* X, int x_type, long long ld, const void* B, 
     DeviceState* d = nullptr;
     int pairs = 0;
     if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
-    const int cap = gx_cap(M, E ? E : 1, E > 0);
-    const GxWork w = gx_work(M, K, cap, pairs, true);
+    const GxForm form = gx_form(M, E ? E : 1, E > 0, true);
+    const GxWork w = gx_work(M, K, form.cap, pairs, true);
     if (w.bytes > work_bytes) return scratch_fail(w.bytes, work_bytes);
     uint8_t* ws = static_cast<uint8_t*>(work);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -356,7 +359,7 @@ BW_API int bw_linear_f8(const void* X, int x_type, long long ld, const void* B, 
     if ((rc = quant_f8_rows(X, x_type, ld, ws + w.q, scale, w.lds, M, K, reinterpret_cast<int*>(ws + w.counters), w.n_counters,
                             st)))
         return rc;
-    return f8_product(*d, pairs, cap, w, ws + w.q, scale, w.lds, B, static_cast<const float*>(b_scale),
+    return f8_product(*d, pairs, form, w, ws + w.q, scale, w.lds, B, static_cast<const float*>(b_scale),
                       static_cast<const int*>(offsets), E, C, M, N, K, x_type, swiglu, ws, true, st);
 }
 
@@ -370,7 +373,7 @@ BW_API int bw_gemm_grouped_work_bytes(int E, int M, int N, int K, int layout, in
     DeviceState* d = nullptr;
     int pairs = 0;
     if ((rc = device_state(&d)) || (rc = gx_pairs(*d, &pairs))) return rc;
-    *bytes = gx_work(M, K, gx_cap(M, E, true), pairs, false).bytes;
+    *bytes = gx_work(M, K, gx_form(M, E, true, false).cap, pairs, false).bytes;
     return BW_OK;
 }
 

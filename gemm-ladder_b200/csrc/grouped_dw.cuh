@@ -52,7 +52,7 @@ __device__ __forceinline__ void dw_tables(const DwParams& p, int* off, int* cum,
     g.E = p.E;
     g.T = p.T;
     g.cap = 64;
-    gx_tables<false>(g, off, cum, lane);  // cum: runs of at most 64, 0 where an expert has no rows
+    gx_tables(g, off, cum, lane);  // cum: runs of at most 64, 0 where an expert has no rows
     __syncwarp();
     // one more for each expert without rows: added from the end of the table on, each entry by the empty experts before it
     const int per = (p.E + 32) / 32;
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             }
             tc_fence_before();
             __syncwarp();
-            if (alive && lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)acc);
+            if (alive && lane == 0) mbar_arrive_remote_relaxed(tempty0 + 8u * (uint32_t)acc);
             acc ^= 1;
             if (acc == 0) aph ^= 1u;
             ++seg;
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     fence_proxy_async_shared();  // the MMAs read what was written, not what was loaded
                     __syncwarp();
                 }
-                if (lane == 0) mbar_arrive_cluster(ready0 + 8u * (uint32_t)stage);
+                if (lane == 0) mbar_arrive_remote(ready0 + 8u * (uint32_t)stage);
                 if (++stage == S) {
                     stage = 0;
                     ph ^= 1u;

@@ -1,22 +1,24 @@
 // grouped_kernel.cuh -- products grouped by expert with ragged numbers of rows, and products in 8-bit floating point with
 // a scale per block of 128: one kernel.
 //
-//   Y[t, n] = sum_k X[t, k] W_e[n, k]     t in the rows of expert e, n < N            (KIND 0: fp16 or bf16)
-//   Y[t, n] = sum_b xs[t, b] ws_e[n / 128, b] sum_{k in block b} X[t, k] W_e[n, k]    (KIND 1: e4m3, blocks of 128 of K)
-// or W as E x K x N (KIND 0), or silu(gate) * up of two of W's rows per output column.  One expert and no offsets: a plain
+//   Y[t, n] = sum_k X[t, k] W_e[n, k]     t in the rows of expert e, n < N            (kGx16: fp16 or bf16)
+//   Y[t, n] = sum_b xs[t, b] ws_e[n / 128, b] sum_{k in block b} X[t, k] W_e[n, k]    (kGxF8*: e4m3, blocks of 128 of K)
+// or W as E x K x N (kGx16), or silu(gate) * up of two of W's rows per output column.  One expert and no offsets: a plain
 // product.
 //
 // A pair of SMs (cta_group::2) holds a tile of 256 weight rows x up to 256 tokens: each block loads its 128 weight rows
 // and half of the tokens, the leader issues the MMA over both blocks' shared memory.  The weights are the MMA's M, so the
 // ragged dimension is its N, set per tile (grouped_sched.h).  Roles of a block's 12 warps:
 //   warp 0      TMA producer: a ring of stages of 128 bytes of K (64 16-bit values or 128 e4m3).
-//   warp 1      tensor memory; one thread of the leader issues the MMAs into one of two accumulators.
-//   warps 2, 3  KIND 1: the products xs ws of a K-block, one per token (a warp 128 of them), into a ring in shared memory.
+//   warp 1      tensor memory; one thread of the leader issues the MMAs into a ring of accumulators (two of 256 columns, up to eight narrower).
+//   warps 2, 3  kGxF8Weights: the products xs ws of a K-block, one per token (a warp 128 of them), into a ring in shared memory.
 //   warps 4-11  epilogue: TMEM lanes 32 (warp % 4) .. + 31 (weight rows), the first or second half of the columns (tokens).
-// KIND 1: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers (128 per
-// thread); the MMAs of the next K-block run into the other accumulator meanwhile.  The scales differ from block to block, so
-// no MMA may run across two.  Per K-block and SM 128 x 256 multiply-adds (256 cycles of its 128 lanes) stand beside 512
-// cycles of MMA at the e4m3 rate.
+// e4m3: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers; the MMAs of
+// the next K-blocks run into the other accumulators meanwhile.  The scales differ from block to block, so no MMA may run
+// across two.  With the weights as M (kGxF8Weights) a column's scale is the same in all lanes and comes from shared memory, 4
+// bytes per product: 256 tokens would take 1024 cycles a K-block (128 bytes a cycle) beside 512 of MMA.  So above 128 tokens
+// per expert the tokens are the M (kGxF8Tokens): a lane is a token with one scale, a half of the columns one block of
+// weights with another, and the product of the two is all a K-block needs.
 // Every wait is bounded (ptx.cuh); after one that gave up the epilogue walks its segments to the end without waiting,
 // reading or writing, so that all threads meet at every barrier.
 #pragma once
@@ -40,10 +42,13 @@ constexpr int kGxScales = 4;          // K-blocks of scale products held
 constexpr int kGxOtherRegs = 72, kGxEpiRegs = 216;
 static_assert(128 * kGxOtherRegs + 256 * kGxEpiRegs <= kGxThreads * 168, "registers moved within what the launch holds");
 constexpr int kGxAhead = 4;           // K-blocks whose scales are on their way
+constexpr int kGxAccs = 8;            // accumulators in tensor memory at most
 constexpr int kGxBufBytes = 8 * 16 * 32 * 4;                    // per epilogue warp 16 tokens x 32 columns of C
 constexpr int kGxScaleBytes = kGxScales * 2 * 256 * 4;          // [K-block][gate, up][token]
-constexpr int kGxBars = 2 * kGxMaxStages + 4 + 2 * kGxScales + 1;
+constexpr int kGxBars = 2 * kGxMaxStages + 2 * kGxAccs + 2 * kGxScales + 1;
 
+// fp16 or bf16; e4m3 with the weight rows as the MMA's M; e4m3 with the tokens as its M.
+enum : int { kGx16 = 0, kGxF8Weights = 1, kGxF8Tokens = 2 };
 // What silu * up pairs: nothing; rows 256 g + i with 256 g + 128 + i; rows f with N / 2 + f.
 enum : int { kGxPlain = 0, kGxGluBlocks = 1, kGxGluHalves = 2 };
 
@@ -52,15 +57,16 @@ struct GxParams {
     int E, T;              // experts, rows of X
     int N, Nout;           // weight rows per expert; columns of C
     int nt, kblocks;       // weight tiles per expert, K-blocks
-    int cap, box;          // the most tokens of a tile; rows of one TMA box of X
+    int cap, box, wbox;    // the most tokens of a tile; rows of one TMA box of X, of W
     int stages, stage_bytes, ring_bytes;
+    int accs;              // accumulators in tensor memory
     int mn_major;          // W is E x K x N
     int glu, out;          // kGx*; BW_TYPE_* (0 fp16, 1 bf16, 2 fp32)
     uint32_t idesc;        // without N
     void* C;               // T x Nout, contiguous
-    const float* xs;       // KIND 1: scale of token t, K-block b at xs[b * xs_ld + t]
+    const float* xs;       // e4m3: scale of token t, K-block b at xs[b * xs_ld + t]
     long long xs_ld;
-    const float* ws;       // KIND 1: [e][block of 128 rows][K-block]
+    const float* ws;       // e4m3: [e][block of 128 rows][K-block]
     int ws_rows;           // blocks of 128 rows per expert
     float* work;           // parts of split tiles: slots of 2 x 128 x cap
     int* counters;         // two per split tile, zero at the start of a call
@@ -86,29 +92,28 @@ __host__ __device__ inline GxSmem gx_smem(int ring_bytes, int E)
 // A tile's rows of X and weight rows.
 struct GxTile {
     int e, n;     // expert, weight tile
-    int t0;       // its first token (may lie before lo: rounded down to 4 rows for the scales)
-    int lo, hi;   // the tokens of C it writes: [lo, hi)
+    int t0, t1;   // its tokens [t0, t1)
     int N;        // MMA N: a multiple of 32
 };
 
 // Follows ascending tile indices through the experts.
 struct GxFind {
     int e = 0;
-    template <bool F8>
+    template <int KIND>
     __device__ __forceinline__ GxTile at(const GxParams& p, const int* off, const int* cum, int tile)
     {
         while (cum[e + 1] * p.nt <= tile) ++e;
         GxTile t;
         t.e = e;
-        const int runs = cum[e + 1] - cum[e], a = off[e], b = off[e + 1], s = F8 ? a & ~3 : a;
+        const int runs = cum[e + 1] - cum[e], a = off[e], b = off[e + 1];
         int m;
         group_place(tile - cum[e] * p.nt, p.nt, runs, m, t.n);
-        const int rows = group_run_rows(s, b, runs);
-        t.t0 = s + m * rows;
-        const int end = t.t0 + rows < b ? t.t0 + rows : b;
-        t.lo = t.t0 < a ? a : t.t0;
-        t.hi = end;
-        t.N = (end - t.t0 + 31) / 32 * 32;
+        const int rows = KIND == kGxF8Tokens ? 256 : group_run_rows(a, b, runs);
+        t.t0 = a + m * rows;
+        t.t1 = t.t0 + rows < b ? t.t0 + rows : b;
+        int n = t.t1 - t.t0;
+        if (KIND == kGxF8Tokens) n = p.glu == kGxPlain && p.N - t.n * 256 < 256 ? p.N - t.n * 256 : 256;
+        t.N = (n + 31) / 32 * 32;
         return t;
     }
 };
@@ -127,9 +132,9 @@ __device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, vol
 }
 
 // 16 tokens x 32 columns of C: v[j] is token tb + j, column f + lane.  Through the warp's buffer, so that a token's 32
-// columns leave as 16-byte pieces; only tokens [lo, hi) and columns below Nout (a multiple of 8) are written.
-__device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[16], void* buf, int tb, int lo, int hi, int f,
-                                           int lane, bool write)
+// columns leave as 16-byte pieces; only tokens below t1 and columns below Nout (a multiple of 8) are written.
+__device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[16], void* buf, int tb, int t1, int f, int lane,
+                                           bool write)
 {
     if (p.out == 2) {
         float* b = static_cast<float*>(buf);
@@ -139,7 +144,7 @@ __device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[1
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = tb + i * 4 + (lane >> 3), c = f + (lane & 7) * 4;
-            if (write && t >= lo && t < hi && c < p.Nout)
+            if (write && t < t1 && c < p.Nout)
                 *reinterpret_cast<float4*>(static_cast<float*>(p.C) + (size_t)t * p.Nout + c) =
                     *reinterpret_cast<const float4*>(b + (i * 4 + (lane >> 3)) * 32 + (lane & 7) * 4);
         }
@@ -162,7 +167,7 @@ __device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[1
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int t = tb + i * 8 + (lane >> 2), c = f + (lane & 3) * 8;
-            if (write && t >= lo && t < hi && c < p.Nout)
+            if (write && t < t1 && c < p.Nout)
                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.C) + (size_t)t * p.Nout + c) =
                     *reinterpret_cast<const uint4*>(b + (i * 8 + (lane >> 2)) * 32 + (lane & 3) * 8);
         }
@@ -177,7 +182,7 @@ __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], u
 {
     uint8_t* mine = bufs + ew * 2048;
     if (p.glu == kGxPlain) {
-        gx_store16(p, v, mine, tb, t.lo, t.hi, f, lane, write);
+        gx_store16(p, v, mine, tb, t.t1, f, lane, write);
         return;
     }
     const uint32_t bar = 2u + (uint32_t)(h * 2 + (q & 1));
@@ -194,8 +199,39 @@ __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], u
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * b[j * 32 + lane];
         named_bar_sync(bar, 64);
-        gx_store16(p, v, mine, tb, t.lo, t.hi, f, lane, write);
+        gx_store16(p, v, mine, tb, t.t1, f, lane, write);
     }
+}
+
+// 16 columns of one token's row of C from column f on (kGxF8Tokens: a lane is a token).
+__device__ __forceinline__ void gx_store_row16(const GxParams& p, const float (&v)[16], int t, int f)
+{
+    const int left = p.Nout - f;
+    const size_t at = (size_t)t * p.Nout + f;
+    if (p.out == 2) {
+        float* d = static_cast<float*>(p.C) + at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * j < left) *reinterpret_cast<float4*>(d + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        return;
+    }
+    uint32_t w[8];
+    if (p.out == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+    }
+    uint16_t* d = static_cast<uint16_t*>(p.C) + at;
+    if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
 // Part `slot` of a split tile: 128 x cap fp32 of this block's rows as [token / 4][row][4].
@@ -204,20 +240,8 @@ __device__ __forceinline__ float4* gx_slot(const GxParams& p, int slot, int rank
     return reinterpret_cast<float4*>(p.work) + ((size_t)(slot * 2 + rank) * (p.cap / 4) + c4) * 128 + row;
 }
 
-// acc[j] += v[j] s[j] for 16 columns, as pairs.
-__device__ __forceinline__ void gx_fma16(uint64_t (&acc)[8], const uint32_t (&r)[16], const float* s)
-{
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(s + 4 * j);  // one address per warp: a broadcast
-        acc[2 * j] = fma_f32x2(pair_f32(r[4 * j], r[4 * j + 1]), x.x, acc[2 * j]);
-        acc[2 * j + 1] = fma_f32x2(pair_f32(r[4 * j + 2], r[4 * j + 3]), x.y, acc[2 * j + 1]);
-    }
-}
-
 // The experts' rows and their running number of runs, in shared memory: off[e], cum[e].  Row numbers are clamped to
 // ascend within [0, T], so that no value of the caller's leads outside X or C.  By the first warp.
-template <bool F8>
 __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum, int lane)
 {
     if (!p.offsets) {
@@ -250,8 +274,7 @@ __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum,
     __syncwarp();
     int n = 0;
     for (int i = i0; i < i1 && i < p.E; ++i) {
-        const int a = F8 ? off[i] & ~3 : off[i];
-        n += off[i + 1] > off[i] ? group_runs(a, off[i + 1], p.cap) : 0;
+        n += group_runs(off[i], off[i + 1], p.cap);
     }
     int sum = n;
     for (int d = 1; d < 32; d *= 2) {
@@ -261,18 +284,16 @@ __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum,
     n = sum - n;
     for (int i = i0; i < i1; ++i) {
         cum[i] = n;
-        if (i < p.E) {
-            const int a = F8 ? off[i] & ~3 : off[i];
-            n += off[i + 1] > off[i] ? group_runs(a, off[i + 1], p.cap) : 0;
-        }
+        if (i < p.E) n += group_runs(off[i], off[i + 1], p.cap);
     }
 }
 
+// What each block's dynamic shared memory and registers hold follows from p and KIND; two blocks make a cluster.
 template <int KIND>
 __global__ void __launch_bounds__(kGxThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const GxParams p)
 {
-    constexpr bool F8 = KIND == 1;
+    constexpr bool F8 = KIND != kGx16, TOK = KIND == kGxF8Tokens;
     constexpr int kRowElems = 64;  // a 128-byte row of a stage in the maps' 16-bit elements
 #ifdef BW_EMULATE
     uint8_t* smem_raw = emu::cta_smem();
@@ -284,8 +305,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
     uint64_t* empty = full + kGxMaxStages;
     uint64_t* tfull = empty + kGxMaxStages;
-    uint64_t* tempty = tfull + 2;
-    uint64_t* sfull = tempty + 2;
+    uint64_t* tempty = tfull + kGxAccs;
+    uint64_t* sfull = tempty + kGxAccs;
     uint64_t* sempty = sfull + kGxScales;
     uint64_t* drain = sempty + kGxScales;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
@@ -300,7 +321,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
     const int S = p.stages;
-    const int tmem_cols = 2 * p.cap;  // a power of two, 64 .. 512
+    const int tmem_cols = p.accs * p.cap;  // a power of two, 256 or 512
 
     if (threadIdx.x == 0) {
         BW_TRACE_CLEAR();
@@ -312,7 +333,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < p.accs; ++i) {
             mbar_init(&tfull[i], 1);
             mbar_init(&tempty[i], 16);  // the epilogue warps of both blocks
         }
@@ -334,7 +355,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_relinquish_pair();
     }
     griddep_wait();  // what the kernel ahead wrote (the offsets, X, its scales, the counters) is visible from here on
-    if (warp == 4) gx_tables<F8>(p, off, cum, lane);
+    if (warp == 4) gx_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // barriers, tables and tensor memory of both blocks are there
@@ -344,9 +365,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     GroupWalk walk(s, c);
     GroupSeg sg;
     GxFind find;
-    // KIND 1 holds 128 sums in registers: the epilogue's 8 warps take registers from the other 4 (384 threads are launched
+    // kGxF8Tokens holds 128 sums in registers: the epilogue's 8 warps take registers from the other 4 (384 threads are launched
     // with 168 each: 128 x 72 + 256 x 216 <= 384 x 168)
-    if (F8 && warp < 4) reg_dec<kGxOtherRegs>();
+    if (TOK && warp < 4) reg_dec<kGxOtherRegs>();
 
     if (warp == 0) {
         // ---------------------------------------------------------- TMA producer
@@ -355,15 +376,23 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         uint32_t ph = 0;
         bool alive = true;
         while (alive && walk.next(s, sg)) {
-            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
-            const int boxes = (t.N / 2 + p.box - 1) / p.box;
+            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
+            const int boxes = TOK ? 1 : (t.N / 2 + p.box - 1) / p.box;
             const uint32_t bytes = 2u * (kGxXBytes + (uint32_t)(boxes * p.box) * 128u);
-            const int tok = t.t0 + rank * (t.N / 2);
-            // this block's weight rows: 128 in a row, or 64 gate and 64 up rows
-            const int w0 = p.glu == kGxPlain ? t.n * 256 + rank * 128
-                           : p.glu == kGxGluBlocks ? t.n * 256 + rank * 64
-                                                   : t.n * 128 + rank * 64;
-            const int w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
+            const int tok = t.t0 + rank * (TOK ? 128 : t.N / 2);
+            // this block's weight rows: 128 in a row, or 64 gate and 64 up rows (TOK: its half of the tile's columns; one block
+            // has the gate rows, the other the up rows)
+            int w0, w1 = 0;
+            if (TOK) {
+                w0 = p.glu == kGxPlain      ? t.n * 256 + rank * (t.N / 2)
+                     : p.glu == kGxGluBlocks ? t.n * 256 + rank * 128
+                                             : t.n * 128 + rank * (p.N / 2);
+            } else {
+                w0 = p.glu == kGxPlain      ? t.n * 256 + rank * 128
+                     : p.glu == kGxGluBlocks ? t.n * 256 + rank * 64
+                                             : t.n * 128 + rank * 64;
+                w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
+            }
             for (int kb = sg.k0; kb < sg.k1; ++kb) {
                 alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg);
                 if (!alive) break;
@@ -371,14 +400,17 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 const uint32_t bar = full0 + 8u * (uint32_t)stage;
                 if (elect_one()) {
                     if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-                    if (p.mn_major) {
+                    if (TOK) {
+                        tma_load_3d_pair(sx, &tmx, kb * kRowElems, tok, 0, bar);
+                        tma_load_3d_pair(sx + kGxXBytes, &tmw, kb * kRowElems, w0, t.e, bar);
+                    } else if (p.mn_major) {
                         tma_load_3d_pair(sx, &tmw, w0, kb * 64, t.e, bar);
                         tma_load_3d_pair(sx + 8192, &tmw, w0 + 64, kb * 64, t.e, bar);
                     } else {
                         tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
                         if (p.glu != kGxPlain) tma_load_3d_pair(sx + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
                     }
-                    for (int i = 0; i < boxes; ++i)
+                    for (int i = 0; !TOK && i < boxes; ++i)
                         tma_load_3d_pair(sx + kGxXBytes + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
                 }
                 ++issued;
@@ -410,7 +442,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             bool alive = true;
             GX_CLOCK(long long w_full = 0, w_acc = 0, n_kb = 0, t_at = 0);
             while (alive && walk.next(s, sg)) {
-                const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+                const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
                 const uint32_t idesc = p.idesc | idesc_n(t.N);
                 for (int kb = sg.k0; kb < sg.k1; ++kb) {
                     GX_CLOCK(t_at = clock64());
@@ -442,8 +474,10 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     }
                     __syncwarp();
                     if (last) {
-                        acc ^= 1;
-                        if (acc == 0) aph ^= 1u;
+                        if (++acc == p.accs) {
+                            acc = 0;
+                            aph ^= 1u;
+                        }
                     }
                     if (++stage == S) {
                         stage = 0;
@@ -467,7 +501,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         __syncwarp();
     } else if (warp >= 4) {
         // ---------------------------------------------------------- epilogue
-        if (F8) reg_inc<kGxEpiRegs>();
+        if (TOK) reg_inc<kGxEpiRegs>();
         const int ew = warp - 4, q = warp & 3, h = ew >> 2;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
@@ -479,157 +513,251 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         auto release = [&](int a) {
             tc_fence_before();
             __syncwarp();
-            if (alive && lane == 0) mbar_arrive_cluster(tempty0 + 8u * (uint32_t)a);
+            if (alive && lane == 0) mbar_arrive_remote_relaxed(tempty0 + 8u * (uint32_t)a);
+        };
+        auto next_acc = [&] {
+            if (++acc == p.accs) {
+                acc = 0;
+                aph ^= 1u;
+            }
         };
         while (walk.next(s, sg)) {
-            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
-            const int nc = t.N / 2, c0 = h * nc;  // this warp's columns
-            const int tb = t.t0 + c0;
-            const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
-            const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
-            if constexpr (F8) {
-                uint64_t sum[8][8];  // 128 columns as pairs
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
-                for (int kb = sg.k0;;) {
-                    if (alive)
-                        alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), seg) &&
-                                gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
-                    if (alive) {
-                        tc_fence_after();
-                        const float* sc = sc_base + si * 512 + c0;
-                        const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
-                        // the next 16 columns leave tensor memory while these are added
-                        uint32_t r[2][16];
-                        tmem_ld16(tm, r[0]);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (i * 16 >= nc) break;
-                            tmem_wait_ld();
-                            if (i < 7 && (i + 1) * 16 < nc) tmem_ld16(tm + (uint32_t)(i * 16 + 16), r[(i + 1) & 1]);
-                            gx_fma16(sum[i], r[i & 1], sc + i * 16);
-                        }
-                    }
-                    __syncwarp();  // every lane has read the scales
-                    if (alive && lane == 0) mbar_arrive(&sempty[si]);
-                    if (++si == kGxScales) {
-                        si = 0;
-                        sph ^= 1u;
-                    }
-                    if (++kb == sg.k1) break;
-                    release(acc);
-                    acc ^= 1;
-                    if (acc == 0) aph ^= 1u;
-                }
-                // the sums go back into the last accumulator, where the code below takes them for both kinds
-                const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (i * 16 >= nc) break;
-                    uint32_t r[16];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
-                    tmem_st16(tm + (uint32_t)(i * 16), r);
-                }
-                tmem_wait_st();
-            } else {
+            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
+            // This warp's columns, in runs of 16: half of the tile's.  TOK: the first or second 128, or with the activation
+            // 64 gate columns and their 64 up columns.
+            const int nc = t.N / 2, c0 = h * nc;
+            auto col = [&](int i) {
+                if (!TOK) return c0 + i * 16;
+                return p.glu == kGxPlain ? h * 128 + i * 16 : (i < 4 ? 0 : 64) + h * 64 + i * 16;
+            };
+            auto in_tile = [&](int i) { return TOK ? col(i) < t.N : i * 16 < nc; };
+            const uint32_t quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+            if constexpr (KIND == kGx16) {
                 if (alive)
                     alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
                 tc_fence_after();
+            } else {
+                constexpr int kRuns = TOK ? 8 : 4;
+                uint64_t sum[kRuns][8];  // 16 columns a run, as pairs
+#pragma unroll
+                for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
+                int kb = sg.k0;
+                if constexpr (TOK) {
+                    // this token's scales and its columns' (one or two blocks of 128 weight rows), two K-blocks ahead
+                    const int tok = t.t0 + rank * 128 + row;
+                    const float* xs = p.xs + (tok < t.t1 ? tok : t.t0);
+                    const int r0 = p.glu == kGxPlain ? 2 * t.n + h : p.glu == kGxGluBlocks ? 2 * t.n : t.n;
+                    const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : r0 + 1;
+                    const float* ws0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
+                    const float* ws1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
+                    struct Scale {
+                        float x, w0, w1;
+                    } ahead[2] = {};
+                    auto load = [&](int k, Scale& a) {
+                        if (k >= sg.k1) return;
+                        a.x = xs[k * p.xs_ld];
+                        a.w0 = ws0[k];
+                        if (p.glu != kGxPlain) a.w1 = ws1[k];
+                    };
+                    load(kb, ahead[0]);
+                    load(kb + 1, ahead[1]);
+                    // one K-block; false after the last
+                    auto block = [&](Scale& a) {
+                        const uint32_t s0 = __float_as_uint(a.x * a.w0), s1 = __float_as_uint(a.x * a.w1);
+                        const uint64_t p0 = pair_f32(s0, s0), p1 = p.glu != kGxPlain ? pair_f32(s1, s1) : p0;
+                        load(kb + 2, a);
+                        if (alive)
+                            alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                        if (alive) {
+                            tc_fence_after();
+                            const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
+#pragma unroll
+                            for (int i = 0; i < 8; i += 2) {  // 32 columns leave tensor memory at a time
+                                uint32_t r[2][16];
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    tmem_ld16(tm + (uint32_t)col(i + j), r[j]);  // (past the tile's: not used)
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k)
+                                        sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1,
+                                                                  sum[i + j][k]);
+                            }
+                        }
+                        if (++kb == sg.k1) return false;
+                        release(acc);
+                        next_acc();
+                        return true;
+                    };
+                    while (block(ahead[0]) && block(ahead[1])) {
+                    }
+                } else {
+                    for (;;) {
+                        if (alive)
+                            alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), seg) &&
+                                    gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                        if (alive) {
+                            tc_fence_after();
+                            const float* sc = sc_base + si * 512 + c0;
+                            const uint32_t tm = quarter + (uint32_t)(acc * p.cap + c0);
+                            uint32_t r[4][16];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (in_tile(i)) tmem_ld16(tm + (uint32_t)(i * 16), r[i]);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (in_tile(i)) {
+#pragma unroll
+                                    for (int k = 0; k < 8; k += 2) {
+                                        uint64_t s0, s1;  // one address per warp: a broadcast
+                                        ld_shared_2b64(sc + i * 16 + 2 * k, s0, s1);
+                                        sum[i][k] = fma_f32x2(pair_f32(r[i][2 * k], r[i][2 * k + 1]), s0, sum[i][k]);
+                                        sum[i][k + 1] = fma_f32x2(pair_f32(r[i][2 * k + 2], r[i][2 * k + 3]), s1, sum[i][k + 1]);
+                                    }
+                                }
+                        }
+                        __syncwarp();  // every lane has read the scales
+                        if (alive && lane == 0) mbar_arrive(&sempty[si]);
+                        if (++si == kGxScales) {
+                            si = 0;
+                            sph ^= 1u;
+                        }
+                        if (++kb == sg.k1) break;
+                        release(acc);
+                        next_acc();
+                    }
+                }
+                // the sums go back into the last accumulator, where the code below takes them for all kinds
+                const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
+#pragma unroll
+                for (int i = 0; i < kRuns; ++i)
+                    if (in_tile(i)) {
+                        uint32_t r[16];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
+                        tmem_st16(tm + (uint32_t)col(i), r);
+                    }
+                tmem_wait_st();
             }
-            const uint32_t tm = lanes + (uint32_t)(acc * p.cap);
+            const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
             // this segment's sum of 16 columns
             auto own = [&](int i, float(&v)[16]) {
                 uint32_t r[16];
-                tmem_ld16(tm + (uint32_t)(i * 16), r);
+                tmem_ld16(tm + (uint32_t)col(i), r);
                 tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
             };
-            if (sg.k0 == 0 && sg.k1 == s.kb) {
-#pragma unroll 1
-                for (int i = 0; i * 16 < nc; ++i) {
-                    float v[16];
-                    own(i, v);
-                    gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
-                }
-            } else {
+            bool done = true;  // this block has the tile's whole sum
+            int first = c, last = c;
+            if (sg.k0 != 0 || sg.k1 != s.kb) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
-                const int first = tile_first_part(s, sg.tile), last = tile_last_part(s, sg.tile);
-                const int nseg = last - first + 1;
+                first = tile_first_part(s, sg.tile);
+                last = tile_last_part(s, sg.tile);
                 int* counter = p.counters + sg.tile * 2 + rank;
                 named_bar_sync(1, kGxEpiThreads);  // the flag of an earlier tile has been read
-                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == nseg - 1 ? 1 : 0;
+                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
-                int go = *reduce_flag;
-                if (!go) {
+                done = *reduce_flag != 0;
+                if (!done) {
                     const int slot = part_slot(s, c, sg.tile);
 #pragma unroll 1
-                    for (int i = 0; i * 16 < nc; ++i) {
+                    for (int i = 0; i < 8 && in_tile(i); ++i) {
                         float v[16];
                         own(i, v);
                         if (alive) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                __stcg(gx_slot(p, slot, rank, row, c0 / 4 + i * 4 + j),
+                                __stcg(gx_slot(p, slot, rank, row, col(i) / 4 + j),
                                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
                         }
                     }
                     named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
                     if (threadIdx.x == kGxEpi0)
-                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == nseg - 1 ? 1 : 0;
+                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == last - first ? 1 : 0;
                     named_bar_sync(1, kGxEpiThreads);
-                    go = *reduce_flag;
+                    done = *reduce_flag != 0;
                 }
-                if (go) {
+            }
+            // the tile's sum of 16 columns
+            auto total = [&](int i, float(&v)[16]) {
+                if (first == last) {
+                    own(i, v);
+                    return;
+                }
+                float mine[16];
+                own(i, mine);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                for (int part = first; part <= last; ++part) {
+                    if (part == c) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] += mine[j];
+                        continue;
+                    }
+                    const int slot = part_slot(s, part, sg.tile);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 x = __ldcg(gx_slot(p, slot, rank, row, col(i) / 4 + j));
+                        v[4 * j] += x.x;
+                        v[4 * j + 1] += x.y;
+                        v[4 * j + 2] += x.z;
+                        v[4 * j + 3] += x.w;
+                    }
+                }
+            };
+            if (done) {
+                if constexpr (TOK) {
+                    const int tok = t.t0 + rank * 128 + row;
+                    const bool write = alive && tok < t.t1;
+                    const bool glu = p.glu != kGxPlain;
 #pragma unroll 1
-                    for (int i = 0; i * 16 < nc; ++i) {
-                        float v[16], mine[16];
-                        own(i, mine);
+                    for (int i = 0; i < (glu ? 4 : 8) && in_tile(i); ++i) {
+                        float v[16];
+                        total(i, v);
+                        if (glu) {
+                            float u[16];
+                            total(i + 4, u);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                        for (int part = first; part <= last; ++part) {
-                            if (part == c) {
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] += mine[j];
-                                continue;
-                            }
-                            const int slot = part_slot(s, part, sg.tile);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 x = __ldcg(gx_slot(p, slot, rank, row, c0 / 4 + i * 4 + j));
-                                v[4 * j] += x.x;
-                                v[4 * j + 1] += x.y;
-                                v[4 * j + 2] += x.z;
-                                v[4 * j + 3] += x.w;
-                            }
+                            for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * u[j];
                         }
+                        if (write) gx_store_row16(p, v, tok, t.n * (glu ? 128 : 256) + col(i));
+                    }
+                } else {
+                    const int tb = t.t0 + c0;
+                    const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
+#pragma unroll 1
+                    for (int i = 0; in_tile(i); ++i) {
+                        float v[16];
+                        total(i, v);
                         gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
                     }
                 }
             }
             release(acc);
-            acc ^= 1;
-            if (acc == 0) aph ^= 1u;
+            next_acc();
             ++seg;
         }
         if (threadIdx.x == kGxEpi0) BW_TRACE_AT(4);
-    } else if (F8) {
+    } else if (KIND == kGxF8Weights) {
         // ---------------------------------------------------------- scale products
         const int t00 = (warp - 2) * 128 + lane;  // this lane's first token of a tile
         int si = 0, seg = 0;
         uint32_t sph = 0;
         bool alive = true;
         while (alive && walk.next(s, sg)) {
-            const GxTile t = find.at<F8>(p, off, cum, sg.tile);
+            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
             // the scale blocks of this block's weight rows (gate and up: of each)
             const int r0 = p.glu == kGxGluHalves ? t.n : p.glu == kGxGluBlocks ? 2 * t.n : 2 * t.n + rank;
             const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : 2 * t.n + 1;
             const float* w0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
             const float* w1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
-            const int have = t.hi - t.t0;
+            const int have = t.t1 - t.t0;
             // loaded kGxAhead K-blocks ahead: a load takes as long as several K-blocks of MMAs
             float x[kGxAhead][4], a[kGxAhead], b[kGxAhead];
             auto load = [&](int kb, float(&x)[4], float& a, float& b) {

@@ -5,19 +5,26 @@
 
 namespace bw {
 
-// The most tokens of a tile for an average of `rows` per expert.  A tile's MMA is as wide as the tokens it has, so a large
-// cap costs little computing; a small one leaves shared memory for more stages of weights, which is what few tokens want.
-inline int gx_cap(int T, int E, bool grouped)
+// The form of a call and the most tokens of a tile, for an average of `rows` tokens per expert.  With the weights as M a
+// tile's MMA is as wide as the tokens it has, so a large cap costs little computing; a small one leaves shared memory for
+// more stages of weights, which is what few tokens want.
+struct GxForm {
+    int kind, cap;
+};
+inline GxForm gx_form(int T, int E, bool grouped, bool f8)
 {
     const long long rows = grouped ? ((long long)T + E - 1) / E : T;
+    if (f8 && rows > 128) return {kGxF8Tokens, 256};
     // (experts' numbers of rows spread around the average: twice it, so that most take one run)
     const long long want = grouped ? 2 * rows : rows;
-    return want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
+    const int cap = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 || f8 ? 128 : 256;
+    return {f8 ? kGxF8Weights : kGx16, cap};
 }
 
-// Everything of a call but its addresses.  cap 0: the rule's.
-inline GxParams gx_params(int E, int T, int N, int K, bool f8, bool bf16, bool mn_major, int glu, int out, int cap)
+// Everything of a call but its addresses.
+inline GxParams gx_params(int E, int T, int N, int K, GxForm form, bool bf16, bool mn_major, int glu, int out)
 {
+    const bool f8 = form.kind != kGx16, tokens = form.kind == kGxF8Tokens;
     GxParams p = {};
     p.E = E;
     p.T = T;
@@ -25,8 +32,10 @@ inline GxParams gx_params(int E, int T, int N, int K, bool f8, bool bf16, bool m
     p.Nout = glu == kGxPlain ? N : N / 2;
     p.nt = glu == kGxGluHalves ? (N / 2 + 127) / 128 : (N + 255) / 256;
     p.kblocks = f8 ? (K + 127) / 128 : (K + 63) / 64;
-    p.cap = cap;
-    p.box = p.cap == 32 ? 16 : 32;
+    p.cap = form.cap;
+    p.box = tokens ? 128 : p.cap == 32 ? 16 : 32;
+    p.wbox = glu == kGxPlain || tokens ? 128 : 64;
+    p.accs = 512 / p.cap < kGxAccs ? 512 / p.cap : kGxAccs;
     p.stage_bytes = kGxXBytes + p.cap / 2 * 128;
     const int fixed = gx_smem(0, E).bytes + 1024;
     p.stages = (BW_SMEM_LIMIT - fixed) / p.stage_bytes;
@@ -56,7 +65,7 @@ inline GxMaps gx_maps(const GxParams& p, int K, long long ldx, bool f8)
         const uint64_t w[6] = {n, k, e, n, n * k, 64};
         for (int i = 0; i < 6; ++i) m.w[i] = w[i];
     } else {
-        const uint64_t w[6] = {k, n, e, k, n * k, p.glu == kGxPlain ? 128u : 64u};
+        const uint64_t w[6] = {k, n, e, k, n * k, (uint64_t)p.wbox};
         for (int i = 0; i < 6; ++i) m.w[i] = w[i];
     }
     const uint64_t x[6] = {k, (uint64_t)p.T, 1, ld, ld * (uint64_t)p.T, (uint64_t)p.box};

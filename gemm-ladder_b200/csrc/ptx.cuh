@@ -83,8 +83,24 @@ __device__ __forceinline__ void record_timeout(volatile int* abort_flag, uint32_
 }
 
 // Spins on (bar, parity) until the phase completes, the block's abort flag rises, or `limit_ns` pass. On a timeout it
-// records `where` and raises the abort flag; returns false on timeout or abort.  (wait_spin in place: for kernels that move
-// registers between warpgroups, which may not call functions.)
+// records `where` and raises the abort flag; returns false on timeout or abort.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
+                                       uint32_t where, int seg)
+{
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 31u) == 0) {
+            if (*abort_flag) return false;
+            if (globaltimer_ns() - t0 > limit_ns) {
+                record_timeout(abort_flag, where, seg);
+                return false;
+            }
+        }
+    }
+}
+
+// The same in place, for kernels that move registers between warpgroups (they may not call functions).
 __device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
                                           uint32_t where, int seg)
 {
@@ -99,11 +115,6 @@ __device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, volatil
             }
         }
     }
-}
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
-                                       uint32_t where, int seg)
-{
-    return wait_spin(bar, parity, abort_flag, limit_ns, where, seg);
 }
 
 __device__ __forceinline__ bool wait_bounded(uint64_t* barp, uint32_t parity, volatile int* abort_flag,
@@ -262,6 +273,19 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t dst, float v)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// The same without a fence, which would wait for the thread's loads and stores in flight (with release at cluster scope 1000
+// cycles and more beside an epilogue's stores, at block scope as long as a load takes).  For an arrival that hands on tensor
+// memory that was read: the loads from it have completed (tmem_wait_ld) and tc_fence_before orders them.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// With release at block scope: hands on this block's shared memory to the async proxy (fence_proxy_async_shared ahead of it).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // 16 bytes into another block's shared memory (`dst`, a shared::cluster address), counted as transaction bytes on
@@ -462,6 +486,12 @@ template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ------------------------------------------------------------------ shared memory by its own address space
+__device__ __forceinline__ void ld_shared_2b64(const void* p, uint64_t& a, uint64_t& b)
+{
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(smem_u32(p)) : "memory");
+}
 
 // ------------------------------------------------------------------ two fp32 operations at once
 // A pair of floats in a 64-bit register: (a.lo b.lo + c.lo, a.hi b.hi + c.hi), each rounded once.

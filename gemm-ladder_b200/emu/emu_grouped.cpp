@@ -109,7 +109,7 @@ EMU_API int bw_emu_grouped(const void* X, long long ldx, const float* xs, long l
 {
     using namespace bw;
     begin();
-    GxParams p = gx_params(E, T, N, K, kind == 1, bf16, mn_major, glu, out, cap);
+    GxParams p = gx_params(E, T, N, K, GxForm{kind, cap}, bf16, mn_major, glu, out);
     if (stages && stages < p.stages) {
         p.stages = stages;
         p.ring_bytes = stages * p.stage_bytes;
@@ -120,14 +120,16 @@ EMU_API int bw_emu_grouped(const void* X, long long ldx, const float* xs, long l
     p.work = work.data(), p.counters = counters.data();
     p.wait_ns = emu::g_wait_ns;
     CUtensorMap mw, mx;
-    const GxMaps m = gx_maps(p, K, ldx, kind == 1);
+    const GxMaps m = gx_maps(p, K, ldx, kind != kGx16);
     map3(&mw, W, m.w[0], m.w[1], m.w[2], m.w[3], m.w[4], (uint32_t)m.w[5]);
     map3(&mx, X, m.x[0], m.x[1], m.x[2], m.x[3], m.x[4], (uint32_t)m.x[5]);
     launch_pairs(pairs, gx_smem(p.ring_bytes, p.E).bytes, [&] {
-        if (kind == 1)
-            grouped_kernel<1>(mw, mx, p);
+        if (kind == kGxF8Weights)
+            grouped_kernel<kGxF8Weights>(mw, mx, p);
+        else if (kind == kGxF8Tokens)
+            grouped_kernel<kGxF8Tokens>(mw, mx, p);
         else
-            grouped_kernel<0>(mw, mx, p);
+            grouped_kernel<kGx16>(mw, mx, p);
     });
     (void)dirty;
     end(status, findings, finding, len);

@@ -197,6 +197,8 @@ inline void mbar_arrive_cluster(uint32_t cluster_addr)
     emu::met(cluster_addr, "an arrival");
     emu::mb_arrive(emu::cta_of(cluster_addr), emu::off_of(cluster_addr), 0);
 }
+inline void mbar_arrive_remote(uint32_t cluster_addr) { mbar_arrive_cluster(cluster_addr); }
+inline void mbar_arrive_remote_relaxed(uint32_t cluster_addr) { mbar_arrive_cluster(cluster_addr); }
 // st.async: the 16 bytes land in the other block later (queued to this block's TMA engine, standing for the path
 // between the blocks), then complete on that block's barrier.
 inline void st_async_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t bar)
@@ -293,6 +295,12 @@ inline void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) { emu::tmem_ld(taddr, r
 inline void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) { emu::tmem_ld(taddr, r); }
 inline void tmem_wait_ld() {}
 inline void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) { emu::tmem_st(taddr, r); }
+inline void ld_shared_2b64(const void* p, uint64_t& a, uint64_t& b)
+{
+    if (emu::offset_of(p) % 16) emu::finding("a 16-byte load from shared memory at offset %u", emu::offset_of(p));
+    std::memcpy(&a, p, 8);
+    std::memcpy(&b, static_cast<const uint8_t*>(p) + 8, 8);
+}
 inline void tmem_wait_st() {}
 
 inline bool elect_one() { return (emu::t_tid & 31) == 0; }

@@ -29,6 +29,8 @@ vp, i32, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
 
 def emulate(L, X, W, off, N, pairs, xs=None, ws=None, mn=False, glu=0, out=None, cap=32, stages=0):
+    """The kernel's form by cap: 8-bit operands with 256 tokens a tile have the tokens as the MMA's M."""
+    kind = 0 if xs is None else 2 if cap == 256 else 1
     T, K = X.shape
     E = 1 if off is None else off.numel() - 1
     out = X.dtype if out is None else out
@@ -36,7 +38,7 @@ def emulate(L, X, W, off, N, pairs, xs=None, ws=None, mn=False, glu=0, out=None,
     st, dirty, nf, msg = (ctypes.c_uint * 4)(), i32(), i32(), ctypes.create_string_buffer(512)
     ptr = lambda t: vp(t.data_ptr()) if t is not None else None
     L.bw_emu_grouped(ptr(X), ll(X.stride(0)), ptr(xs), ll(xs.stride(1) if xs is not None else 0), ptr(W), ptr(ws), ptr(off),
-                     ptr(C), E, T, N, K, pairs, int(xs is not None), int(X.dtype == torch.bfloat16), int(mn), glu,
+                     ptr(C), E, T, N, K, pairs, kind, int(X.dtype == torch.bfloat16), int(mn), glu,
                      OUT[out], cap, stages, st, ctypes.byref(dirty), ctypes.byref(nf), msg, 512)
     assert nf.value == 0, msg.value.decode()
     return C, list(st)
@@ -107,7 +109,12 @@ CASES8 = [  # counts (None offsets: one), N, K, pairs, out, activation, cap
     ([5, 0, 38, 1], 264, 400, 2, torch.float16, 0, 32, True),
     ([66, 3], 512, 160, 3, torch.bfloat16, 2, 64, True),
     ([18], 512, 1040, 3, torch.bfloat16, 1, 32, False),                 # split tiles with the activation
-    ([200], 256, 144, 1, torch.float16, 0, 256, False),
+    ([100], 256, 144, 1, torch.float16, 0, 128, False),
+    ([200], 256, 144, 1, torch.float16, 0, 256, False),                 # the tokens as the MMA's M from here on
+    ([130, 0, 300], 328, 400, 2, torch.float32, 0, 256, True),
+    ([5], 264, 1168, 3, torch.bfloat16, 0, 256, False),                 # split tiles
+    ([290], 512, 272, 2, torch.bfloat16, 1, 256, False),
+    ([3, 140], 512, 400, 3, torch.float16, 2, 256, True),
 ]
 
 
