@@ -68,7 +68,7 @@ int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CU
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs));
     cfg.blockDim = dim3(kGxThreads);
-    cfg.dynamicSmemBytes = (size_t)(1024 + gx_smem(p.ring_bytes, p.E).bytes);
+    cfg.dynamicSmemBytes = (size_t)(1024 + gx_smem(KIND, p.ring_bytes, p.E).bytes);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -31,12 +31,13 @@ struct DwParams {
 };
 
 struct DwSmem {
-    int bars, misc, tables, bytes;
+    int buf, bars, misc, tables, bytes;
 };
 __host__ __device__ inline DwSmem dw_smem(int ring_bytes, int E)
 {
     DwSmem m;
-    m.bars = ring_bytes;
+    m.buf = ring_bytes;
+    m.bars = m.buf + 8 * kGxLineBytes;
     m.misc = m.bars + (3 * kDwMaxStages + 5) * 8;
     m.misc = (m.misc + 15) / 16 * 16;
     m.tables = m.misc + 64;
@@ -71,32 +72,6 @@ __device__ __forceinline__ void dw_tables(const DwParams& p, int* off, int* cum,
     }
 }
 
-// 16 columns of one row of dW.
-__device__ __forceinline__ void dw_store16(const DwParams& p, const float (&v)[16], size_t at, int left)
-{
-    if (p.out == 2) {
-        float* d = static_cast<float*>(p.dW) + at;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (4 * j < left) *reinterpret_cast<float4*>(d + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        return;
-    }
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        if (p.out == 1) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&x);
-        } else {
-            const __half2 x = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&x);
-        }
-    }
-    uint16_t* d = static_cast<uint16_t*>(p.dW) + at;
-    if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-}
-
 __global__ void __launch_bounds__(kGxThreads, 1)
     grouped_dw_kernel(const __grid_constant__ CUtensorMap tmy, const __grid_constant__ CUtensorMap tmx, const DwParams p)
 {
@@ -119,7 +94,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     int* off = reinterpret_cast<int*>(smem + L.tables);
     int* cum = off + p.E + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
@@ -170,36 +145,35 @@ __global__ void __launch_bounds__(kGxThreads, 1)
 
     if (warp == 0) {
         // ---------------------------------------------------------- TMA producer
-        if (lane == 0) {
-            int stage = 0, issued = 0, seg = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            while (ok && walk.next(s, off, cum, sg)) {
-                int n0, k0, width;
-                place(n0, k0, width);
-                const int t0 = off[sg.e], rows = off[sg.e + 1] - t0;
-                const int boxes = (width / 2 + 63) / 64;
-                for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
-                    if (!wait_bounded(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t* sy = smem + stage * kDwStageBytes;
-                    uint8_t* sx = sy + 16384;
+        int stage = 0, issued = 0, seg = 0;
+        uint32_t ph = 0;
+        bool alive = true;
+        while (alive && walk.next(s, off, cum, sg)) {
+            int n0, k0, width;
+            place(n0, k0, width);
+            const int t0 = off[sg.e], rows = off[sg.e + 1] - t0;
+            const int boxes = (width / 2 + 63) / 64;
+            for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg);
+                if (!alive) break;
+                uint8_t* sy = smem + stage * kDwStageBytes;
+                const int t = t0 + kb * 64, y = n0 + rank * 128, x = k0 + rank * (width / 2);
+                if (elect_one()) {
                     mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 + boxes) * 8192u);
-                    const int t = t0 + kb * 64;
-                    tma_load_3d(sy, &tmy, n0 + rank * 128, t, 0, &full[stage]);
-                    tma_load_3d(sy + 8192, &tmy, n0 + rank * 128 + 64, t, 0, &full[stage]);
-                    for (int i = 0; i < boxes; ++i)
-                        tma_load_3d(sx + i * 8192, &tmx, k0 + rank * (width / 2) + 64 * i, t, 0, &full[stage]);
-                    ++issued;
-                    if (++stage == S) {
-                        stage = 0;
-                        ph ^= 1u;
-                    }
+                    tma_load_3d(sy, &tmy, y, t, 0, &full[stage]);
+                    tma_load_3d(sy + 8192, &tmy, y + 64, t, 0, &full[stage]);
+                    tma_load_3d(sy + 16384, &tmx, x, t, 0, &full[stage]);
+                    if (boxes > 1) tma_load_3d(sy + 24576, &tmx, x + 64, t, 0, &full[stage]);
                 }
-                ++seg;
+                ++issued;
+                if (++stage == S) {
+                    stage = 0;
+                    ph ^= 1u;
+                }
             }
+            ++seg;
+        }
+        if (lane == 0) {
             const int n = issued < S ? issued : S;
             for (int i = 1; i <= n; ++i) {
                 const int q = issued - i;
@@ -208,53 +182,59 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA issuer
-        if (lane == 0 && leader) {
+        if (leader) {
+            const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
+            const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
+            const uint64_t dy = desc_mnmajor(smem_u32(smem), 0), dx = desc_mnmajor(smem_u32(smem) + 16384u, 0);
             int stage = 0, acc = 0, seg = 0;
             uint32_t ph = 0, aph = 0;
-            bool ok = true;
-            while (ok && walk.next(s, off, cum, sg)) {
+            bool alive = true;
+            while (alive && walk.next(s, off, cum, sg)) {
                 int n0, k0, width;
                 place(n0, k0, width);
                 const int rows = off[sg.e + 1] - off[sg.e];
-                if (rows > 0) {
-                    if (!wait_bounded(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg)) break;
-                    const uint32_t idesc = p.idesc | idesc_n(width);
-                    const uint32_t d = tmem_base + (uint32_t)(acc * 256);
-                    for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                        if (!wait_bounded(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t sy = smem_u32(smem + stage * kDwStageBytes), sx = sy + 16384u;
-                        const int here = rows - kb * 64 < 64 ? rows - kb * 64 : 64;
+                ++seg;
+                if (rows == 0) continue;
+                alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg);
+                const uint32_t idesc = p.idesc | idesc_n(width);
+                const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+                for (int kb = sg.k0; alive && kb < sg.k1; ++kb) {
+                    alive = gx_warp_wait(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg);
+                    if (!alive) break;
+                    tc_fence_after();
+                    const uint64_t ad = dy + (uint64_t)((uint32_t)stage * (kDwStageBytes >> 4));
+                    const uint64_t bd = dx + (uint64_t)((uint32_t)stage * (kDwStageBytes >> 4));
+                    const int here = rows - kb * 64;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (k * 16 < here)
-                                mma_f16_pair(d, desc_mnmajor(sy, k), desc_mnmajor(sx, k), idesc,
-                                             kb > sg.k0 || k > 0 ? 1u : 0u);
-                        mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 0));
-                        mma_commit_pair(mapa_shared(smem_u32(&empty[stage]), 1));
-                        if (++stage == S) {
-                            stage = 0;
-                            ph ^= 1u;
+                            if (k * 16 < here) mma_f16_pair(d, ad + 128 * k, bd + 128 * k, idesc, kb > sg.k0 || k > 0 ? 1u : 0u);
+                        mma_commit_pair(empty0[0] + 8u * (uint32_t)stage);
+                        mma_commit_pair(empty0[1] + 8u * (uint32_t)stage);
+                        if (kb + 1 == sg.k1) {
+                            mma_commit_pair(tfull0[0] + 8u * (uint32_t)acc);
+                            mma_commit_pair(tfull0[1] + 8u * (uint32_t)acc);
                         }
                     }
-                    if (!ok) break;
-                    mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 0));
-                    mma_commit_pair(mapa_shared(smem_u32(&tfull[acc]), 1));
-                    acc ^= 1;
-                    if (acc == 0) aph ^= 1u;
+                    __syncwarp();
+                    if (++stage == S) {
+                        stage = 0;
+                        ph ^= 1u;
+                    }
                 }
-                ++seg;
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
             }
-            mma_commit_pair(mapa_shared(smem_u32(drain), 0));
-            wait_drain(drain, 0, p.wait_ns);
+            if (elect_one()) {
+                mma_commit_pair(mapa_shared(smem_u32(drain), 0));
+                wait_drain(drain, 0, p.wait_ns);
+            }
         }
         __syncwarp();
     } else if (warp >= 4) {
         // ---------------------------------------------------------- epilogue
-        const int ew = warp - 4, q = warp & 3, h = ew >> 2;
+        const int q = warp & 3, h = (warp - 4) >> 2, per = gx_per_line(p.out);
+        uint8_t* line = smem + L.buf + (warp - 4) * kGxLineBytes;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
         int acc = 0, seg = 0;
@@ -265,77 +245,81 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             place(n0, k0, width);
             const int rows = off[sg.e + 1] - off[sg.e];
             const int nc = width / 2, c0 = h * nc;
-            const int n = n0 + rank * 128 + row, k = k0 + c0;
-            const size_t at = ((size_t)sg.e * p.N + n) * p.K + k;
-            const bool mine = alive && n < p.N;
+            const int r0 = n0 + rank * 128 + q * 32, k = k0 + c0;
+            uint8_t* base = static_cast<uint8_t*>(p.dW) + (size_t)sg.e * p.N * p.K * (p.out == 2 ? 4 : 2);
+            // as whole lines; past this warp's columns (k + nc) another warp or tile writes
+            const int k1 = k + nc < p.K ? k + nc : p.K;
+            auto store = [&](int i, const float(&v)[16]) {
+                const int at = i / 16 % per;
+                gx_put16(p.out, line, at, lane, v);
+                if (at == per - 1 || i + 16 >= nc)
+                    gx_flush(p.out, line, base, (size_t)p.K, r0, alive ? p.N : 0, k + i - at * 16, k1, lane);
+            };
             if (rows == 0) {
                 float z[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) z[j] = 0.f;
-                for (int i = 0; mine && i < nc; i += 16) dw_store16(p, z, at + i, p.K - k - i);
+#pragma unroll 1
+                for (int i = 0; i < nc; i += 16) store(i, z);
                 ++seg;
                 continue;
             }
             if (alive) alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
             tc_fence_after();
-            const bool write = alive && n < p.N;
             const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256 + c0);
-            auto own = [&](int i, float(&v)[16]) {
-                uint32_t r[16];
-                tmem_ld16(tm + (uint32_t)i, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+            auto slot_at = [&](int part, int i) {
+                return reinterpret_cast<float4*>(p.work) +
+                       ((size_t)(dw_slot(s, part, sg.u0) * 2 + rank) * 64 + (c0 + i) / 4) * 128 + row;
             };
-            if (sg.k0 == 0 && sg.k1 == sg.kb) {
-#pragma unroll 1
-                for (int i = 0; i < nc; i += 16) {
-                    float v[16];
-                    own(i, v);
-                    if (write) dw_store16(p, v, at + i, p.K - k - i);
-                }
-            } else {
+            bool done = true;  // this block has the tile's whole sum
+            int first = c, last = c;
+            if (sg.k0 != 0 || sg.k1 != sg.kb) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
-                const int first = dw_part_of(s, sg.u0), last = dw_part_of(s, sg.u0 + sg.kb - 1);
-                const int nseg = last - first + 1;
+                first = dw_part_of(s, sg.u0);
+                last = dw_part_of(s, sg.u0 + sg.kb - 1);
                 int* counter = p.counters + sg.tile * 2 + rank;
-                auto slot_at = [&](int part, int i) {
-                    return reinterpret_cast<float4*>(p.work) +
-                           ((size_t)(dw_slot(s, part, sg.u0) * 2 + rank) * 64 + (c0 + i) / 4) * 128 + row;
-                };
                 named_bar_sync(1, kGxEpiThreads);
-                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == nseg - 1 ? 1 : 0;
+                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
-                int go = *reduce_flag;
-                if (!go) {
+                done = *reduce_flag != 0;
+                if (!done) {
 #pragma unroll 1
                     for (int i = 0; i < nc; i += 16) {
-                        float v[16];
-                        own(i, v);
+                        uint32_t r[16];
+                        tmem_ld16(tm + (uint32_t)i, r);
+                        tmem_wait_ld();
                         if (alive) {
                             float4* to = slot_at(c, i);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                __stcg(to + j * 128, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                                __stcg(to + j * 128, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                                 __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
                         }
                     }
                     named_bar_sync(1, kGxEpiThreads);
                     if (threadIdx.x == kGxEpi0)
-                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == nseg - 1 ? 1 : 0;
+                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == last - first ? 1 : 0;
                     named_bar_sync(1, kGxEpiThreads);
-                    go = *reduce_flag;
+                    done = *reduce_flag != 0;
                 }
-                if (go) {
+            }
+            if (done) {
 #pragma unroll 1
-                    for (int i = 0; i < nc; i += 16) {
-                        float v[16], o[16];
-                        own(i, o);
+                for (int i = 0; i < nc; i += 16) {
+                    uint32_t r[16];
+                    float v[16];
+                    tmem_ld16(tm + (uint32_t)i, r);
+                    tmem_wait_ld();
+                    if (first == last) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                    } else {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) v[j] = 0.f;
                         for (int part = first; part <= last; ++part) {
                             if (part == c) {
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] += o[j];
+                                for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
                                 continue;
                             }
                             const float4* from = slot_at(part, i);
@@ -348,8 +332,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                                 v[4 * j + 3] += x.w;
                             }
                         }
-                        if (write) dw_store16(p, v, at + i, p.K - k - i);
                     }
+                    store(i, v);
                 }
             }
             tc_fence_before();

@@ -37,7 +37,7 @@ inline GxParams gx_params(int E, int T, int N, int K, GxForm form, bool bf16, bo
     p.wbox = glu == kGxPlain || tokens ? 128 : 64;
     p.accs = 512 / p.cap < kGxAccs ? 512 / p.cap : kGxAccs;
     p.stage_bytes = kGxXBytes + p.cap / 2 * 128;
-    const int fixed = gx_smem(0, E).bytes + 1024;
+    const int fixed = gx_smem(form.kind, 0, E).bytes + 1024;
     p.stages = (BW_SMEM_LIMIT - fixed) / p.stage_bytes;
     if (p.stages > kGxMaxStages) p.stages = kGxMaxStages;
     p.ring_bytes = p.stages * p.stage_bytes;
@@ -84,7 +84,8 @@ inline DwParams dw_params(int E, int T, int N, int K, bool bf16, int out)
     p.tn = (N + 255) / 256;
     p.tk = (K + 255) / 256;
     p.width = ((K + p.tk - 1) / p.tk + 31) / 32 * 32;
-    p.stages = kDwMaxStages;
+    p.stages = (BW_SMEM_LIMIT - 1024 - dw_smem(0, E).bytes) / kDwStageBytes;
+    if (p.stages > kDwMaxStages) p.stages = kDwMaxStages;
     p.ring_bytes = p.stages * kDwStageBytes;
     p.out = out;
     p.idesc = idesc_16_f32_m(256, bf16, true, true);

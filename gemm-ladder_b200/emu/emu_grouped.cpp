@@ -123,7 +123,7 @@ EMU_API int bw_emu_grouped(const void* X, long long ldx, const float* xs, long l
     const GxMaps m = gx_maps(p, K, ldx, kind != kGx16);
     map3(&mw, W, m.w[0], m.w[1], m.w[2], m.w[3], m.w[4], (uint32_t)m.w[5]);
     map3(&mx, X, m.x[0], m.x[1], m.x[2], m.x[3], m.x[4], (uint32_t)m.x[5]);
-    launch_pairs(pairs, gx_smem(p.ring_bytes, p.E).bytes, [&] {
+    launch_pairs(pairs, gx_smem(kind, p.ring_bytes, p.E).bytes, [&] {
         if (kind == kGxF8Weights)
             grouped_kernel<kGxF8Weights>(mw, mx, p);
         else if (kind == kGxF8Tokens)
