@@ -48,7 +48,7 @@ GxWork gx_work(int T, int K, int cap, int pairs, bool linear)
     w.parts = at;
     at = up256(at + gx_work_bytes(pairs, cap));
     w.counters = at;
-    w.n_counters = 2 * pairs;
+    w.n_counters = 2 * pairs + 1;
     w.bytes = up256(at + (size_t)w.n_counters * sizeof(int));
     return w;
 }
@@ -90,6 +90,7 @@ int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m,
 {
     p.work = reinterpret_cast<float*>(work + w.parts);
     p.counters = reinterpret_cast<int*>(work + w.counters);
+    p.next = p.counters + 2 * pairs;
     p.wait_ns = g_wait_ns;
     if (!zeroed) {
         cudaError_t e = cudaMemsetAsync(p.counters, 0, (size_t)w.n_counters * sizeof(int), st);
@@ -179,6 +180,7 @@ int gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx,
     p.dW = dW;
     p.work = static_cast<float*>(work);
     p.counters = reinterpret_cast<int*>(static_cast<uint8_t*>(work) + at);
+    p.next = p.counters + dw_counters(p, pairs) - 1;
     p.wait_ns = g_wait_ns;
     e = cudaMemsetAsync(p.counters, 0, (size_t)dw_counters(p, pairs) * sizeof(int), st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync (counters)");

@@ -7,7 +7,7 @@
 // the rows after them are another expert's (perhaps not finite), so they are overwritten with zeros up to the next 16 (an
 // MMA's depth) between the load and the MMAs.  For that each block's loads complete on its own barrier; its warp 2 waits
 // there, clears what has to be cleared and arrives on the leader's barrier, where the MMA issuer waits for both blocks.
-// Roles otherwise as in grouped_kernel.cuh; a TMEM lane is a row of dW, a column a column.
+// Warp 3 plans; roles otherwise as in grouped_kernel.cuh; a TMEM lane is a row of dW, a column a column.
 #pragma once
 #include "grouped_kernel.cuh"
 
@@ -27,6 +27,7 @@ struct DwParams {
     void* dW;        // E x N x K
     float* work;     // parts of split tiles
     int* counters;   // two per split tile, zero at the start of a call
+    int* next;       // the whole tiles given out, zero at the start of a call
     unsigned long long wait_ns;
 };
 
@@ -38,12 +39,24 @@ __host__ __device__ inline DwSmem dw_smem(int ring_bytes, int E)
     DwSmem m;
     m.buf = ring_bytes;
     m.bars = m.buf + 8 * kGxLineBytes;
-    m.misc = m.bars + (3 * kDwMaxStages + 5) * 8;
+    m.misc = m.bars + (3 * kDwMaxStages + 5 + 2 * kGxQueue + 2 * kGxDescs) * 8;
     m.misc = (m.misc + 15) / 16 * 16;
-    m.tables = m.misc + 64;
+    m.tables = m.misc + 64 + kGxDescs * 64;
     m.bytes = m.tables + 2 * (E + 1) * 4;
     return m;
 }
+
+// A segment: a tile, its K-blocks, and, of a split tile, the parts' numbers.
+struct DwDesc {
+    int e, rows;      // expert (-1: no segment left), its rows
+    int t0;           // its first row
+    int n0, c0;       // the tile's first row and column of dW_e
+    int width;        // its columns: the MMA's N
+    int k0, k1;       // K-blocks
+    int tile, first, last;
+    long long u0;     // the tile's first unit (split tiles)
+};
+static_assert(sizeof(DwDesc) <= 64, "room for the descriptors");
 
 // Row numbers as gx_tables has them, and the running number of K-blocks of one tile of each expert.  By one warp.
 __device__ __forceinline__ void dw_tables(const DwParams& p, int* off, int* cum, int lane)
@@ -88,9 +101,16 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     uint64_t* tfull = empty + kDwMaxStages;
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
+    uint64_t* qfull = drain + 1;
+    uint64_t* qempty = qfull + kGxQueue;
+    uint64_t* dfull = qempty + kGxQueue;
+    uint64_t* dempty = dfull + kGxDescs;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* reduce_flag = abort_flag + 1;
+    volatile int* epi_go = abort_flag + 2;      // two, alternating
+    volatile int* queue_tile = abort_flag + 4;  // kGxQueue entries
+    DwDesc* descs = reinterpret_cast<DwDesc*>(smem + L.misc + 64);
     int* off = reinterpret_cast<int*>(smem + L.tables);
     int* cum = off + p.E + 1;
 
@@ -112,6 +132,14 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&tempty[i], 16);
         }
         mbar_init(drain, 1);
+        for (int i = 0; i < kGxQueue; ++i) {
+            mbar_init(&qfull[i], 1);
+            mbar_init(&qempty[i], 2);  // both blocks' plans
+        }
+        for (int i = 0; i < kGxDescs; ++i) {
+            mbar_init(&dfull[i], 1);
+            mbar_init(&dempty[i], 10u + (leader ? 1u : 0u));  // producer, warp 2, epilogue, MMA issuer
+        }
         *abort_flag = 0;
         *reduce_flag = 0;
         fence_barrier_init();
@@ -131,33 +159,33 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
-    DwWalk walk(s, c);
-    DwSeg sg = {};
-    // a tile's place and columns: neighbouring tiles share dY's columns
-    auto place = [&](int& n0, int& k0, int& width) {
-        const int i = sg.tile - sg.e * s.per;
-        n0 = i / p.tk * 256;
-        k0 = i % p.tk * p.width;
-        const int left = p.K - k0;
-        width = left < p.width ? (left + 31) / 32 * 32 : p.width;
+    int asked = 0;
+    // a warp's next descriptor (false: none left, or the wait gave up)
+    auto next = [&](DwDesc& d, bool& alive) {
+        const int at = asked % kGxDescs;
+        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, p.wait_ns,
+                                      site(3, 10, (uint32_t)at), asked);
+        if (!alive) return false;
+        d = descs[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dempty[at]);
+        ++asked;
+        return d.e >= 0;
     };
 
     if (warp == 0) {
         // ---------------------------------------------------------- TMA producer
-        int stage = 0, issued = 0, seg = 0;
+        int stage = 0, issued = 0;
         uint32_t ph = 0;
         bool alive = true;
-        while (alive && walk.next(s, off, cum, sg)) {
-            int n0, k0, width;
-            place(n0, k0, width);
-            const int t0 = off[sg.e], rows = off[sg.e + 1] - t0;
-            const int boxes = (width / 2 + 63) / 64;
-            for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
-                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg);
+        DwDesc d;
+        while (next(d, alive)) {
+            const int boxes = (d.width / 2 + 63) / 64;
+            for (int kb = d.k0; d.rows > 0 && kb < d.k1; ++kb) {
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), asked);
                 if (!alive) break;
                 uint8_t* sy = smem + stage * kDwStageBytes;
-                const int t = t0 + kb * 64, y = n0 + rank * 128, x = k0 + rank * (width / 2);
+                const int t = d.t0 + kb * 64, y = d.n0 + rank * 128, x = d.c0 + rank * (d.width / 2);
                 if (elect_one()) {
                     mbar_arrive_expect_tx(&full[stage], (uint32_t)(2 + boxes) * 8192u);
                     tma_load_3d(sy, &tmy, y, t, 0, &full[stage]);
@@ -171,7 +199,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     ph ^= 1u;
                 }
             }
-            ++seg;
         }
         if (lane == 0) {
             const int n = issued < S ? issued : S;
@@ -186,32 +213,29 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
             const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
             const uint64_t dy = desc_mnmajor(smem_u32(smem), 0), dx = desc_mnmajor(smem_u32(smem) + 16384u, 0);
-            int stage = 0, acc = 0, seg = 0;
+            int stage = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool alive = true;
-            while (alive && walk.next(s, off, cum, sg)) {
-                int n0, k0, width;
-                place(n0, k0, width);
-                const int rows = off[sg.e + 1] - off[sg.e];
-                ++seg;
-                if (rows == 0) continue;
-                alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg);
-                const uint32_t idesc = p.idesc | idesc_n(width);
+            DwDesc t;
+            while (next(t, alive)) {
+                if (t.rows == 0) continue;
+                alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), asked);
+                const uint32_t idesc = p.idesc | idesc_n(t.width);
                 const uint32_t d = tmem_base + (uint32_t)(acc * 256);
-                for (int kb = sg.k0; alive && kb < sg.k1; ++kb) {
-                    alive = gx_warp_wait(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg);
+                for (int kb = t.k0; alive && kb < t.k1; ++kb) {
+                    alive = gx_warp_wait(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), asked);
                     if (!alive) break;
                     tc_fence_after();
                     const uint64_t ad = dy + (uint64_t)((uint32_t)stage * (kDwStageBytes >> 4));
                     const uint64_t bd = dx + (uint64_t)((uint32_t)stage * (kDwStageBytes >> 4));
-                    const int here = rows - kb * 64;
+                    const int here = t.rows - kb * 64;
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (k * 16 < here) mma_f16_pair(d, ad + 128 * k, bd + 128 * k, idesc, kb > sg.k0 || k > 0 ? 1u : 0u);
+                            if (k * 16 < here) mma_f16_pair(d, ad + 128 * k, bd + 128 * k, idesc, kb > t.k0 || k > 0 ? 1u : 0u);
                         mma_commit_pair(empty0[0] + 8u * (uint32_t)stage);
                         mma_commit_pair(empty0[1] + 8u * (uint32_t)stage);
-                        if (kb + 1 == sg.k1) {
+                        if (kb + 1 == t.k1) {
                             mma_commit_pair(tfull0[0] + 8u * (uint32_t)acc);
                             mma_commit_pair(tfull0[1] + 8u * (uint32_t)acc);
                         }
@@ -229,6 +253,10 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 mma_commit_pair(mapa_shared(smem_u32(drain), 0));
                 wait_drain(drain, 0, p.wait_ns);
             }
+        } else if (lane == 0) {
+            const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
+            const GxQueue queue = {qfull, qempty, queue_tile, 0};
+            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, p.wait_ns);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -237,16 +265,26 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         uint8_t* line = smem + L.buf + (warp - 4) * kGxLineBytes;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
-        int acc = 0, seg = 0;
+        int acc = 0;
         uint32_t aph = 0;
         bool alive = true;
-        while (walk.next(s, off, cum, sg)) {
-            int n0, k0, width;
-            place(n0, k0, width);
-            const int rows = off[sg.e + 1] - off[sg.e];
-            const int nc = width / 2, c0 = h * nc;
-            const int r0 = n0 + rank * 128 + q * 32, k = k0 + c0;
-            uint8_t* base = static_cast<uint8_t*>(p.dW) + (size_t)sg.e * p.N * p.K * (p.out == 2 ? 4 : 2);
+        for (;; ++asked) {
+            // one thread waits for the descriptor and tells the others, as in grouped_kernel.cuh
+            const int at = asked % kGxDescs;
+            if (threadIdx.x == kGxEpi0) {
+                const uint32_t bar = smem_u32(&dfull[at]), ph = (uint32_t)(asked / kGxDescs & 1);
+                const bool ok = alive && (mbar_try_wait(bar, ph) ||
+                                          wait_spin(bar, ph, abort_flag, p.wait_ns, site(2, 10, (uint32_t)at), asked));
+                epi_go[asked & 1] = ok && descs[at].e >= 0 ? 1 : 0;
+            }
+            named_bar_sync(1, kGxEpiThreads);
+            if (!epi_go[asked & 1]) break;
+            const DwDesc t = descs[at];
+            __syncwarp();
+            if (alive && lane == 0) mbar_arrive(&dempty[at]);
+            const int nc = t.width / 2, c0 = h * nc;
+            const int r0 = t.n0 + rank * 128 + q * 32, k = t.c0 + c0;
+            uint8_t* base = static_cast<uint8_t*>(p.dW) + (size_t)t.e * p.N * p.K * (p.out == 2 ? 4 : 2);
             // as whole lines; past this warp's columns (k + nc) another warp or tile writes
             const int k1 = k + nc < p.K ? k + nc : p.K;
             auto store = [&](int i, const float(&v)[16]) {
@@ -255,29 +293,27 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 if (at == per - 1 || i + 16 >= nc)
                     gx_flush(p.out, line, base, (size_t)p.K, r0, alive ? p.N : 0, k + i - at * 16, k1, lane);
             };
-            if (rows == 0) {
+            if (t.rows == 0) {
                 float z[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) z[j] = 0.f;
 #pragma unroll 1
                 for (int i = 0; i < nc; i += 16) store(i, z);
-                ++seg;
                 continue;
             }
-            if (alive) alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+            if (alive) alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
             tc_fence_after();
             const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256 + c0);
             auto slot_at = [&](int part, int i) {
+                const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
                 return reinterpret_cast<float4*>(p.work) +
-                       ((size_t)(dw_slot(s, part, sg.u0) * 2 + rank) * 64 + (c0 + i) / 4) * 128 + row;
+                       ((size_t)(dw_slot(s, part, t.u0) * 2 + rank) * 64 + (c0 + i) / 4) * 128 + row;
             };
             bool done = true;  // this block has the tile's whole sum
-            int first = c, last = c;
-            if (sg.k0 != 0 || sg.k1 != sg.kb) {
+            const int first = t.first, last = t.last;
+            if (first != last) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
-                first = dw_part_of(s, sg.u0);
-                last = dw_part_of(s, sg.u0 + sg.kb - 1);
-                int* counter = p.counters + sg.tile * 2 + rank;
+                int* counter = p.counters + t.tile * 2 + rank;
                 named_bar_sync(1, kGxEpiThreads);
                 if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
@@ -341,20 +377,19 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             if (alive && lane == 0) mbar_arrive_remote_relaxed(tempty0 + 8u * (uint32_t)acc);
             acc ^= 1;
             if (acc == 0) aph ^= 1u;
-            ++seg;
         }
     } else if (warp == 2) {
         // ---------------------------------------------------------- stages handed on, an expert's last one cleared behind it
         const uint32_t ready0 = mapa_shared(smem_u32(&ready[0]), 0);
-        int stage = 0, seg = 0;
+        int stage = 0;
         uint32_t ph = 0;
         bool alive = true;
-        while (alive && walk.next(s, off, cum, sg)) {
-            const int rows = off[sg.e + 1] - off[sg.e];
-            for (int kb = sg.k0; rows > 0 && kb < sg.k1; ++kb) {
-                alive = gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(5, 0, (uint32_t)stage), seg);
+        DwDesc t;
+        while (next(t, alive)) {
+            for (int kb = t.k0; t.rows > 0 && kb < t.k1; ++kb) {
+                alive = gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(4, 0, (uint32_t)stage), asked);
                 if (!alive) break;
-                const int here = rows - kb * 64;
+                const int here = t.rows - kb * 64;
                 if (here < 64 && here % 16) {
                     const int r1 = (here + 15) / 16 * 16;
                     uint4* box = reinterpret_cast<uint4*>(smem + stage * kDwStageBytes);  // 4 boxes of 64 rows of 8 pieces
@@ -369,7 +404,54 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     ph ^= 1u;
                 }
             }
-            ++seg;
+        }
+    } else {
+        // ---------------------------------------------------------- plan
+        const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
+        GxQueue queue = {qfull, qempty, queue_tile, 0};
+        DwWalk walk(s, c);
+        bool alive = true;
+        for (int i = 0; alive; ++i) {
+            DwSeg sg;
+            DwDesc d = {};
+            bool some = walk.next_part(s, off, cum, sg);
+            if (!some) {
+                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, p.wait_ns);
+                if (!alive) break;
+                some = tile >= 0;
+                if (some) DwWalk::whole(s, off, tile, sg);
+            }
+            if (some) {
+                d.e = sg.e;
+                d.t0 = off[sg.e];
+                d.rows = off[sg.e + 1] - d.t0;
+                const int j = sg.tile - sg.e * s.per;  // neighbouring tiles share dY's columns
+                d.n0 = j / p.tk * 256;
+                d.c0 = j % p.tk * p.width;
+                d.width = p.K - d.c0 < p.width ? (p.K - d.c0 + 31) / 32 * 32 : p.width;
+                d.k0 = sg.k0;
+                d.k1 = sg.k1;
+                d.tile = sg.tile;
+                d.u0 = sg.u0;
+                if (sg.k0 != 0 || sg.k1 != sg.kb) {
+                    d.first = dw_part_of(s, sg.u0);
+                    d.last = dw_part_of(s, sg.u0 + sg.kb - 1);
+                } else {
+                    d.first = d.last = c;
+                }
+            } else {
+                d.e = -1;
+            }
+            const int at = i % kGxDescs;
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, p.wait_ns, site(5, 11, (uint32_t)at),
+                                 i);
+            if (!alive) break;
+            if (lane == 0) {
+                descs[at] = d;
+                mbar_arrive(&dfull[at]);
+            }
+            __syncwarp();
+            if (!some) break;
         }
     }
 

@@ -10,18 +10,25 @@
 // and half of the tokens, the leader issues the MMA over both blocks' shared memory.  The weights are the MMA's M, so the
 // ragged dimension is its N, set per tile (grouped_sched.h).  Roles of a block's 12 warps:
 //   warp 0      TMA producer: a ring of stages of 128 bytes of K (64 16-bit values or 128 e4m3).
-//   warp 1      tensor memory; one thread of the leader issues the MMAs into a ring of accumulators (two of 256 columns, up to eight narrower).
-//   warps 2, 3  kGxF8Weights: the products xs ws of a K-block, one per token (a warp 128 of them), into a ring in shared memory.
-//   warps 4-11  epilogue: TMEM lanes 32 (warp % 4) .. + 31 (weight rows), the first or second half of the columns (tokens).
+//   warp 1      tensor memory; one lane of the leader's issues the MMAs into a ring of accumulators.  One lane of the other
+//               block's deals out the whole tiles.
+//   warp 2      the plan: the pair's segments (a tile and its K-blocks) one after the other, as descriptors in a ring in
+//               shared memory that the other warps follow.  (Each warp on its own held the schedule's state in registers that
+//               the epilogue's sums need.)
+//   warp 3      e4m3: the products of two scales, four K-blocks at a time, into a ring in shared memory.
+//   warps 4-11  epilogue: TMEM lanes 32 (warp % 4) .. + 31, the first or second half of the columns.
 // e4m3: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers; the MMAs of
 // the next K-blocks run into the other accumulators meanwhile.  The scales differ from block to block, so no MMA may run
 // across two.  With the weights as M (kGxF8Weights) a column's scale is the same in all lanes and comes from shared memory, 4
 // bytes per product: 256 tokens would take 1024 cycles a K-block (128 bytes a cycle) beside 512 of MMA.  So above 128 tokens
 // per expert the tokens are the M (kGxF8Tokens): a lane is a token with one scale, a half of the columns one block of
-// weights with another, and the product of the two is all a K-block needs.
-// Every wait is bounded (ptx.cuh); after one that gave up the epilogue walks its segments to the end without waiting,
-// reading or writing, so that all threads meet at every barrier.
+// weights with another, and the product of the two is all a K-block needs.  Few tokens: the K-blocks go to the epilogue in
+// groups of 128 columns (4 K-blocks of 32 tokens), since a hand-over costs more than the sums of 32 columns.
+// Every wait is bounded (ptx.cuh); after one that gave up the epilogue goes on to the end of its segment without waiting or
+// writing, so that all its threads meet at every barrier, and then leaves.
 #pragma once
+#include <type_traits>
+
 #include "grouped_sched.h"
 #include "kernel_common.cuh"
 
@@ -38,13 +45,15 @@ constexpr int kGxEpi0 = 128;         // the first epilogue thread
 constexpr int kGxEpiThreads = 256;
 constexpr int kGxXBytes = 128 * 128;  // a block's weight rows of a stage
 constexpr int kGxMaxStages = 12;
-constexpr int kGxScales = 4;          // K-blocks of scale products held
+constexpr int kGxBatch = 4;           // K-blocks whose scale products are handed over at once
+constexpr int kGxBatches = 2;         // such batches held
+constexpr int kGxDescs = 4;           // descriptors held
+constexpr int kGxQueue = 4;           // whole tiles dealt ahead
 constexpr int kGxOtherRegs = 72, kGxEpiRegs = 216;
 static_assert(128 * kGxOtherRegs + 256 * kGxEpiRegs <= kGxThreads * 168, "registers moved within what the launch holds");
-constexpr int kGxAhead = 4;           // K-blocks whose scales are on their way
 constexpr int kGxAccs = 8;            // accumulators in tensor memory at most
-constexpr int kGxScaleBytes = kGxScales * 2 * 256 * 4;          // [K-block][gate, up][token]
-constexpr int kGxBars = 2 * kGxMaxStages + 2 * kGxAccs + 2 * kGxScales + 1;
+constexpr int kGxScaleBytes = kGxBatches * kGxBatch * 2 * 128 * 4;  // [batch][K-block][gate, up or half][token]
+constexpr int kGxBars = 2 * kGxMaxStages + 2 * kGxAccs + 2 * kGxBatches + 2 * kGxDescs + 2 * kGxQueue + 1;
 
 // fp16 or bf16; e4m3 with the weight rows as the MMA's M; e4m3 with the tokens as its M.
 enum : int { kGx16 = 0, kGxF8Weights = 1, kGxF8Tokens = 2 };
@@ -58,7 +67,7 @@ struct GxParams {
     int nt, kblocks;       // weight tiles per expert, K-blocks
     int cap, box, wbox;    // the most tokens of a tile; rows of one TMA box of X, of W
     int stages, stage_bytes, ring_bytes;
-    int accs;              // accumulators in tensor memory
+    int accs, group;       // accumulators in tensor memory; K-blocks of one (e4m3), cap columns each
     int mn_major;          // W is E x K x N
     int glu, out;          // kGx*; BW_TYPE_* (0 fp16, 1 bf16, 2 fp32)
     uint32_t idesc;        // without N
@@ -69,6 +78,7 @@ struct GxParams {
     int ws_rows;           // blocks of 128 rows per expert
     float* work;           // parts of split tiles: slots of 2 x 128 x cap
     int* counters;         // two per split tile, zero at the start of a call
+    int* next;             // the whole tiles given out, zero at the start of a call
     unsigned long long wait_ns;
 };
 
@@ -82,30 +92,34 @@ __host__ __device__ inline GxSmem gx_smem(int kind, int ring_bytes, int E)
     GxSmem m;
     m.buf = ring_bytes;
     m.scales = m.buf + 8 * (kind == 2 ? 4096 : 2048);
-    m.bars = m.scales + (kind == 1 ? kGxScaleBytes : 0);
+    m.bars = m.scales + (kind ? kGxScaleBytes : 0);
     m.misc = m.bars + kGxBars * 8;
     m.misc = (m.misc + 15) / 16 * 16;
-    m.tables = m.misc + 64;
+    m.tables = m.misc + 64 + kGxDescs * 64;
     m.bytes = m.tables + 2 * (E + 1) * 4;
     return m;
 }
 
-// A tile's rows of X and weight rows.
-struct GxTile {
-    int e, n;     // expert, weight tile
-    int t0, t1;   // its tokens [t0, t1)
-    int N;        // MMA N: a multiple of 32
+// A segment: a tile (its rows of X, its weight rows), its K-blocks, and, of a tile split along K, the parts' numbers.
+struct GxDesc {
+    int e, n;         // expert (-1: no segment left), weight tile
+    int t0, t1;       // tokens [t0, t1)
+    int N;            // MMA N: a multiple of 32
+    int k0, k1;       // K-blocks
+    int tile;         // its number, for a split tile's counters
+    int first, last;  // parts of the tile: this pair's alone where equal
 };
+static_assert(sizeof(GxDesc) <= 64, "room for the descriptors");
 
-// Follows ascending tile indices through the experts.
+// Follows ascending tile numbers through the experts.
 struct GxFind {
     int e = 0;
     template <int KIND>
-    __device__ __forceinline__ GxTile at(const GxParams& p, const int* off, const int* cum, int tile)
+    __device__ __forceinline__ void at(const GxParams& p, const int* off, const int* cum, int tile, GxDesc& t)
     {
         while (cum[e + 1] * p.nt <= tile) ++e;
-        GxTile t;
         t.e = e;
+        t.tile = tile;
         const int runs = cum[e + 1] - cum[e], a = off[e], b = off[e + 1];
         int m;
         group_place(tile - cum[e] * p.nt, p.nt, runs, m, t.n);
@@ -115,7 +129,6 @@ struct GxFind {
         int n = t.t1 - t.t0;
         if (KIND == kGxF8Tokens) n = p.glu == kGxPlain && p.N - t.n * 256 < 256 ? p.N - t.n * 256 : 256;
         t.N = (n + 31) / 32 * 32;
-        return t;
     }
 };
 
@@ -130,6 +143,46 @@ __device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, vol
     ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
     if (ok) mbar_try_wait(b, parity);  // complete: this lane acquires too
     return ok != 0;
+}
+
+// Whole tiles on demand.  The first of a pair is its own; for the others one lane of the pair's second block (warp 1) draws
+// numbers from the call's counter, ahead of need, into a queue of kGxQueue entries in both blocks' shared memory (-1: none
+// left), and reuses an entry once all the pair's readers have read it.
+struct GxQueue {
+    uint64_t* full;   // an entry is there (each block's own)
+    uint64_t* empty;  // the second block's count
+    volatile int* tile;
+    int i;            // tiles this reader has asked for
+};
+__device__ __forceinline__ void gx_deal(const GxQueue& q, int* counter, int first, int tiles, volatile int* abort_flag,
+                                        uint64_t limit_ns)
+{
+    const uint32_t other = mapa_shared(smem_u32(const_cast<int*>(q.tile)), 0), full0 = mapa_shared(smem_u32(q.full), 0);
+    for (int i = 0;; ++i) {
+        const int at = i % kGxQueue;
+        const uint32_t bar = smem_u32(&q.empty[at]), ph = (uint32_t)(i / kGxQueue & 1) ^ 1u;
+        if (!mbar_try_wait(bar, ph) && !wait_spin(bar, ph, abort_flag, limit_ns, site(6, 9, (uint32_t)at), i)) return;
+        int t = first + atomicAdd(counter, 1);
+        if (t >= tiles) t = -1;
+        q.tile[at] = t;
+        st_cluster_f32(other + 4u * (uint32_t)at, __int_as_float(t));
+        mbar_arrive(&q.full[at]);
+        mbar_arrive_cluster(full0 + 8u * (uint32_t)at);
+        if (t < 0) return;
+    }
+}
+// The next whole tile, by one warp; -1: none left, or the wait gave up (alive false).
+__device__ __forceinline__ int gx_next_tile(GxQueue& q, int own, int tiles, bool& alive, volatile int* abort_flag,
+                                            uint64_t limit_ns)
+{
+    if (q.i++ == 0) return own < tiles ? own : -1;
+    const int at = (q.i - 2) % kGxQueue;
+    alive = gx_warp_wait(&q.full[at], (uint32_t)((q.i - 2) / kGxQueue & 1), abort_flag, limit_ns, site(5, 9, (uint32_t)at), q.i);
+    if (!alive) return -1;
+    const int t = q.tile[at];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive_remote(mapa_shared(smem_u32(&q.empty[at]), 1));
+    return t;
 }
 
 // 16 tokens x 32 columns of C: v[j] is token tb + j, column f + lane.  Through the warp's buffer, so that a token's 32
@@ -179,11 +232,11 @@ __device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[1
 // 16 tokens of a finished sum to C.  With the activation a warp of gate rows (quarters 0 and 1) takes the up rows' sums
 // from the warp of the same columns two quarters on, through that warp's buffer; the two meet twice.
 __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], uint8_t* bufs, int ew, int q, int h, int tb,
-                                            const GxTile& t, int f, int lane, bool write)
+                                            int t1, int f, int lane, bool write)
 {
     uint8_t* mine = bufs + ew * 2048;
     if (p.glu == kGxPlain) {
-        gx_store16(p, v, mine, tb, t.t1, f, lane, write);
+        gx_store16(p, v, mine, tb, t1, f, lane, write);
         return;
     }
     const uint32_t bar = 2u + (uint32_t)(h * 2 + (q & 1));
@@ -200,7 +253,7 @@ __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], u
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * b[j * 32 + lane];
         named_bar_sync(bar, 64);
-        gx_store16(p, v, mine, tb, t.t1, f, lane, write);
+        gx_store16(p, v, mine, tb, t1, f, lane, write);
     }
 }
 
@@ -309,7 +362,6 @@ __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum,
     }
 }
 
-// What each block's dynamic shared memory and registers hold follows from p and KIND; two blocks make a cluster.
 template <int KIND>
 __global__ void __launch_bounds__(kGxThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const GxParams p)
@@ -328,11 +380,18 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     uint64_t* tfull = empty + kGxMaxStages;
     uint64_t* tempty = tfull + kGxAccs;
     uint64_t* sfull = tempty + kGxAccs;
-    uint64_t* sempty = sfull + kGxScales;
-    uint64_t* drain = sempty + kGxScales;
+    uint64_t* sempty = sfull + kGxBatches;
+    uint64_t* dfull = sempty + kGxBatches;
+    uint64_t* dempty = dfull + kGxDescs;
+    uint64_t* qfull = dempty + kGxDescs;
+    uint64_t* qempty = qfull + kGxQueue;
+    uint64_t* drain = qempty + kGxQueue;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* reduce_flag = abort_flag + 1;
+    volatile int* epi_go = abort_flag + 2;      // two, alternating
+    volatile int* queue_tile = abort_flag + 4;  // kGxQueue entries
+    GxDesc* descs = reinterpret_cast<GxDesc*>(smem + L.misc + 64);
     float* scales = reinterpret_cast<float*>(smem + L.scales);
     int* off = reinterpret_cast<int*>(smem + L.tables);
     int* cum = off + p.E + 1;
@@ -342,7 +401,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
     const int S = p.stages;
-    const int tmem_cols = p.accs * p.cap;  // a power of two, 256 or 512
+    const int acc_cols = p.group * p.cap;       // columns of an accumulator
+    const int tmem_cols = p.accs * acc_cols;    // a power of two, 256 or 512
 
     if (threadIdx.x == 0) {
         BW_TRACE_CLEAR();
@@ -358,9 +418,17 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&tfull[i], 1);
             mbar_init(&tempty[i], 16);  // the epilogue warps of both blocks
         }
-        for (int i = 0; i < kGxScales; ++i) {
-            mbar_init(&sfull[i], 2);
-            mbar_init(&sempty[i], 8);
+        for (int i = 0; i < kGxBatches; ++i) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sempty[i], 8);  // the epilogue warps
+        }
+        for (int i = 0; i < kGxDescs; ++i) {
+            mbar_init(&dfull[i], 1);
+            mbar_init(&dempty[i], 9u + (leader ? 1u : 0u) + (F8 ? 1u : 0u));  // producer, epilogue, MMA issuer, scales
+        }
+        for (int i = 0; i < kGxQueue; ++i) {
+            mbar_init(&qfull[i], 1);
+            mbar_init(&qempty[i], 2);  // both blocks' plans
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -376,28 +444,38 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_relinquish_pair();
     }
     griddep_wait();  // what the kernel ahead wrote (the offsets, X, its scales, the counters) is visible from here on
-    if (warp == 4) gx_tables(p, off, cum, lane);
+    if (warp == 2) gx_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // barriers, tables and tensor memory of both blocks are there
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-    GroupWalk walk(s, c);
-    GroupSeg sg;
-    GxFind find;
-    // kGxF8Tokens holds 128 sums in registers: the epilogue's 8 warps take registers from the other 4 (384 threads are launched
+    // e4m3 holds up to 128 sums in registers: the epilogue's 8 warps take registers from the other 4 (384 threads are launched
     // with 168 each: 128 x 72 + 256 x 216 <= 384 x 168)
-    if (TOK && warp < 4) reg_dec<kGxOtherRegs>();
+    if (F8 && warp < 4) reg_dec<kGxOtherRegs>();
+
+    // a warp's next descriptor (false: none left, or the wait gave up)
+    int asked = 0;
+    auto next = [&](GxDesc& d, bool& alive) {
+        const int at = asked % kGxDescs;
+        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, p.wait_ns,
+                                      site(3, 10, (uint32_t)at), asked);
+        if (!alive) return false;
+        d = descs[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dempty[at]);
+        ++asked;
+        return d.e >= 0;
+    };
 
     if (warp == 0) {
         // ---------------------------------------------------------- TMA producer
         const uint32_t full0 = mapa_shared(smem_u32(full), 0);  // both blocks complete the leader's barriers
-        int stage = 0, issued = 0, seg = 0;
+        int stage = 0, issued = 0;
         uint32_t ph = 0;
         bool alive = true;
-        while (alive && walk.next(s, sg)) {
-            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
+        GxDesc t;
+        while (next(t, alive)) {
             const int boxes = TOK ? 1 : (t.N / 2 + p.box - 1) / p.box;
             const uint32_t bytes = 2u * (kGxXBytes + (uint32_t)(boxes * p.box) * 128u);
             const int tok = t.t0 + rank * (TOK ? 128 : t.N / 2);
@@ -414,8 +492,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                                              : t.n * 128 + rank * 64;
                 w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
             }
-            for (int kb = sg.k0; kb < sg.k1; ++kb) {
-                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), seg);
+            for (int kb = t.k0; kb < t.k1; ++kb) {
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), asked);
                 if (!alive) break;
                 uint8_t* sx = smem + stage * p.stage_bytes;
                 const uint32_t bar = full0 + 8u * (uint32_t)stage;
@@ -440,7 +518,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     ph ^= 1u;
                 }
             }
-            ++seg;
         }
         if (leader && lane == 0) {  // loads in flight land before the blocks may leave (after an abort; else they have landed)
             const int n = issued < S ? issued : S;
@@ -450,37 +527,38 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             }
         }
     } else if (warp == 1) {
-        // ---------------------------------------------------------- MMA issuer
         if (leader) {
+            // ------------------------------------------------------ MMA issuer
             const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
             const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
             // the descriptors' low words (a 16-byte step of the address is a step of 1) and their constant high words
             const uint64_t dx = !F8 && p.mn_major ? desc_mnmajor(smem_u32(smem), 0) : desc_kmajor(smem_u32(smem), 0);
             const uint64_t dy = desc_kmajor(smem_u32(smem) + kGxXBytes, 0);
             const uint32_t step = (uint32_t)p.stage_bytes >> 4, kx = !F8 && p.mn_major ? 128u : 2u;
-            int stage = 0, acc = 0, seg = 0;
+            int stage = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool alive = true;
+            GxDesc t;
             GX_CLOCK(long long w_full = 0, w_acc = 0, n_kb = 0, t_at = 0);
-            while (alive && walk.next(s, sg)) {
-                const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
+            while (next(t, alive)) {
                 const uint32_t idesc = p.idesc | idesc_n(t.N);
-                for (int kb = sg.k0; kb < sg.k1; ++kb) {
+                int in_group = 0;
+                for (int kb = t.k0; kb < t.k1; ++kb) {
                     GX_CLOCK(t_at = clock64());
-                    if (F8 || kb == sg.k0)
-                        alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), seg);
+                    if (F8 ? in_group == 0 : kb == t.k0)
+                        alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), asked);
                     GX_CLOCK(w_acc += clock64() - t_at; t_at = clock64());
-                    alive = alive && gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), seg);
+                    alive = alive && gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), asked);
                     if (!alive) break;
                     GX_CLOCK(w_full += clock64() - t_at; if (n_kb++ == 0 && lane == 0) BW_TRACE_AT(2));
                     tc_fence_after();
                     const uint64_t ad = dx + (uint64_t)(step * (uint32_t)stage), bd = dy + (uint64_t)(step * (uint32_t)stage);
-                    const uint32_t d = tmem_base + (uint32_t)(acc * p.cap);
-                    const bool last = F8 || kb + 1 == sg.k1;
+                    const uint32_t d = tmem_base + (uint32_t)(acc * acc_cols + in_group * p.cap);
+                    const bool last = kb + 1 == t.k1 || (F8 && in_group + 1 == p.group);
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t accumulate = ((!F8 && kb > sg.k0) || k > 0) ? 1u : 0u;
+                            const uint32_t accumulate = ((!F8 && kb > t.k0) || k > 0) ? 1u : 0u;
                             if constexpr (F8)
                                 mma_f8_pair(d, ad + kx * k, bd + 2 * k, idesc, accumulate);
                             else
@@ -494,7 +572,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         }
                     }
                     __syncwarp();
+                    if (F8) ++in_group;
                     if (last) {
+                        in_group = 0;
                         if (++acc == p.accs) {
                             acc = 0;
                             aph ^= 1u;
@@ -505,7 +585,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         ph ^= 1u;
                     }
                 }
-                ++seg;
             }
             if (lane == 0) {
                 BW_TRACE_AT(3);
@@ -518,19 +597,122 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 mma_commit_pair(mapa_shared(smem_u32(drain), 0));
                 wait_drain(drain, 0, p.wait_ns);
             }
+        } else if (lane == 0) {
+            // ------------------------------------------------------ whole tiles dealt out
+            const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+            const GxQueue queue = {qfull, qempty, queue_tile, 0};
+            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, p.wait_ns);
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp == 2) {
+        // ---------------------------------------------------------- plan
+        const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+        GxQueue queue = {qfull, qempty, queue_tile, 0};
+        GroupWalk walk(s, c);
+        GxFind find;
+        bool alive = true;
+        for (int i = 0; alive; ++i) {
+            GroupSeg sg;
+            GxDesc d = {};
+            bool some = walk.next_part(s, sg);
+            if (!some) {
+                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, p.wait_ns);
+                if (!alive) break;
+                some = tile >= 0;
+                if (some) GroupWalk::whole(s, tile, sg);
+            }
+            if (some) {
+                find.at<KIND>(p, off, cum, sg.tile, d);
+                d.k0 = sg.k0;
+                d.k1 = sg.k1;
+                if (sg.k0 != 0 || sg.k1 != s.kb) {
+                    d.first = tile_first_part(s, sg.tile);
+                    d.last = tile_last_part(s, sg.tile);
+                }
+            } else {
+                d.e = -1;
+            }
+            const int at = i % kGxDescs;
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, p.wait_ns, site(5, 11, (uint32_t)at),
+                                 i);
+            if (!alive) break;
+            if (lane == 0) {
+                descs[at] = d;
+                mbar_arrive(&dfull[at]);
+            }
+            __syncwarp();
+            if (!some) break;
+        }
+    } else if (warp == 3) {
+        // ---------------------------------------------------------- scale products
+        if constexpr (F8) {
+            int si = 0;
+            uint32_t sph = 0;
+            bool alive = true;
+            GxDesc t;
+            while (next(t, alive)) {
+                // the scale blocks of the weight rows: kGxF8Weights, of this block's rows (gate and up: of each); kGxF8Tokens, of the
+                // tile's two halves of columns
+                int r0, r1;
+                if (p.glu == kGxGluHalves) {
+                    r0 = t.n;
+                    r1 = p.ws_rows / 2 + t.n;
+                } else {
+                    r0 = 2 * t.n + (!TOK && p.glu == kGxPlain ? rank : 0);
+                    r1 = 2 * t.n + 1;
+                }
+                const bool two = TOK || p.glu != kGxPlain;
+                const float* w0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
+                const float* w1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
+                const int tok = t.t0 + (TOK ? rank * 128 : 0) + lane, have = t.t1 - tok;  // this lane's: every 32nd from tok on
+                // a batch is loaded while the one before it is in use: a load takes as long as several K-blocks of MMAs
+                float x[kGxBatch][4], a[kGxBatch], b[kGxBatch];
+                auto load = [&](int kb, float(&x)[4], float& a, float& b) {
+                    if (kb >= t.k1) return;
+                    const float* xs = p.xs + kb * p.xs_ld + tok;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = i * 32 < have ? xs[i * 32] : 0.f;
+                    a = w0[kb];
+                    b = two ? w1[kb] : 0.f;
+                };
+#pragma unroll
+                for (int d = 0; d < kGxBatch; ++d) load(t.k0 + d, x[d], a[d], b[d]);
+                for (int kb = t.k0; kb < t.k1; kb += kGxBatch) {
+                    alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), asked);
+                    if (!alive) break;
+                    float* to = scales + si * kGxBatch * 256 + lane;
+#pragma unroll
+                    for (int d = 0; d < kGxBatch; ++d) {
+                        if (kb + d >= t.k1) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (!TOK && i * 32 >= t.N) break;
+                            to[d * 256 + i * 32] = x[d][i] * a[d];
+                            if (two) to[d * 256 + 128 + i * 32] = x[d][i] * b[d];
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[si]);
+                    if (++si == kGxBatches) {
+                        si = 0;
+                        sph ^= 1u;
+                    }
+#pragma unroll
+                    for (int d = 0; d < kGxBatch; ++d) load(kb + kGxBatch + d, x[d], a[d], b[d]);
+                }
+            }
+        }
+    } else {
         // ---------------------------------------------------------- epilogue
-        if (TOK) reg_inc<kGxEpiRegs>();
+        if (F8) reg_inc<kGxEpiRegs>();
         const int ew = warp - 4, q = warp & 3, h = ew >> 2;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
+        const uint32_t quarter = tmem_base + ((uint32_t)(q * 32) << 16);
         uint8_t* bufs = smem + L.buf;
-        int acc = 0, seg = 0, si = 0;
+        int acc = 0, si = 0;
         uint32_t aph = 0, sph = 0;
         bool alive = true;
-        const float* sc_base = scales + (p.glu != kGxPlain && q >= 2 ? 256 : 0);
         auto release = [&](int a) {
             tc_fence_before();
             __syncwarp();
@@ -542,130 +724,137 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 aph ^= 1u;
             }
         };
-        while (walk.next(s, sg)) {
-            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
+        for (;; ++asked) {
+            // one thread waits for the descriptor and tells the other 255, so that all of them go on to the same barriers, or none
+            const GxDesc& t = descs[asked % kGxDescs];
+            if (threadIdx.x == kGxEpi0) {
+                const uint32_t bar = smem_u32(&dfull[asked % kGxDescs]), ph = (uint32_t)(asked / kGxDescs & 1);
+                const bool ok = alive && (mbar_try_wait(bar, ph) || wait_spin(bar, ph, abort_flag, p.wait_ns,
+                                                                              site(2, 10, (uint32_t)(asked % kGxDescs)), asked));
+                epi_go[asked & 1] = ok && t.e >= 0 ? 1 : 0;
+            }
+            named_bar_sync(1, kGxEpiThreads);
+            if (!epi_go[asked & 1]) break;
+            const int N = t.N;
             // This warp's columns, in runs of 16: half of the tile's.  TOK: the first or second 128, or with the activation
             // 64 gate columns and their 64 up columns.
-            const int nc = t.N / 2, c0 = h * nc;
+            const int nc = N / 2, c0 = h * nc;
             auto col = [&](int i) {
                 if (!TOK) return c0 + i * 16;
                 return p.glu == kGxPlain ? h * 128 + i * 16 : (i < 4 ? 0 : 64) + h * 64 + i * 16;
             };
-            auto in_tile = [&](int i) { return TOK ? col(i) < t.N : i * 16 < nc; };
-            const uint32_t quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+            auto in_tile = [&](int i) { return TOK ? col(i) < N : i * 16 < nc; };
             if constexpr (KIND == kGx16) {
                 if (alive)
-                    alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                    alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
                 tc_fence_after();
             } else {
-                constexpr int kRuns = TOK ? 8 : 4;
-                uint64_t sum[kRuns][8];  // 16 columns a run, as pairs
+                const int blocks = t.k1 - t.k0;
+                // The segment's scaled sums, and back into its last accumulator, where the code below takes them for all kinds.
+                // R: runs of 16 columns that this warp holds.
+                auto accumulate = [&](auto runs) {
+                    constexpr int R = decltype(runs)::value;
+                    uint64_t sum[R][8];  // 16 columns a run, as pairs
 #pragma unroll
-                for (int i = 0; i < kRuns; ++i)
+                    for (int i = 0; i < R; ++i)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
-                int kb = sg.k0;
-                if constexpr (TOK) {
-                    // this token's scales and its columns' (one or two blocks of 128 weight rows), two K-blocks ahead
-                    const int tok = t.t0 + rank * 128 + row;
-                    const float* xs = p.xs + (tok < t.t1 ? tok : t.t0);
-                    const int r0 = p.glu == kGxPlain ? 2 * t.n + h : p.glu == kGxGluBlocks ? 2 * t.n : t.n;
-                    const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : r0 + 1;
-                    const float* ws0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
-                    const float* ws1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
-                    struct Scale {
-                        float x, w0, w1;
-                    } ahead[2] = {};
-                    auto load = [&](int k, Scale& a) {
-                        if (k >= sg.k1) return;
-                        a.x = xs[k * p.xs_ld];
-                        a.w0 = ws0[k];
-                        if (p.glu != kGxPlain) a.w1 = ws1[k];
-                    };
-                    load(kb, ahead[0]);
-                    load(kb + 1, ahead[1]);
-                    // one K-block; false after the last
-                    auto block = [&](Scale& a) {
-                        const uint32_t s0 = __float_as_uint(a.x * a.w0), s1 = __float_as_uint(a.x * a.w1);
-                        const uint64_t p0 = pair_f32(s0, s0), p1 = p.glu != kGxPlain ? pair_f32(s1, s1) : p0;
-                        load(kb + 2, a);
-                        if (alive)
-                            alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
-                        if (alive) {
-                            tc_fence_after();
-                            const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
-#pragma unroll
-                            for (int i = 0; i < 8; i += 2) {  // 32 columns leave tensor memory at a time
-                                uint32_t r[2][16];
-#pragma unroll
-                                for (int j = 0; j < 2; ++j)
-                                    tmem_ld16(tm + (uint32_t)col(i + j), r[j]);  // (past the tile's: not used)
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                    for (int k = 0; k < 8; ++k)
-                                        sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1,
-                                                                  sum[i + j][k]);
-                            }
+                        for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
+                    for (int kb = 0;;) {
+                        if (alive && kb % kGxBatch == 0)
+                            alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), asked);
+                        const float* sc = scales + (si * kGxBatch + kb % kGxBatch) * 256;
+                        uint64_t p0 = 0, p1 = 0;
+                        if (TOK) {
+                            const uint32_t s0 = __float_as_uint(sc[p.glu == kGxPlain ? h * 128 + row : row]);
+                            const uint32_t s1 = p.glu == kGxPlain ? s0 : __float_as_uint(sc[128 + row]);
+                            p0 = pair_f32(s0, s0);
+                            p1 = pair_f32(s1, s1);
                         }
-                        if (++kb == sg.k1) return false;
-                        release(acc);
-                        next_acc();
-                        return true;
-                    };
-                    while (block(ahead[0]) && block(ahead[1])) {
-                    }
-                } else {
-                    for (;;) {
                         if (alive)
-                            alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), seg) &&
-                                    gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), seg);
+                            alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
                         if (alive) {
                             tc_fence_after();
-                            const float* sc = sc_base + si * 512 + c0;
-                            const uint32_t tm = quarter + (uint32_t)(acc * p.cap + c0);
-                            uint32_t r[4][16];
+                            if constexpr (TOK) {
+                                const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (in_tile(i)) tmem_ld16(tm + (uint32_t)(i * 16), r[i]);
-                            tmem_wait_ld();
+                                for (int i = 0; i < 8; i += 2) {  // 32 columns leave tensor memory at a time
+                                    uint32_t r[2][16];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (in_tile(i)) {
+                                    for (int j = 0; j < 2; ++j)
+                                        tmem_ld16(tm + (uint32_t)col(i + j), r[j]);  // (past the tile's: not used)
+                                    tmem_wait_ld();
 #pragma unroll
-                                    for (int k = 0; k < 8; k += 2) {
-                                        uint64_t s0, s1;  // one address per warp: a broadcast
-                                        ld_shared_2b64(sc + i * 16 + 2 * k, s0, s1);
-                                        sum[i][k] = fma_f32x2(pair_f32(r[i][2 * k], r[i][2 * k + 1]), s0, sum[i][k]);
-                                        sum[i][k + 1] = fma_f32x2(pair_f32(r[i][2 * k + 2], r[i][2 * k + 3]), s1, sum[i][k + 1]);
+                                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                        for (int k = 0; k < 8; ++k)
+                                            sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1,
+                                                                      sum[i + j][k]);
+                                }
+                            } else {
+                                // the accumulator's K-blocks, 4 / R of them, cap columns each
+                                const uint32_t tm = quarter + (uint32_t)(acc * acc_cols + c0);
+                                const float* from = sc + (p.glu != kGxPlain && q >= 2 ? 128 : 0) + c0;
+#pragma unroll
+                                for (int w = 0; w < 4; w += 2) {
+                                    uint32_t r[2][16];
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+                                        const int u = w + j;
+                                        if (kb + u / R < blocks && u % R * 16 < nc)
+                                            tmem_ld16(tm + (uint32_t)(u / R * (R * 32) + u % R * 16), r[j]);
+                                    }
+                                    tmem_wait_ld();
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+                                        const int u = w + j;
+                                        if (kb + u / R < blocks && u % R * 16 < nc) {
+#pragma unroll
+                                            for (int k = 0; k < 8; k += 2) {
+                                                uint64_t s0, s1;  // one address per warp: a broadcast
+                                                ld_shared_2b64(from + u / R * 256 + u % R * 16 + 2 * k, s0, s1);
+                                                uint64_t(&to)[8] = sum[u % R];
+                                                to[k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), s0, to[k]);
+                                                to[k + 1] = fma_f32x2(pair_f32(r[j][2 * k + 2], r[j][2 * k + 3]), s1, to[k + 1]);
+                                            }
+                                        }
                                     }
                                 }
+                            }
                         }
-                        __syncwarp();  // every lane has read the scales
-                        if (alive && lane == 0) mbar_arrive(&sempty[si]);
-                        if (++si == kGxScales) {
-                            si = 0;
-                            sph ^= 1u;
+                        kb += TOK ? 1 : 4 / R;
+                        if (kb % kGxBatch == 0 || kb >= blocks) {
+                            __syncwarp();  // every lane has read the scales
+                            if (alive && lane == 0) mbar_arrive(&sempty[si]);
+                            if (++si == kGxBatches) {
+                                si = 0;
+                                sph ^= 1u;
+                            }
                         }
-                        if (++kb == sg.k1) break;
+                        if (kb >= blocks) break;
                         release(acc);
                         next_acc();
                     }
-                }
-                // the sums go back into the last accumulator, where the code below takes them for all kinds
-                const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
+                    const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
 #pragma unroll
-                for (int i = 0; i < kRuns; ++i)
-                    if (in_tile(i)) {
-                        uint32_t r[16];
+                    for (int i = 0; i < R; ++i)
+                        if (in_tile(i)) {
+                            uint32_t r[16];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
-                        tmem_st16(tm + (uint32_t)col(i), r);
-                    }
-                tmem_wait_st();
+                            for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
+                            tmem_st16(tm + (uint32_t)col(i), r);
+                        }
+                    tmem_wait_st();
+                };
+                if constexpr (TOK)
+                    accumulate(std::integral_constant<int, 8>());
+                else if (p.cap == 128)
+                    accumulate(std::integral_constant<int, 4>());
+                else if (p.cap == 64)
+                    accumulate(std::integral_constant<int, 2>());
+                else
+                    accumulate(std::integral_constant<int, 1>());
             }
-            const uint32_t tm = quarter + (uint32_t)(acc * p.cap);
+            const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
             // this segment's sum of 16 columns
             auto own = [&](int i, float(&v)[16]) {
                 uint32_t r[16];
@@ -675,18 +864,17 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
             };
             bool done = true;  // this block has the tile's whole sum
-            int first = c, last = c;
-            if (sg.k0 != 0 || sg.k1 != s.kb) {
+            const int first = t.first, last = t.last, tile = t.tile;
+            if (first != last) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
-                first = tile_first_part(s, sg.tile);
-                last = tile_last_part(s, sg.tile);
-                int* counter = p.counters + sg.tile * 2 + rank;
+                const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+                int* counter = p.counters + tile * 2 + rank;
                 named_bar_sync(1, kGxEpiThreads);  // the flag of an earlier tile has been read
                 if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
                 done = *reduce_flag != 0;
                 if (!done) {
-                    const int slot = part_slot(s, c, sg.tile);
+                    const int slot = part_slot(s, c, tile);
 #pragma unroll 1
                     for (int i = 0; i < 8 && in_tile(i); ++i) {
                         float v[16];
@@ -711,6 +899,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     own(i, v);
                     return;
                 }
+                const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
                 float mine[16];
                 own(i, mine);
 #pragma unroll
@@ -721,7 +910,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         for (int j = 0; j < 16; ++j) v[j] += mine[j];
                         continue;
                     }
-                    const int slot = part_slot(s, part, sg.tile);
+                    const int slot = part_slot(s, part, tile);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float4 x = __ldcg(gx_slot(p, slot, rank, row, col(i) / 4 + j));
@@ -735,7 +924,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             if (done) {
                 if constexpr (TOK) {
                     const bool glu = p.glu != kGxPlain;
-                    const int r0 = t.t0 + rank * 128 + q * 32, f0 = t.n * (glu ? 128 : 256);
+                    const int r0 = t.t0 + rank * 128 + q * 32, r1 = alive ? t.t1 : 0, f0 = t.n * (glu ? 128 : 256);
                     const int per = gx_per_line(p.out), runs = glu ? 4 : 8;
                     uint8_t* line = bufs + ew * kGxLineBytes;
 #pragma unroll 1
@@ -750,75 +939,25 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         }
                         gx_put16(p.out, line, i % per, lane, v);
                         if (i % per == per - 1 || i + 1 == runs || !in_tile(i + 1))
-                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, alive ? t.t1 : 0, f0 + col(i - i % per),
+                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, r1, f0 + col(i - i % per),
                                      f0 + col(i) + 16 < p.Nout ? f0 + col(i) + 16 : p.Nout, lane);
                     }
                 } else {
-                    const int tb = t.t0 + c0;
+                    const int tb = t.t0 + c0, t1 = t.t1;
                     const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
 #pragma unroll 1
                     for (int i = 0; in_tile(i); ++i) {
                         float v[16];
                         total(i, v);
-                        gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t, f, lane, alive);
+                        gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t1, f, lane, alive);
                     }
                 }
             }
             release(acc);
             next_acc();
-            ++seg;
+            if (alive && lane == 0) mbar_arrive(&dempty[asked % kGxDescs]);  // (release met the warp: the descriptor has been read)
         }
         if (threadIdx.x == kGxEpi0) BW_TRACE_AT(4);
-    } else if (KIND == kGxF8Weights) {
-        // ---------------------------------------------------------- scale products
-        const int t00 = (warp - 2) * 128 + lane;  // this lane's first token of a tile
-        int si = 0, seg = 0;
-        uint32_t sph = 0;
-        bool alive = true;
-        while (alive && walk.next(s, sg)) {
-            const GxTile t = find.at<KIND>(p, off, cum, sg.tile);
-            // the scale blocks of this block's weight rows (gate and up: of each)
-            const int r0 = p.glu == kGxGluHalves ? t.n : p.glu == kGxGluBlocks ? 2 * t.n : 2 * t.n + rank;
-            const int r1 = p.glu == kGxGluHalves ? p.ws_rows / 2 + t.n : 2 * t.n + 1;
-            const float* w0 = p.ws + ((size_t)t.e * p.ws_rows + (r0 < p.ws_rows ? r0 : p.ws_rows - 1)) * p.kblocks;
-            const float* w1 = p.ws + ((size_t)t.e * p.ws_rows + (r1 < p.ws_rows ? r1 : p.ws_rows - 1)) * p.kblocks;
-            const int have = t.t1 - t.t0;
-            // loaded kGxAhead K-blocks ahead: a load takes as long as several K-blocks of MMAs
-            float x[kGxAhead][4], a[kGxAhead], b[kGxAhead];
-            auto load = [&](int kb, float(&x)[4], float& a, float& b) {
-                if (kb >= sg.k1) return;
-                const float* xs = p.xs + kb * p.xs_ld + t.t0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = t00 + i * 32 < have ? xs[t00 + i * 32] : 0.f;
-                a = w0[kb];
-                b = p.glu != kGxPlain ? w1[kb] : 0.f;
-            };
-#pragma unroll
-            for (int d = 0; d < kGxAhead; ++d) load(sg.k0 + d, x[d], a[d], b[d]);
-            for (int kb = sg.k0; alive && kb < sg.k1; kb += kGxAhead) {
-#pragma unroll
-                for (int d = 0; d < kGxAhead; ++d) {
-                    if (kb + d >= sg.k1) break;
-                    alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), seg);
-                    if (!alive) break;
-                    float* to = scales + si * 512;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (t00 + i * 32 >= t.N) break;
-                        to[t00 + i * 32] = x[d][i] * a[d];
-                        if (p.glu != kGxPlain) to[256 + t00 + i * 32] = x[d][i] * b[d];
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sfull[si]);
-                    if (++si == kGxScales) {
-                        si = 0;
-                        sph ^= 1u;
-                    }
-                    load(kb + d + kGxAhead, x[d], a[d], b[d]);
-                }
-            }
-            ++seg;
-        }
     }
 
     __syncwarp();

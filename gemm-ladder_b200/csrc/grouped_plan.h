@@ -35,7 +35,8 @@ inline GxParams gx_params(int E, int T, int N, int K, GxForm form, bool bf16, bo
     p.cap = form.cap;
     p.box = tokens ? 128 : p.cap == 32 ? 16 : 32;
     p.wbox = glu == kGxPlain || tokens ? 128 : 64;
-    p.accs = 512 / p.cap < kGxAccs ? 512 / p.cap : kGxAccs;
+    p.group = form.kind == kGxF8Weights ? 128 / p.cap : 1;
+    p.accs = 512 / (p.cap * p.group) < kGxAccs ? 512 / (p.cap * p.group) : kGxAccs;
     p.stage_bytes = kGxXBytes + p.cap / 2 * 128;
     const int fixed = gx_smem(form.kind, 0, E).bytes + 1024;
     p.stages = (BW_SMEM_LIMIT - fixed) / p.stage_bytes;
@@ -91,10 +92,11 @@ inline DwParams dw_params(int E, int T, int N, int K, bool bf16, int out)
     p.idesc = idesc_16_f32_m(256, bf16, true, true);
     return p;
 }
+// (two counters per split tile, and the number of whole tiles given out)
 inline int dw_counters(const DwParams& p, int pairs)
 {
     const long long tiles = (long long)p.E * p.tn * p.tk;
-    return 2 * (int)(tiles <= kDwFewWaves * pairs ? tiles : tiles % pairs);
+    return 2 * (int)(tiles <= kDwFewWaves * pairs ? tiles : tiles % pairs) + 1;
 }
 
 }  // namespace bw

@@ -10,8 +10,9 @@
 // runs share a weight tile while it is in L2 and the weight tiles a run of tokens.
 //
 // Dealing: with `tiles` tiles on P pairs, the first tiles % P are split along K over all pairs (the K-blocks of those
-// tiles cut into P even ranges), then every pair takes the same number of whole tiles.  The parts of a split tile are
-// summed by the last pair to finish it, in the order of K, so results repeat bit for bit.
+// tiles cut into P even ranges), then the others go whole to whichever pair asks next (a counter in global memory: tiles
+// differ in their tokens; dealt out in turn, SMs were idle for a fifth of the time).  The parts of a split tile are summed by
+// the last pair to finish it, in the order of K, so results repeat bit for bit.
 #pragma once
 #include <cstdint>
 
@@ -70,7 +71,7 @@ struct GroupSeg {
     int k0, k1;  // its K-blocks [k0, k1)
 };
 
-// A pair's segments in order: its range of the split tiles, then its whole tiles.
+// A pair's segments in order: its range of the split tiles, then whole tiles.
 struct GroupWalk {
     long long u, uend;
     int tile;
@@ -83,7 +84,8 @@ struct GroupWalk {
         }
         tile = s.split + c;
     }
-    BW_GS bool next(const GroupSched& s, GroupSeg& g)
+    // its next range of a split tile
+    BW_GS bool next_part(const GroupSched& s, GroupSeg& g)
     {
         if (u < uend) {
             g.tile = (int)(u / s.kb);
@@ -93,10 +95,20 @@ struct GroupWalk {
             u = end > uend ? uend : end;
             return true;
         }
-        if (tile >= s.tiles) return false;
+        return false;
+    }
+    static BW_GS void whole(const GroupSched& s, int tile, GroupSeg& g)
+    {
         g.tile = tile;
         g.k0 = 0;
         g.k1 = s.kb;
+    }
+    // the same with the whole tiles dealt out in turn
+    BW_GS bool next(const GroupSched& s, GroupSeg& g)
+    {
+        if (next_part(s, g)) return true;
+        if (tile >= s.tiles) return false;
+        whole(s, tile, g);
         tile += s.pairs;
         return true;
     }
@@ -122,7 +134,7 @@ BW_GS void group_place(int j, int nt, int runs, int& m, int& n)
 // dW_e (N x K) in tiles of 256 rows x up to 256 columns; a tile's K-blocks are runs of 64 of expert e's rows (an expert without
 // rows: one unit that only writes zeros).  Tiles in the order of experts, `per` each.  The experts' lengths differ, so the
 // split tiles are dealt out by units (K-blocks): with few tiles all of them, else the first tiles % pairs; the others whole,
-// one pair after the other, so that the pairs work on the same expert's rows at a time.
+// to whichever pair asks next, so that the pairs work on the same expert's rows at a time.
 constexpr int kDwFewWaves = 4;
 
 struct DwSched {
@@ -174,7 +186,7 @@ struct DwWalk {
         tile = s.split + c;
         e = 0;
     }
-    BW_GS bool next(const DwSched& s, const int* off, const int* cum, DwSeg& g)
+    BW_GS bool next_part(const DwSched& s, const int* off, const int* cum, DwSeg& g)
     {
         if (u < uend) {
             while ((long long)s.per * cum[e + 1] <= u) ++e;
@@ -190,15 +202,16 @@ struct DwWalk {
             u = end > uend ? uend : end;
             return true;
         }
-        if (tile >= s.tiles) return false;
+        return false;
+    }
+    static BW_GS void whole(const DwSched& s, const int* off, int tile, DwSeg& g)
+    {
         g.e = tile / s.per;
         g.kb = dw_blocks(off[g.e + 1] - off[g.e]);
         g.tile = tile;
         g.k0 = 0;
         g.k1 = g.kb;
         g.u0 = 0;
-        tile += s.pairs;
-        return true;
     }
 };
 

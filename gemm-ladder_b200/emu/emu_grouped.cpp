@@ -116,8 +116,8 @@ EMU_API int bw_emu_grouped(const void* X, long long ldx, const float* xs, long l
     }
     p.offsets = offsets, p.C = C, p.xs = xs, p.xs_ld = xs_ld, p.ws = ws;
     std::vector<float> work(gx_work_bytes(pairs, p.cap) / 4, NAN);
-    std::vector<int> counters(2 * (size_t)pairs, 0);
-    p.work = work.data(), p.counters = counters.data();
+    std::vector<int> counters(2 * (size_t)pairs + 1, 0);
+    p.work = work.data(), p.counters = counters.data(), p.next = p.counters + 2 * pairs;
     p.wait_ns = emu::g_wait_ns;
     CUtensorMap mw, mx;
     const GxMaps m = gx_maps(p, K, ldx, kind != kGx16);
@@ -149,8 +149,8 @@ EMU_API int bw_emu_grouped_dw(const void* dY, long long ldy, const void* X, long
     }
     p.offsets = offsets, p.dW = dW;
     std::vector<float> work(gx_work_bytes(pairs, 256) / 4, NAN);
-    std::vector<int> counters((size_t)dw_counters(p, pairs) + 1, 0);
-    p.work = work.data(), p.counters = counters.data();
+    std::vector<int> counters((size_t)dw_counters(p, pairs), 0);
+    p.work = work.data(), p.counters = counters.data(), p.next = p.counters + counters.size() - 1;
     p.wait_ns = emu::g_wait_ns;
     CUtensorMap my, mx;
     map3(&my, dY, (uint64_t)N, (uint64_t)T, 1, (uint64_t)ldy, (uint64_t)ldy * T, 64);
