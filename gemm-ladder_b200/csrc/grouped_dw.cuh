@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
     const int S = p.stages;
+    const uint32_t limit = lean_limit(p.wait_ns);
 
     griddep_launch();
     if (threadIdx.x == 0) {
@@ -163,8 +164,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     // a warp's next descriptor (false: none left, or the wait gave up)
     auto next = [&](DwDesc& d, bool& alive) {
         const int at = asked % kGxDescs;
-        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, p.wait_ns,
-                                      site(3, 10, (uint32_t)at), asked);
+        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, limit,
+                                      site(3, 10, (uint32_t)at));
         if (!alive) return false;
         d = descs[at];
         __syncwarp();
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         while (next(d, alive)) {
             const int boxes = (d.width / 2 + 63) / 64;
             for (int kb = d.k0; d.rows > 0 && kb < d.k1; ++kb) {
-                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), asked);
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, limit, site(0, 1, stage));
                 if (!alive) break;
                 uint8_t* sy = smem + stage * kDwStageBytes;
                 const int t = d.t0 + kb * 64, y = d.n0 + rank * 128, x = d.c0 + rank * (d.width / 2);
@@ -210,8 +211,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA issuer
         if (leader) {
-            const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
-            const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
             const uint64_t dy = desc_mnmajor(smem_u32(smem), 0), dx = desc_mnmajor(smem_u32(smem) + 16384u, 0);
             int stage = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
@@ -219,11 +218,11 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             DwDesc t;
             while (next(t, alive)) {
                 if (t.rows == 0) continue;
-                alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), asked);
+                alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, limit, site(1, 3, acc));
                 const uint32_t idesc = p.idesc | idesc_n(t.width);
                 const uint32_t d = tmem_base + (uint32_t)(acc * 256);
                 for (int kb = t.k0; alive && kb < t.k1; ++kb) {
-                    alive = gx_warp_wait(&ready[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), asked);
+                    alive = gx_warp_wait(&ready[stage], ph, abort_flag, limit, site(1, 0, stage));
                     if (!alive) break;
                     tc_fence_after();
                     const uint64_t ad = dy + (uint64_t)((uint32_t)stage * (kDwStageBytes >> 4));
@@ -233,12 +232,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (k * 16 < here) mma_f16_pair(d, ad + 128 * k, bd + 128 * k, idesc, kb > t.k0 || k > 0 ? 1u : 0u);
-                        mma_commit_pair(empty0[0] + 8u * (uint32_t)stage);
-                        mma_commit_pair(empty0[1] + 8u * (uint32_t)stage);
-                        if (kb + 1 == t.k1) {
-                            mma_commit_pair(tfull0[0] + 8u * (uint32_t)acc);
-                            mma_commit_pair(tfull0[1] + 8u * (uint32_t)acc);
-                        }
+                        if (kb + 1 == t.k1) mma_commit_both(smem_u32(&tfull[acc]));
+                        mma_commit_both(smem_u32(&empty[stage]));
                     }
                     __syncwarp();
                     if (++stage == S) {
@@ -256,7 +251,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         } else if (lane == 0) {
             const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
             const GxQueue queue = {qfull, qempty, queue_tile, 0};
-            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, p.wait_ns);
+            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -272,9 +267,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             // one thread waits for the descriptor and tells the others, as in grouped_kernel.cuh
             const int at = asked % kGxDescs;
             if (threadIdx.x == kGxEpi0) {
-                const uint32_t bar = smem_u32(&dfull[at]), ph = (uint32_t)(asked / kGxDescs & 1);
-                const bool ok = alive && (mbar_try_wait(bar, ph) ||
-                                          wait_spin(bar, ph, abort_flag, p.wait_ns, site(2, 10, (uint32_t)at), asked));
+                const bool ok = alive && wait_lean(smem_u32(&dfull[at]), (uint32_t)(asked / kGxDescs & 1), abort_flag, limit,
+                                                   site(2, 10, (uint32_t)at));
                 epi_go[asked & 1] = ok && descs[at].e >= 0 ? 1 : 0;
             }
             named_bar_sync(1, kGxEpiThreads);
@@ -301,7 +295,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 for (int i = 0; i < nc; i += 16) store(i, z);
                 continue;
             }
-            if (alive) alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
+            alive = alive && gx_warp_wait(&tfull[acc], aph, abort_flag, limit, site(2, 2, (uint32_t)acc));
             tc_fence_after();
             const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * 256 + c0);
             auto slot_at = [&](int part, int i) {
@@ -387,7 +381,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         DwDesc t;
         while (next(t, alive)) {
             for (int kb = t.k0; t.rows > 0 && kb < t.k1; ++kb) {
-                alive = gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(4, 0, (uint32_t)stage), asked);
+                alive = gx_warp_wait(&full[stage], ph, abort_flag, limit, site(4, 0, (uint32_t)stage));
                 if (!alive) break;
                 const int here = t.rows - kb * 64;
                 if (here < 64 && here % 16) {
@@ -416,7 +410,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             DwDesc d = {};
             bool some = walk.next_part(s, off, cum, sg);
             if (!some) {
-                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, p.wait_ns);
+                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, limit);
                 if (!alive) break;
                 some = tile >= 0;
                 if (some) DwWalk::whole(s, off, tile, sg);
@@ -443,8 +437,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 d.e = -1;
             }
             const int at = i % kGxDescs;
-            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, p.wait_ns, site(5, 11, (uint32_t)at),
-                                 i);
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
             if (!alive) break;
             if (lane == 0) {
                 descs[at] = d;
@@ -463,6 +456,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, 512u);
     }
+    if (threadIdx.x == 0) record_abort(abort_flag);
 }
 
 }  // namespace bw

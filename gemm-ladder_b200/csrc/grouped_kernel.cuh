@@ -24,8 +24,8 @@
 // per expert the tokens are the M (kGxF8Tokens): a lane is a token with one scale, a half of the columns one block of
 // weights with another, and the product of the two is all a K-block needs.  Few tokens: the K-blocks go to the epilogue in
 // groups of 128 columns (4 K-blocks of 32 tokens), since a hand-over costs more than the sums of 32 columns.
-// Every wait is bounded (ptx.cuh); after one that gave up the epilogue goes on to the end of its segment without waiting or
-// writing, so that all its threads meet at every barrier, and then leaves.
+// Every wait is bounded (wait_lean, ptx.cuh).  A thread of the epilogue whose wait gave up goes on to the end of its segment
+// without waiting or writing, through every barrier and every instruction that its warp executes as one, and then leaves.
 #pragma once
 #include <type_traits>
 
@@ -132,18 +132,22 @@ struct GxFind {
     }
 };
 
-// Warp-uniform bounded wait: all lanes see the phase complete (and what it orders), or none goes on.
-__device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
-                                             uint32_t where, int seg)
+// A wait after which a warp goes on, or gives up, as one.
+__device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit_ns,
+                                             uint32_t where)
 {
     const uint32_t b = smem_u32(bar);
     if (__all_sync(0xFFFFFFFFu, mbar_try_wait(b, parity))) return true;
-    uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = wait_spin(b, parity, abort_flag, limit_ns, where, seg) ? 1u : 0u;
-    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-    if (ok) mbar_try_wait(b, parity);  // complete: this lane acquires too
-    return ok != 0;
+    return __all_sync(0xFFFFFFFFu, wait_lean(b, parity, abort_flag, limit_ns, where));
 }
+
+// An accumulator as the epilogue of kGxF8Tokens sees it: its tensor memory, its barriers, the phase it waits for next.
+struct GxAcc {
+    uint32_t tm;
+    uint64_t* full;
+    uint32_t empty;  // the leader's
+    uint32_t ph;
+};
 
 // Whole tiles on demand.  The first of a pair is its own; for the others one lane of the pair's second block (warp 1) draws
 // numbers from the call's counter, ahead of need, into a queue of kGxQueue entries in both blocks' shared memory (-1: none
@@ -155,13 +159,13 @@ struct GxQueue {
     int i;            // tiles this reader has asked for
 };
 __device__ __forceinline__ void gx_deal(const GxQueue& q, int* counter, int first, int tiles, volatile int* abort_flag,
-                                        uint64_t limit_ns)
+                                        uint32_t limit_ns)
 {
     const uint32_t other = mapa_shared(smem_u32(const_cast<int*>(q.tile)), 0), full0 = mapa_shared(smem_u32(q.full), 0);
     for (int i = 0;; ++i) {
         const int at = i % kGxQueue;
-        const uint32_t bar = smem_u32(&q.empty[at]), ph = (uint32_t)(i / kGxQueue & 1) ^ 1u;
-        if (!mbar_try_wait(bar, ph) && !wait_spin(bar, ph, abort_flag, limit_ns, site(6, 9, (uint32_t)at), i)) return;
+        if (!wait_lean(smem_u32(&q.empty[at]), (uint32_t)(i / kGxQueue & 1) ^ 1u, abort_flag, limit_ns, site(6, 9, (uint32_t)at)))
+            return;
         int t = first + atomicAdd(counter, 1);
         if (t >= tiles) t = -1;
         q.tile[at] = t;
@@ -173,11 +177,11 @@ __device__ __forceinline__ void gx_deal(const GxQueue& q, int* counter, int firs
 }
 // The next whole tile, by one warp; -1: none left, or the wait gave up (alive false).
 __device__ __forceinline__ int gx_next_tile(GxQueue& q, int own, int tiles, bool& alive, volatile int* abort_flag,
-                                            uint64_t limit_ns)
+                                            uint32_t limit_ns)
 {
     if (q.i++ == 0) return own < tiles ? own : -1;
     const int at = (q.i - 2) % kGxQueue;
-    alive = gx_warp_wait(&q.full[at], (uint32_t)((q.i - 2) / kGxQueue & 1), abort_flag, limit_ns, site(5, 9, (uint32_t)at), q.i);
+    alive = gx_warp_wait(&q.full[at], (uint32_t)((q.i - 2) / kGxQueue & 1), abort_flag, limit_ns, site(5, 9, (uint32_t)at));
     if (!alive) return -1;
     const int t = q.tile[at];
     __syncwarp();
@@ -401,6 +405,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     const bool leader = rank == 0;
     const int pairs = gridDim.x / 2, c = blockIdx.x / 2;
     const int S = p.stages;
+    const uint32_t limit = lean_limit(p.wait_ns);
     const int acc_cols = p.group * p.cap;       // columns of an accumulator
     const int tmem_cols = p.accs * acc_cols;    // a power of two, 256 or 512
 
@@ -458,8 +463,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     int asked = 0;
     auto next = [&](GxDesc& d, bool& alive) {
         const int at = asked % kGxDescs;
-        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, p.wait_ns,
-                                      site(3, 10, (uint32_t)at), asked);
+        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, limit,
+                                      site(3, 10, (uint32_t)at));
         if (!alive) return false;
         d = descs[at];
         __syncwarp();
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
             }
             for (int kb = t.k0; kb < t.k1; ++kb) {
-                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, p.wait_ns, site(0, 1, stage), asked);
+                alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, limit, site(0, 1, stage));
                 if (!alive) break;
                 uint8_t* sx = smem + stage * p.stage_bytes;
                 const uint32_t bar = full0 + 8u * (uint32_t)stage;
@@ -529,8 +534,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     } else if (warp == 1) {
         if (leader) {
             // ------------------------------------------------------ MMA issuer
-            const uint32_t empty0[2] = {mapa_shared(smem_u32(empty), 0), mapa_shared(smem_u32(empty), 1)};
-            const uint32_t tfull0[2] = {mapa_shared(smem_u32(tfull), 0), mapa_shared(smem_u32(tfull), 1)};
             // the descriptors' low words (a 16-byte step of the address is a step of 1) and their constant high words
             const uint64_t dx = !F8 && p.mn_major ? desc_mnmajor(smem_u32(smem), 0) : desc_kmajor(smem_u32(smem), 0);
             const uint64_t dy = desc_kmajor(smem_u32(smem) + kGxXBytes, 0);
@@ -544,17 +547,18 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 const uint32_t idesc = p.idesc | idesc_n(t.N);
                 int in_group = 0;
                 for (int kb = t.k0; kb < t.k1; ++kb) {
-                    GX_CLOCK(t_at = clock64());
-                    if (F8 ? in_group == 0 : kb == t.k0)
-                        alive = gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, p.wait_ns, site(1, 3, acc), asked);
-                    GX_CLOCK(w_acc += clock64() - t_at; t_at = clock64());
-                    alive = alive && gx_warp_wait(&full[stage], ph, abort_flag, p.wait_ns, site(1, 0, stage), asked);
-                    if (!alive) break;
-                    GX_CLOCK(w_full += clock64() - t_at; if (n_kb++ == 0 && lane == 0) BW_TRACE_AT(2));
-                    tc_fence_after();
                     const uint64_t ad = dx + (uint64_t)(step * (uint32_t)stage), bd = dy + (uint64_t)(step * (uint32_t)stage);
                     const uint32_t d = tmem_base + (uint32_t)(acc * acc_cols + in_group * p.cap);
                     const bool last = kb + 1 == t.k1 || (F8 && in_group + 1 == p.group);
+                    GX_CLOCK(t_at = clock64());
+                    alive = gx_warp_wait(&full[stage], ph, abort_flag, limit, site(1, 0, stage));
+                    GX_CLOCK(w_full += clock64() - t_at; if (n_kb++ == 0 && lane == 0) BW_TRACE_AT(2); t_at = clock64());
+                    // (the accumulator last: e4m3, it is what the MMAs wait for)
+                    if (F8 ? in_group == 0 : kb == t.k0)
+                        alive = alive && gx_warp_wait(&tempty[acc], aph ^ 1u, abort_flag, limit, site(1, 3, acc));
+                    GX_CLOCK(w_acc += clock64() - t_at);
+                    if (!alive) break;
+                    tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -564,12 +568,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                             else
                                 mma_f16_pair(d, ad + kx * k, bd + 2 * k, idesc, accumulate);
                         }
-                        mma_commit_pair(empty0[0] + 8u * (uint32_t)stage);
-                        mma_commit_pair(empty0[1] + 8u * (uint32_t)stage);
-                        if (last) {
-                            mma_commit_pair(tfull0[0] + 8u * (uint32_t)acc);
-                            mma_commit_pair(tfull0[1] + 8u * (uint32_t)acc);
-                        }
+                        if (last) mma_commit_both(smem_u32(&tfull[acc]));
+                        mma_commit_both(smem_u32(&empty[stage]));
                     }
                     __syncwarp();
                     if (F8) ++in_group;
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             // ------------------------------------------------------ whole tiles dealt out
             const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
             const GxQueue queue = {qfull, qempty, queue_tile, 0};
-            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, p.wait_ns);
+            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             GxDesc d = {};
             bool some = walk.next_part(s, sg);
             if (!some) {
-                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, p.wait_ns);
+                const int tile = gx_next_tile(queue, s.split + c, s.tiles, alive, abort_flag, limit);
                 if (!alive) break;
                 some = tile >= 0;
                 if (some) GroupWalk::whole(s, tile, sg);
@@ -633,8 +633,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 d.e = -1;
             }
             const int at = i % kGxDescs;
-            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, p.wait_ns, site(5, 11, (uint32_t)at),
-                                 i);
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
             if (!alive) break;
             if (lane == 0) {
                 descs[at] = d;
@@ -678,7 +677,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
 #pragma unroll
                 for (int d = 0; d < kGxBatch; ++d) load(t.k0 + d, x[d], a[d], b[d]);
                 for (int kb = t.k0; kb < t.k1; kb += kGxBatch) {
-                    alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, p.wait_ns, site(4, 13, (uint32_t)si), asked);
+                    alive = gx_warp_wait(&sempty[si], sph ^ 1u, abort_flag, limit, site(4, 13, (uint32_t)si));
                     if (!alive) break;
                     float* to = scales + si * kGxBatch * 256 + lane;
 #pragma unroll
@@ -713,13 +712,19 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         int acc = 0, si = 0;
         uint32_t aph = 0, sph = 0;
         bool alive = true;
-        auto release = [&](int a) {
+        // kGxF8Tokens: its two accumulators, the next to be used first
+        GxAcc acc_a = {quarter, &tfull[0], tempty0, 0u}, acc_b = {quarter + (uint32_t)p.cap, &tfull[1], tempty0 + 8u, 0u};
+        auto release = [&] {
             tc_fence_before();
             __syncwarp();
-            if (alive && lane == 0) mbar_arrive_remote_relaxed(tempty0 + 8u * (uint32_t)a);
+            if (alive && lane == 0) mbar_arrive_remote_relaxed(TOK ? acc_a.empty : tempty0 + 8u * (uint32_t)acc);
         };
         auto next_acc = [&] {
-            if (++acc == p.accs) {
+            if (TOK) {
+                const GxAcc x = acc_a;
+                acc_a = acc_b;
+                acc_b = x;
+            } else if (++acc == p.accs) {
                 acc = 0;
                 aph ^= 1u;
             }
@@ -728,9 +733,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             // one thread waits for the descriptor and tells the other 255, so that all of them go on to the same barriers, or none
             const GxDesc& t = descs[asked % kGxDescs];
             if (threadIdx.x == kGxEpi0) {
-                const uint32_t bar = smem_u32(&dfull[asked % kGxDescs]), ph = (uint32_t)(asked / kGxDescs & 1);
-                const bool ok = alive && (mbar_try_wait(bar, ph) || wait_spin(bar, ph, abort_flag, p.wait_ns,
-                                                                              site(2, 10, (uint32_t)(asked % kGxDescs)), asked));
+                const bool ok = alive && wait_lean(smem_u32(&dfull[asked % kGxDescs]), (uint32_t)(asked / kGxDescs & 1),
+                                                   abort_flag, limit, site(2, 10, (uint32_t)(asked % kGxDescs)));
                 epi_go[asked & 1] = ok && t.e >= 0 ? 1 : 0;
             }
             named_bar_sync(1, kGxEpiThreads);
@@ -745,116 +749,155 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             };
             auto in_tile = [&](int i) { return TOK ? col(i) < N : i * 16 < nc; };
             if constexpr (KIND == kGx16) {
-                if (alive)
-                    alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
+                alive = alive && gx_warp_wait(&tfull[acc], aph, abort_flag, limit, site(2, 2, (uint32_t)acc));
                 tc_fence_after();
             } else {
                 const int blocks = t.k1 - t.k0;
-                // The segment's scaled sums, and back into its last accumulator, where the code below takes them for all kinds.
-                // R: runs of 16 columns that this warp holds.
-                auto accumulate = [&](auto runs) {
-                    constexpr int R = decltype(runs)::value;
-                    uint64_t sum[R][8];  // 16 columns a run, as pairs
-#pragma unroll
-                    for (int i = 0; i < R; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
-                    for (int kb = 0;;) {
-                        if (alive && kb % kGxBatch == 0)
-                            alive = gx_warp_wait(&sfull[si], sph, abort_flag, p.wait_ns, site(2, 13, (uint32_t)si), asked);
-                        const float* sc = scales + (si * kGxBatch + kb % kGxBatch) * 256;
-                        uint64_t p0 = 0, p1 = 0;
-                        if (TOK) {
-                            const uint32_t s0 = __float_as_uint(sc[p.glu == kGxPlain ? h * 128 + row : row]);
-                            const uint32_t s1 = p.glu == kGxPlain ? s0 : __float_as_uint(sc[128 + row]);
-                            p0 = pair_f32(s0, s0);
-                            p1 = pair_f32(s1, s1);
-                        }
-                        if (alive)
-                            alive = gx_warp_wait(&tfull[acc], aph, abort_flag, p.wait_ns, site(2, 2, (uint32_t)acc), asked);
-                        if (alive) {
-                            tc_fence_after();
-                            if constexpr (TOK) {
-                                const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
-#pragma unroll
-                                for (int i = 0; i < 8; i += 2) {  // 32 columns leave tensor memory at a time
-                                    uint32_t r[2][16];
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j)
-                                        tmem_ld16(tm + (uint32_t)col(i + j), r[j]);  // (past the tile's: not used)
-                                    tmem_wait_ld();
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                                        for (int k = 0; k < 8; ++k)
-                                            sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1,
-                                                                      sum[i + j][k]);
-                                }
-                            } else {
-                                // the accumulator's K-blocks, 4 / R of them, cap columns each
-                                const uint32_t tm = quarter + (uint32_t)(acc * acc_cols + c0);
-                                const float* from = sc + (p.glu != kGxPlain && q >= 2 ? 128 : 0) + c0;
-#pragma unroll
-                                for (int w = 0; w < 4; w += 2) {
-                                    uint32_t r[2][16];
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j) {
-                                        const int u = w + j;
-                                        if (kb + u / R < blocks && u % R * 16 < nc)
-                                            tmem_ld16(tm + (uint32_t)(u / R * (R * 32) + u % R * 16), r[j]);
-                                    }
-                                    tmem_wait_ld();
-#pragma unroll
-                                    for (int j = 0; j < 2; ++j) {
-                                        const int u = w + j;
-                                        if (kb + u / R < blocks && u % R * 16 < nc) {
-#pragma unroll
-                                            for (int k = 0; k < 8; k += 2) {
-                                                uint64_t s0, s1;  // one address per warp: a broadcast
-                                                ld_shared_2b64(from + u / R * 256 + u % R * 16 + 2 * k, s0, s1);
-                                                uint64_t(&to)[8] = sum[u % R];
-                                                to[k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), s0, to[k]);
-                                                to[k + 1] = fma_f32x2(pair_f32(r[j][2 * k + 2], r[j][2 * k + 3]), s1, to[k + 1]);
-                                            }
-                                        }
-                                    }
-                                }
-                            }
-                        }
-                        kb += TOK ? 1 : 4 / R;
-                        if (kb % kGxBatch == 0 || kb >= blocks) {
-                            __syncwarp();  // every lane has read the scales
-                            if (alive && lane == 0) mbar_arrive(&sempty[si]);
-                            if (++si == kGxBatches) {
-                                si = 0;
-                                sph ^= 1u;
-                            }
-                        }
-                        if (kb >= blocks) break;
-                        release(acc);
-                        next_acc();
+                // this batch's scales have been read: the next
+                auto next_batch = [&] {
+                    __syncwarp();
+                    if (alive && lane == 0) mbar_arrive(&sempty[si]);
+                    if (++si == kGxBatches) {
+                        si = 0;
+                        sph ^= 1u;
                     }
-                    const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
+                };
+                auto wait_scales = [&] {
+                    alive = alive && gx_warp_wait(&sfull[si], sph, abort_flag, limit, site(2, 13, (uint32_t)si));
+                };
+                // The segment's scaled sums, and back into its last accumulator, where the code below takes them for all kinds.
+                if constexpr (TOK) {
+                    uint64_t sum[8][8];  // 8 runs of 16 columns, as pairs
 #pragma unroll
-                    for (int i = 0; i < R; ++i)
+                    for (int i = 0; i < 64; ++i) sum[i / 8][i % 8] = 0ull;
+                    // this token's scale with the weights of this warp's first 64 columns, and of the others
+                    const float* sc = scales + (p.glu == kGxPlain ? h * 128 : 0) + row;
+                    const int sc1 = p.glu == kGxPlain ? 0 : 128, ca = col(0), cb = col(4);
+                    int left = blocks, at = 0;  // K-blocks to come; of the batch, read
+                    wait_scales();
+                    float s0 = sc[si * kGxBatch * 256], s1 = sc[si * kGxBatch * 256 + sc1];
+                    // one K-block; false after the last, whose accumulator is kept
+                    auto block = [&](GxAcc& a) {
+                        const uint64_t p0 = pair_f32(__float_as_uint(s0), __float_as_uint(s0));
+                        const uint64_t p1 = pair_f32(__float_as_uint(s1), __float_as_uint(s1));
+                        alive = alive && gx_warp_wait(a.full, a.ph, abort_flag, limit, site(2, 2, 0));
+                        a.ph ^= 1u;
+                        tc_fence_after();
+                        --left;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {  // 32 columns leave tensor memory at a time
+                            uint32_t r[2][16];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)  // (past the tile's columns: not used)
+                                tmem_ld16(a.tm + (uint32_t)((i < 4 ? ca : cb) + (i + j) % 4 * 16), r[j]);
+                            tmem_wait_ld();
+                            if (i == 6 && left) {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (alive && lane == 0) mbar_arrive_remote_relaxed(a.empty);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+                                    sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1, sum[i + j][k]);
+                        }
+                        if (!left) return false;
+                        if (++at == kGxBatch) {
+                            at = 0;
+                            next_batch();
+                            wait_scales();
+                        }
+                        const float* x = sc + (si * kGxBatch + at) * 256;
+                        s0 = x[0];
+                        s1 = x[sc1];
+                        return true;
+                    };
+                    while (block(acc_a) && block(acc_b)) {
+                    }
+                    next_batch();
+                    if (blocks % 2 == 0) {  // the segment ended in the second: it comes first, as the one in use
+                        const GxAcc x = acc_a;
+                        acc_a = acc_b;
+                        acc_b = x;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
                         if (in_tile(i)) {
                             uint32_t r[16];
 #pragma unroll
                             for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
-                            tmem_st16(tm + (uint32_t)col(i), r);
+                            tmem_st16(acc_a.tm + (uint32_t)col(i), r);
                         }
                     tmem_wait_st();
-                };
-                if constexpr (TOK)
-                    accumulate(std::integral_constant<int, 8>());
-                else if (p.cap == 128)
-                    accumulate(std::integral_constant<int, 4>());
-                else if (p.cap == 64)
-                    accumulate(std::integral_constant<int, 2>());
-                else
-                    accumulate(std::integral_constant<int, 1>());
+                } else {
+                    // R: runs of 16 columns that this warp holds
+                    auto accumulate = [&](auto runs) {
+                        constexpr int R = decltype(runs)::value;
+                        uint64_t sum[R][8];
+#pragma unroll
+                        for (int i = 0; i < R; ++i)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sum[i][j] = 0ull;
+                        for (int kb = 0;;) {
+                            if (kb % kGxBatch == 0) wait_scales();
+                            alive = alive && gx_warp_wait(&tfull[acc], aph, abort_flag, limit, site(2, 2, (uint32_t)acc));
+                            tc_fence_after();
+                            // the accumulator's K-blocks, 4 / R of them, cap columns each
+                            const uint32_t tm = quarter + (uint32_t)(acc * acc_cols + c0);
+                            const float* from =
+                                scales + (si * kGxBatch + kb % kGxBatch) * 256 + (p.glu != kGxPlain && q >= 2 ? 128 : 0) + c0;
+#pragma unroll
+                            for (int w = 0; w < 4; w += 2) {
+                                uint32_t r[2][16];
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const int u = w + j;
+                                    if (kb + u / R < blocks && u % R * 16 < nc)
+                                        tmem_ld16(tm + (uint32_t)(u / R * (R * 32) + u % R * 16), r[j]);
+                                }
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const int u = w + j;
+                                    if (kb + u / R < blocks && u % R * 16 < nc) {
+#pragma unroll
+                                        for (int k = 0; k < 8; k += 2) {
+                                            uint64_t s0, s1;  // one address per warp: a broadcast
+                                            ld_shared_2b64(from + u / R * 256 + u % R * 16 + 2 * k, s0, s1);
+                                            uint64_t(&to)[8] = sum[u % R];
+                                            to[k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), s0, to[k]);
+                                            to[k + 1] = fma_f32x2(pair_f32(r[j][2 * k + 2], r[j][2 * k + 3]), s1, to[k + 1]);
+                                        }
+                                    }
+                                }
+                            }
+                            kb += 4 / R;
+                            if (kb % kGxBatch == 0 || kb >= blocks) next_batch();
+                            if (kb >= blocks) break;
+                            release();
+                            next_acc();
+                        }
+                        const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
+#pragma unroll
+                        for (int i = 0; i < R; ++i)
+                            if (in_tile(i)) {
+                                uint32_t r[16];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
+                                tmem_st16(tm + (uint32_t)col(i), r);
+                            }
+                        tmem_wait_st();
+                    };
+                    if (p.cap == 128)
+                        accumulate(std::integral_constant<int, 4>());
+                    else if (p.cap == 64)
+                        accumulate(std::integral_constant<int, 2>());
+                    else
+                        accumulate(std::integral_constant<int, 1>());
+                }
             }
-            const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
+            const uint32_t tm = TOK ? acc_a.tm : quarter + (uint32_t)(acc * acc_cols);
             // this segment's sum of 16 columns
             auto own = [&](int i, float(&v)[16]) {
                 uint32_t r[16];
@@ -953,7 +996,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     }
                 }
             }
-            release(acc);
+            release();
             next_acc();
             if (alive && lane == 0) mbar_arrive(&dempty[asked % kGxDescs]);  // (release met the warp: the descriptor has been read)
         }
@@ -968,7 +1011,10 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, (uint32_t)tmem_cols);
     }
-    if (threadIdx.x == 0) BW_TRACE_AT(5);
+    if (threadIdx.x == 0) {
+        record_abort(abort_flag);
+        BW_TRACE_AT(5);
+    }
 }
 
 }  // namespace bw

@@ -62,6 +62,20 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok != 0;
 }
 
+// The same without waiting at all (try_wait suspends the thread for a while before it says no).
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // ------------------------------------------------------------------ the device status word
 // [0]: status code (0 ok, 3 a bounded wait gave up); [1]: the first site that gave up (role << 16 | barrier id);
 // [2]: blockIdx.x of that block; [3]: the segment it was on.  Cleared by the host.
@@ -100,21 +114,38 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile i
     }
 }
 
-// The same in place, for kernels that move registers between warpgroups (they may not call functions).
-__device__ __forceinline__ bool wait_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns,
-                                          uint32_t where, int seg)
+// Spins on (bar, parity) in place: for kernels that move registers between warpgroups, which may not call functions, and for
+// waits inside a hot loop, where code that rarely runs costs instruction fetches (a wait with the whole of wait_slow in it
+// took 150 cycles more).  Gives up after `limit_ns` (at most 4 s) or when the block's abort flag rises; raises the flag with
+// `where`, which the block's end records (record_abort).  Threads that gave up and threads that did not go on together: a
+// caller whose warp must act as one votes.
+__device__ __forceinline__ uint32_t globaltimer_lo()
 {
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 31u) == 0) {
-            if (*abort_flag) return false;
-            if (globaltimer_ns() - t0 > limit_ns) {
-                record_timeout(abort_flag, where, seg);
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+__device__ __forceinline__ bool wait_lean(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit_ns,
+                                          uint32_t where)
+{
+    uint32_t n = 0, t0 = 0;
+    while (!mbar_try_wait(bar, parity)) {  // (one that fails takes 1.4 us)
+        if ((++n & 7u) == 0) {
+            const uint32_t t = globaltimer_lo();
+            if (n == 8u) t0 = t;
+            if (t - t0 > limit_ns || *abort_flag) {
+                if (!*abort_flag) *abort_flag = (int)where;
                 return false;
             }
         }
     }
+    return true;
+}
+__device__ __forceinline__ uint32_t lean_limit(uint64_t limit_ns) { return limit_ns < 4000000000ull ? (uint32_t)limit_ns : 4000000000u; }
+// By one thread of a block whose waits are wait_lean's, at its end.
+__device__ __forceinline__ void record_abort(volatile int* abort_flag)
+{
+    if (*abort_flag) record_timeout(abort_flag, (uint32_t)*abort_flag, 0);
 }
 
 __device__ __forceinline__ bool wait_bounded(uint64_t* barp, uint32_t parity, volatile int* abort_flag,
@@ -421,10 +452,19 @@ __device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uin
 
 // Arrives once on the barrier at shared::cluster address `bar` (this block's or the other block's of the pair) when
 // every tcgen05 operation the leader has issued so far has completed.  The pair's barriers in both blocks are reached
-// by one such commit each (no multicast form is used anywhere in this library).
+// by one such commit each (the grouped kernels reach both with one, mma_commit_both).
 __device__ __forceinline__ void mma_commit_pair(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// The same on the barrier at offset `bar` of both blocks of the pair: an arrival in each, no data.
+__device__ __forceinline__ void mma_commit_both(uint32_t bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
 }
 
 // Arrives once on `bar` when every tcgen05 operation issued so far by this thread has completed.

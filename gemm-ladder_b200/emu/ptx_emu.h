@@ -44,6 +44,8 @@ inline bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return emu::mb_try_wait(emu::cta_of(bar), emu::off_of(bar), parity);
 }
 
+inline bool mbar_test_wait(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity); }
+
 inline unsigned int g_status[4];
 inline thread_local unsigned int* t_status = g_status;  // the status word of the emulated GPU this thread runs on
 enum : uint32_t { kStatusTimeout = 3u };
@@ -89,9 +91,23 @@ inline bool wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, u
     }
 }
 
-inline bool wait_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns, uint32_t where, int seg)
+inline bool wait_lean(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit_ns, uint32_t where)
 {
-    return wait_slow(bar, parity, abort_flag, limit_ns, where, seg);
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+        spin_pause(i);
+        if (*abort_flag) return false;
+        if ((i & 31u) == 0 && globaltimer_ns() - t0 > limit_ns) {
+            *abort_flag = (int)where;
+            return false;
+        }
+    }
+    return true;
+}
+inline uint32_t lean_limit(uint64_t limit_ns) { return limit_ns < 4000000000ull ? (uint32_t)limit_ns : 4000000000u; }
+inline void record_abort(volatile int* abort_flag)
+{
+    if (*abort_flag) record_timeout(abort_flag, (uint32_t)*abort_flag, 0);
 }
 
 // ------------------------------------------------------------------ system scope (the emulated GPUs of one process)
@@ -283,6 +299,12 @@ inline void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_
 inline void mma_commit_pair(uint32_t bar)
 {
     emu::t_cta->tc.post([=] { emu::mb_arrive(emu::cta_of(bar), emu::off_of(bar), 0); });
+}
+inline void mma_commit_both(uint32_t bar)
+{
+    emu::t_cta->tc.post([=] {
+        for (int r = 0; r < 2; ++r) emu::mb_arrive(emu::t_cta->cluster->cta[r], emu::off_of(bar), 0);
+    });
 }
 inline void mma_commit(uint64_t* bar)
 {
