@@ -39,7 +39,7 @@ __host__ __device__ inline DwSmem dw_smem(int ring_bytes, int E)
     DwSmem m;
     m.buf = ring_bytes;
     m.bars = m.buf + 8 * kGxLineBytes;
-    m.misc = m.bars + (3 * kDwMaxStages + 5 + 2 * kGxQueue + 2 * kGxDescs) * 8;
+    m.misc = m.bars + (3 * kDwMaxStages + 5 + 2 + 2 * kGxDescs) * 8;
     m.misc = (m.misc + 15) / 16 * 16;
     m.tables = m.misc + 64 + kGxDescs * 64;
     m.bytes = m.tables + 2 * (E + 1) * 4;
@@ -102,14 +102,14 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     uint64_t* tempty = tfull + 2;
     uint64_t* drain = tempty + 2;
     uint64_t* qfull = drain + 1;
-    uint64_t* qempty = qfull + kGxQueue;
-    uint64_t* dfull = qempty + kGxQueue;
+    uint64_t* qasked = qfull + 1;
+    uint64_t* dfull = qasked + 1;
     uint64_t* dempty = dfull + kGxDescs;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* reduce_flag = abort_flag + 1;
     volatile int* epi_go = abort_flag + 2;      // two, alternating
-    volatile int* queue_tile = abort_flag + 4;  // kGxQueue entries
+    volatile int* queue_tile = abort_flag + 4;
     DwDesc* descs = reinterpret_cast<DwDesc*>(smem + L.misc + 64);
     int* off = reinterpret_cast<int*>(smem + L.tables);
     int* cum = off + p.E + 1;
@@ -133,10 +133,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&tempty[i], 16);
         }
         mbar_init(drain, 1);
-        for (int i = 0; i < kGxQueue; ++i) {
-            mbar_init(&qfull[i], 1);
-            mbar_init(&qempty[i], 2);  // both blocks' plans
-        }
+        mbar_init(qfull, 1);
+        mbar_init(qasked, 2);  // both blocks' plans
         for (int i = 0; i < kGxDescs; ++i) {
             mbar_init(&dfull[i], 1);
             mbar_init(&dempty[i], 10u + (leader ? 1u : 0u));  // producer, warp 2, epilogue, MMA issuer
@@ -201,13 +199,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 }
             }
         }
-        if (lane == 0) {
-            const int n = issued < S ? issued : S;
-            for (int i = 1; i <= n; ++i) {
-                const int q = issued - i;
-                wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
-            }
-        }
+        if (lane == 0) gx_drain(full, issued, S, p.wait_ns);
     } else if (warp == 1) {
         // ---------------------------------------------------------- MMA issuer
         if (leader) {
@@ -250,8 +242,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             }
         } else if (lane == 0) {
             const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
-            const GxQueue queue = {qfull, qempty, queue_tile, 0};
-            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
+            const GxQueue queue = {qfull, qasked, queue_tile, 0};
+            if (s.split + c < s.tiles)  // (else the plans ask for nothing)
+                gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -307,61 +300,37 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const int first = t.first, last = t.last;
             if (first != last) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
-                int* counter = p.counters + t.tile * 2 + rank;
+#pragma unroll 1
+                for (int i = 0; i < nc; i += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(tm + (uint32_t)i, r);
+                    tmem_wait_ld();
+                    if (alive) {
+                        float4* to = slot_at(c, i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            __stcg(to + j * 128, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                             __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
+                    }
+                }
                 named_bar_sync(1, kGxEpiThreads);
-                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
+                if (threadIdx.x == kGxEpi0)
+                    *reduce_flag = alive && atom_add_acq_rel_gpu(p.counters + t.tile * 2 + rank, 1) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
                 done = *reduce_flag != 0;
-                if (!done) {
-#pragma unroll 1
-                    for (int i = 0; i < nc; i += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(tm + (uint32_t)i, r);
-                        tmem_wait_ld();
-                        if (alive) {
-                            float4* to = slot_at(c, i);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                __stcg(to + j * 128, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                                                 __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
-                        }
-                    }
-                    named_bar_sync(1, kGxEpiThreads);
-                    if (threadIdx.x == kGxEpi0)
-                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == last - first ? 1 : 0;
-                    named_bar_sync(1, kGxEpiThreads);
-                    done = *reduce_flag != 0;
-                }
             }
             if (done) {
 #pragma unroll 1
                 for (int i = 0; i < nc; i += 16) {
-                    uint32_t r[16];
                     float v[16];
-                    tmem_ld16(tm + (uint32_t)i, r);
-                    tmem_wait_ld();
                     if (first == last) {
+                        uint32_t r[16];
+                        tmem_ld16(tm + (uint32_t)i, r);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
                     } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                        for (int part = first; part <= last; ++part) {
-                            if (part == c) {
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
-                                continue;
-                            }
-                            const float4* from = slot_at(part, i);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 x = __ldcg(from + j * 128);
-                                v[4 * j] += x.x;
-                                v[4 * j + 1] += x.y;
-                                v[4 * j + 2] += x.z;
-                                v[4 * j + 3] += x.w;
-                            }
-                        }
+                        gx_sum_parts<4>(v, first, last, [&](int part) { return slot_at(part, i); });
                     }
                     store(i, v);
                 }
@@ -402,10 +371,13 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     } else {
         // ---------------------------------------------------------- plan
         const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
-        GxQueue queue = {qfull, qempty, queue_tile, 0};
+        GxQueue queue = {qfull, qasked, queue_tile, 0};
         DwWalk walk(s, c);
         bool alive = true;
-        for (int i = 0; alive; ++i) {
+        for (int i = 0;; ++i) {
+            const int at = i % kGxDescs;
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
+            if (!alive) break;
             DwSeg sg;
             DwDesc d = {};
             bool some = walk.next_part(s, off, cum, sg);
@@ -436,9 +408,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             } else {
                 d.e = -1;
             }
-            const int at = i % kGxDescs;
-            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
-            if (!alive) break;
             if (lane == 0) {
                 descs[at] = d;
                 mbar_arrive(&dfull[at]);

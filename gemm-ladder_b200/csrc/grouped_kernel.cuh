@@ -47,13 +47,12 @@ constexpr int kGxXBytes = 128 * 128;  // a block's weight rows of a stage
 constexpr int kGxMaxStages = 12;
 constexpr int kGxBatch = 4;           // K-blocks whose scale products are handed over at once
 constexpr int kGxBatches = 2;         // such batches held
-constexpr int kGxDescs = 4;           // descriptors held
-constexpr int kGxQueue = 4;           // whole tiles dealt ahead
+constexpr int kGxDescs = 4;           // descriptors held at most
 constexpr int kGxOtherRegs = 72, kGxEpiRegs = 216;
 static_assert(128 * kGxOtherRegs + 256 * kGxEpiRegs <= kGxThreads * 168, "registers moved within what the launch holds");
 constexpr int kGxAccs = 8;            // accumulators in tensor memory at most
 constexpr int kGxScaleBytes = kGxBatches * kGxBatch * 2 * 128 * 4;  // [batch][K-block][gate, up or half][token]
-constexpr int kGxBars = 2 * kGxMaxStages + 2 * kGxAccs + 2 * kGxBatches + 2 * kGxDescs + 2 * kGxQueue + 1;
+constexpr int kGxBars = 2 * kGxMaxStages + 2 * kGxAccs + 2 * kGxBatches + 2 * kGxDescs + 2 + 1;
 
 // fp16 or bf16; e4m3 with the weight rows as the MMA's M; e4m3 with the tokens as its M.
 enum : int { kGx16 = 0, kGxF8Weights = 1, kGxF8Tokens = 2 };
@@ -67,6 +66,7 @@ struct GxParams {
     int nt, kblocks;       // weight tiles per expert, K-blocks
     int cap, box, wbox;    // the most tokens of a tile; rows of one TMA box of X, of W
     int stages, stage_bytes, ring_bytes;
+    int descs;             // descriptors held: tiles planned ahead
     int accs, group;       // accumulators in tensor memory; K-blocks of one (e4m3), cap columns each
     int mn_major;          // W is E x K x N
     int glu, out;          // kGx*; BW_TYPE_* (0 fp16, 1 bf16, 2 fp32)
@@ -141,6 +141,17 @@ __device__ __forceinline__ bool gx_warp_wait(uint64_t* bar, uint32_t parity, vol
     return __all_sync(0xFFFFFFFFu, wait_lean(b, parity, abort_flag, limit_ns, where));
 }
 
+// The stages still on their way, of `issued`, within one limit for all (the other block of an aborted pair may not have sent its
+// half).
+__device__ __forceinline__ void gx_drain(uint64_t* full, int issued, int S, uint64_t limit_ns)
+{
+    const uint64_t t0 = globaltimer_ns();
+    if (limit_ns < 1000000000ull) limit_ns = 1000000000ull;
+    for (int q = issued < S ? 0 : issued - S; q < issued; ++q)
+        while (!mbar_try_wait(smem_u32(&full[q % S]), (uint32_t)((q / S) & 1)))
+            if (globaltimer_ns() - t0 > limit_ns) return;
+}
+
 // An accumulator as the epilogue of kGxF8Tokens sees it: its tensor memory, its barriers, the phase it waits for next.
 struct GxAcc {
     uint32_t tm;
@@ -149,29 +160,27 @@ struct GxAcc {
     uint32_t ph;
 };
 
-// Whole tiles on demand.  The first of a pair is its own; for the others one lane of the pair's second block (warp 1) draws
-// numbers from the call's counter, ahead of need, into a queue of kGxQueue entries in both blocks' shared memory (-1: none
-// left), and reuses an entry once all the pair's readers have read it.
+// Whole tiles on demand.  A pair's first is its own; for each of the others the plans of both blocks ask (q.asked), and one lane
+// of the second block (warp 1) draws a number from the call's counter and hands it to both (-1: none left).  Nothing is drawn
+// ahead of need: with four tiles drawn ahead, pairs of 6 tiles each ended between 141 and 282 us.
 struct GxQueue {
-    uint64_t* full;   // an entry is there (each block's own)
-    uint64_t* empty;  // the second block's count
+    uint64_t* full;   // the tile is there (each block's own)
+    uint64_t* asked;  // the second block's: both have asked
     volatile int* tile;
-    int i;            // tiles this reader has asked for
+    int i;            // tiles asked for
 };
 __device__ __forceinline__ void gx_deal(const GxQueue& q, int* counter, int first, int tiles, volatile int* abort_flag,
                                         uint32_t limit_ns)
 {
     const uint32_t other = mapa_shared(smem_u32(const_cast<int*>(q.tile)), 0), full0 = mapa_shared(smem_u32(q.full), 0);
-    for (int i = 0;; ++i) {
-        const int at = i % kGxQueue;
-        if (!wait_lean(smem_u32(&q.empty[at]), (uint32_t)(i / kGxQueue & 1) ^ 1u, abort_flag, limit_ns, site(6, 9, (uint32_t)at)))
-            return;
+    for (uint32_t i = 0;; ++i) {
+        if (!wait_lean(smem_u32(q.asked), i & 1u, abort_flag, limit_ns, site(6, 9, 0))) return;
         int t = first + atomicAdd(counter, 1);
         if (t >= tiles) t = -1;
-        q.tile[at] = t;
-        st_cluster_f32(other + 4u * (uint32_t)at, __int_as_float(t));
-        mbar_arrive(&q.full[at]);
-        mbar_arrive_cluster(full0 + 8u * (uint32_t)at);
+        *q.tile = t;
+        st_cluster_f32(other, __int_as_float(t));
+        mbar_arrive(q.full);
+        mbar_arrive_cluster(full0);
         if (t < 0) return;
     }
 }
@@ -180,13 +189,10 @@ __device__ __forceinline__ int gx_next_tile(GxQueue& q, int own, int tiles, bool
                                             uint32_t limit_ns)
 {
     if (q.i++ == 0) return own < tiles ? own : -1;
-    const int at = (q.i - 2) % kGxQueue;
-    alive = gx_warp_wait(&q.full[at], (uint32_t)((q.i - 2) / kGxQueue & 1), abort_flag, limit_ns, site(5, 9, (uint32_t)at));
-    if (!alive) return -1;
-    const int t = q.tile[at];
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive_remote(mapa_shared(smem_u32(&q.empty[at]), 1));
-    return t;
+    __syncwarp();  // the last answer has been read
+    if ((threadIdx.x & 31) == 0) mbar_arrive_remote(mapa_shared(smem_u32(q.asked), 1));
+    alive = gx_warp_wait(q.full, (uint32_t)(q.i & 1), abort_flag, limit_ns, site(5, 9, 0));
+    return alive ? *q.tile : -1;
 }
 
 // 16 tokens x 32 columns of C: v[j] is token tb + j, column f + lane.  Through the warp's buffer, so that a token's 32
@@ -366,6 +372,36 @@ __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum,
     }
 }
 
+// v = the sum of 16 columns over the parts [first, last] in their order, each at at(part) and 128 vectors on.  U parts are on
+// their way at once (one at a time, a tile split in 8 took 100 us to sum).
+template <int U, class F>
+__device__ __forceinline__ void gx_sum_parts(float (&v)[16], int first, int last, F at)
+{
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = 0.f;
+#pragma unroll 1
+    for (int part = first; part <= last; part += U) {
+        float4 x[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float4* from = at(part + u <= last ? part + u : last);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][j] = __ldcg(from + j * 128);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (part + u > last) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[4 * j] += x[u][j].x;
+                v[4 * j + 1] += x[u][j].y;
+                v[4 * j + 2] += x[u][j].z;
+                v[4 * j + 3] += x[u][j].w;
+            }
+        }
+    }
+}
+
 template <int KIND>
 __global__ void __launch_bounds__(kGxThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const GxParams p)
@@ -388,13 +424,13 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     uint64_t* dfull = sempty + kGxBatches;
     uint64_t* dempty = dfull + kGxDescs;
     uint64_t* qfull = dempty + kGxDescs;
-    uint64_t* qempty = qfull + kGxQueue;
-    uint64_t* drain = qempty + kGxQueue;
+    uint64_t* qasked = qfull + 1;
+    uint64_t* drain = qasked + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* reduce_flag = abort_flag + 1;
     volatile int* epi_go = abort_flag + 2;      // two, alternating
-    volatile int* queue_tile = abort_flag + 4;  // kGxQueue entries
+    volatile int* queue_tile = abort_flag + 4;
     GxDesc* descs = reinterpret_cast<GxDesc*>(smem + L.misc + 64);
     float* scales = reinterpret_cast<float*>(smem + L.scales);
     int* off = reinterpret_cast<int*>(smem + L.tables);
@@ -431,10 +467,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             mbar_init(&dfull[i], 1);
             mbar_init(&dempty[i], 9u + (leader ? 1u : 0u) + (F8 ? 1u : 0u));  // producer, epilogue, MMA issuer, scales
         }
-        for (int i = 0; i < kGxQueue; ++i) {
-            mbar_init(&qfull[i], 1);
-            mbar_init(&qempty[i], 2);  // both blocks' plans
-        }
+        mbar_init(qfull, 1);
+        mbar_init(qasked, 2);  // both blocks' plans
         mbar_init(drain, 1);
         *abort_flag = 0;
         *reduce_flag = 0;
@@ -462,8 +496,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
     // a warp's next descriptor (false: none left, or the wait gave up)
     int asked = 0;
     auto next = [&](GxDesc& d, bool& alive) {
-        const int at = asked % kGxDescs;
-        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / kGxDescs & 1), abort_flag, limit,
+        const int at = asked % p.descs;
+        alive = alive && gx_warp_wait(&dfull[at], (uint32_t)(asked / p.descs & 1), abort_flag, limit,
                                       site(3, 10, (uint32_t)at));
         if (!alive) return false;
         d = descs[at];
@@ -525,11 +559,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             }
         }
         if (leader && lane == 0) {  // loads in flight land before the blocks may leave (after an abort; else they have landed)
-            const int n = issued < S ? issued : S;
-            for (int i = 1; i <= n; ++i) {
-                const int q = issued - i;
-                wait_drain(&full[q % S], (uint32_t)((q / S) & 1), p.wait_ns);
-            }
+            gx_drain(full, issued, S, p.wait_ns);
         }
     } else if (warp == 1) {
         if (leader) {
@@ -600,18 +630,22 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         } else if (lane == 0) {
             // ------------------------------------------------------ whole tiles dealt out
             const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-            const GxQueue queue = {qfull, qempty, queue_tile, 0};
-            gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
+            const GxQueue queue = {qfull, qasked, queue_tile, 0};
+            if (s.split + c < s.tiles)  // (else the plans ask for nothing)
+                gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
         __syncwarp();
     } else if (warp == 2) {
         // ---------------------------------------------------------- plan
         const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-        GxQueue queue = {qfull, qempty, queue_tile, 0};
+        GxQueue queue = {qfull, qasked, queue_tile, 0};
         GroupWalk walk(s, c);
         GxFind find;
         bool alive = true;
-        for (int i = 0; alive; ++i) {
+        for (int i = 0;; ++i) {
+            const int at = i % p.descs;
+            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / p.descs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
+            if (!alive) break;
             GroupSeg sg;
             GxDesc d = {};
             bool some = walk.next_part(s, sg);
@@ -632,9 +666,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             } else {
                 d.e = -1;
             }
-            const int at = i % kGxDescs;
-            alive = gx_warp_wait(&dempty[at], (uint32_t)(i / kGxDescs & 1) ^ 1u, abort_flag, limit, site(5, 11, (uint32_t)at));
-            if (!alive) break;
             if (lane == 0) {
                 descs[at] = d;
                 mbar_arrive(&dfull[at]);
@@ -731,10 +762,10 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         };
         for (;; ++asked) {
             // one thread waits for the descriptor and tells the other 255, so that all of them go on to the same barriers, or none
-            const GxDesc& t = descs[asked % kGxDescs];
+            const GxDesc& t = descs[asked % p.descs];
             if (threadIdx.x == kGxEpi0) {
-                const bool ok = alive && wait_lean(smem_u32(&dfull[asked % kGxDescs]), (uint32_t)(asked / kGxDescs & 1),
-                                                   abort_flag, limit, site(2, 10, (uint32_t)(asked % kGxDescs)));
+                const bool ok = alive && wait_lean(smem_u32(&dfull[asked % p.descs]), (uint32_t)(asked / p.descs & 1),
+                                                   abort_flag, limit, site(2, 10, (uint32_t)(asked % p.descs)));
                 epi_go[asked & 1] = ok && t.e >= 0 ? 1 : 0;
             }
             named_bar_sync(1, kGxEpiThreads);
@@ -911,30 +942,23 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             if (first != last) {
                 // a part of a split tile: the last block to finish sums all parts in the order of K
                 const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-                int* counter = p.counters + tile * 2 + rank;
-                named_bar_sync(1, kGxEpiThreads);  // the flag of an earlier tile has been read
-                if (threadIdx.x == kGxEpi0) *reduce_flag = alive && ld_acquire_gpu(counter) == last - first ? 1 : 0;
+                const int slot = part_slot(s, c, tile);
+#pragma unroll 1
+                for (int i = 0; i < 8 && in_tile(i); ++i) {
+                    float v[16];
+                    own(i, v);
+                    if (alive) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            __stcg(gx_slot(p, slot, rank, row, col(i) / 4 + j),
+                                   make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    }
+                }
+                named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
+                if (threadIdx.x == kGxEpi0)
+                    *reduce_flag = alive && atom_add_acq_rel_gpu(p.counters + tile * 2 + rank, 1) == last - first ? 1 : 0;
                 named_bar_sync(1, kGxEpiThreads);
                 done = *reduce_flag != 0;
-                if (!done) {
-                    const int slot = part_slot(s, c, tile);
-#pragma unroll 1
-                    for (int i = 0; i < 8 && in_tile(i); ++i) {
-                        float v[16];
-                        own(i, v);
-                        if (alive) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                __stcg(gx_slot(p, slot, rank, row, col(i) / 4 + j),
-                                       make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                        }
-                    }
-                    named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
-                    if (threadIdx.x == kGxEpi0)
-                        *reduce_flag = alive && atom_add_acq_rel_gpu(counter, 1) == last - first ? 1 : 0;
-                    named_bar_sync(1, kGxEpiThreads);
-                    done = *reduce_flag != 0;
-                }
             }
             // the tile's sum of 16 columns
             auto total = [&](int i, float(&v)[16]) {
@@ -943,26 +967,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     return;
                 }
                 const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-                float mine[16];
-                own(i, mine);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                for (int part = first; part <= last; ++part) {
-                    if (part == c) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] += mine[j];
-                        continue;
-                    }
-                    const int slot = part_slot(s, part, tile);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float4 x = __ldcg(gx_slot(p, slot, rank, row, col(i) / 4 + j));
-                        v[4 * j] += x.x;
-                        v[4 * j + 1] += x.y;
-                        v[4 * j + 2] += x.z;
-                        v[4 * j + 3] += x.w;
-                    }
-                }
+                gx_sum_parts<4>(v, first, last, [&](int part) {
+                    return gx_slot(p, part_slot(s, part, tile), rank, row, col(i) / 4);
+                });
             };
             if (done) {
                 if constexpr (TOK) {
@@ -998,7 +1005,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             }
             release();
             next_acc();
-            if (alive && lane == 0) mbar_arrive(&dempty[asked % kGxDescs]);  // (release met the warp: the descriptor has been read)
+            if (alive && lane == 0) mbar_arrive(&dempty[asked % p.descs]);  // (release met the warp: the descriptor has been read)
         }
         if (threadIdx.x == kGxEpi0) BW_TRACE_AT(4);
     }

@@ -97,14 +97,14 @@ inline bool wait_lean(uint32_t bar, uint32_t parity, volatile int* abort_flag, u
     for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
         spin_pause(i);
         if (*abort_flag) return false;
-        if ((i & 31u) == 0 && globaltimer_ns() - t0 > limit_ns) {
+        if ((i & 31u) == 0 && globaltimer_ns() - t0 > limit_ns * 1000000ull) {
             *abort_flag = (int)where;
             return false;
         }
     }
     return true;
 }
-inline uint32_t lean_limit(uint64_t limit_ns) { return limit_ns < 4000000000ull ? (uint32_t)limit_ns : 4000000000u; }
+inline uint32_t lean_limit(uint64_t limit_ns) { return (uint32_t)(limit_ns / 1000000u); }  // (here milliseconds: the host is slow)
 inline void record_abort(volatile int* abort_flag)
 {
     if (*abort_flag) record_timeout(abort_flag, (uint32_t)*abort_flag, 0);
