@@ -562,12 +562,6 @@ def _f8(t, what, dim, device):
         raise ValueError(f"{what} must be a contiguous {dim}-D float8_e4m3fn tensor on one device with the others")
 
 
-def _f8_scales(rows, cols, like):
-    """Scales of rows x cols stored column by column, each column on 16 bytes."""
-    blocks = -(-cols // F8_BLOCK)
-    return like.new_empty((blocks, (rows + 3) // 4 * 4), dtype=torch.float32)[:, :rows].t()
-
-
 def _f8_scale_ld(scale, rows, cols, device, what):
     """Elements from column to column of a rows x blocks scale tensor stored column by column."""
     blocks = -(-cols // F8_BLOCK)
@@ -589,9 +583,11 @@ def quantize_f8(X, Q=None, scale=None, stream=None):
         _out(Q, X, rows, cols, torch.float8_e4m3fn, "Q")
 
     def call(s):
-        q = _out(Q, X, rows, cols, torch.float8_e4m3fn, "Q")
-        sc = _f8_scales(rows, cols, X) if scale is None else scale
-        n = _f8_scale_ld(sc, rows, cols, X.device, "scale") if lds is None else lds
+        q = X.new_empty((rows, cols), dtype=torch.float8_e4m3fn) if Q is None else Q
+        sc, n = scale, lds
+        if sc is None:  # column by column, each column on 16 bytes
+            n = (rows + 3) // 4 * 4
+            sc = X.new_empty_strided((rows, -(-cols // F8_BLOCK)), (1, n), dtype=torch.float32)
         check(lib().bw_quant_f8(X.data_ptr(), code, ld, q.data_ptr(), sc.data_ptr(), n, rows, cols, s))
         return q, sc
 
@@ -625,18 +621,23 @@ def quantize_blocks_f8(W, Q=None, scale=None, stream=None):
 
 def _f8_weight(B, b_scale, offsets, K, device):
     """(E, N) of a weight: E 0 without offsets."""
-    _f8(B, "B", 2 if offsets is None else 3, device)
-    if B.shape[-1] != K:
-        raise ValueError(f"A's rows have {K} columns but B is {tuple(B.shape)}")
-    N = B.shape[-2]
-    shape = (*B.shape[:-2], -(-N // F8_BLOCK), -(-K // F8_BLOCK))
-    if b_scale.dtype != torch.float32 or tuple(b_scale.shape) != shape or b_scale.device != device or \
+    dim = 2 if offsets is None else 3
+    if B.dtype != torch.float8_e4m3fn or B.dim() != dim or B.device != device or not B.is_contiguous():
+        raise ValueError(f"B must be a contiguous {dim}-D float8_e4m3fn tensor on one device with the others")
+    shape = B.shape
+    N = shape[-2]
+    if shape[-1] != K:
+        raise ValueError(f"A's rows have {K} columns but B is {tuple(shape)}")
+    sizes = b_scale.shape
+    if b_scale.dtype != torch.float32 or len(sizes) != dim or sizes[-1] != -(-K // F8_BLOCK) or \
+            sizes[-2] != -(-N // F8_BLOCK) or sizes[0] != (shape[0] if dim == 3 else sizes[0]) or b_scale.device != device or \
             not b_scale.is_contiguous():
-        raise ValueError(f"b_scale must be a contiguous fp32 tensor of {shape} on B's device")
-    if offsets is None:
+        raise ValueError(f"b_scale must be a contiguous fp32 tensor on B's device, a scale for each 128 x 128 block of B "
+                         f"{tuple(shape)}")
+    if dim == 2:
         return 0, N
-    _offsets(offsets, device, B.shape[0])
-    return B.shape[0], N
+    _offsets(offsets, device, shape[0])
+    return shape[0], N
 
 
 def gemm_f8(A, a_scale, B, b_scale, offsets=None, C=None, dtype=None, swiglu=False, stream=None):

@@ -53,22 +53,23 @@ GxWork gx_work(int T, int K, int cap, int pairs, bool linear)
     return w;
 }
 
-template <int KIND>
-int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CUtensorMap& mx, int pairs, bool pdl,
-              cudaStream_t st)
+// A kernel on pairs of SMs, overlapping with the one ahead of it on the stream, which is the call's own and launched in plain
+// stream order.
+template <class P>
+int launch_pairs(DeviceState& d, void (*kernel)(CUtensorMap, CUtensorMap, P), std::atomic<bool>* limit_set, const CUtensorMap& m0,
+                 const CUtensorMap& m1, const P& p, int pairs, int smem, cudaStream_t st)
 {
-    static std::atomic<bool> limit_set[kMaxDevices];  // the kernel's shared-memory limit, once per device
-    std::atomic<bool>& done = limit_set[&d - g_dev];
+    std::atomic<bool>& done = limit_set[&d - g_dev];  // the kernel's shared-memory limit, once per device
     cudaError_t e;
     if (!done.load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(grouped_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, BW_SMEM_LIMIT);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BW_SMEM_LIMIT);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
         done.store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * pairs));
     cfg.blockDim = dim3(kGxThreads);
-    cfg.dynamicSmemBytes = (size_t)(1024 + gx_smem(KIND, p.ring_bytes, p.E).bytes);
+    cfg.dynamicSmemBytes = (size_t)(1024 + smem);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -78,13 +79,26 @@ int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CU
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, grouped_kernel<KIND>, mw, mx, p);
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, kernel, m0, m1, p);
     return e == cudaSuccess ? BW_OK : cuda_fail(e, "kernel launch (grouped)");
 }
+int zero_counters(int* counters, int n, cudaStream_t st)
+{
+    gx_zero_kernel<<<1, 256, 0, st>>>(counters, n);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? BW_OK : cuda_fail(e, "kernel launch (counters)");
+}
 
-// The product of p (its addresses but C's workspace filled in); zeroed: the counters are zero already, by a kernel that the
-// launch may overlap.
+template <int KIND>
+int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CUtensorMap& mx, int pairs, cudaStream_t st)
+{
+    static std::atomic<bool> limit_set[kMaxDevices];
+    return launch_pairs(d, grouped_kernel<KIND>, limit_set, mw, mx, p, pairs, gx_smem(KIND, p.ring_bytes, p.E).bytes, st);
+}
+
+// The product of p (its addresses but the workspace's filled in); zeroed: the kernel ahead of it on the stream, one of the
+// call's own launched in plain order, zeroes the counters.
 int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m, const void* X, const void* W, const GxWork& w, uint8_t* work,
                int pairs, bool zeroed, cudaStream_t st)
 {
@@ -92,20 +106,20 @@ int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m,
     p.counters = reinterpret_cast<int*>(work + w.counters);
     p.next = p.counters + 2 * pairs;
     p.wait_ns = g_wait_ns;
-    if (!zeroed) {
-        cudaError_t e = cudaMemsetAsync(p.counters, 0, (size_t)w.n_counters * sizeof(int), st);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync (counters)");
-    }
     CUtensorMap mw, mx;
     if (!moe_map(&mw, W, 0, m.w[0], m.w[1], m.w[2], m.w[3], m.w[4], (uint32_t)m.w[5]) ||
         !moe_map(&mx, X, 0, m.x[0], m.x[1], m.x[2], m.x[3], m.x[4], (uint32_t)m.x[5])) {
         snprintf(g_errbuf, sizeof g_errbuf, "cuTensorMapEncodeTiled failed");
         return BW_ERR_LAUNCH;
     }
+    if (!zeroed) {
+        const int rc = zero_counters(p.counters, w.n_counters, st);
+        if (rc) return rc;
+    }
     switch (form.kind) {
-    case kGxF8Tokens: return gx_launch<kGxF8Tokens>(d, p, mw, mx, pairs, zeroed, st);
-    case kGxF8Weights: return gx_launch<kGxF8Weights>(d, p, mw, mx, pairs, zeroed, st);
-    default: return gx_launch<kGx16>(d, p, mw, mx, pairs, zeroed, st);
+    case kGxF8Tokens: return gx_launch<kGxF8Tokens>(d, p, mw, mx, pairs, st);
+    case kGxF8Weights: return gx_launch<kGxF8Weights>(d, p, mw, mx, pairs, st);
+    default: return gx_launch<kGx16>(d, p, mw, mx, pairs, st);
     }
 }
 
@@ -182,8 +196,6 @@ int gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx,
     p.counters = reinterpret_cast<int*>(static_cast<uint8_t*>(work) + at);
     p.next = p.counters + dw_counters(p, pairs) - 1;
     p.wait_ns = g_wait_ns;
-    e = cudaMemsetAsync(p.counters, 0, (size_t)dw_counters(p, pairs) * sizeof(int), st);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync (counters)");
     CUtensorMap my, mx;
     if (!moe_map(&my, dY, 0, (uint64_t)N, (uint64_t)M, 1, (uint64_t)ldy, (uint64_t)ldy * M, 64) ||
         !moe_map(&mx, X, 0, (uint64_t)K, (uint64_t)M, 1, (uint64_t)ldx, (uint64_t)ldx * M, 64)) {
@@ -191,26 +203,8 @@ int gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long ldx,
         return BW_ERR_LAUNCH;
     }
     static std::atomic<bool> limit_set[kMaxDevices];
-    std::atomic<bool>& done = limit_set[d - g_dev];
-    if (!done.load(std::memory_order_acquire)) {
-        e = cudaFuncSetAttribute(grouped_dw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BW_SMEM_LIMIT);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-        done.store(true, std::memory_order_release);
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs));
-    cfg.blockDim = dim3(kGxThreads);
-    cfg.dynamicSmemBytes = (size_t)(1024 + dw_smem(p.ring_bytes, E).bytes);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, grouped_dw_kernel, my, mx, p);
-    return e == cudaSuccess ? BW_OK : cuda_fail(e, "kernel launch (grouped gradient)");
+    if ((rc = zero_counters(p.counters, dw_counters(p, pairs), st))) return rc;
+    return launch_pairs(*d, grouped_dw_kernel, limit_set, my, mx, p, pairs, dw_smem(p.ring_bytes, E).bytes, st);
 }
 
 int f8_check(int E, int M, int N, int K, int out_type, int swiglu)

@@ -151,7 +151,6 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_alloc_pair(tmem_slot, 512u);
         tmem_relinquish_pair();
     }
-    griddep_wait();
     if (warp == 4) dw_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
@@ -243,6 +242,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         } else if (lane == 0) {
             const DwSched s = dw_sched(off, cum, p.E, p.tn * p.tk, pairs);
             const GxQueue queue = {qfull, qasked, queue_tile, 0};
+            griddep_wait();  // the counters are zero (a kernel of the call's own ahead of this one writes nothing else)
             if (s.split + c < s.tiles)  // (else the plans ask for nothing)
                 gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         uint8_t* line = smem + L.buf + (warp - 4) * kGxLineBytes;
         const int row = q * 32 + lane;
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
+        griddep_wait();
         int acc = 0;
         uint32_t aph = 0;
         bool alive = true;

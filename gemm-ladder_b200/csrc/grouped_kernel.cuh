@@ -339,11 +339,15 @@ __device__ __forceinline__ void gx_tables(const GxParams& p, int* off, int* cum,
     }
     const int per = (p.E + 32) / 32;  // E + 1 numbers
     const int i0 = lane * per, i1 = i0 + per < p.E + 1 ? i0 + per : p.E + 1;
+#pragma unroll 4
+    for (int i = lane; i < p.E + 1; i += 32) {  // (loads that do not wait for one another)
+        const int v = p.offsets[i];
+        off[i] = v < 0 ? 0 : v > p.T ? p.T : v;
+    }
+    __syncwarp();
     int top = 0;
     for (int i = i0; i < i1; ++i) {
-        int v = p.offsets[i];
-        v = v < 0 ? 0 : v > p.T ? p.T : v;
-        top = v > top ? v : top;
+        top = off[i] > top ? off[i] : top;
         off[i] = top;
     }
     int run = top;
@@ -400,6 +404,13 @@ __device__ __forceinline__ void gx_sum_parts(float (&v)[16], int first, int last
             }
         }
     }
+}
+
+// The counters' zeros, as a kernel of the call's own ahead of its product, whose set-up it overlaps.
+__global__ void gx_zero_kernel(int* p, int n)
+{
+    griddep_launch();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
 }
 
 template <int KIND>
@@ -482,7 +493,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_alloc_pair(tmem_slot, (uint32_t)tmem_cols);
         tmem_relinquish_pair();
     }
-    griddep_wait();  // what the kernel ahead wrote (the offsets, X, its scales, the counters) is visible from here on
+    // The kernel ahead is the call's own (zero_counters or the quantiser): it writes the counters, and in bw_linear_f8 X and its scales.  Whoever
+    // uses one of these waits for it (griddep_wait); W, its scales and the offsets were complete before it began.
     if (warp == 2) gx_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
@@ -531,25 +543,49 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                                              : t.n * 128 + rank * 64;
                 w1 = p.glu == kGxPlain ? w0 + 64 : p.glu == kGxGluBlocks ? w0 + 128 : p.N / 2 + w0;
             }
-            for (int kb = t.k0; kb < t.k1; ++kb) {
+            auto load_w = [&](int kb, int st) {
+                const uint32_t bar = full0 + 8u * (uint32_t)st;
+                uint8_t* to = smem + st * p.stage_bytes;
+                if (leader) mbar_arrive_expect_tx(&full[st], bytes);
+                if (TOK) {
+                    tma_load_3d_pair(to + kGxXBytes, &tmw, kb * kRowElems, w0, t.e, bar);
+                } else if (p.mn_major) {
+                    tma_load_3d_pair(to, &tmw, w0, kb * 64, t.e, bar);
+                    tma_load_3d_pair(to + 8192, &tmw, w0 + 64, kb * 64, t.e, bar);
+                } else {
+                    tma_load_3d_pair(to, &tmw, kb * kRowElems, w0, t.e, bar);
+                    if (p.glu != kGxPlain) tma_load_3d_pair(to + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
+                }
+            };
+            auto load_x = [&](int kb, int st) {
+                const uint32_t bar = full0 + 8u * (uint32_t)st;
+                uint8_t* to = smem + st * p.stage_bytes;
+                if (TOK) {
+                    tma_load_3d_pair(to, &tmx, kb * kRowElems, tok, 0, bar);
+                } else {
+                    for (int i = 0; i < boxes; ++i)
+                        tma_load_3d_pair(to + kGxXBytes + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
+                }
+            };
+            int kb = t.k0;
+            if (issued == 0) {  // the first stages' weights while the kernel ahead runs
+                const int n = t.k1 - kb < S ? t.k1 - kb : S;
+                if (elect_one())
+                    for (int i = 0; i < n; ++i) load_w(kb + i, i);
+                griddep_wait();
+                if (elect_one())
+                    for (int i = 0; i < n; ++i) load_x(kb + i, i);
+                kb += n;
+                issued = n;
+                if (n == S) ph ^= 1u;
+                else stage = n;
+            }
+            for (; kb < t.k1; ++kb) {
                 alive = gx_warp_wait(&empty[stage], ph ^ 1u, abort_flag, limit, site(0, 1, stage));
                 if (!alive) break;
-                uint8_t* sx = smem + stage * p.stage_bytes;
-                const uint32_t bar = full0 + 8u * (uint32_t)stage;
                 if (elect_one()) {
-                    if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-                    if (TOK) {
-                        tma_load_3d_pair(sx, &tmx, kb * kRowElems, tok, 0, bar);
-                        tma_load_3d_pair(sx + kGxXBytes, &tmw, kb * kRowElems, w0, t.e, bar);
-                    } else if (p.mn_major) {
-                        tma_load_3d_pair(sx, &tmw, w0, kb * 64, t.e, bar);
-                        tma_load_3d_pair(sx + 8192, &tmw, w0 + 64, kb * 64, t.e, bar);
-                    } else {
-                        tma_load_3d_pair(sx, &tmw, kb * kRowElems, w0, t.e, bar);
-                        if (p.glu != kGxPlain) tma_load_3d_pair(sx + 8192, &tmw, kb * kRowElems, w1, t.e, bar);
-                    }
-                    for (int i = 0; !TOK && i < boxes; ++i)
-                        tma_load_3d_pair(sx + kGxXBytes + i * p.box * 128, &tmx, kb * kRowElems, tok + i * p.box, 0, bar);
+                    load_w(kb, stage);
+                    load_x(kb, stage);
                 }
                 ++issued;
                 if (++stage == S) {
@@ -631,6 +667,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             // ------------------------------------------------------ whole tiles dealt out
             const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
             const GxQueue queue = {qfull, qasked, queue_tile, 0};
+            griddep_wait();
             if (s.split + c < s.tiles)  // (else the plans ask for nothing)
                 gx_deal(queue, p.next, s.split + pairs, s.tiles, abort_flag, limit);
         }
@@ -680,6 +717,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             uint32_t sph = 0;
             bool alive = true;
             GxDesc t;
+            griddep_wait();
             while (next(t, alive)) {
                 // the scale blocks of the weight rows: kGxF8Weights, of this block's rows (gate and up: of each); kGxF8Tokens, of the
                 // tile's two halves of columns
@@ -740,6 +778,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0);
         const uint32_t quarter = tmem_base + ((uint32_t)(q * 32) << 16);
         uint8_t* bufs = smem + L.buf;
+        griddep_wait();
         int acc = 0, si = 0;
         uint32_t aph = 0, sph = 0;
         bool alive = true;
