@@ -11,7 +11,7 @@ namespace {
 // Sizes within the tensor maps' and the schedule's 32-bit indices.
 bool gx_sizes_ok(int E, int T, int N, int K)
 {
-    if (E < 1 || E > kGroupMax || T < 0 || N < 1 || K < 1 || N > (1 << 20) || K > (1 << 20)) return false;
+    if (E < 1 || E > kGroupMax || T < 0 || T > (1 << 30) || N < 1 || K < 1 || N > (1 << 20) || K > (1 << 20)) return false;
     return ((long long)T / 32 + E) * ((N + 255) / 256) < (1LL << 30) && (long long)E * N <= 0x7FFFFFFFLL;
 }
 

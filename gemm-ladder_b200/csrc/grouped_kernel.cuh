@@ -812,7 +812,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
             const int N = t.N;
             // This warp's columns, in runs of 16: half of the tile's.  TOK: the first or second 128, or with the activation
             // 64 gate columns and their 64 up columns.
-            const int nc = N / 2, c0 = h * nc;
+            const int c0 = h * (N / 2), have = t.t1 - t.t0 - c0;
+            const int nc = have < N / 2 ? have : N / 2;  // (those of tokens: not TOK)
             auto col = [&](int i) {
                 if (!TOK) return c0 + i * 16;
                 return p.glu == kGxPlain ? h * 128 + i * 16 : (i < 4 ? 0 : 64) + h * 64 + i * 16;

@@ -45,11 +45,9 @@ BW_GS GroupSched group_sched(int nt, int kb, int pairs, int runs)
     s.pairs = pairs;
     s.tiles = nt * runs;
     s.split = s.tiles % pairs;
-    const long long units = (long long)s.split * kb;
-    long long parts = units / kGroupMinUnits;
-    if (parts > pairs) parts = pairs;
-    if (parts < s.split) parts = s.split;
-    s.parts = (int)parts;
+    s.parts = s.split * kb / kGroupMinUnits;
+    if (s.parts > pairs) s.parts = pairs;
+    if (s.parts < s.split) s.parts = s.split;
     // a remainder that fills most of a wave is as quick in whole tiles
     if (s.tiles > pairs && s.split * 8 > pairs * 7) s.parts = s.split;
     return s;
@@ -59,11 +57,12 @@ BW_GS GroupSched group_sched(int nt, int kb, int pairs, int runs)
 BW_GS int group_runs(int a, int b, int cap) { return b > a ? (b - a + cap - 1) / cap : 0; }
 BW_GS int group_run_rows(int a, int b, int runs) { return ((b - a + runs - 1) / runs + 31) / 32 * 32; }
 
-// The first K-block (of split tile x kb) of part c, and the part that holds K-block u.
-BW_GS long long part_begin(const GroupSched& s, int c) { return (long long)s.split * s.kb * c / s.parts; }
-BW_GS int part_of(const GroupSched& s, long long u)
+// The first K-block (of split tile x kb) of part c, and the part that holds K-block u.  (Fewer than `pairs` tiles of at most
+// 2^14 K-blocks are split into at most `pairs` parts: 32 bits hold the products, and divide in a quarter of the time.)
+BW_GS int part_begin(const GroupSched& s, int c) { return (int)((unsigned)(s.split * s.kb) * (unsigned)c / (unsigned)s.parts); }
+BW_GS int part_of(const GroupSched& s, int u)
 {
-    return (int)(((u + 1) * s.parts - 1) / ((long long)s.split * s.kb));
+    return (int)(((unsigned)(u + 1) * (unsigned)s.parts - 1u) / (unsigned)(s.split * s.kb));
 }
 
 struct GroupSeg {
@@ -73,7 +72,7 @@ struct GroupSeg {
 
 // A pair's segments in order: its range of the split tiles, then whole tiles.
 struct GroupWalk {
-    long long u, uend;
+    int u, uend;
     int tile;
     BW_GS GroupWalk(const GroupSched& s, int c)
     {
@@ -88,10 +87,10 @@ struct GroupWalk {
     BW_GS bool next_part(const GroupSched& s, GroupSeg& g)
     {
         if (u < uend) {
-            g.tile = (int)(u / s.kb);
-            g.k0 = (int)(u - (long long)g.tile * s.kb);
-            const long long end = (long long)(g.tile + 1) * s.kb;
-            g.k1 = s.kb - (int)(end > uend ? end - uend : 0);
+            g.tile = u / s.kb;
+            g.k0 = u - g.tile * s.kb;
+            const int end = (g.tile + 1) * s.kb;
+            g.k1 = s.kb - (end > uend ? end - uend : 0);
             u = end > uend ? uend : end;
             return true;
         }
@@ -115,8 +114,8 @@ struct GroupWalk {
 };
 
 // The parts of split tile t: [first, last]; part c's slot for it (a part's range touches at most two tiles).
-BW_GS int tile_first_part(const GroupSched& s, int t) { return part_of(s, (long long)t * s.kb); }
-BW_GS int tile_last_part(const GroupSched& s, int t) { return part_of(s, (long long)(t + 1) * s.kb - 1); }
+BW_GS int tile_first_part(const GroupSched& s, int t) { return part_of(s, t * s.kb); }
+BW_GS int tile_last_part(const GroupSched& s, int t) { return part_of(s, (t + 1) * s.kb - 1); }
 BW_GS int part_slot(const GroupSched& s, int c, int t) { return 2 * c + (part_begin(s, c) / s.kb == t ? 0 : 1); }
 
 // A tile's place in its expert: weight tile n and run m, of `runs` runs; j counts the expert's tiles.

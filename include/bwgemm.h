@@ -327,7 +327,9 @@ int bw_gemm_device_plan(int M, int N, int K, int variant, int noalloc, bw_plan* 
  * finished accumulator, 3 a free accumulator, 4 partials copied in, 5 and 6 a K-split cluster's pieces and go signal,
  * 7 another rank's partial of the fused reduce-scatter (index: the sender), 8 a rank's ack of the previous call, 9 an
  * entry of the block's queue of units (a plan with dyn 1); of the mixture-of-experts kernel (role 3: its tokens'
- * producer) 10 an expert's activations, 11 a split output tile's other partials, 12 a stage's tokens.
+ * producer) 10 an expert's activations, 11 a split output tile's other partials, 12 a stage's tokens; of the grouped and
+ * e4m3 kernels (roles 0 to 2 as above, 3 a descriptor's reader, 4 the scales or the gradient's hand-over, 5 the plan, 6 the
+ * dealer of whole tiles) 9 a tile asked for, 10 a descriptor, 11 a descriptor's place, 13 a batch of scales.
  * Returns a CUDA error as BW_ERR_LAUNCH.
  * No reference counterpart as a function: the reference traps in its guarded wait (hopper/step2.cuh:128-145); this
  * rung's waits return instead and leave the context usable.
