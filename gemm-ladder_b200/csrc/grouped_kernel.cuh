@@ -787,17 +787,32 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         auto release = [&] {
             tc_fence_before();
             __syncwarp();
-            if (alive && lane == 0) mbar_arrive_remote_relaxed(TOK ? acc_a.empty : tempty0 + 8u * (uint32_t)acc);
+            if (alive && lane == 0) mbar_arrive_remote_relaxed(tempty0 + 8u * (uint32_t)acc);
         };
         auto next_acc = [&] {
-            if (TOK) {
-                const GxAcc x = acc_a;
-                acc_a = acc_b;
-                acc_b = x;
-            } else if (++acc == p.accs) {
+            if (++acc == p.accs) {
                 acc = 0;
                 aph ^= 1u;
             }
+        };
+        // a part of a split tile has been stored: true in the last block of `parts` to come here, which sums them
+        auto count_part = [&](int tile, int parts) {
+            named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
+            if (threadIdx.x == kGxEpi0)
+                *reduce_flag = alive && atom_add_acq_rel_gpu(p.counters + tile * 2 + rank, 1) == parts - 1 ? 1 : 0;
+            named_bar_sync(1, kGxEpiThreads);
+            return *reduce_flag != 0;
+        };
+        auto store_part = [&](int slot, int column, const float(&v)[16]) {
+            if (!alive) return;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                __stcg(gx_slot(p, slot, rank, row, column / 4 + j),
+                       make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+        };
+        auto sum_parts = [&](const GroupSched& s, int tile, int first, int last, int column, float(&v)[16]) {
+            gx_sum_parts<4>(v, first, last,
+                            [&](int part) { return gx_slot(p, part_slot(s, part, tile), rank, row, column / 4); });
         };
         for (;; ++asked) {
             // one thread waits for the descriptor and tells the other 255, so that all of them go on to the same barriers, or none
@@ -836,7 +851,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 auto wait_scales = [&] {
                     alive = alive && gx_warp_wait(&sfull[si], sph, abort_flag, limit, site(2, 13, (uint32_t)si));
                 };
-                // The segment's scaled sums, and back into its last accumulator, where the code below takes them for all kinds.
+                // The segment's scaled sums.  TOK: on to C from their registers, while the MMAs of the next segment run.  (Through
+                // tensor memory, as below, a tile took 6 us past its sums, 10 with the activation.)  Else back into the segment's
+                // last accumulator, where the code below takes them as it does other types'.
                 if constexpr (TOK) {
                     uint64_t sum[8][8];  // 8 runs of 16 columns, as pairs
 #pragma unroll
@@ -847,7 +864,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     int left = blocks, at = 0;  // K-blocks to come; of the batch, read
                     wait_scales();
                     float s0 = sc[si * kGxBatch * 256], s1 = sc[si * kGxBatch * 256 + sc1];
-                    // one K-block; false after the last, whose accumulator is kept
+                    // one K-block; false after the last
                     auto block = [&](GxAcc& a) {
                         const uint64_t p0 = pair_f32(__float_as_uint(s0), __float_as_uint(s0));
                         const uint64_t p1 = pair_f32(__float_as_uint(s1), __float_as_uint(s1));
@@ -862,7 +879,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                             for (int j = 0; j < 2; ++j)  // (past the tile's columns: not used)
                                 tmem_ld16(a.tm + (uint32_t)((i < 4 ? ca : cb) + (i + j) % 4 * 16), r[j]);
                             tmem_wait_ld();
-                            if (i == 6 && left) {
+                            if (i == 6) {
                                 tc_fence_before();
                                 __syncwarp();
                                 if (alive && lane == 0) mbar_arrive_remote_relaxed(a.empty);
@@ -887,20 +904,75 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     while (block(acc_a) && block(acc_b)) {
                     }
                     next_batch();
-                    if (blocks % 2 == 0) {  // the segment ended in the second: it comes first, as the one in use
+                    if (blocks % 2) {  // the segment ended in the first: the second is used next
                         const GxAcc x = acc_a;
                         acc_a = acc_b;
                         acc_b = x;
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (in_tile(i)) {
-                            uint32_t r[16];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) unpair_f32(sum[i][j], r[2 * j], r[2 * j + 1]);
-                            tmem_st16(acc_a.tm + (uint32_t)col(i), r);
+                    const bool glu = p.glu != kGxPlain;
+                    const int r0 = t.t0 + rank * 128 + q * 32, r1 = alive ? t.t1 : 0, f0 = t.n * (glu ? 128 : 256);
+                    const int per = gx_per_line(p.out);
+                    uint8_t* line = bufs + ew * kGxLineBytes;
+                    // columns of C in runs of 16; the tile ends after an even number of them
+                    auto put = [&](int i, const float(&v)[16]) {
+                        gx_put16(p.out, line, i % per, lane, v);
+                        if (i % 2 == 1 && (i % per == per - 1 || !in_tile(i + 1))) {
+                            const int at = f0 + col(i);
+                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, r1, at - i % per * 16, at + 16 < p.Nout ? at + 16 : p.Nout, lane);
                         }
-                    tmem_wait_st();
+                    };
+                    auto run = [&](int i, float(&v)[16]) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            uint32_t a, b;
+                            unpair_f32(sum[i][j], a, b);
+                            v[2 * j] = __uint_as_float(a);
+                            v[2 * j + 1] = __uint_as_float(b);
+                        }
+                    };
+                    auto activate = [&](float(&v)[16], const float(&u)[16]) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * u[j];
+                    };
+                    const int first = t.first, last = t.last, tile = t.tile;
+                    if (first == last) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if ((glu && i >= 4) || !in_tile(i)) break;
+                            float v[16];
+                            run(i, v);
+                            if (glu && i < 4) {
+                                float u[16];
+                                run((i + 4) % 8, u);
+                                activate(v, u);
+                            }
+                            put(i, v);
+                        }
+                    } else {
+                        const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+                        const int slot = part_slot(s, c, tile);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (in_tile(i)) {
+                                float v[16];
+                                run(i, v);
+                                store_part(slot, col(i), v);
+                            }
+                        if (count_part(tile, last - first + 1)) {
+                            const int runs = glu ? 4 : 8;
+#pragma unroll 1
+                            for (int i = 0; i < runs && in_tile(i); ++i) {
+                                float v[16];
+                                sum_parts(s, tile, first, last, col(i), v);
+                                if (glu) {
+                                    float u[16];
+                                    sum_parts(s, tile, first, last, col(i + 4), u);
+                                    activate(v, u);
+                                }
+                                put(i, v);
+                            }
+                        }
+                    }
                 } else {
                     // R: runs of 16 columns that this warp holds
                     auto accumulate = [&](auto runs) {
@@ -968,84 +1040,48 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         accumulate(std::integral_constant<int, 1>());
                 }
             }
-            const uint32_t tm = TOK ? acc_a.tm : quarter + (uint32_t)(acc * acc_cols);
-            // this segment's sum of 16 columns
-            auto own = [&](int i, float(&v)[16]) {
-                uint32_t r[16];
-                tmem_ld16(tm + (uint32_t)col(i), r);
-                tmem_wait_ld();
+            if constexpr (!TOK) {
+                const uint32_t tm = quarter + (uint32_t)(acc * acc_cols);
+                // this segment's sum of 16 columns
+                auto own = [&](int i, float(&v)[16]) {
+                    uint32_t r[16];
+                    tmem_ld16(tm + (uint32_t)col(i), r);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-            };
-            bool done = true;  // this block has the tile's whole sum
-            const int first = t.first, last = t.last, tile = t.tile;
-            if (first != last) {
-                // a part of a split tile: the last block to finish sums all parts in the order of K
-                const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-                const int slot = part_slot(s, c, tile);
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                };
+                bool done = true;  // this block has the tile's whole sum
+                const int first = t.first, last = t.last, tile = t.tile;
+                if (first != last) {
+                    // a part of a split tile: the last block to finish sums all parts in the order of K
+                    const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
+                    const int slot = part_slot(s, c, tile);
 #pragma unroll 1
-                for (int i = 0; i < 8 && in_tile(i); ++i) {
-                    float v[16];
-                    own(i, v);
-                    if (alive) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            __stcg(gx_slot(p, slot, rank, row, col(i) / 4 + j),
-                                   make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
-                    }
-                }
-                named_bar_sync(1, kGxEpiThreads);  // every thread's stores come before the count
-                if (threadIdx.x == kGxEpi0)
-                    *reduce_flag = alive && atom_add_acq_rel_gpu(p.counters + tile * 2 + rank, 1) == last - first ? 1 : 0;
-                named_bar_sync(1, kGxEpiThreads);
-                done = *reduce_flag != 0;
-            }
-            // the tile's sum of 16 columns
-            auto total = [&](int i, float(&v)[16]) {
-                if (first == last) {
-                    own(i, v);
-                    return;
-                }
-                const GroupSched s = group_sched(p.nt, p.kblocks, pairs, cum[p.E]);
-                gx_sum_parts<4>(v, first, last, [&](int part) {
-                    return gx_slot(p, part_slot(s, part, tile), rank, row, col(i) / 4);
-                });
-            };
-            if (done) {
-                if constexpr (TOK) {
-                    const bool glu = p.glu != kGxPlain;
-                    const int r0 = t.t0 + rank * 128 + q * 32, r1 = alive ? t.t1 : 0, f0 = t.n * (glu ? 128 : 256);
-                    const int per = gx_per_line(p.out), runs = glu ? 4 : 8;
-                    uint8_t* line = bufs + ew * kGxLineBytes;
-#pragma unroll 1
-                    for (int i = 0; i < runs && in_tile(i); ++i) {
+                    for (int i = 0; in_tile(i); ++i) {
                         float v[16];
-                        total(i, v);
-                        if (glu) {
-                            float u[16];
-                            total(i + 4, u);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * u[j];
-                        }
-                        gx_put16(p.out, line, i % per, lane, v);
-                        if (i % per == per - 1 || i + 1 == runs || !in_tile(i + 1))
-                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, r1, f0 + col(i - i % per),
-                                     f0 + col(i) + 16 < p.Nout ? f0 + col(i) + 16 : p.Nout, lane);
+                        own(i, v);
+                        store_part(slot, col(i), v);
                     }
-                } else {
+                    done = count_part(tile, last - first + 1);
+                }
+                if (done) {
                     const int tb = t.t0 + c0, t1 = t.t1;
                     const int f = p.glu == kGxPlain ? t.n * 256 + rank * 128 + q * 32 : t.n * 128 + rank * 64 + (q & 1) * 32;
 #pragma unroll 1
                     for (int i = 0; in_tile(i); ++i) {
                         float v[16];
-                        total(i, v);
+                        if (first == last)
+                            own(i, v);
+                        else
+                            sum_parts(group_sched(p.nt, p.kblocks, pairs, cum[p.E]), tile, first, last, col(i), v);
                         gx_finish16(p, v, bufs, ew, q, h, tb + i * 16, t1, f, lane, alive);
                     }
                 }
+                release();
+                next_acc();
             }
-            release();
-            next_acc();
-            if (alive && lane == 0) mbar_arrive(&dempty[asked % p.descs]);  // (release met the warp: the descriptor has been read)
+            __syncwarp();  // the descriptor has been read
+            if (alive && lane == 0) mbar_arrive(&dempty[asked % p.descs]);
         }
         if (threadIdx.x == kGxEpi0) BW_TRACE_AT(4);
     }
