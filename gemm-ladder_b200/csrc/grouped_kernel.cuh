@@ -239,6 +239,10 @@ __device__ __forceinline__ void gx_store16(const GxParams& p, const float (&v)[1
     __syncwarp();
 }
 
+// Within 5 + 1.2 |g| steps of fp32.  (The fast quotient is 0 where the exponential passes 2^126, at g < -87.3: silu(g) u is then
+// within 1.1e-36 |u| of it.  With the correctly rounded one the finish of a tile took 4.3 us more.)
+__device__ __forceinline__ float gx_silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+
 // 16 tokens of a finished sum to C.  With the activation a warp of gate rows (quarters 0 and 1) takes the up rows' sums
 // from the warp of the same columns two quarters on, through that warp's buffer; the two meet twice.
 __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], uint8_t* bufs, int ew, int q, int h, int tb,
@@ -261,7 +265,7 @@ __device__ __forceinline__ void gx_finish16(const GxParams& p, float (&v)[16], u
         // the up rows' warp: the same half, quarter q + 2
         const float* b = reinterpret_cast<const float*>(bufs + (ew + 2) * 2048);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * b[j * 32 + lane];
+        for (int j = 0; j < 16; ++j) v[j] = gx_silu(v[j]) * b[j * 32 + lane];
         named_bar_sync(bar, 64);
         gx_store16(p, v, mine, tb, t1, f, lane, write);
     }
@@ -932,7 +936,7 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                     };
                     auto activate = [&](float(&v)[16], const float(&u)[16]) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = v[j] / (1.0f + __expf(-v[j])) * u[j];
+                        for (int j = 0; j < 16; ++j) v[j] = gx_silu(v[j]) * u[j];
                     };
                     const int first = t.first, last = t.last, tile = t.tile;
                     if (first == last) {
