@@ -252,7 +252,7 @@ int gemm_f8(const void* A, const void* a_scale, long long lds, const void* B, co
 int quant_f8_check(const void* X, int type, long long ld, int rows, int cols)
 {
     if (type != BW_TYPE_F16 && type != BW_TYPE_BF16) return BW_ERR_ARG;
-    if (rows < 0 || cols < 1 || cols % 16 || cols > (1 << 20) || ld < cols || ld % 8) return BW_ERR_SHAPE;
+    if (rows < 0 || rows > (1 << 30) || cols < 1 || cols % 16 || cols > (1 << 20) || ld < cols || ld % 8) return BW_ERR_SHAPE;
     if ((long long)(rows / kF8Rows + 1) * ((cols + 255) / 256) > 0x7FFFFFFFLL) return BW_ERR_SHAPE;  // blocks of the grid
     if (rows && !aligned(X, 16)) return BW_ERR_ARG;
     return BW_OK;

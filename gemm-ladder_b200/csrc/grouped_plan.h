@@ -5,9 +5,7 @@
 
 namespace bw {
 
-// The form of a call and the most tokens of a tile, for an average of `rows` tokens per expert.  With the weights as M a
-// tile's MMA is as wide as the tokens it has, so a large cap costs little computing; a small one leaves shared memory for
-// more stages of weights, which is what few tokens want.
+// The form of a call and the most tokens of a tile, for an average of `rows` tokens per expert.
 struct GxForm {
     int kind, cap;
 };
@@ -17,10 +15,13 @@ inline GxForm gx_form(int T, int E, bool grouped, bool f8)
     // e4m3, the tokens as M: measured, 32 experts of 4096 x 4096 with 32 / 64 / 128 rows each in 188 / 190 / 190 us against
     // 133 / 194 / 238 with the weights as M; one matrix of 8192 x 8192 at 128 / 160 tokens in 55 / 55 against 49 / 59
     if (f8 && rows > (grouped ? 48 : 128)) return {kGxF8Tokens, 256};
-    // (experts' numbers of rows spread around the average: twice it, so that most take one run)
+    // fp16 and bf16: a tile's MMA is as wide as the tokens it has, and a smaller cap, for more stages of weights, gained nothing
+    // (64 experts of 2048 x 2048 with 28 rows each in 108 us with 64 and with 256, 8 of 4096 x 4096 with 20 in 66 with both)
+    if (!f8) return {kGx16, 256};
+    // e4m3, the weights as M: the smaller the cap, the more K-blocks are handed over at once (17 tokens, 8192 x 8192: 31 us with 32,
+    // 35 with 128).  Experts' numbers of rows spread around the average: twice it, so that most take one run.
     const long long want = grouped ? 2 * rows : rows;
-    const int cap = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 || f8 ? 128 : 256;
-    return {f8 ? kGxF8Weights : kGx16, cap};
+    return {kGxF8Weights, want <= 32 ? 32 : want <= 64 ? 64 : 128};
 }
 
 // Everything of a call but its addresses.
@@ -37,7 +38,9 @@ inline GxParams gx_params(int E, int T, int N, int K, GxForm form, bool bf16, bo
     p.cap = form.cap;
     p.box = tokens ? 128 : p.cap == 32 ? 16 : 32;
     p.wbox = glu == kGxPlain || tokens ? 128 : 64;
-    // short tiles: more of them planned ahead, to keep the stage ring full
+    // short tiles: more of them planned ahead, to keep the stage ring full (16 experts of 8192 x 256 with 100 rows each: 31.8 us,
+    // 35.8 with two); long ones: two, since a tile planned ahead cannot go to a pair that is done earlier (64 of 2048 x 2816 with
+    // 256 rows: 186 us, 190 with four)
     p.descs = p.kblocks < 8 ? kGxDescs : 2;
     p.group = form.kind == kGxF8Weights ? 128 / p.cap : 1;
     p.accs = 512 / (p.cap * p.group) < kGxAccs ? 512 / (p.cap * p.group) : kGxAccs;

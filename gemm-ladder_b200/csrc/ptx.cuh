@@ -62,20 +62,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok != 0;
 }
 
-// The same without waiting at all (try_wait suspends the thread for a while before it says no).
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // ------------------------------------------------------------------ the device status word
 // [0]: status code (0 ok, 3 a bounded wait gave up); [1]: the first site that gave up (role << 16 | barrier id);
 // [2]: blockIdx.x of that block; [3]: the segment it was on.  Cleared by the host.

@@ -44,8 +44,6 @@ inline bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return emu::mb_try_wait(emu::cta_of(bar), emu::off_of(bar), parity);
 }
 
-inline bool mbar_test_wait(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity); }
-
 inline unsigned int g_status[4];
 inline thread_local unsigned int* t_status = g_status;  // the status word of the emulated GPU this thread runs on
 enum : uint32_t { kStatusTimeout = 3u };

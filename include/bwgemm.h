@@ -154,7 +154,8 @@ int bw_moe_mlp(const void* X, long long ldx, const void* R, const void* W1, cons
  *                            (the layout of bw_moe_mlp's W1; N % 16 == 0)
  * with fp32 sums, C in X's type, rounded once.  Rows before offsets[0] and from offsets[E] on are not written.  Row numbers
  * outside [0, M], or below an earlier one, are taken as the nearest that are not.
- * N % 8 == 0, K % 8 == 0 (both layouts), ldx >= K, ldx % 8 == 0, 1 <= E <= 1024; X, B and C 16-byte aligned, C contiguous.
+ * N % 8 == 0, K % 8 == 0 (both layouts), ldx >= K, ldx % 8 == 0, 1 <= E <= 1024, N and K <= 2^20, M <= 2^30; X, B and C
+ * 16-byte aligned, C contiguous.
  * `work` (bw_gemm_grouped_work_bytes), overlap and capture: as for the 8-bit entries.  M == 0 is a call that does nothing.
  * The kernel that reads the offsets runs on `stream`: they may be written by a kernel ahead of the call.
  * No reference counterpart.
@@ -197,7 +198,7 @@ int bw_gemm_grouped_dw(const void* dY, long long ldy, const void* X, long long l
  * of 128 gate then 128 up rows (as bw_gemm_i8_swiglu takes them); E >= 1: B_e's first N/2 rows gate, its last up.
  * bw_linear_f8 is both in one call: X (fp16 or bf16) quantised as bw_quant_f8 does on the way, C in X's type.
  *
- * K % 16 == 0, N % 8 == 0, E <= 1024; X, Q, A, B and C 16-byte aligned, scales 4-byte aligned.
+ * K % 16 == 0, N % 8 == 0, E <= 1024, N and K <= 2^20, M <= 2^30; X, Q, A, B and C 16-byte aligned, scales 4-byte aligned.
  * `work` (bw_gemm_f8_work_bytes, linear 1 for bw_linear_f8), overlap and capture: as for the 8-bit integer entries.
  * M == 0 is a call that does nothing.  No reference counterpart.
  */

@@ -448,7 +448,8 @@ def test_refusals_of_the_f8_entries(abi):
     def quant(type=0, ld=128, Q=P, s=P, lds=100, rows=100, cols=128, X=P):
         return L.bw_quant_f8(X, type, ld, Q, s, lds, rows, cols, None)
 
-    for bad in (dict(ld=120), dict(ld=132), dict(lds=99), dict(rows=-1), dict(cols=0), dict(cols=24, ld=24)):
+    for bad in (dict(ld=120), dict(ld=132), dict(lds=99), dict(rows=-1), dict(cols=0), dict(cols=24, ld=24),
+                dict(rows=2 ** 30 + 1, lds=2 ** 31)):
         assert quant(**bad) == b.BW_ERR_SHAPE, bad
     for bad in (dict(type=2), dict(X=P + 8), dict(Q=P + 8), dict(s=0)):
         assert quant(**bad) == b.BW_ERR_ARG, bad
