@@ -1,6 +1,6 @@
 // grouped.cuh -- host side of the products grouped by expert and in 8-bit floating point (bw_gemm_grouped,
-// bw_gemm_grouped_dw, bw_quant_f8, bw_quant_blocks_f8, bw_gemm_f8, bw_linear_f8 of bwgemm.h), included by bwgemm.cu: argument checks, the tensor
-// maps, the caller's workspace, the launches.
+// bw_gemm_grouped_dw, bw_quant_f8, bw_quant_blocks_f8, bw_gemm_f8, bw_linear_f8 of bwgemm.h), included by bwgemm.cu:
+// argument checks, the tensor maps, the caller's workspace, the launches.
 #pragma once
 #include "grouped_plan.h"
 #include "quant_f8.cuh"
@@ -99,8 +99,8 @@ int gx_launch(DeviceState& d, const GxParams& p, const CUtensorMap& mw, const CU
 
 // The product of p (its addresses but the workspace's filled in); zeroed: the kernel ahead of it on the stream, one of the
 // call's own launched in plain order, zeroes the counters.
-int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m, const void* X, const void* W, const GxWork& w, uint8_t* work,
-               int pairs, bool zeroed, cudaStream_t st)
+int gx_product(DeviceState& d, GxParams& p, const GxForm& form, const GxMaps& m, const void* X, const void* W,
+               const GxWork& w, uint8_t* work, int pairs, bool zeroed, cudaStream_t st)
 {
     p.work = reinterpret_cast<float*>(work + w.parts);
     p.counters = reinterpret_cast<int*>(work + w.counters);
@@ -147,7 +147,8 @@ int gemm_grouped(const void* X, long long ldx, const void* B, const int* offsets
     const GxForm form = gx_form(M, E, true, false);
     const GxWork w = gx_work(M, K, form.cap, pairs, false);
     if (w.bytes > work_bytes) return scratch_fail(w.bytes, work_bytes);
-    GxParams p = gx_params(E, M, N, K, form, type == BW_TYPE_BF16, layout == BW_LAYOUT_KN, swiglu ? kGxGluHalves : kGxPlain, type);
+    GxParams p = gx_params(E, M, N, K, form, type == BW_TYPE_BF16, layout == BW_LAYOUT_KN, swiglu ? kGxGluHalves : kGxPlain,
+                           type);
     p.offsets = offsets;
     p.C = C;
     return gx_product(*d, p, form, gx_maps(p, K, ldx, false), X, B, w, static_cast<uint8_t*>(work), pairs, false, st);

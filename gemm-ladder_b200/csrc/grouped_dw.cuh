@@ -8,6 +8,10 @@
 // MMA's depth) between the load and the MMAs.  For that each block's loads complete on its own barrier; its warp 2 waits
 // there, clears what has to be cleared and arrives on the leader's barrier, where the MMA issuer waits for both blocks.
 // Warp 3 plans; roles otherwise as in grouped_kernel.cuh; a TMEM lane is a row of dW, a column a column.
+// What bounds it (one B200, bursts): 16384 rows over 64 experts, 2816 x 2048, bf16: 253 us, 746 TFLOP/s.  The gradient's 738 MB
+// alone, written as zeros by the same stores, take 151 us (torch's fill 190; a DRAM that is only written takes 4 to 5 TB/s), and
+// the MMAs and loads of 4 K-blocks a tile do not hide behind them whole.  1000 rows over 16, 1352 x 2048: 49 us, of which 18 are
+// the 89 MB of writes; 10 tiles a pair, each with its own start and end.
 #pragma once
 #include "grouped_kernel.cuh"
 

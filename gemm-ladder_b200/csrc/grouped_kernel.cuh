@@ -20,10 +20,19 @@
 // e4m3: the accumulator is taken out of tensor memory once per K-block of 128, scaled and added in fp32 registers; the MMAs of
 // the next K-blocks run into the other accumulators meanwhile.  The scales differ from block to block, so no MMA may run
 // across two.  With the weights as M (kGxF8Weights) a column's scale is the same in all lanes and comes from shared memory, 4
-// bytes per product: 256 tokens would take 1024 cycles a K-block (128 bytes a cycle) beside 512 of MMA.  So above 128 tokens
-// per expert the tokens are the M (kGxF8Tokens): a lane is a token with one scale, a half of the columns one block of
+// bytes per product: 256 tokens would take 1024 cycles a K-block (128 bytes a cycle) beside 512 of MMA.  So with more
+// tokens (gx_form has the bounds) they are the M (kGxF8Tokens): a lane is a token with one scale, a half of the columns one block of
 // weights with another, and the product of the two is all a K-block needs.  Few tokens: the K-blocks go to the epilogue in
 // groups of 128 columns (4 K-blocks of 32 tokens), since a hand-over costs more than the sums of 32 columns.
+// What bounds it (one B200, device time of a call in bursts on a cold L2):
+//   16384 rows over 64 experts of 2048 x 2816, bf16: 182 us, 1037 TFLOP/s (8191 rows, 32 x (5760, 2880), activation: 266 us, 1021):
+//     the operands' way from L2 to the SMs.  A K-block is 64 KB per pair for 512 cycles of MMA, 10 TB/s over all SMs; the tensor
+//     pipe is active 56 % of the cycles and DRAM 63 %.
+//   24 rows over 64 experts of 2048 x 1024, bf16: 31 us, 22 in a graph: two launches, one tile's latency, a split tile's sum.
+//   8192^3 in e4m3, the quantiser included: 581 us, 1890 TFLOP/s: the sums in the epilogue (0.55 us per K-block of a 256 x 256
+//     tile; MMAs and loads alone 0.39).  8192 rows over 64 experts of 4096 x 2048: 200 us: the same, and tiles half empty.
+//   17 x 8192 x 28672 in e4m3: 65 us, the weights at 3.6 TB/s: the parts of the split tiles (3.4 MB out and in), start
+//     and quantiser beside 36 us of weights.
 // Every wait is bounded (wait_lean, ptx.cuh).  A thread of the epilogue whose wait gave up goes on to the end of its segment
 // without waiting or writing, through every barrier and every instruction that its warp executes as one, and then leaves.
 #pragma once
@@ -497,8 +506,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
         tmem_alloc_pair(tmem_slot, (uint32_t)tmem_cols);
         tmem_relinquish_pair();
     }
-    // The kernel ahead is the call's own (zero_counters or the quantiser): it writes the counters, and in bw_linear_f8 X and its scales.  Whoever
-    // uses one of these waits for it (griddep_wait); W, its scales and the offsets were complete before it began.
+    // The kernel ahead is the call's own (zero_counters or the quantiser): it writes the counters, and in bw_linear_f8 X and
+    // its scales.  Whoever uses one of these waits for it (griddep_wait); W, its scales and the offsets were complete before it
+    // began.
     if (warp == 2) gx_tables(p, off, cum, lane);
     __syncwarp();
     tc_fence_before();
@@ -855,9 +865,9 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                 auto wait_scales = [&] {
                     alive = alive && gx_warp_wait(&sfull[si], sph, abort_flag, limit, site(2, 13, (uint32_t)si));
                 };
-                // The segment's scaled sums.  TOK: on to C from their registers, while the MMAs of the next segment run.  (Through
-                // tensor memory, as below, a tile took 6 us past its sums, 10 with the activation.)  Else back into the segment's
-                // last accumulator, where the code below takes them as it does other types'.
+                // The segment's scaled sums.  TOK: on to C from their registers, while the MMAs of the next segment run.
+                // (Through tensor memory, as below, a tile took 6 us past its sums, 10 with the activation.)  Else back into the
+                // segment's last accumulator, where the code below takes them as it does other types'.
                 if constexpr (TOK) {
                     uint64_t sum[8][8];  // 8 runs of 16 columns, as pairs
 #pragma unroll
@@ -892,7 +902,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                             for (int j = 0; j < 2; ++j)
 #pragma unroll
                                 for (int k = 0; k < 8; ++k)
-                                    sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1, sum[i + j][k]);
+                                    sum[i + j][k] = fma_f32x2(pair_f32(r[j][2 * k], r[j][2 * k + 1]), i < 4 ? p0 : p1,
+                                                              sum[i + j][k]);
                         }
                         if (!left) return false;
                         if (++at == kGxBatch) {
@@ -922,7 +933,8 @@ __global__ void __launch_bounds__(kGxThreads, 1)
                         gx_put16(p.out, line, i % per, lane, v);
                         if (i % 2 == 1 && (i % per == per - 1 || !in_tile(i + 1))) {
                             const int at = f0 + col(i);
-                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, r1, at - i % per * 16, at + 16 < p.Nout ? at + 16 : p.Nout, lane);
+                            gx_flush(p.out, line, p.C, (size_t)p.Nout, r0, r1, at - i % per * 16,
+                                     at + 16 < p.Nout ? at + 16 : p.Nout, lane);
                         }
                     };
                     auto run = [&](int i, float(&v)[16]) {

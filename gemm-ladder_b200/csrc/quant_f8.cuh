@@ -7,7 +7,8 @@
 // and q 0 (its products are NaN, as the unquantised ones' would be).
 //
 // Bound by its bytes: 2 read and 1 written per element, in one pass, a group held in registers between its maximum and its
-// rounding.
+// rounding.  10240 x 8192 by blocks: 41 us, 0.94 of the copy bandwidth; 4099 x 7184 by rows: 21 us, 0.65 (14 us of bytes; 3.2
+// waves of blocks, their start and the launch).
 #pragma once
 #include <cuda_fp8.h>
 

@@ -122,7 +122,8 @@ class TPMLPI8:
     """One rank's part of the block in 8 bits.  W1, W2: (int8 rows, fp32 scales) of quantize_shards.
     linear(X, rows, scales, swiglu) -> X's product with its rows quantised (bwgemm.linear_i8); over several ranks also
     quantize_rows(A) -> (int8, scales) and gemm_f32(q, q_scales, rows, scales) -> fp32 (bwgemm.gemm_i8), each rank
-    quantising its own shard of the activation, and reduce_scatter as TPMLP's."""
+    quantising its own shard of the activation, and reduce_scatter as TPMLP's. On one rank also in 8-bit
+    floating point: linear bwgemm.linear_f8, W1 and W2 bwgemm.quantize_blocks_f8 of the same shards (N x K)."""
 
     def __init__(self, W1, W2, rank, world, linear, quantize_rows=None, gemm_f32=None, reduce_scatter=None):
         self.W1, self.W2 = W1, W2
