@@ -484,3 +484,50 @@ def test_mlp_block_in_8_bit_floating_point(dtype, M):
     # e4m3's rounding is at most 2^-4 of a value, as a uniform error 2^-4 / sqrt(3) = 3.6 %, about 2.6 % over the values of a
     # step; six quantised operands (X twice, gate, up, A, W2), the activation's slope at most 1.1: below 9 %
     assert (Y.double() - want).norm() <= 0.09 * want.norm()
+
+
+@pytest.mark.parametrize("N", [8, 72, 136, 264, 392])
+def test_f8_columns_that_end_inside_a_tile_of_many_tokens(N):
+    for M, K in ((300, 272), (129, 4112)):
+        X, Q, s, B, t = f8_operands(M, 0, N, K, F16, N)
+        for dtype in (F16, F32):
+            check(bwgemm.gemm_f8(Q, s, B, t, dtype=dtype), *reference8(Q, s, B, t, None, N, False)[:2])
+
+
+@pytest.mark.parametrize("most", [4, 120])
+def test_as_many_experts_as_there_may_be(most):
+    E, N, K = bwgemm.GROUP_MAX_EXPERTS, 72, 144
+    counts = torch.randint(0, most, (E,), generator=torch.Generator().manual_seed(most)).tolist()
+    T = sum(counts) + 5
+    off = ref.offsets_of(counts, 2, "cuda")
+    X, dY = rows(T, K, BF16, 1), rows(T, N, BF16, 2)
+    for mn in (False, True):
+        W = weights(E, N, K, BF16, 3, mn)
+        C = (bwgemm.gemm_grouped if mn else bwgemm.gemm_grouped_tn)(X, W, off)
+        y, err, covered = reference16(X, W, off, N, mn)
+        check(C[covered], y[covered], err[covered])
+    check(bwgemm.gemm_grouped_dw(dY, X, off), *ref.weight_gradient(dY, X, off))
+    Q, s = bwgemm.quantize_f8(X)
+    B, t = bwgemm.quantize_blocks_f8(weights(E, N, K, BF16, 4))
+    C = bwgemm.gemm_f8(Q, s, B, t, offsets=off, dtype=BF16)
+    y, err, covered = reference8(Q, s, B, t, off, N, False)
+    check(C[covered], y[covered], err[covered])
+
+
+@pytest.mark.parametrize("N,K", [(8, 8), (16, 8), (8, 16), (24, 40)])
+def test_the_smallest_widths(N, K):
+    counts = [3, 0, 1, 70]
+    T, E = sum(counts) + 4, len(counts)
+    off = ref.offsets_of(counts, 2, "cuda")
+    X, dY = rows(T, K, F16, 1), rows(T, N, F16, 2)
+    for mn in (False, True):
+        W = weights(E, N, K, F16, 3, mn)
+        C = (bwgemm.gemm_grouped if mn else bwgemm.gemm_grouped_tn)(X, W, off)
+        y, err, covered = reference16(X, W, off, N, mn)
+        check(C[covered], y[covered], err[covered])
+    check(bwgemm.gemm_grouped_dw(dY, X, off, dtype=F32), *ref.weight_gradient(dY, X, off))
+    for M in (1, 200):
+        X, Q, s, B, t = f8_operands(M, 0, N, 16 * K, F16, N)
+        check(bwgemm.gemm_f8(Q, s, B, t), *reference8(Q, s, B, t, None, N, False)[:2])
+        X, Q, s, B, t = f8_operands(M, 0, N, 16, F16, N)
+        check(bwgemm.gemm_f8(Q, s, B, t), *reference8(Q, s, B, t, None, N, False)[:2])
